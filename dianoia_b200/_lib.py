@@ -17,6 +17,25 @@ HEADER = os.path.join(os.path.dirname(PKG), "include", "dianoia_b200.h")
 _i64 = ctypes.c_int64
 _p = ctypes.c_void_p
 
+
+
+class PagedCache(ctypes.Structure):
+    """dn_paged_cache (include/dianoia_b200.h)."""
+    _fields_ = [("keys", _p), ("values", _p), ("table", _p), ("type", _i64), ("pages", _i64),
+                ("page_size", _i64), ("kv_heads", _i64), ("hd", _i64), ("sequences", _i64),
+                ("table_stride", _i64), ("page_stride", _i64)]
+
+
+class LogitRules(ctypes.Structure):
+    """dn_logit_rules (include/dianoia_b200.h)."""
+    _fields_ = [("tokens", _p), ("history", _p), ("generated", _p), ("repetition", _p), ("frequency", _p),
+                ("presence", _p), ("bias_tokens", _p), ("bias", _p), ("bias_start", _p), ("mask", _p),
+                ("mask_row", _p), ("mask_rows", _i64), ("mask_stride", _i64)]
+
+
+_cache_p = ctypes.POINTER(PagedCache)
+_rules_p = ctypes.POINTER(LogitRules)
+
 # Every exported function with its ctypes signature (restype, argtypes).
 SIGNATURES = {
     "lab_alloc": (_p, [_i64]),
@@ -78,6 +97,12 @@ SIGNATURES = {
     "dn_quantize_qa": (_i64, [_p, _p, _i64, _i64, _i64, _p]),
     "dn_rms_norm": (_i64, [_p, _p, _p, _p, _i64, _i64, _i64, ctypes.c_double, _i64, _i64, _p]),
     "dn_swiglu": (_i64, [_p, _p, _p, _i64, _i64, _p]),
+    "dn_paged_append": (_i64, [_cache_p, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _p, _p, _i64, _i64, _p, _p,
+                               ctypes.c_double, _p, _i64, _i64, _i64, _i64, _p]),
+    "dn_paged_attention_workspace": (_i64, [_cache_p, _i64, _i64, _i64, _i64]),
+    "dn_paged_attention": (_i64, [_cache_p, _p, _i64, _p, _p, _p, _i64, _i64, ctypes.c_double, _i64, _p, _i64, _i64,
+                                  _i64, _p, _i64, _i64, _p]),
+    "dn_logits_apply": (_i64, [_i64, _p, _i64, _p, _i64, _i64, _i64, _rules_p, _i64, _p]),
     "dn_linear_qa": (_i64, [_i64, _p, _p, _p, _i64, _p, _i64, _p, _i64, _i64, _i64, _i64, _i64, _p]),
     "dn_linear_allgather": (_i64, [_i64, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _p, _p, _i64, _p]),
     "dn_linear_qa_allgather": (_i64, [_i64, _p, _p, _p, _i64, _i64, _i64, _p, _p, _i64, _i64, _p]),
@@ -107,6 +132,7 @@ SIGNATURES = {
 # Status codes (include/dianoia_b200.h).
 DN_OK, DN_ERR_ARGS, DN_ERR_CUDA, DN_ERR_NO_DEVICE, DN_ERR_UNSUPPORTED, DN_ERR_TOO_LARGE = 0, -1, -2, -3, -4, -5
 DN_Q8, DN_Q4 = 0, 1
+DN_F32, DN_F16, DN_BF16 = 0, 1, 2
 DN_PATH_AUTO, DN_PATH_GEMV, DN_PATH_TC, DN_PATH_GENERIC = -1, 0, 1, 2
 DN_FLAG_PDL = 1
 (DN_BATCH_Q8, DN_BATCH_Q4, DN_BATCH_RMS_NORM, DN_BATCH_SWIGLU, DN_BATCH_ADD, DN_BATCH_COPY, DN_BATCH_STEER,

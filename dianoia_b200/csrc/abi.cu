@@ -382,6 +382,64 @@ bool status_words(uint32_t** dev, volatile uint32_t** host) {
 
 // ======================================================================= lab_*
 
+namespace {
+
+// ------------------------------------------------ the batched step's checks
+
+constexpr int64_t kMaxStride = (int64_t)1 << 32;  // elements: rows * stride * size stays inside 63 bits
+
+bool elem_type(int64_t t) { return t == DN_F32 || t == DN_F16 || t == DN_BF16; }
+
+// Whether `rows` rows of `acols` and `bcols` elements, strides apart, share a
+// byte. Rows of equal byte strides may interleave (parts of one fused
+// product); with unequal ones the whole extents must be apart.
+bool overlaps(const void* a, int64_t astride, int64_t acols, int64_t atype, const void* b, int64_t bstride,
+              int64_t bcols, int64_t btype, int64_t rows) {
+  if (rows <= 0 || acols <= 0 || bcols <= 0) return false;
+  const int64_t as = astride * dn::elem_size(atype), ab = acols * dn::elem_size(atype);
+  const int64_t bs = bstride * dn::elem_size(btype), bb = bcols * dn::elem_size(btype);
+  const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+  if (x >= y + (uintptr_t)((rows - 1) * bs + bb) || y >= x + (uintptr_t)((rows - 1) * as + ab)) return false;
+  if (as != bs || rows == 1) return true;
+  const int64_t ahead = y >= x ? (int64_t)(y - x) % as : (as - (int64_t)(x - y) % as) % as;  // of b's row in a's
+  return ahead < ab || as - ahead < bb;
+}
+
+// A launch the runtime refused: its sticky-free error is taken off the thread.
+int64_t launch_failed() {
+  cudaGetLastError();
+  return DN_ERR_CUDA;
+}
+
+int64_t check_cache(const dn_paged_cache* c) {
+  static_assert(sizeof(dn_paged_cache) == sizeof(dn::PagedCache), "cache layouts differ");
+  static_assert(sizeof(dn_logit_rules) == sizeof(dn::LogitRules), "rule layouts differ");
+  if (c == nullptr || !elem_type(c->type) || c->pages < 0 || c->page_size < 1 || c->kv_heads < 1 || c->hd < 1 ||
+      c->sequences < 0 || c->table_stride < 0)
+    return DN_ERR_ARGS;
+  if (c->hd > dn::kMaxPagedHd || c->page_size > (1 << 20) || c->kv_heads > 65535 || c->pages > INT32_MAX ||
+      c->sequences > (1 << 24) || c->table_stride > INT32_MAX || c->page_stride > kMaxStride)
+    return DN_ERR_TOO_LARGE;
+  if (c->page_stride < c->kv_heads * c->page_size * c->hd) return DN_ERR_ARGS;
+  // Positions are int32.
+  if (c->table_stride * c->page_size > (int64_t)1 << 30) return DN_ERR_TOO_LARGE;
+  if (c->pages > 0 && (c->keys == nullptr || c->values == nullptr)) return DN_ERR_ARGS;
+  if (c->sequences > 0 && c->table_stride > 0 && c->table == nullptr) return DN_ERR_ARGS;
+  const uintptr_t es = (uintptr_t)dn::elem_size(c->type) - 1;
+  if ((((uintptr_t)c->keys | (uintptr_t)c->values) & es) != 0 || ((uintptr_t)c->table & 3) != 0) return DN_ERR_ARGS;
+  return DN_OK;
+}
+
+int64_t check_attention(const dn_paged_cache* c, int64_t heads, int64_t n, int64_t prefix, int64_t max_length) {
+  if (heads < 1 || heads % c->kv_heads != 0 || n < 0 || prefix < 0 || max_length < 0) return DN_ERR_ARGS;
+  if (heads > (1 << 20) || n > (int64_t)1 << 24 || n * heads > (int64_t)1 << 30 || prefix > (int64_t)1 << 30 ||
+      max_length > (int64_t)1 << 30)
+    return DN_ERR_TOO_LARGE;
+  return DN_OK;
+}
+
+}  // namespace
+
 extern "C" {
 
 void* lab_alloc(int64_t bytes) {
@@ -588,6 +646,146 @@ int64_t dn_swiglu(float* g, const float* u, uint8_t* qa, int64_t count, int64_t 
                  cudaSuccess
              ? DN_OK
              : DN_ERR_CUDA;
+}
+
+int64_t dn_paged_append(const dn_paged_cache* cache, int64_t type, const void* q, int64_t q_stride,
+                        const void* k, int64_t k_stride, const void* v, int64_t v_stride,
+                        const int32_t* seq, const int32_t* pos, const float* rope, int64_t rope_rows,
+                        int64_t rot, const float* q_norm, const float* k_norm, double eps, void* q_out,
+                        int64_t q_out_stride, int64_t heads, int64_t n, int64_t flags, void* stream) {
+  if (int64_t rc = check_cache(cache); rc != DN_OK) return rc;
+  if (!elem_type(type) || n < 0 || heads < 0 || rot < 0 || rot % 2 != 0 || rot > cache->hd || rope_rows < 0)
+    return DN_ERR_ARGS;
+  const int64_t kv = cache->kv_heads * cache->hd, qd = heads * cache->hd;
+  if (heads > (1 << 20) || q_stride > kMaxStride || k_stride > kMaxStride || v_stride > kMaxStride ||
+      q_out_stride > kMaxStride)
+    return DN_ERR_TOO_LARGE;
+  if (k_stride < kv || v_stride < kv || q_stride < qd || q_out_stride < qd) return DN_ERR_ARGS;
+  // A group of lanes for each (token, head): the launch's block count fits 31 bits.
+  if (n > (int64_t)0x7fffffff / (heads + 2 * cache->kv_heads)) return DN_ERR_TOO_LARGE;
+  if (n == 0) return DN_OK;
+  if (k == nullptr || v == nullptr || seq == nullptr || pos == nullptr || (rot > 0 && rope == nullptr) ||
+      (heads > 0 && (q == nullptr || q_out == nullptr)))
+    return DN_ERR_ARGS;
+  const uintptr_t es = (uintptr_t)dn::elem_size(type) - 1, cs = (uintptr_t)dn::elem_size(cache->type) - 1;
+  if ((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v) & es) != 0 || ((uintptr_t)q_out & cs) != 0 ||
+      (((uintptr_t)seq | (uintptr_t)pos | (uintptr_t)rope | (uintptr_t)q_norm | (uintptr_t)k_norm) & 3) != 0)
+    return DN_ERR_ARGS;
+  if (heads > 0 && overlaps(q, q_stride, qd, type, q_out, q_out_stride, qd, cache->type, n) &&
+      !(q == q_out && type == cache->type && q_stride == q_out_stride))
+    return DN_ERR_ARGS;
+  if (device_state() == nullptr) return DN_ERR_NO_DEVICE;
+  dn::PagedAppendArgs a{};
+  memcpy(&a.cache, cache, sizeof a.cache);
+  a.type = type;
+  a.q = q;
+  a.k = k;
+  a.v = v;
+  a.q_stride = q_stride;
+  a.k_stride = k_stride;
+  a.v_stride = v_stride;
+  a.seq = seq;
+  a.pos = pos;
+  a.rope = rope;
+  a.rope_rows = rope_rows;
+  a.rot = rot;
+  a.q_norm = q_norm;
+  a.k_norm = k_norm;
+  a.eps = (float)eps;
+  a.q_out = q_out;
+  a.q_out_stride = q_out_stride;
+  a.heads = heads;
+  a.n = n;
+  return dn::launch_paged_append(a, static_cast<cudaStream_t>(stream), (flags & DN_FLAG_PDL) != 0) == cudaSuccess
+             ? DN_OK
+             : launch_failed();
+}
+
+int64_t dn_paged_attention_workspace(const dn_paged_cache* cache, int64_t heads, int64_t n, int64_t prefix,
+                                     int64_t max_length) {
+  if (int64_t rc = check_cache(cache); rc != DN_OK) return rc;
+  if (int64_t rc = check_attention(cache, heads, n, prefix, max_length); rc != DN_OK) return rc;
+  dn::PagedCache c;
+  memcpy(&c, cache, sizeof c);
+  return dn::paged_attention_workspace(c, heads, n, prefix, max_length);
+}
+
+int64_t dn_paged_attention(const dn_paged_cache* cache, const void* q, int64_t q_stride,
+                           const int32_t* q_start, const int32_t* lengths, const int32_t* prefix_pages,
+                           int64_t prefix, int64_t max_length, double scale, int64_t window, void* out,
+                           int64_t out_stride, int64_t heads, int64_t n, void* workspace,
+                           int64_t workspace_bytes, int64_t flags, void* stream) {
+  if (int64_t rc = check_cache(cache); rc != DN_OK) return rc;
+  if (int64_t rc = check_attention(cache, heads, n, prefix, max_length); rc != DN_OK) return rc;
+  const int64_t row = heads * cache->hd;
+  if (window < 0 || window > INT32_MAX || q_stride < row || out_stride < row || workspace_bytes < 0)
+    return DN_ERR_ARGS;
+  if (q_stride > kMaxStride || out_stride > kMaxStride) return DN_ERR_TOO_LARGE;
+  if (q_start == nullptr && n != cache->sequences) return DN_ERR_ARGS;
+  if (n == 0) return DN_OK;
+  if (q == nullptr || lengths == nullptr || out == nullptr || workspace == nullptr ||
+      (prefix > 0 && prefix_pages == nullptr))
+    return DN_ERR_ARGS;
+  const uintptr_t es = (uintptr_t)dn::elem_size(cache->type) - 1;
+  if ((((uintptr_t)q | (uintptr_t)out) & es) != 0 || ((uintptr_t)workspace & 15) != 0 ||
+      (((uintptr_t)q_start | (uintptr_t)lengths | (uintptr_t)prefix_pages) & 3) != 0)
+    return DN_ERR_ARGS;
+  if (overlaps(q, q_stride, row, cache->type, out, out_stride, row, cache->type, n) &&
+      !(q == out && q_stride == out_stride))
+    return DN_ERR_ARGS;
+  dn::PagedAttentionArgs a{};
+  memcpy(&a.cache, cache, sizeof a.cache);
+  if (workspace_bytes < dn::paged_attention_workspace(a.cache, heads, n, prefix, max_length)) return DN_ERR_ARGS;
+  if (device_state() == nullptr) return DN_ERR_NO_DEVICE;
+  a.q = q;
+  a.q_stride = q_stride;
+  a.q_start = q_start;
+  a.lengths = lengths;
+  a.prefix_pages = prefix_pages;
+  a.prefix = prefix;
+  a.max_length = max_length;
+  a.scale = (float)scale;
+  a.window = window;
+  a.out = out;
+  a.out_stride = out_stride;
+  a.heads = heads;
+  a.n = n;
+  a.workspace = workspace;
+  return dn::launch_paged_attention(a, static_cast<cudaStream_t>(stream), (flags & DN_FLAG_PDL) != 0) ==
+                 cudaSuccess
+             ? DN_OK
+             : launch_failed();
+}
+
+int64_t dn_logits_apply(int64_t type, const void* logits, int64_t stride, void* out, int64_t out_stride,
+                        int64_t n, int64_t vocab, const dn_logit_rules* rules, int64_t flags, void* stream) {
+  if (!elem_type(type) || n < 0 || vocab < 0 || stride < vocab || out_stride < vocab || rules == nullptr)
+    return DN_ERR_ARGS;
+  if (vocab > (1 << 30) || n > INT32_MAX || stride > kMaxStride || out_stride > kMaxStride)
+    return DN_ERR_TOO_LARGE;
+  if (n > INT32_MAX / (vocab / 4096 + 2)) return DN_ERR_TOO_LARGE;  // the launch's blocks fit 31 bits
+  const dn_logit_rules& r = *rules;
+  if (r.history != nullptr && r.tokens == nullptr) return DN_ERR_ARGS;
+  if (r.bias_start != nullptr && (r.bias_tokens == nullptr || r.bias == nullptr)) return DN_ERR_ARGS;
+  if (r.mask != nullptr && (r.mask_rows < 0 || r.mask_stride < (vocab + 31) / 32)) return DN_ERR_ARGS;
+  if (r.mask != nullptr && r.mask_row == nullptr && r.mask_rows < n) return DN_ERR_ARGS;
+  if ((((uintptr_t)r.tokens | (uintptr_t)r.generated | (uintptr_t)r.repetition | (uintptr_t)r.frequency |
+        (uintptr_t)r.presence | (uintptr_t)r.bias_tokens | (uintptr_t)r.bias | (uintptr_t)r.mask |
+        (uintptr_t)r.mask_row) & 3) != 0 ||
+      (((uintptr_t)r.history | (uintptr_t)r.bias_start) & 7) != 0)
+    return DN_ERR_ARGS;
+  if (n == 0 || vocab == 0) return DN_OK;
+  const uintptr_t es = (uintptr_t)dn::elem_size(type) - 1;
+  if (logits == nullptr || out == nullptr || (((uintptr_t)logits | (uintptr_t)out) & es) != 0) return DN_ERR_ARGS;
+  if (overlaps(logits, stride, vocab, type, out, out_stride, vocab, type, n) &&
+      !(logits == out && stride == out_stride))
+    return DN_ERR_ARGS;
+  if (device_state() == nullptr) return DN_ERR_NO_DEVICE;
+  dn::LogitsArgs a{type, logits, out, stride, out_stride, n, vocab, {}};
+  memcpy(&a.rules, rules, sizeof a.rules);
+  return dn::launch_logits(a, static_cast<cudaStream_t>(stream), (flags & DN_FLAG_PDL) != 0) == cudaSuccess
+             ? DN_OK
+             : launch_failed();
 }
 
 int64_t dn_linear_qa(int64_t format, const void* qs, const void* scales, const uint8_t* xa,

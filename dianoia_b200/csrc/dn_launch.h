@@ -196,6 +196,79 @@ struct SteerArgs {
 };
 cudaError_t launch_steer(const SteerArgs& a, cudaStream_t stream, bool pdl);
 
+// Element types of the paged cache and of logits.
+enum ElemType : int64_t { kF32 = 0, kF16 = 1, kBF16 = 2 };
+inline int64_t elem_size(int64_t type) { return type == kF32 ? 4 : 2; }
+
+// A paged cache (dn_paged_cache, whose layout this is).
+struct PagedCache {
+  void* keys;
+  void* values;
+  const int32_t* table;
+  int64_t type, pages, page_size, kv_heads, hd, sequences, table_stride, page_stride;
+};
+constexpr int64_t kMaxPagedHd = 256;
+
+// A step's keys and values into the cache, its queries rotated (paged_append.cu).
+struct PagedAppendArgs {
+  PagedCache cache;
+  int64_t type;  // of q, k and v
+  const void* q;
+  const void* k;
+  const void* v;
+  int64_t q_stride, k_stride, v_stride;
+  const int32_t* seq;
+  const int32_t* pos;
+  const float* rope;
+  int64_t rope_rows, rot;
+  const float* q_norm;
+  const float* k_norm;
+  float eps;
+  void* q_out;
+  int64_t q_out_stride, heads, n;
+};
+cudaError_t launch_paged_append(const PagedAppendArgs& a, cudaStream_t stream, bool pdl);
+
+// Attention over the cache for a batch with a shared prefix (paged_attention.cu).
+struct PagedAttentionArgs {
+  PagedCache cache;
+  const void* q;
+  const int32_t* q_start;  // [sequences + 1], or null: one token for each sequence
+  const int32_t* lengths;
+  const int32_t* prefix_pages;
+  void* out;
+  int64_t q_stride, out_stride, prefix, max_length, window, heads, n;
+  float scale;
+  void* workspace;
+};
+int64_t paged_attention_workspace(const PagedCache& c, int64_t heads, int64_t n, int64_t prefix,
+                                  int64_t max_length);
+cudaError_t launch_paged_attention(const PagedAttentionArgs& a, cudaStream_t stream, bool pdl);
+
+// The rules on a batch's logits (dn_logit_rules, whose layout this is; logits.cu).
+struct LogitRules {
+  const int32_t* tokens;
+  const int64_t* history;
+  const int32_t* generated;
+  const float* repetition;
+  const float* frequency;
+  const float* presence;
+  const int32_t* bias_tokens;
+  const float* bias;
+  const int64_t* bias_start;
+  const uint32_t* mask;
+  const int32_t* mask_row;
+  int64_t mask_rows, mask_stride;
+};
+struct LogitsArgs {
+  int64_t type;
+  const void* logits;
+  void* out;
+  int64_t stride, out_stride, n, vocab;
+  LogitRules rules;
+};
+cudaError_t launch_logits(const LogitsArgs& a, cudaStream_t stream, bool pdl);
+
 // The decode GEMV on either activation form (gemv.cu).
 int64_t launch_gemv_ex(const GemvArgs& g, cudaStream_t stream, bool pdl);
 bool gemv_ex_supported(const GemvArgs& g);

@@ -1,0 +1,330 @@
+// Attention over a paged cache for a batch whose sequences share a prefix
+// (dn_paged_attention): out = softmax(scale q . k) v over the positions a
+// query sees, the shared ones read once for every query of the batch.
+// paged_attention.cuh says how the work is divided and joined.
+#include "paged_attention.cuh"
+
+namespace dn {
+namespace {
+
+using namespace paged;
+
+constexpr int kLanes = 32;
+
+// ------------------------------------------------------- the f32 arithmetic
+//
+// Any type, head size up to 256 and alignment. A block of 4 warps takes 16
+// rows; each tile of 32 keys is brought to shared memory as f32 for all of
+// them. Warp w owns rows 4 w .. 4 w + 3: lane j scores key j for each (f32
+// FMAs along the head), the tile's maximum and sum are warp reductions, and
+// for the values lane j owns dimensions 4 j .. 4 j + 3 (and 128 more on).
+constexpr int kSimtThreads = 128;
+constexpr int kSimtRows = 16;
+constexpr int kSimtKeys = 32;
+constexpr int kWarpRows = 4;
+
+// Floats of a row of keys, values or queries in shared memory: 16-byte
+// aligned, and eight rows apart by 16 bytes of banks.
+__host__ __device__ constexpr int simt_pitch(int hd) { return (hd + 31) / 32 * 32 + 4; }
+
+template <typename T, int V>
+__global__ void __launch_bounds__(kSimtThreads) attention_simt_kernel(const __grid_constant__ Params p) {
+  pdl_launch_dependents();
+  pdl_wait();
+  extern __shared__ float smem[];
+  const int hd = (int)p.a.cache.hd, pitch = simt_pitch(hd);
+  float* qs = smem;                            // [kSimtRows][pitch]
+  float* ks = qs + kSimtRows * pitch;          // [kSimtKeys][pitch]
+  float* vs = ks + kSimtKeys * pitch;          // [kSimtKeys][pitch]
+  float* ps = vs + kSimtKeys * pitch;          // [4 warps][kSimtKeys][kWarpRows]
+  __shared__ int row_low[kSimtRows], row_high[kSimtRows], span[2];
+  __shared__ int key_page[kSimtKeys];
+  Work w;
+  if (!find_work(p, w)) return;
+  const int tid = threadIdx.x, warp = tid / kLanes, lane = tid % kLanes;
+  if (tid < kSimtRows) {
+    int low = 0, high = -1;
+    if (tid < w.rows) {
+      const int t = (w.row0 + tid) / p.group;
+      sees(p, w.prefix ? seq_of(p, t) : w.seq, t, low, high);
+    }
+    row_low[tid] = low;
+    row_high[tid] = high;
+    const bool any = high >= low;
+    const int lo = __reduce_min_sync(0xffffu, any ? low : INT32_MAX);
+    const int hi = __reduce_max_sync(0xffffu, any ? high : -1);
+    if (tid == 0) {
+      span[0] = lo;
+      span[1] = hi;
+    }
+  }
+  for (int i = tid; i < kSimtRows * pitch; i += kSimtThreads) {
+    const int r = i / pitch, d = i % pitch;
+    float x = 0.0f;
+    if (r < w.rows && d < hd) {
+      int t, head;
+      out_index(p, w, r, t, head);
+      x = to_f32<T>(static_cast<const T*>(p.a.q)[t * p.a.q_stride + (int64_t)head * hd + d]);
+    }
+    qs[i] = x;
+  }
+  __syncthreads();
+  int begin, end;
+  slice_keys(p, w, span[0], span[1], kSimtKeys, begin, end);
+
+  float m[kWarpRows], l[kWarpRows], acc[kWarpRows][2][4];
+#pragma unroll
+  for (int r = 0; r < kWarpRows; r++) {
+    m[r] = -INFINITY;
+    l[r] = 0.0f;
+#pragma unroll
+    for (int u = 0; u < 2; u++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) acc[r][u][e] = 0.0f;
+  }
+  const int row_base = warp * kWarpRows;
+  int low[kWarpRows], high[kWarpRows];
+#pragma unroll
+  for (int r = 0; r < kWarpRows; r++) {
+    low[r] = row_low[row_base + r];
+    high[r] = row_high[row_base + r];
+  }
+  for (int k0 = begin; k0 < end; k0 += kSimtKeys) {
+    __syncthreads();  // the last tile is read
+    if (tid < kSimtKeys) key_page[tid] = k0 + tid < end ? page_of(p, w, k0 + tid) : -1;
+    __syncthreads();
+    const int runs = pitch / V;
+    for (int i = tid; i < kSimtKeys * runs; i += kSimtThreads) {
+      const int j = i / runs, d = i % runs * V;
+      float x[V] = {}, y[V] = {};
+      if (key_page[j] >= 0 && d < hd) {
+        const int slot = (k0 + j) % (int)p.a.cache.page_size;
+        const int64_t at = key_page[j] * p.a.cache.page_stride +
+                           ((int64_t)w.head * p.a.cache.page_size + slot) * hd + d;
+        load_run<T, V>(static_cast<const T*>(p.a.cache.keys) + at, x);
+        load_run<T, V>(static_cast<const T*>(p.a.cache.values) + at, y);
+      }
+#pragma unroll
+      for (int e = 0; e < V; e++) {
+        ks[j * pitch + d + e] = x[e];
+        vs[j * pitch + d + e] = y[e];
+      }
+    }
+    __syncthreads();
+    // Scores of key `lane` for the warp's rows.
+    float s[kWarpRows] = {};
+    const float4* kv = reinterpret_cast<const float4*>(ks + lane * pitch);
+    for (int d = 0; d < (hd + 3) / 4; d++) {
+      const float4 k = kv[d];
+#pragma unroll
+      for (int r = 0; r < kWarpRows; r++) {
+        const float4 q = reinterpret_cast<const float4*>(qs + (row_base + r) * pitch)[d];
+        s[r] = fmaf(q.x, k.x, s[r]);
+        s[r] = fmaf(q.y, k.y, s[r]);
+        s[r] = fmaf(q.z, k.z, s[r]);
+        s[r] = fmaf(q.w, k.w, s[r]);
+      }
+    }
+    const bool there = key_page[lane] >= 0;
+    float pr[kWarpRows];
+    bool all = true;  // every row that sees a key of the tile sees all of it
+#pragma unroll
+    for (int r = 0; r < kWarpRows; r++) {
+      const bool seen = there && k0 + lane >= low[r] && k0 + lane <= high[r];
+      const float x = seen ? s[r] * p.scale_log2 : -INFINITY;
+      float top = x;
+#pragma unroll
+      for (int off = 16; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+      const float next = fmaxf(m[r], top);
+      const float base = next == -INFINITY ? 0.0f : next;
+      const float keep = exp2f(m[r] - base);
+      pr[r] = seen ? exp2f(x - base) : 0.0f;
+      m[r] = next;
+      l[r] = l[r] * keep + pr[r];  // a lane's share; summed over the lanes at the end
+#pragma unroll
+      for (int u = 0; u < 2; u++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) acc[r][u][e] *= keep;
+      all = all && seen;
+    }
+    float4* pw = reinterpret_cast<float4*>(ps) + warp * kSimtKeys;
+    pw[lane] = make_float4(pr[0], pr[1], pr[2], pr[3]);
+    __syncwarp();
+    const bool fast = __all_sync(0xffffffffu, all);
+    for (int j = 0; j < kSimtKeys; j++) {
+      const float4 q = pw[j];
+      const float pj[kWarpRows] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+      for (int u = 0; u < 2; u++) {
+        const int d = 4 * lane + 128 * u;
+        if (d >= hd) break;
+        const float4 v = *reinterpret_cast<const float4*>(vs + j * pitch + d);
+        const float ve[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int r = 0; r < kWarpRows; r++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            // A key that a row does not see adds nothing, infinite or not.
+            if (fast || pj[r] != 0.0f) acc[r][u][e] = fmaf(pj[r], ve[e], acc[r][u][e]);
+          }
+      }
+    }
+    __syncwarp();
+  }
+#pragma unroll
+  for (int r = 0; r < kWarpRows; r++) {
+    float sum = l[r];
+#pragma unroll
+    for (int off = 16; off >= 1; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+    if (row_base + r >= w.rows) continue;
+    int t, head;
+    const int64_t row = out_index(p, w, row_base + r, t, head);
+    if (p.direct) {
+      const float inv = sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum;  // NaN stays
+      T* out = static_cast<T*>(p.a.out) + t * p.a.out_stride + (int64_t)head * hd;
+#pragma unroll
+      for (int u = 0; u < 2; u++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const int d = 4 * lane + 128 * u + e;
+          if (d < hd) out[d] = from_f32<T>(sum == 0.0f ? 0.0f : acc[r][u][e] * inv);
+        }
+    } else {
+      const int64_t at = slice_index(p, w) * (p.a.n * p.a.heads) + row;
+      if (lane == 0) p.ml[at] = make_float2(m[r], sum);
+#pragma unroll
+      for (int u = 0; u < 2; u++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const int d = 4 * lane + 128 * u + e;
+          if (d < hd) p.acc[at * hd + d] = acc[r][u][e];
+        }
+    }
+  }
+}
+
+// ------------------------------------------------------------------ the join
+
+constexpr int kJoinThreads = 128;
+
+// One warp for each (token, head).
+template <typename T>
+__global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(const __grid_constant__ Params p) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int64_t rows = p.a.n * p.a.heads;
+  const int64_t row = (int64_t)blockIdx.x * (kJoinThreads / kLanes) + threadIdx.x / kLanes;
+  if (row >= rows) return;
+  const int lane = threadIdx.x % kLanes, hd = (int)p.a.cache.hd;
+  const int t = (int)(row / p.a.heads), head = (int)(row % p.a.heads);
+  if (p.a.q_start != nullptr && seq_of(p, t) < 0) return;
+  const int slices = p.prefix_splits + p.own_splits;
+  float m = -INFINITY;
+  for (int i = 0; i < slices; i++) m = fmaxf(m, p.ml[i * rows + row].x);
+  const float base = m == -INFINITY ? 0.0f : m;
+  float l = 0.0f, acc[kMaxPagedHd / kLanes] = {};
+  for (int i = 0; i < slices; i++) {
+    const float2 ml = p.ml[i * rows + row];
+    if (ml.y == 0.0f) continue;
+    const float f = exp2f(ml.x - base);
+    l += ml.y * f;
+    const float* a = p.acc + (i * rows + row) * hd;
+#pragma unroll
+    for (int u = 0; u < kMaxPagedHd / kLanes; u++)
+      if (lane + kLanes * u < hd) acc[u] += a[lane + kLanes * u] * f;
+  }
+  T* out = static_cast<T*>(p.a.out) + t * p.a.out_stride + (int64_t)head * hd;
+#pragma unroll
+  for (int u = 0; u < kMaxPagedHd / kLanes; u++)
+    if (lane + kLanes * u < hd) out[lane + kLanes * u] = from_f32<T>(l == 0.0f ? 0.0f : acc[u] / l);
+}
+
+// ------------------------------------------------------------------ the host
+
+// How the work is divided, from sizes that the host knows.
+Params plan(const PagedCache& c, int64_t heads, int64_t n, int64_t prefix, int64_t max_length) {
+  Params p{};
+  p.group = (int)(heads / c.kv_heads);
+  p.tile_rows = kSimtRows;
+  p.min_slice = 128;
+  const int64_t rows = n * p.group;
+  const int64_t tiles = (rows + p.tile_rows - 1) / p.tile_rows;
+  p.prefix_tiles = prefix > 0 ? (int)tiles : 0;
+  p.own_slots = (int)(rows / p.tile_rows + c.sequences);
+  // Enough blocks to give every SM two, as long as a slice has min_slice keys.
+  auto splits = [&](int64_t blocks, int64_t keys) {
+    const int64_t want = (2 * 148 + blocks - 1) / (blocks > 0 ? blocks : 1);
+    const int64_t most = (keys + p.min_slice - 1) / p.min_slice;
+    return (int)(want < most ? want : most > 1 ? most : 1);
+  };
+  p.prefix_splits = prefix > 0 ? splits(tiles * c.kv_heads, prefix) : 0;
+  const int64_t own = max_length > prefix ? max_length - prefix : 1;
+  p.own_splits = splits((int64_t)p.own_slots * c.kv_heads, own);
+  p.direct = p.prefix_splits + p.own_splits == 1;
+  return p;
+}
+
+template <typename K>
+cudaError_t launch_ex(K kern, const Params& p, dim3 grid, int threads, size_t smem, cudaStream_t stream, bool pdl) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = pdl ? 1 : 0;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, p);
+}
+
+template <typename T, int V>
+cudaError_t launch_simt(const Params& p, cudaStream_t stream, bool pdl) {
+  const size_t smem = ((kSimtRows + 2 * kSimtKeys) * (size_t)simt_pitch((int)p.a.cache.hd) +
+                       kSimtThreads / kLanes * kSimtKeys * kWarpRows) * sizeof(float);
+  if (cudaError_t e = cudaFuncSetAttribute(attention_simt_kernel<T, V>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                           (int)smem);
+      e != cudaSuccess)
+    return e;
+  const dim3 grid((unsigned)(p.prefix_tiles * p.prefix_splits + p.own_slots * p.own_splits),
+                  (unsigned)p.a.cache.kv_heads);
+  return launch_ex(attention_simt_kernel<T, V>, p, grid, kSimtThreads, smem, stream, pdl);
+}
+
+template <typename T>
+cudaError_t launch_type(Params& p, cudaStream_t stream, bool pdl) {
+  constexpr int V = 16 / sizeof(T);
+  const PagedCache& c = p.a.cache;
+  const bool runs = (((uintptr_t)c.keys | (uintptr_t)c.values) & 15) == 0 && (c.page_stride | c.hd) % V == 0;
+  cudaError_t e = runs ? launch_simt<T, V>(p, stream, pdl) : launch_simt<T, 1>(p, stream, pdl);
+  if (e != cudaSuccess || p.direct) return e;
+  const int64_t warps = p.a.n * p.a.heads, per = kJoinThreads / kLanes;
+  return launch_ex(attention_join_kernel<T>, p, dim3((unsigned)((warps + per - 1) / per)), kJoinThreads, 0, stream,
+                   true);
+}
+
+}  // namespace
+
+int64_t paged_attention_workspace(const PagedCache& c, int64_t heads, int64_t n, int64_t prefix,
+                                  int64_t max_length) {
+  const Params p = plan(c, heads, n, prefix, max_length);
+  return (p.prefix_splits + p.own_splits) * n * heads * (c.hd + 2) * (int64_t)sizeof(float) + 16;
+}
+
+cudaError_t launch_paged_attention(const PagedAttentionArgs& a, cudaStream_t stream, bool pdl) {
+  if (a.n <= 0) return cudaSuccess;
+  Params p = plan(a.cache, a.heads, a.n, a.prefix, a.max_length);
+  p.a = a;
+  p.scale_log2 = a.scale * kLog2e;
+  const int64_t rows = (p.prefix_splits + p.own_splits) * a.n * a.heads;
+  p.ml = static_cast<float2*>(a.workspace);
+  p.acc = reinterpret_cast<float*>(p.ml + (rows + 1) / 2 * 2);
+  switch (a.cache.type) {
+    case kF32: return launch_type<float>(p, stream, pdl);
+    case kF16: return launch_type<__half>(p, stream, pdl);
+    default: return launch_type<__nv_bfloat16>(p, stream, pdl);
+  }
+}
+
+}  // namespace dn

@@ -1,0 +1,167 @@
+// The pieces that the paged attention's kernels share: how a launch's blocks
+// map to work, what a row of queries sees, and where partial results go.
+//
+// A row is one head's query of one token; the rows of a kv head's group lie
+// together, row = token * group + g. The keys a row sees, positions low ..
+// high, fall in two parts: the shared prefix (positions below `prefix`, read
+// through one page list for the whole batch) and the sequence's own. A block
+// takes a tile of rows of one kv head and a slice of one part's keys and
+// leaves, for each row, the running maximum m of its scores (in log2 units),
+// the sum l of 2^(score - m) and the weighted values acc; the join is
+//   m = max m_i, l = sum l_i 2^(m_i - m), out = sum acc_i 2^(m_i - m) / l.
+#pragma once
+
+#include "dn_common.cuh"
+#include "dn_launch.h"
+#include "elem.cuh"
+
+namespace dn {
+namespace paged {
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct Params {
+  PagedAttentionArgs a;
+  int group;            // query heads of a kv head
+  int tile_rows;        // rows of a block
+  int prefix_tiles, prefix_splits;
+  int own_slots, own_splits;
+  int min_slice;        // keys: slices are not made shorter than this
+  float* acc;           // [prefix_splits + own_splits][n * heads][hd]
+  float2* ml;           // [prefix_splits + own_splits][n * heads]: m, l
+  float scale_log2;
+  bool direct;          // one slice in all: blocks write `out` themselves
+};
+
+// A block's work: rows row0 .. row0 + rows - 1 of kv head `head`, slice
+// `slice` of the part's keys, whose pages are `pages`.
+struct Work {
+  bool prefix;
+  int head, row0, rows, slice, splits, seq;
+};
+
+__device__ __forceinline__ int seq_start(const Params& p, int s) {
+  if (p.a.q_start == nullptr) return s;
+  const int v = p.a.q_start[s];
+  return v < 0 ? 0 : v > (int)p.a.n ? (int)p.a.n : v;
+}
+
+// The sequence that token t belongs to, or -1.
+__device__ __forceinline__ int seq_of(const Params& p, int t) {
+  const int seqs = (int)p.a.cache.sequences;
+  if (p.a.q_start == nullptr) return t < seqs ? t : -1;
+  int lo = 0, hi = seqs;  // the last s with seq_start(s) <= t
+  while (lo < hi) {
+    const int mid = (lo + hi) / 2;
+    if (seq_start(p, mid) <= t) lo = mid + 1;
+    else hi = mid;
+  }
+  const int s = lo - 1;
+  return s >= 0 && t < seq_start(p, s + 1) ? s : -1;
+}
+
+// Positions low .. high that token t of sequence s sees (high < low: none).
+__device__ __forceinline__ void sees(const Params& p, int s, int t, int& low, int& high) {
+  low = 0;
+  high = -1;
+  if (s < 0) return;
+  high = p.a.lengths[s] - (seq_start(p, s + 1) - t);
+  if (p.a.window > 0) low = max(0, high - (int)p.a.window + 1);
+}
+
+// Slots of own work: sequence s has slots first(s) .. first(s + 1) - 1, at
+// least its ceil(rows / tile_rows); first(sequences) = own_slots at most.
+__device__ __forceinline__ int first_slot(const Params& p, int s) {
+  return (int)((int64_t)seq_start(p, s) * p.group / p.tile_rows) + s;
+}
+
+__device__ __forceinline__ bool find_work(const Params& p, Work& w) {
+  int b = blockIdx.x;
+  w.head = blockIdx.y;
+  const int prefix_blocks = p.prefix_tiles * p.prefix_splits;
+  w.prefix = b < prefix_blocks;
+  if (w.prefix) {
+    w.seq = -1;
+    w.splits = p.prefix_splits;
+    w.slice = b / p.prefix_tiles;
+    w.row0 = b % p.prefix_tiles * p.tile_rows;
+    w.rows = min(p.tile_rows, (int)p.a.n * p.group - w.row0);
+    return w.rows > 0;
+  }
+  b -= prefix_blocks;
+  w.splits = p.own_splits;
+  w.slice = b / p.own_slots;
+  const int slot = b % p.own_slots;
+  const int seqs = (int)p.a.cache.sequences;
+  if (p.a.q_start == nullptr && p.group <= p.tile_rows) {
+    w.seq = slot;
+    w.row0 = slot * p.group;
+    w.rows = p.group;
+    return slot < seqs;
+  }
+  int lo = 0, hi = seqs;  // the last s with first_slot(s) <= slot
+  while (lo < hi) {
+    const int mid = (lo + hi) / 2;
+    if (first_slot(p, mid) <= slot) lo = mid + 1;
+    else hi = mid;
+  }
+  w.seq = lo - 1;
+  if (w.seq < 0) return false;
+  const int end = seq_start(p, w.seq + 1) * p.group;
+  w.row0 = seq_start(p, w.seq) * p.group + (slot - first_slot(p, w.seq)) * p.tile_rows;
+  w.rows = min(p.tile_rows, end - w.row0);
+  return w.rows > 0;
+}
+
+// The page of a position of the part, or -1 where there is none.
+__device__ __forceinline__ int page_of(const Params& p, const Work& w, int pos) {
+  const int entry = pos / (int)p.a.cache.page_size;
+  int page;
+  if (w.prefix) {
+    page = p.a.prefix_pages[entry];
+  } else {
+    if (entry >= (int)p.a.cache.table_stride) return -1;
+    page = p.a.cache.table[(int64_t)w.seq * p.a.cache.table_stride + entry];
+  }
+  return page >= 0 && page < (int)p.a.cache.pages ? page : -1;
+}
+
+// The slice's keys, begin .. end - 1, of the positions low .. high that the
+// tile's rows see between them; slices start at multiples of `tile`.
+__device__ __forceinline__ void slice_keys(const Params& p, const Work& w, int low, int high, int tile, int& begin,
+                                           int& end) {
+  const int prefix = (int)p.a.prefix;
+  int lo = w.prefix ? low : max(low, prefix);
+  int hi = w.prefix ? min(high, prefix - 1) : high;
+  if (!w.prefix) {
+    const int last = (int)(p.a.cache.table_stride * p.a.cache.page_size) - 1;
+    hi = min(hi, last);
+  }
+  lo = lo / tile * tile;
+  if (!w.prefix) lo = max(lo, prefix);
+  const int keys = hi - lo + 1;
+  if (keys <= 0) {
+    begin = end = 0;
+    return;
+  }
+  int per = max((keys + w.splits - 1) / w.splits, p.min_slice);
+  per = (per + tile - 1) / tile * tile;
+  const int64_t b = lo + (int64_t)w.slice * per;
+  begin = (int)min((int64_t)hi + 1, b);
+  end = (int)min((int64_t)hi + 1, b + per);
+}
+
+// Index of a row of the tile in the workspace: token * heads + head.
+__device__ __forceinline__ int64_t out_index(const Params& p, const Work& w, int r, int& token, int& head) {
+  const int row = w.row0 + r;
+  token = row / p.group;
+  head = w.head * p.group + row % p.group;
+  return (int64_t)token * p.a.heads + head;
+}
+
+__device__ __forceinline__ int slice_index(const Params& p, const Work& w) {
+  return w.prefix ? w.slice : p.prefix_splits + w.slice;
+}
+
+}  // namespace paged
+}  // namespace dn

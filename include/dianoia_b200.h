@@ -396,6 +396,129 @@ int64_t dn_linear_qa(int64_t format, const void* qs, const void* scales, const u
                      int64_t xa_stride, float* ys, int64_t ldy, uint8_t* ya, int64_t ya_stride,
                      int64_t rows, int64_t cols, int64_t n, int64_t flags, void* stream);
 
+/* ------------------------------------------- dn_* (a batched decode step's neighbours)
+ *
+ * What a step that serves many requests at once needs beside the products: a
+ * paged key / value cache, attention over it that reads a prefix the requests
+ * share once for all of them, and the rules on the logits that the sampler
+ * reads. No counterpart in the reference, which runs one sequence over a
+ * contiguous f32 cache (lab_gpu_enc_attention). Device pointers throughout,
+ * asynchronous on `stream`, nothing allocated, capturable in a CUDA graph. */
+
+/* Element types. */
+#define DN_F32 0
+#define DN_F16 1
+#define DN_BF16 2
+
+/* A paged cache as a caller keeps it. Position p of sequence s is slot
+ * p % page_size of page table[s * table_stride + p / page_size]; a page holds
+ * [kv_heads, page_size, hd] elements of `type`, page i starting at element
+ * i * page_stride of `keys` and of `values` (page_stride = kv_heads *
+ * page_size * hd for a pool of its own; more where pools are interleaved).
+ * keys and values are aligned to their element; with both 16-byte aligned and
+ * hd and page_stride multiples of 16 bytes the kernels move 16 bytes at a
+ * time. hd is at most 256. A table entry outside [0, pages) names no page:
+ * nothing is written through it, and no query sees its positions (a window's
+ * freed pages may be marked -1). A position past the table's table_stride
+ * pages does not exist. */
+typedef struct dn_paged_cache {
+  void* keys;
+  void* values;
+  const int32_t* table;
+  int64_t type, pages, page_size, kv_heads, hd, sequences, table_stride, page_stride;
+} dn_paged_cache;
+
+/* Appends n tokens' keys and values to a paged cache and rotates their
+ * queries, in one launch. Token t belongs to sequence seq[t] at position
+ * pos[t]; its q, k and v are `heads`, kv_heads and kv_heads rows of hd
+ * elements of `type` at element t * q_stride of q, t * k_stride of k and
+ * t * v_stride of v (three parts of one fused product, say). Queries and keys
+ * are first normalized per head where q_norm / k_norm (hd f32 weights) are not
+ * NULL, w * x / sqrt(mean(x^2) + eps), and then rotated: values j and j + rot / 2
+ * (j < rot / 2) of a head by the cosines and sines of the token's row of
+ * `rope`, [cos(rot / 2), sin(rot / 2)] at rope + pos[t] * rot (the half-split
+ * form of lab_gpu_enc_head_norm_rope); values rot .. hd - 1 stay. rot is even,
+ * at most hd; 0 (rope may be NULL) rotates nothing. Arithmetic is in f32 and
+ * each result is rounded once, to the cache's type: keys and values into the
+ * token's slot, queries to q_out (`heads` rows of hd at t * q_out_stride).
+ * heads 0 (q and q_out may be NULL) appends without queries. q_out must not
+ * overlap q unless it has the same address, type and stride.
+ * A token is skipped - nothing appended, its q_out row zeros - where seq[t] is
+ * outside [0, sequences), pos[t] is negative, past the table or (rot > 0) past
+ * the rope_rows rows of `rope`, or its table entry names no page. Two tokens
+ * of one call in the same slot leave either's values. */
+int64_t dn_paged_append(const dn_paged_cache* cache, int64_t type, const void* q, int64_t q_stride,
+                        const void* k, int64_t k_stride, const void* v, int64_t v_stride,
+                        const int32_t* seq, const int32_t* pos, const float* rope, int64_t rope_rows,
+                        int64_t rot, const float* q_norm, const float* k_norm, double eps, void* q_out,
+                        int64_t q_out_stride, int64_t heads, int64_t n, int64_t flags, void* stream);
+
+/* Causal grouped-query attention of a batch over a paged cache whose
+ * sequences share their first `prefix` positions: those keys and values are
+ * read once, through prefix_pages (the ceil(prefix / page_size) pages that
+ * hold them; NULL with prefix 0), for every query of the batch; positions from
+ * `prefix` on are read through each sequence's own table row. Queries are
+ * ragged: sequence s has tokens q_start[s] .. q_start[s + 1] - 1 of q (n =
+ * q_start[sequences]; q_start NULL is one token for each sequence), its last
+ * ones, so that token t is at position lengths[s] - (q_start[s + 1] - t) and
+ * sees the positions up to its own, the window - 1 before it with window > 0.
+ * q and out are `heads` rows of hd elements of the cache's type a token, at
+ * t * q_stride and t * out_stride; heads is a multiple of kv_heads, head h
+ * reading kv head h / (heads / kv_heads). out = softmax(scale * q . k) v; a
+ * query that sees no position (a slot of the batch with length 0) gives zeros,
+ * and what lies in positions that a query does not see (infinities and NaN
+ * too) does not reach its output. Scores, softmax and sums are in f32; for
+ * 16-bit types the probabilities are rounded to that type before they multiply
+ * the values, as the tensor cores take them. out may be q (the same address
+ * and stride). Tokens at and past q_start[sequences] are left alone.
+ * max_length is the longest length the batch may have: a hint that sizes the
+ * split of long sequences, any lengths are computed right. `workspace`
+ * (16-byte aligned, at least dn_paged_attention_workspace bytes, from the same
+ * cache, heads, n, prefix and max_length) is undefined before and after, and
+ * calls that overlap in time need one each. */
+int64_t dn_paged_attention_workspace(const dn_paged_cache* cache, int64_t heads, int64_t n, int64_t prefix,
+                                     int64_t max_length);
+int64_t dn_paged_attention(const dn_paged_cache* cache, const void* q, int64_t q_stride,
+                           const int32_t* q_start, const int32_t* lengths, const int32_t* prefix_pages,
+                           int64_t prefix, int64_t max_length, double scale, int64_t window, void* out,
+                           int64_t out_stride, int64_t heads, int64_t n, void* workspace,
+                           int64_t workspace_bytes, int64_t flags, void* stream);
+
+/* The rules on a batch's logits, all of them optional. */
+typedef struct dn_logit_rules {
+  /* Penalties for repeated tokens (history NULL: none). Row r's tokens so far
+   * are tokens[history[r]] .. tokens[history[r + 1] - 1]; its last
+   * generated[r] of them were generated (generated NULL: all). Ids outside
+   * [0, vocab) are ignored. NULL penalties are neutral. */
+  const int32_t* tokens;
+  const int64_t* history;   /* [n + 1] */
+  const int32_t* generated; /* [n] */
+  const float* repetition;  /* [n], > 0: a token seen: x / r where x > 0, else x * r */
+  const float* frequency;   /* [n]: less f for each time a token was generated */
+  const float* presence;    /* [n]: less p for a token generated at all */
+  /* Biases (bias_start NULL: none): bias[i] is added to row r's logit of
+   * bias_tokens[i], bias_start[r] <= i < bias_start[r + 1], in that order. */
+  const int32_t* bias_tokens;
+  const float* bias;
+  const int64_t* bias_start; /* [n + 1] */
+  /* Grammar masks (mask NULL: none): mask row m is mask_stride words, token v
+   * allowed where bit v % 32 of word v / 32 is set. Row r takes mask row
+   * mask_row[r] (mask_row NULL: r), and none where that is outside
+   * [0, mask_rows). */
+  const uint32_t* mask;
+  const int32_t* mask_row; /* [n] */
+  int64_t mask_rows, mask_stride;
+} dn_logit_rules;
+
+/* Applies the rules to n rows of `vocab` logits of `type`, row r at element
+ * r * stride of logits, into out (row r at r * out_stride; out may be logits,
+ * with the same stride, and must not overlap it otherwise), in the order
+ * repetition, frequency and presence, bias, mask. A token that the mask does
+ * not allow gives minus infinity whatever its logit was (a mask that allows
+ * none leaves a row of them). Arithmetic is in f32, rounded once to `type`. */
+int64_t dn_logits_apply(int64_t type, const void* logits, int64_t stride, void* out, int64_t out_stride,
+                        int64_t n, int64_t vocab, const dn_logit_rules* rules, int64_t flags, void* stream);
+
 /* A decode chain: the quantized products of one token (or any sequence of
  * GEMVs on QA activations) run by ONE persistent kernel, so HBM keeps
  * streaming weights across the dependencies between them. Op i reads QA
