@@ -5,11 +5,10 @@
 #include "paged_attention.cuh"
 
 namespace dn {
-namespace {
 
 using namespace paged;
 
-constexpr int kLanes = 32;
+namespace {
 
 // ------------------------------------------------------- the f32 arithmetic
 //
@@ -241,16 +240,24 @@ __global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(const __gr
 
 // ------------------------------------------------------------------ the host
 
+// Whether the tensor-core kernel takes a cache: 16-bit elements whose rows are
+// whole, aligned runs of 16 bytes.
+bool mma_cache(const PagedCache& c) {
+  return c.type != kF32 && (((uintptr_t)c.keys | (uintptr_t)c.values) & 15) == 0 && (c.page_stride | c.hd) % 8 == 0;
+}
+
 // How the work is divided, from sizes that the host knows.
 Params plan(const PagedCache& c, int64_t heads, int64_t n, int64_t prefix, int64_t max_length) {
+  const bool mma = mma_cache(c);
   Params p{};
   p.group = (int)(heads / c.kv_heads);
-  p.tile_rows = kSimtRows;
-  p.min_slice = 128;
   const int64_t rows = n * p.group;
-  const int64_t tiles = (rows + p.tile_rows - 1) / p.tile_rows;
+  p.prefix_rows = mma && rows > 2 * kThinRows ? kWideRows : kThinRows;
+  p.own_rows = mma && rows > 2 * kThinRows * c.sequences ? kWideRows : kThinRows;
+  p.min_slice = 128;
+  const int64_t tiles = (rows + p.prefix_rows - 1) / p.prefix_rows;
   p.prefix_tiles = prefix > 0 ? (int)tiles : 0;
-  p.own_slots = (int)(rows / p.tile_rows + c.sequences);
+  p.own_slots = (int)(rows / p.own_rows + c.sequences);
   // Enough blocks to give every SM two, as long as a slice has min_slice keys.
   auto splits = [&](int64_t blocks, int64_t keys) {
     const int64_t want = (2 * 148 + blocks - 1) / (blocks > 0 ? blocks : 1);
@@ -264,21 +271,6 @@ Params plan(const PagedCache& c, int64_t heads, int64_t n, int64_t prefix, int64
   return p;
 }
 
-template <typename K>
-cudaError_t launch_ex(K kern, const Params& p, dim3 grid, int threads, size_t smem, cudaStream_t stream, bool pdl) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3((unsigned)threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = pdl ? 1 : 0;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kern, p);
-}
-
 template <typename T, int V>
 cudaError_t launch_simt(const Params& p, cudaStream_t stream, bool pdl) {
   const size_t smem = ((kSimtRows + 2 * kSimtKeys) * (size_t)simt_pitch((int)p.a.cache.hd) +
@@ -287,17 +279,17 @@ cudaError_t launch_simt(const Params& p, cudaStream_t stream, bool pdl) {
                                            (int)smem);
       e != cudaSuccess)
     return e;
-  const dim3 grid((unsigned)(p.prefix_tiles * p.prefix_splits + p.own_slots * p.own_splits),
-                  (unsigned)p.a.cache.kv_heads);
-  return launch_ex(attention_simt_kernel<T, V>, p, grid, kSimtThreads, smem, stream, pdl);
+  return launch_ex(attention_simt_kernel<T, V>, p, attention_grid(p), kSimtThreads, smem, stream, pdl);
 }
 
 template <typename T>
-cudaError_t launch_type(Params& p, cudaStream_t stream, bool pdl) {
+cudaError_t launch_type(const Params& p, cudaStream_t stream, bool pdl) {
   constexpr int V = 16 / sizeof(T);
   const PagedCache& c = p.a.cache;
   const bool runs = (((uintptr_t)c.keys | (uintptr_t)c.values) & 15) == 0 && (c.page_stride | c.hd) % V == 0;
-  cudaError_t e = runs ? launch_simt<T, V>(p, stream, pdl) : launch_simt<T, 1>(p, stream, pdl);
+  cudaError_t e = mma_cache(c) ? launch_attention_mma(p, stream, pdl)
+                  : runs       ? launch_simt<T, V>(p, stream, pdl)
+                               : launch_simt<T, 1>(p, stream, pdl);
   if (e != cudaSuccess || p.direct) return e;
   const int64_t warps = p.a.n * p.a.heads, per = kJoinThreads / kLanes;
   return launch_ex(attention_join_kernel<T>, p, dim3((unsigned)((warps + per - 1) / per)), kJoinThreads, 0, stream,
@@ -316,6 +308,7 @@ cudaError_t launch_paged_attention(const PagedAttentionArgs& a, cudaStream_t str
   if (a.n <= 0) return cudaSuccess;
   Params p = plan(a.cache, a.heads, a.n, a.prefix, a.max_length);
   p.a = a;
+  p.pairs = (((uintptr_t)a.q | (uintptr_t)a.out) & 3) == 0 && (a.q_stride | a.out_stride) % 2 == 0;
   p.scale_log2 = a.scale * kLog2e;
   const int64_t rows = (p.prefix_splits + p.own_splits) * a.n * a.heads;
   p.ml = static_cast<float2*>(a.workspace);

@@ -23,13 +23,14 @@ constexpr float kLog2e = 1.4426950408889634f;
 struct Params {
   PagedAttentionArgs a;
   int group;            // query heads of a kv head
-  int tile_rows;        // rows of a block
+  int prefix_rows, own_rows;  // rows of a block's tile, by the part
   int prefix_tiles, prefix_splits;
   int own_slots, own_splits;
   int min_slice;        // keys: slices are not made shorter than this
   float* acc;           // [prefix_splits + own_splits][n * heads][hd]
   float2* ml;           // [prefix_splits + own_splits][n * heads]: m, l
   float scale_log2;
+  bool pairs;           // rows of q and out are 4-byte aligned
   bool direct;          // one slice in all: blocks write `out` themselves
 };
 
@@ -70,9 +71,9 @@ __device__ __forceinline__ void sees(const Params& p, int s, int t, int& low, in
 }
 
 // Slots of own work: sequence s has slots first(s) .. first(s + 1) - 1, at
-// least its ceil(rows / tile_rows); first(sequences) = own_slots at most.
+// least its ceil(rows / own_rows); first(sequences) = own_slots at most.
 __device__ __forceinline__ int first_slot(const Params& p, int s) {
-  return (int)((int64_t)seq_start(p, s) * p.group / p.tile_rows) + s;
+  return (int)((int64_t)seq_start(p, s) * p.group / p.own_rows) + s;
 }
 
 __device__ __forceinline__ bool find_work(const Params& p, Work& w) {
@@ -84,8 +85,8 @@ __device__ __forceinline__ bool find_work(const Params& p, Work& w) {
     w.seq = -1;
     w.splits = p.prefix_splits;
     w.slice = b / p.prefix_tiles;
-    w.row0 = b % p.prefix_tiles * p.tile_rows;
-    w.rows = min(p.tile_rows, (int)p.a.n * p.group - w.row0);
+    w.row0 = b % p.prefix_tiles * p.prefix_rows;
+    w.rows = min(p.prefix_rows, (int)p.a.n * p.group - w.row0);
     return w.rows > 0;
   }
   b -= prefix_blocks;
@@ -93,7 +94,7 @@ __device__ __forceinline__ bool find_work(const Params& p, Work& w) {
   w.slice = b / p.own_slots;
   const int slot = b % p.own_slots;
   const int seqs = (int)p.a.cache.sequences;
-  if (p.a.q_start == nullptr && p.group <= p.tile_rows) {
+  if (p.a.q_start == nullptr && p.group <= p.own_rows) {
     w.seq = slot;
     w.row0 = slot * p.group;
     w.rows = p.group;
@@ -108,8 +109,8 @@ __device__ __forceinline__ bool find_work(const Params& p, Work& w) {
   w.seq = lo - 1;
   if (w.seq < 0) return false;
   const int end = seq_start(p, w.seq + 1) * p.group;
-  w.row0 = seq_start(p, w.seq) * p.group + (slot - first_slot(p, w.seq)) * p.tile_rows;
-  w.rows = min(p.tile_rows, end - w.row0);
+  w.row0 = seq_start(p, w.seq) * p.group + (slot - first_slot(p, w.seq)) * p.own_rows;
+  w.rows = min(p.own_rows, end - w.row0);
   return w.rows > 0;
 }
 
@@ -162,6 +163,35 @@ __device__ __forceinline__ int64_t out_index(const Params& p, const Work& w, int
 __device__ __forceinline__ int slice_index(const Params& p, const Work& w) {
   return w.prefix ? w.slice : p.prefix_splits + w.slice;
 }
+
+// Rows of a block: thin tiles for few rows a sequence, wide ones for many.
+constexpr int kThinRows = 16;
+constexpr int kWideRows = 64;
+constexpr int kLanes = 32;
+
+inline dim3 attention_grid(const Params& p) {
+  return dim3((unsigned)(p.prefix_tiles * p.prefix_splits + p.own_slots * p.own_splits),
+              (unsigned)p.a.cache.kv_heads);
+}
+
+template <typename K>
+inline cudaError_t launch_ex(K kern, const Params& p, dim3 grid, int threads, size_t smem, cudaStream_t stream, bool pdl) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = pdl ? 1 : 0;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, p);
+}
+
+// The tensor-core kernel (paged_attention_mma.cu), for the caches that
+// mma_cache (paged_attention.cu) lets through.
+cudaError_t launch_attention_mma(const Params& p, cudaStream_t stream, bool pdl);
 
 }  // namespace paged
 }  // namespace dn
