@@ -736,7 +736,9 @@ int64_t dn_paged_attention(const dn_paged_cache* cache, const void* q, int64_t q
   dn::PagedAttentionArgs a{};
   memcpy(&a.cache, cache, sizeof a.cache);
   if (workspace_bytes < dn::paged_attention_workspace(a.cache, heads, n, prefix, max_length)) return DN_ERR_ARGS;
-  if (device_state() == nullptr) return DN_ERR_NO_DEVICE;
+  DeviceState* d = device_state();
+  if (d == nullptr) return DN_ERR_NO_DEVICE;
+  a.status = d->status_dev;
   a.q = q;
   a.q_stride = q_stride;
   a.q_start = q_start;

@@ -240,6 +240,7 @@ struct PagedAttentionArgs {
   int64_t q_stride, out_stride, prefix, max_length, window, heads, n;
   float scale;
   void* workspace;
+  uint32_t* status;
 };
 int64_t paged_attention_workspace(const PagedCache& c, int64_t heads, int64_t n, int64_t prefix,
                                   int64_t max_length);

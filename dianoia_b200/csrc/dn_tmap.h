@@ -34,4 +34,13 @@ bool encode_tmap_2d_sw64(CUtensorMap* map, const void* base, CUtensorMapDataType
 bool encode_tmap_row_chunks(CUtensorMap* map, const void* base, uint64_t rows, uint64_t row_bytes,
                             uint32_t box_rows, uint32_t chunks);
 
+// A 4-D map over pages of 16-bit elements, [pages][heads][slots][hd] with
+// page_stride elements between pages: boxes of box_slots rows of 64 elements
+// of one head of one page, 128-byte swizzled; columns past hd and pages past
+// the last read as zeros. Coordinates (element, slot, head, page). Returns
+// false if the driver refuses the map (hd and page_stride must be multiples
+// of 8 and the base 16-byte aligned).
+bool encode_tmap_pages(CUtensorMap* map, const void* base, bool bf16, uint64_t hd, uint64_t slots, uint64_t heads,
+                       uint64_t pages, uint64_t page_stride, uint32_t box_slots);
+
 }  // namespace dn

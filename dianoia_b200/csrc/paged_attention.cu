@@ -18,7 +18,6 @@ namespace {
 // FMAs along the head), the tile's maximum and sum are warp reductions, and
 // for the values lane j owns dimensions 4 j .. 4 j + 3 (and 128 more on).
 constexpr int kSimtThreads = 128;
-constexpr int kSimtRows = 16;
 constexpr int kSimtKeys = 32;
 constexpr int kWarpRows = 4;
 
@@ -45,7 +44,7 @@ __global__ void __launch_bounds__(kSimtThreads) attention_simt_kernel(const __gr
     int low = 0, high = -1;
     if (tid < w.rows) {
       const int t = (w.row0 + tid) / p.group;
-      sees(p, w.prefix ? seq_of(p, t) : w.seq, t, low, high);
+      sees(p, w.prefix, w.prefix ? seq_of(p, t) : w.seq, t, low, high);
     }
     row_low[tid] = low;
     row_high[tid] = high;
@@ -248,12 +247,17 @@ bool mma_cache(const PagedCache& c) {
 
 // How the work is divided, from sizes that the host knows.
 Params plan(const PagedCache& c, int64_t heads, int64_t n, int64_t prefix, int64_t max_length) {
-  const bool mma = mma_cache(c);
   Params p{};
   p.group = (int)(heads / c.kv_heads);
   const int64_t rows = n * p.group;
-  p.prefix_rows = mma && rows > 2 * kThinRows ? kWideRows : kThinRows;
-  p.own_rows = mma && rows > 2 * kThinRows * c.sequences ? kWideRows : kThinRows;
+  if (mma_cache(c)) {
+    // 8 rows to a block where a sequence's rows, and the whole batch's on the
+    // prefix, are that few; else 16.
+    const bool few = rows <= 8 * (c.sequences > 1 ? c.sequences : 1) && (prefix == 0 || rows <= 8);
+    p.own_rows = p.prefix_rows = few ? 8 : 16;
+  } else {
+    p.own_rows = p.prefix_rows = kSimtRows;
+  }
   p.min_slice = 128;
   const int64_t tiles = (rows + p.prefix_rows - 1) / p.prefix_rows;
   p.prefix_tiles = prefix > 0 ? (int)tiles : 0;
@@ -279,7 +283,7 @@ cudaError_t launch_simt(const Params& p, cudaStream_t stream, bool pdl) {
                                            (int)smem);
       e != cudaSuccess)
     return e;
-  return launch_ex(attention_simt_kernel<T, V>, p, attention_grid(p), kSimtThreads, smem, stream, pdl);
+  return launch_ex(attention_simt_kernel<T, V>, attention_grid(p), kSimtThreads, smem, stream, pdl, p);
 }
 
 template <typename T>
@@ -287,13 +291,13 @@ cudaError_t launch_type(const Params& p, cudaStream_t stream, bool pdl) {
   constexpr int V = 16 / sizeof(T);
   const PagedCache& c = p.a.cache;
   const bool runs = (((uintptr_t)c.keys | (uintptr_t)c.values) & 15) == 0 && (c.page_stride | c.hd) % V == 0;
-  cudaError_t e = mma_cache(c) ? launch_attention_mma(p, stream, pdl)
+  cudaError_t e = mma_cache(c) ? launch_attention_thin(p, stream, pdl)
                   : runs       ? launch_simt<T, V>(p, stream, pdl)
                                : launch_simt<T, 1>(p, stream, pdl);
   if (e != cudaSuccess || p.direct) return e;
   const int64_t warps = p.a.n * p.a.heads, per = kJoinThreads / kLanes;
-  return launch_ex(attention_join_kernel<T>, p, dim3((unsigned)((warps + per - 1) / per)), kJoinThreads, 0, stream,
-                   true);
+  return launch_ex(attention_join_kernel<T>, dim3((unsigned)((warps + per - 1) / per)), kJoinThreads, 0, stream, true,
+                   p);
 }
 
 }  // namespace
@@ -308,6 +312,10 @@ cudaError_t launch_paged_attention(const PagedAttentionArgs& a, cudaStream_t str
   if (a.n <= 0) return cudaSuccess;
   Params p = plan(a.cache, a.heads, a.n, a.prefix, a.max_length);
   p.a = a;
+  p.status = a.status;
+  p.page_shift = -1;
+  for (int s = 0; s <= 20; s++)
+    if (a.cache.page_size == (int64_t)1 << s) p.page_shift = s;
   p.pairs = (((uintptr_t)a.q | (uintptr_t)a.out) & 3) == 0 && (a.q_stride | a.out_stride) % 2 == 0;
   p.scale_log2 = a.scale * kLog2e;
   const int64_t rows = (p.prefix_splits + p.own_splits) * a.n * a.heads;

@@ -30,6 +30,8 @@ struct Params {
   float* acc;           // [prefix_splits + own_splits][n * heads][hd]
   float2* ml;           // [prefix_splits + own_splits][n * heads]: m, l
   float scale_log2;
+  int page_shift;       // log2 of the page size, or -1
+  uint32_t* status;     // bounded waits' status word
   bool pairs;           // rows of q and out are 4-byte aligned
   bool direct;          // one slice in all: blocks write `out` themselves
 };
@@ -61,13 +63,20 @@ __device__ __forceinline__ int seq_of(const Params& p, int t) {
   return s >= 0 && t < seq_start(p, s + 1) ? s : -1;
 }
 
-// Positions low .. high that token t of sequence s sees (high < low: none).
-__device__ __forceinline__ void sees(const Params& p, int s, int t, int& low, int& high) {
+// Positions low .. high of the prefix, or of sequence s's own part, that its
+// token t sees (high < low: none).
+__device__ __forceinline__ void sees(const Params& p, bool in_prefix, int s, int t, int& low, int& high) {
   low = 0;
   high = -1;
   if (s < 0) return;
   high = p.a.lengths[s] - (seq_start(p, s + 1) - t);
   if (p.a.window > 0) low = max(0, high - (int)p.a.window + 1);
+  if (in_prefix) {
+    high = min(high, (int)p.a.prefix - 1);
+  } else {
+    low = max(low, (int)p.a.prefix);
+    high = min(high, (int)(p.a.cache.table_stride * p.a.cache.page_size) - 1);
+  }
 }
 
 // Slots of own work: sequence s has slots first(s) .. first(s + 1) - 1, at
@@ -114,9 +123,15 @@ __device__ __forceinline__ bool find_work(const Params& p, Work& w) {
   return w.rows > 0;
 }
 
+// A position's entry of the page list (a shift for the usual page sizes: a
+// division by a variable takes some twenty instructions).
+__device__ __forceinline__ int entry_of(const Params& p, int pos) {
+  return p.page_shift >= 0 ? pos >> p.page_shift : pos / (int)p.a.cache.page_size;
+}
+
 // The page of a position of the part, or -1 where there is none.
 __device__ __forceinline__ int page_of(const Params& p, const Work& w, int pos) {
-  const int entry = pos / (int)p.a.cache.page_size;
+  const int entry = entry_of(p, pos);
   int page;
   if (w.prefix) {
     page = p.a.prefix_pages[entry];
@@ -131,25 +146,25 @@ __device__ __forceinline__ int page_of(const Params& p, const Work& w, int pos) 
 // tile's rows see between them; slices start at multiples of `tile`.
 __device__ __forceinline__ void slice_keys(const Params& p, const Work& w, int low, int high, int tile, int& begin,
                                            int& end) {
-  const int prefix = (int)p.a.prefix;
-  int lo = w.prefix ? low : max(low, prefix);
-  int hi = w.prefix ? min(high, prefix - 1) : high;
-  if (!w.prefix) {
-    const int last = (int)(p.a.cache.table_stride * p.a.cache.page_size) - 1;
-    hi = min(hi, last);
-  }
-  lo = lo / tile * tile;
-  if (!w.prefix) lo = max(lo, prefix);
-  const int keys = hi - lo + 1;
-  if (keys <= 0) {
-    begin = end = 0;
-    return;
-  }
+  begin = end = 0;
+  if (high < low) return;
+  const int lo = low / tile * tile, keys = high - lo + 1;
   int per = max((keys + w.splits - 1) / w.splits, p.min_slice);
   per = (per + tile - 1) / tile * tile;
   const int64_t b = lo + (int64_t)w.slice * per;
-  begin = (int)min((int64_t)hi + 1, b);
-  end = (int)min((int64_t)hi + 1, b + per);
+  begin = (int)min((int64_t)high + 1, b);
+  end = (int)min((int64_t)high + 1, b + per);
+}
+
+// Element offset, in the pools, of the row of position pos (low <= pos < end)
+// of the block's kv head, or -1.
+__device__ __forceinline__ int64_t row_at(const Params& p, const Work& w, int pos, int low, int end) {
+  if (pos < low || pos >= end) return -1;
+  const int page = page_of(p, w, pos);
+  if (page < 0) return -1;
+  const int size = (int)p.a.cache.page_size;
+  const int slot = p.page_shift >= 0 ? pos & (size - 1) : pos % size;
+  return page * p.a.cache.page_stride + ((int64_t)w.head * size + slot) * p.a.cache.hd;
 }
 
 // Index of a row of the tile in the workspace: token * heads + head.
@@ -164,9 +179,9 @@ __device__ __forceinline__ int slice_index(const Params& p, const Work& w) {
   return w.prefix ? w.slice : p.prefix_splits + w.slice;
 }
 
-// Rows of a block: thin tiles for few rows a sequence, wide ones for many.
-constexpr int kThinRows = 16;
-constexpr int kWideRows = 64;
+// Rows of a block by kernel: the f32 one and the thin one (8 or 16), the wide one.
+constexpr int kSimtRows = 16;
+constexpr int kWideRows = 128;
 constexpr int kLanes = 32;
 
 inline dim3 attention_grid(const Params& p) {
@@ -174,8 +189,9 @@ inline dim3 attention_grid(const Params& p) {
               (unsigned)p.a.cache.kv_heads);
 }
 
-template <typename K>
-inline cudaError_t launch_ex(K kern, const Params& p, dim3 grid, int threads, size_t smem, cudaStream_t stream, bool pdl) {
+template <typename K, typename... Args>
+inline cudaError_t launch_ex(K kern, dim3 grid, int threads, size_t smem, cudaStream_t stream, bool pdl,
+                             const Args&... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = dim3((unsigned)threads);
@@ -186,12 +202,12 @@ inline cudaError_t launch_ex(K kern, const Params& p, dim3 grid, int threads, si
   attr[0].val.programmaticStreamSerializationAllowed = pdl ? 1 : 0;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kern, p);
+  return cudaLaunchKernelEx(&cfg, kern, args...);
 }
 
-// The tensor-core kernel (paged_attention_mma.cu), for the caches that
-// mma_cache (paged_attention.cu) lets through.
-cudaError_t launch_attention_mma(const Params& p, cudaStream_t stream, bool pdl);
+// The tensor-core kernels for the caches that mma_cache (paged_attention.cu)
+// lets through: few rows of a tile (paged_attention_thin.cu), many.
+cudaError_t launch_attention_thin(const Params& p, cudaStream_t stream, bool pdl);
 
 }  // namespace paged
 }  // namespace dn

@@ -58,6 +58,20 @@ bool encode_tmap_row_chunks(CUtensorMap* map, const void* base, uint64_t rows, u
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+bool encode_tmap_pages(CUtensorMap* map, const void* base, bool bf16, uint64_t hd, uint64_t slots, uint64_t heads,
+                       uint64_t pages, uint64_t page_stride, uint32_t box_slots) {
+  auto fn = encode_fn();
+  if (fn == nullptr) return false;
+  const cuuint64_t dims[4] = {hd, slots, heads, pages};
+  const cuuint64_t strides[3] = {hd * 2, slots * hd * 2, page_stride * 2};
+  const cuuint32_t box[4] = {64, box_slots, 1, 1};
+  const cuuint32_t estrides[4] = {1, 1, 1, 1};
+  return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+            const_cast<void*>(base), dims, strides, box, estrides, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 bool encode_tmap_2d_sw64(CUtensorMap* map, const void* base, CUtensorMapDataType type,
                          uint64_t row_elems, uint64_t rows, uint64_t row_bytes, uint32_t box_elems,
                          uint32_t box_rows) {
