@@ -44,7 +44,7 @@ __global__ void __launch_bounds__(kSimtThreads) attention_simt_kernel(const __gr
     int low = 0, high = -1;
     if (tid < w.rows) {
       const int t = (w.row0 + tid) / p.group;
-      sees(p, w.prefix, w.prefix ? seq_of(p, t) : w.seq, t, low, high);
+      sees(p, w, t, low, high);
     }
     row_low[tid] = low;
     row_high[tid] = high;
@@ -135,8 +135,8 @@ __global__ void __launch_bounds__(kSimtThreads) attention_simt_kernel(const __gr
       for (int off = 16; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
       const float next = fmaxf(m[r], top);
       const float base = next == -INFINITY ? 0.0f : next;
-      const float keep = exp2f(m[r] - base);
-      pr[r] = seen ? exp2f(x - base) : 0.0f;
+      const float keep = exp2_fast(m[r] - base);
+      pr[r] = seen ? exp2_fast(x - base) : 0.0f;
       m[r] = next;
       l[r] = l[r] * keep + pr[r];  // a lane's share; summed over the lanes at the end
 #pragma unroll
@@ -224,7 +224,7 @@ __global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(const __gr
   for (int i = 0; i < slices; i++) {
     const float2 ml = p.ml[i * rows + row];
     if (ml.y == 0.0f) continue;
-    const float f = exp2f(ml.x - base);
+    const float f = exp2_fast(ml.x - base);
     l += ml.y * f;
     const float* a = p.acc + (i * rows + row) * hd;
 #pragma unroll
@@ -258,6 +258,7 @@ Params plan(const PagedCache& c, int64_t heads, int64_t n, int64_t prefix, int64
   } else {
     p.own_rows = p.prefix_rows = kSimtRows;
   }
+  p.own_rows_log2 = 31 - __builtin_clz((unsigned)p.own_rows);
   p.min_slice = 128;
   const int64_t tiles = (rows + p.prefix_rows - 1) / p.prefix_rows;
   p.prefix_tiles = prefix > 0 ? (int)tiles : 0;

@@ -23,7 +23,8 @@ constexpr float kLog2e = 1.4426950408889634f;
 struct Params {
   PagedAttentionArgs a;
   int group;            // query heads of a kv head
-  int prefix_rows, own_rows;  // rows of a block's tile, by the part
+  int prefix_rows, own_rows;  // rows of a block's tile, by the part (a power of two)
+  int own_rows_log2;
   int prefix_tiles, prefix_splits;
   int own_slots, own_splits;
   int min_slice;        // keys: slices are not made shorter than this
@@ -40,8 +41,15 @@ struct Params {
 // `slice` of the part's keys, whose pages are `pages`.
 struct Work {
   bool prefix;
-  int head, row0, rows, slice, splits, seq;
+  int head, row0, rows, slice, splits;
+  int seq, seq_end, length;  // own work: the sequence, its last token + 1, its length
 };
+
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 
 __device__ __forceinline__ int seq_start(const Params& p, int s) {
   if (p.a.q_start == nullptr) return s;
@@ -49,10 +57,12 @@ __device__ __forceinline__ int seq_start(const Params& p, int s) {
   return v < 0 ? 0 : v > (int)p.a.n ? (int)p.a.n : v;
 }
 
-// The sequence that token t belongs to, or -1.
+// The sequence that token t belongs to, or -1. A batch of one token a
+// sequence is recognized in one round of loads.
 __device__ __forceinline__ int seq_of(const Params& p, int t) {
   const int seqs = (int)p.a.cache.sequences;
   if (p.a.q_start == nullptr) return t < seqs ? t : -1;
+  if (t < seqs && seq_start(p, t) == t && seq_start(p, t + 1) == t + 1) return t;
   int lo = 0, hi = seqs;  // the last s with seq_start(s) <= t
   while (lo < hi) {
     const int mid = (lo + hi) / 2;
@@ -63,15 +73,20 @@ __device__ __forceinline__ int seq_of(const Params& p, int t) {
   return s >= 0 && t < seq_start(p, s + 1) ? s : -1;
 }
 
-// Positions low .. high of the prefix, or of sequence s's own part, that its
+// Positions low .. high of the prefix, or of the sequence's own part, that
 // token t sees (high < low: none).
-__device__ __forceinline__ void sees(const Params& p, bool in_prefix, int s, int t, int& low, int& high) {
+__device__ __forceinline__ void sees(const Params& p, const Work& w, int t, int& low, int& high) {
   low = 0;
   high = -1;
-  if (s < 0) return;
-  high = p.a.lengths[s] - (seq_start(p, s + 1) - t);
+  if (w.prefix) {
+    const int s = seq_of(p, t);
+    if (s < 0) return;
+    high = p.a.lengths[s] - (seq_start(p, s + 1) - t);
+  } else {
+    high = w.length - (w.seq_end - t);
+  }
   if (p.a.window > 0) low = max(0, high - (int)p.a.window + 1);
-  if (in_prefix) {
+  if (w.prefix) {
     high = min(high, (int)p.a.prefix - 1);
   } else {
     low = max(low, (int)p.a.prefix);
@@ -81,10 +96,11 @@ __device__ __forceinline__ void sees(const Params& p, bool in_prefix, int s, int
 
 // Slots of own work: sequence s has slots first(s) .. first(s + 1) - 1, at
 // least its ceil(rows / own_rows); first(sequences) = own_slots at most.
-__device__ __forceinline__ int first_slot(const Params& p, int s) {
-  return (int)((int64_t)seq_start(p, s) * p.group / p.own_rows) + s;
+__device__ __forceinline__ int first_slot(const Params& p, int start, int s) {
+  return ((start * p.group) >> p.own_rows_log2) + s;
 }
 
+// Called by every thread of a block of whole warps.
 __device__ __forceinline__ bool find_work(const Params& p, Work& w) {
   int b = blockIdx.x;
   w.head = blockIdx.y;
@@ -104,23 +120,40 @@ __device__ __forceinline__ bool find_work(const Params& p, Work& w) {
   const int slot = b % p.own_slots;
   const int seqs = (int)p.a.cache.sequences;
   if (p.a.q_start == nullptr && p.group <= p.own_rows) {
+    if (slot >= seqs) return false;
     w.seq = slot;
     w.row0 = slot * p.group;
     w.rows = p.group;
-    return slot < seqs;
+    w.seq_end = slot + 1;
+    w.length = p.a.lengths[slot];
+    return true;
   }
-  int lo = 0, hi = seqs;  // the last s with first_slot(s) <= slot
-  while (lo < hi) {
-    const int mid = (lo + hi) / 2;
-    if (first_slot(p, mid) <= slot) lo = mid + 1;
-    else hi = mid;
+  if (seqs == 0) return false;
+  // The last s < seqs with first_slot(s) <= slot: by 32-fold sections, the
+  // first of them around where one token a sequence would put it.
+  const int lane = threadIdx.x % 32;
+  int lo = 0, hi = seqs;  // the answer lies in lo .. hi - 1
+  const int guess = (int)((int64_t)slot * p.own_rows / (p.own_rows + p.group)) - 16;
+  int at = max(0, min(guess, seqs - 32)), step = 1;
+  for (;;) {
+    const int s = at + lane * step;
+    const bool under = s < hi && first_slot(p, seq_start(p, s), s) <= slot;
+    const unsigned votes = __ballot_sync(0xffffffffu, under);
+    const int count = __popc(votes);  // monotone: lanes 0 .. count - 1
+    if (count > 0) lo = max(lo, at + (count - 1) * step);
+    if (count < 32) hi = min(hi, at + count * step);
+    if (hi - lo <= 1) break;
+    step = max(1, (hi - lo + 31) / 32);
+    at = lo;
   }
-  w.seq = lo - 1;
-  if (w.seq < 0) return false;
-  const int end = seq_start(p, w.seq + 1) * p.group;
-  w.row0 = seq_start(p, w.seq) * p.group + (slot - first_slot(p, w.seq)) * p.own_rows;
-  w.rows = min(p.own_rows, end - w.row0);
-  return w.rows > 0;
+  w.seq = lo;
+  const int start = seq_start(p, lo);
+  w.seq_end = seq_start(p, lo + 1);
+  w.length = p.a.lengths[lo];
+  const int tile = slot - first_slot(p, start, lo);
+  w.row0 = start * p.group + tile * p.own_rows;
+  w.rows = min(p.own_rows, w.seq_end * p.group - w.row0);
+  return tile >= 0 && w.rows > 0;
 }
 
 // A position's entry of the page list (a shift for the usual page sizes: a

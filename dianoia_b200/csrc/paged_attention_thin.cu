@@ -109,7 +109,7 @@ __device__ __forceinline__ void thin_block(const Params& p, const Maps& maps, co
   int lo = 0, hi = -1;
   if (lane < w.rows) {
     const int t = (w.row0 + lane) / p.group;
-    sees(p, w.prefix, w.prefix ? seq_of(p, t) : w.seq, t, lo, hi);
+    sees(p, w, t, lo, hi);
   }
   const bool mine = lane < w.rows, any = hi >= lo;
   const int all_low = __reduce_max_sync(0xffffffffu, mine ? any ? lo : INT32_MAX : 0);
@@ -258,7 +258,7 @@ __device__ __forceinline__ void thin_block(const Params& p, const Maps& maps, co
 #pragma unroll
             for (int off = 4; off <= 16; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
             const float next = fmaxf(m[n][h], top);
-            const float keep = next == -INFINITY ? 1.0f : exp2f(m[n][h] - next);
+            const float keep = next == -INFINITY ? 1.0f : exp2_fast(m[n][h] - next);
             m[n][h] = next;
             l[n][h] *= keep;
 #pragma unroll
@@ -274,7 +274,7 @@ __device__ __forceinline__ void thin_block(const Params& p, const Maps& maps, co
 #pragma unroll
         for (int e = 0; e < 4; e++) {
           const float base_m = m[n][e & 1] == -INFINITY ? 0.0f : m[n][e & 1];
-          s[n][e] = exp2f(s[n][e] - base_m);
+          s[n][e] = exp2_fast(s[n][e] - base_m);
           l[n][e & 1] += s[n][e];  // a lane's share of the row's sum
         }
         pf[n][0] = transposed(Pair<T>::pack(s[n][0], s[n][1]));
@@ -354,7 +354,7 @@ __device__ __forceinline__ void thin_block(const Params& p, const Maps& maps, co
     for (int k = 0; k < kWarps; k++) {
       const float2 part = ml[k * kRows + r];
       if (part.y == 0.0f) continue;  // (a NaN goes on)
-      const float f = exp2f(part.x - base);
+      const float f = exp2_fast(part.x - base);
       const float2 v = *reinterpret_cast<const float2*>(os + (k * kRows + r) * kOut + d);
       sum += part.y * f;
       x += v.x * f;
