@@ -249,31 +249,51 @@ bool mma_cache(const PagedCache& c) {
 Params plan(const PagedCache& c, int64_t heads, int64_t n, int64_t prefix, int64_t max_length) {
   Params p{};
   p.group = (int)(heads / c.kv_heads);
-  const int64_t rows = n * p.group;
-  if (mma_cache(c)) {
-    // 8 rows to a block where a sequence's rows, and the whole batch's on the
-    // prefix, are that few; else 16.
-    const bool few = rows <= 8 * (c.sequences > 1 ? c.sequences : 1) && (prefix == 0 || rows <= 8);
-    p.own_rows = p.prefix_rows = few ? 8 : 16;
-  } else {
-    p.own_rows = p.prefix_rows = kSimtRows;
-  }
+  const int64_t rows = n * p.group, seqs = c.sequences > 1 ? c.sequences : 1;
+  const bool wide = mma_cache(c) && c.page_size % 16 == 0 && c.pages > 0;
+  p.prefix_wide = wide && prefix > 0 && rows > kWideFrom;
+  p.own_wide = wide && rows > kWideFrom * seqs;
+  // 8 rows to a thin block where a sequence's rows, and the whole batch's on
+  // the prefix, are that few; else 16.
+  const bool few = rows <= 8 * seqs && (prefix == 0 || p.prefix_wide || rows <= 8);
+  p.thin_rows = mma_cache(c) ? few ? 8 : 16 : kSimtRows;
+  p.prefix_rows = p.prefix_wide ? kWideRows : p.thin_rows;
+  p.own_rows = p.own_wide ? kWideRows : p.thin_rows;
   p.own_rows_log2 = 31 - __builtin_clz((unsigned)p.own_rows);
   p.min_slice = 128;
   const int64_t tiles = (rows + p.prefix_rows - 1) / p.prefix_rows;
   p.prefix_tiles = prefix > 0 ? (int)tiles : 0;
   p.own_slots = (int)(rows / p.own_rows + c.sequences);
-  // Enough blocks to give every SM two, as long as a slice has min_slice keys.
-  auto splits = [&](int64_t blocks, int64_t keys) {
-    const int64_t want = (2 * 148 + blocks - 1) / (blocks > 0 ? blocks : 1);
-    const int64_t most = (keys + p.min_slice - 1) / p.min_slice;
-    return (int)(want < most ? want : most > 1 ? most : 1);
+  // A part's keys are split as long as blocks are wanting and a slice keeps
+  // min_slice keys: two thin blocks to an SM, one wide.
+  auto splits = [&](int64_t blocks, int64_t keys, bool on_wide) {
+    const int64_t want = on_wide ? 148 / (blocks > 0 ? blocks : 1) : (2 * 148 + blocks - 1) / (blocks > 0 ? blocks : 1);
+    const int64_t most = (keys + p.min_slice - 1) / p.min_slice, least = want < most ? want : most;
+    return (int)(least > 1 ? least : 1);
   };
-  p.prefix_splits = prefix > 0 ? splits(tiles * c.kv_heads, prefix) : 0;
+  p.prefix_splits = prefix > 0 ? splits(tiles * c.kv_heads, prefix, p.prefix_wide) : 0;
   const int64_t own = max_length > prefix ? max_length - prefix : 1;
-  p.own_splits = splits((int64_t)p.own_slots * c.kv_heads, own);
+  p.own_splits = splits((int64_t)p.own_slots * c.kv_heads, own, p.own_wide);
   p.direct = p.prefix_splits + p.own_splits == 1;
   return p;
+}
+
+// The tensor-core kernels on the parts that are theirs; the thin one runs
+// beside the wide one, whose blocks leave it half of each SM.
+cudaError_t launch_mma(const Params& p, cudaStream_t stream, bool pdl) {
+  const bool wide = p.prefix_wide || p.own_wide;
+  if (wide) {
+    Params part = p;
+    if (!p.prefix_wide) part.prefix_tiles = 0;
+    if (!p.own_wide) part.own_slots = 0;
+    if (cudaError_t e = launch_attention_wide(part, stream, pdl); e != cudaSuccess) return e;
+  }
+  Params part = p;
+  part.beside = wide;
+  if (p.prefix_wide) part.prefix_tiles = 0;
+  if (p.own_wide) part.own_slots = 0;
+  if (part.prefix_tiles == 0 && part.own_slots == 0) return cudaSuccess;
+  return launch_attention_thin(part, stream, pdl || wide);
 }
 
 template <typename T, int V>
@@ -292,7 +312,7 @@ cudaError_t launch_type(const Params& p, cudaStream_t stream, bool pdl) {
   constexpr int V = 16 / sizeof(T);
   const PagedCache& c = p.a.cache;
   const bool runs = (((uintptr_t)c.keys | (uintptr_t)c.values) & 15) == 0 && (c.page_stride | c.hd) % V == 0;
-  cudaError_t e = mma_cache(c) ? launch_attention_thin(p, stream, pdl)
+  cudaError_t e = mma_cache(c) ? launch_mma(p, stream, pdl)
                   : runs       ? launch_simt<T, V>(p, stream, pdl)
                                : launch_simt<T, 1>(p, stream, pdl);
   if (e != cudaSuccess || p.direct) return e;

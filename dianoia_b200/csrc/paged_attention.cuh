@@ -25,6 +25,9 @@ struct Params {
   int group;            // query heads of a kv head
   int prefix_rows, own_rows;  // rows of a block's tile, by the part (a power of two)
   int own_rows_log2;
+  int thin_rows;        // of the thin kernel's tiles: 8 or 16
+  bool prefix_wide, own_wide;  // which parts the wide kernel takes
+  bool beside;          // this launch runs beside the one before it
   int prefix_tiles, prefix_splits;
   int own_slots, own_splits;
   int min_slice;        // keys: slices are not made shorter than this
@@ -167,6 +170,7 @@ __device__ __forceinline__ int page_of(const Params& p, const Work& w, int pos) 
   const int entry = entry_of(p, pos);
   int page;
   if (w.prefix) {
+    if (pos >= (int)p.a.prefix) return -1;
     page = p.a.prefix_pages[entry];
   } else {
     if (entry >= (int)p.a.cache.table_stride) return -1;
@@ -215,6 +219,7 @@ __device__ __forceinline__ int slice_index(const Params& p, const Work& w) {
 // Rows of a block by kernel: the f32 one and the thin one (8 or 16), the wide one.
 constexpr int kSimtRows = 16;
 constexpr int kWideRows = 128;
+constexpr int kWideFrom = 32;  // rows (of the batch, of a sequence on average) from which the wide one runs
 constexpr int kLanes = 32;
 
 inline dim3 attention_grid(const Params& p) {
@@ -239,8 +244,10 @@ inline cudaError_t launch_ex(K kern, dim3 grid, int threads, size_t smem, cudaSt
 }
 
 // The tensor-core kernels for the caches that mma_cache (paged_attention.cu)
-// lets through: few rows of a tile (paged_attention_thin.cu), many.
+// lets through: few rows of a tile (paged_attention_thin.cu), many
+// (paged_attention_wide.cu).
 cudaError_t launch_attention_thin(const Params& p, cudaStream_t stream, bool pdl);
+cudaError_t launch_attention_wide(const Params& p, cudaStream_t stream, bool pdl);
 
 }  // namespace paged
 }  // namespace dn

@@ -378,12 +378,14 @@ template <typename T, int HDP, int NT, bool TMA>
 __global__ void __launch_bounds__(kThreads)
     attention_thin_kernel(const __grid_constant__ Params p, const __grid_constant__ Maps maps) {
   pdl_launch_dependents();
-  pdl_wait();
+  // Beside the wide kernel, whose start already followed the inputs, there is
+  // nothing to wait for but its end, before this grid's: one block does.
+  if (!p.beside) pdl_wait();
   extern __shared__ __align__(1024) char smem[];
   __shared__ uint64_t bars[kWarps * Shape<HDP>::kStages];
   Work w;
-  if (!find_work(p, w)) return;
-  thin_block<T, HDP, NT, TMA>(p, maps, w, smem, bars);
+  if (find_work(p, w)) thin_block<T, HDP, NT, TMA>(p, maps, w, smem, bars);
+  if (p.beside && blockIdx.x == 0 && blockIdx.y == 0) pdl_wait();
 }
 
 template <typename T, int HDP, int NT, bool TMA>
@@ -408,7 +410,7 @@ cudaError_t launch_rows(const Params& p, cudaStream_t stream, bool pdl) {
                encode_tmap_pages(&maps.values, c.values, c.type == kBF16, c.hd, c.page_size, c.kv_heads, c.pages,
                                  c.page_stride, kStep)))
     return cudaErrorInvalidValue;
-  if (p.own_rows == 8)
+  if (p.thin_rows == 8)
     return tma ? launch_copies<T, HDP, 1, true>(p, maps, stream, pdl) : launch_copies<T, HDP, 1, false>(p, maps, stream, pdl);
   return tma ? launch_copies<T, HDP, 2, true>(p, maps, stream, pdl) : launch_copies<T, HDP, 2, false>(p, maps, stream, pdl);
 }
