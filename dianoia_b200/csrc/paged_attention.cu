@@ -143,7 +143,7 @@ __global__ void __launch_bounds__(kSimtThreads) attention_simt_kernel(const __gr
       for (int u = 0; u < 2; u++)
 #pragma unroll
         for (int e = 0; e < 4; e++) acc[r][u][e] *= keep;
-      all = all && seen;
+      all = all && (seen || high[r] < low[r]);  // (a row that sees nothing has only zeros to add)
     }
     float4* pw = reinterpret_cast<float4*>(ps) + warp * kSimtKeys;
     pw[lane] = make_float4(pr[0], pr[1], pr[2], pr[3]);

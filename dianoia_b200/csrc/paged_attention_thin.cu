@@ -111,9 +111,10 @@ __device__ __forceinline__ void thin_block(const Params& p, const Maps& maps, co
     const int t = (w.row0 + lane) / p.group;
     sees(p, w, t, lo, hi);
   }
-  const bool mine = lane < w.rows, any = hi >= lo;
-  const int all_low = __reduce_max_sync(0xffffffffu, mine ? any ? lo : INT32_MAX : 0);
-  const int all_high = __reduce_min_sync(0xffffffffu, mine ? hi : INT32_MAX);
+  // (Rows that see nothing take part unmasked; their results are dropped.)
+  const bool any = hi >= lo;
+  const int all_low = __reduce_max_sync(0xffffffffu, any ? lo : 0);
+  const int all_high = __reduce_min_sync(0xffffffffu, any ? hi : INT32_MAX);
   const int any_low = __reduce_min_sync(0xffffffffu, any ? lo : INT32_MAX);
   const int any_high = __reduce_max_sync(0xffffffffu, any ? hi : -1);
   int begin, end;
@@ -322,6 +323,15 @@ __device__ __forceinline__ void thin_block(const Params& p, const Maps& maps, co
     for (int h = 0; h < 2; h++)
 #pragma unroll
       for (int off = 4; off <= 16; off <<= 1) l[n][h] += __shfl_xor_sync(0xffffffffu, l[n][h], off);
+
+#pragma unroll
+  for (int n = 0; n < NT; n++)
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+      if (high[n][h] < low[n][h]) {
+        m[n][h] = -INFINITY;
+        l[n][h] = 0.0f;
+      }
 
   // The four warps' parts, through shared memory.
   __syncthreads();

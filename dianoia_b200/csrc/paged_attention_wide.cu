@@ -264,6 +264,10 @@ __device__ __forceinline__ void softmax_rows(const Params& p, const Work& w, cha
   const bool there = r < w.rows;
   const int64_t row = there ? out_index(p, w, r, t, head) : 0;
   const int64_t to = slice_index(p, w) * (p.a.n * p.a.heads) + row;
+  if (high < low) {  // a row that sees nothing took part unmasked
+    m = -INFINITY;
+    l = 0.0f;
+  }
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   if (there && !p.direct) p.ml[to] = make_float2(m, l);
   if (tiles == 0 && !p.direct) return;  // the join reads no values of a row with l = 0
@@ -332,8 +336,8 @@ __global__ void __launch_bounds__(kThreads)
     const bool mine = tid < w.rows;
     if (mine) sees(p, w, (w.row0 + tid) / p.group, low, high);
     const bool any = high >= low;
-    const int all_lo = __reduce_max_sync(0xffffffffu, mine ? any ? low : INT32_MAX : 0);
-    const int all_hi = __reduce_min_sync(0xffffffffu, mine ? high : INT32_MAX);
+    const int all_lo = __reduce_max_sync(0xffffffffu, any ? low : 0);
+    const int all_hi = __reduce_min_sync(0xffffffffu, any ? high : INT32_MAX);
     const int any_lo = __reduce_min_sync(0xffffffffu, any ? low : INT32_MAX);
     const int any_hi = __reduce_max_sync(0xffffffffu, any ? high : -1);
     if (lane == 0) {
