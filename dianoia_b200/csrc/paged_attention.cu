@@ -205,36 +205,64 @@ __global__ void __launch_bounds__(kSimtThreads) attention_simt_kernel(const __gr
 
 constexpr int kJoinThreads = 128;
 
-// One warp for each (token, head).
-template <typename T>
+// One warp for each (token, head): its lanes take a slice's maximum and sum
+// each, then four (V) or one dimension each of every slice's values.
+template <typename T, int V>
 __global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(const __grid_constant__ Params p) {
   pdl_launch_dependents();
   pdl_wait();
   const int64_t rows = p.a.n * p.a.heads;
   const int64_t row = (int64_t)blockIdx.x * (kJoinThreads / kLanes) + threadIdx.x / kLanes;
   if (row >= rows) return;
+  constexpr int kRuns = kMaxPagedHd / (kLanes * V);
   const int lane = threadIdx.x % kLanes, hd = (int)p.a.cache.hd;
-  const int t = (int)(row / p.a.heads), head = (int)(row % p.a.heads);
+  const int t = (int)((uint32_t)row / (uint32_t)p.a.heads), head = (int)((uint32_t)row % (uint32_t)p.a.heads);
   if (p.a.q_start != nullptr && seq_of(p, t) < 0) return;
-  const int slices = p.prefix_splits + p.own_splits;
+  const int slices = p.slices;
   float m = -INFINITY;
-  for (int i = 0; i < slices; i++) m = fmaxf(m, p.ml[i * rows + row].x);
-  const float base = m == -INFINITY ? 0.0f : m;
-  float l = 0.0f, acc[kMaxPagedHd / kLanes] = {};
-  for (int i = 0; i < slices; i++) {
-    const float2 ml = p.ml[i * rows + row];
-    if (ml.y == 0.0f) continue;
-    const float f = exp2_fast(ml.x - base);
-    l += ml.y * f;
-    const float* a = p.acc + (i * rows + row) * hd;
+  for (int i = lane; i < slices; i += kLanes) m = fmaxf(m, p.ml[i * rows + row].x);
 #pragma unroll
-    for (int u = 0; u < kMaxPagedHd / kLanes; u++)
-      if (lane + kLanes * u < hd) acc[u] += a[lane + kLanes * u] * f;
+  for (int off = 16; off >= 1; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
+  const float base = m == -INFINITY ? 0.0f : m;
+  float l = 0.0f, acc[kRuns][V] = {};
+  for (int i0 = 0; i0 < slices; i0 += kLanes) {
+    const float2 ml = i0 + lane < slices ? p.ml[(i0 + lane) * rows + row] : make_float2(-INFINITY, 0.0f);
+    const float mine = ml.y == 0.0f ? 0.0f : exp2_fast(ml.x - base);
+    l += ml.y * mine;
+    unsigned left = __ballot_sync(0xffffffffu, ml.y != 0.0f);  // (a slice with l = 0 may hold anything)
+    const int count = min(kLanes, slices - i0);
+#pragma unroll 4
+    for (int i = 0; i < count; i++) {
+      const float f = __shfl_sync(0xffffffffu, mine, i);
+      const float* a = p.acc + ((i0 + i) * rows + row) * hd;
+      if ((left >> i & 1u) == 0) continue;
+#pragma unroll
+      for (int u = 0; u < kRuns; u++) {
+        const int d = (u * kLanes + lane) * V;
+        if (d >= hd) continue;
+        float x[V];
+        load_run<float, V>(a + d, x);
+#pragma unroll
+        for (int e = 0; e < V; e++) acc[u][e] += x[e] * f;
+      }
+    }
   }
+#pragma unroll
+  for (int off = 16; off >= 1; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
   T* out = static_cast<T*>(p.a.out) + t * p.a.out_stride + (int64_t)head * hd;
 #pragma unroll
-  for (int u = 0; u < kMaxPagedHd / kLanes; u++)
-    if (lane + kLanes * u < hd) out[lane + kLanes * u] = from_f32<T>(l == 0.0f ? 0.0f : acc[u] / l);
+  for (int u = 0; u < kRuns; u++) {
+    const int d = (u * kLanes + lane) * V;
+    if (d >= hd) continue;
+#pragma unroll
+    for (int e = 0; e < V; e++) acc[u][e] = l == 0.0f ? 0.0f : acc[u][e] / l;
+    if (p.runs) {
+      store_run<T, V>(out + d, acc[u]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; e++) out[d + e] = from_f32<T>(acc[u][e]);
+    }
+  }
 }
 
 // ------------------------------------------------------------------ the host
@@ -245,12 +273,19 @@ bool mma_cache(const PagedCache& c) {
   return c.type != kF32 && (((uintptr_t)c.keys | (uintptr_t)c.values) & 15) == 0 && (c.page_stride | c.hd) % 8 == 0;
 }
 
+constexpr int64_t kSoloKeys = 512;    // of the longest sequence
+constexpr int64_t kSoloReads = 8192;  // keys of the prefix, once for each sequence
+
 // How the work is divided, from sizes that the host knows.
 Params plan(const PagedCache& c, int64_t heads, int64_t n, int64_t prefix, int64_t max_length) {
   Params p{};
   p.group = (int)(heads / c.kv_heads);
   const int64_t rows = n * p.group, seqs = c.sequences > 1 ? c.sequences : 1;
   const bool wide = mma_cache(c) && c.page_size % 16 == 0 && c.pages > 0;
+  // Short sequences in all: each reads the prefix for itself, from L2, which
+  // saves the second launch that joins two parts.
+  p.solo = prefix > 0 && prefix % 16 == 0 && max_length <= kSoloKeys && c.sequences * prefix <= kSoloReads;
+  if (p.solo) prefix = 0;
   p.prefix_wide = wide && prefix > 0 && rows > kWideFrom;
   p.own_wide = wide && rows > kWideFrom * seqs;
   // 8 rows to a thin block where a sequence's rows, and the whole batch's on
@@ -274,7 +309,9 @@ Params plan(const PagedCache& c, int64_t heads, int64_t n, int64_t prefix, int64
   p.prefix_splits = prefix > 0 ? splits(tiles * c.kv_heads, prefix, p.prefix_wide) : 0;
   const int64_t own = max_length > prefix ? max_length - prefix : 1;
   p.own_splits = splits((int64_t)p.own_slots * c.kv_heads, own, p.own_wide);
-  p.direct = p.prefix_splits + p.own_splits == 1;
+  p.prefix_slices = p.prefix_splits * (p.prefix_wide ? wide_groups(c.hd) : 1);
+  p.slices = p.prefix_slices + p.own_splits * (p.own_wide ? wide_groups(c.hd) : 1);
+  p.direct = p.slices == 1;
   return p;
 }
 
@@ -317,8 +354,9 @@ cudaError_t launch_type(const Params& p, cudaStream_t stream, bool pdl) {
                                : launch_simt<T, 1>(p, stream, pdl);
   if (e != cudaSuccess || p.direct) return e;
   const int64_t warps = p.a.n * p.a.heads, per = kJoinThreads / kLanes;
-  return launch_ex(attention_join_kernel<T>, dim3((unsigned)((warps + per - 1) / per)), kJoinThreads, 0, stream, true,
-                   p);
+  const dim3 grid((unsigned)((warps + per - 1) / per));
+  return c.hd % 4 == 0 ? launch_ex(attention_join_kernel<T, 4>, grid, kJoinThreads, 0, stream, true, p)
+                       : launch_ex(attention_join_kernel<T, 1>, grid, kJoinThreads, 0, stream, true, p);
 }
 
 }  // namespace
@@ -326,7 +364,7 @@ cudaError_t launch_type(const Params& p, cudaStream_t stream, bool pdl) {
 int64_t paged_attention_workspace(const PagedCache& c, int64_t heads, int64_t n, int64_t prefix,
                                   int64_t max_length) {
   const Params p = plan(c, heads, n, prefix, max_length);
-  return (p.prefix_splits + p.own_splits) * n * heads * (c.hd + 2) * (int64_t)sizeof(float) + 16;
+  return p.slices * n * heads * (c.hd + 2) * (int64_t)sizeof(float) + 16;
 }
 
 cudaError_t launch_paged_attention(const PagedAttentionArgs& a, cudaStream_t stream, bool pdl) {
@@ -337,9 +375,13 @@ cudaError_t launch_paged_attention(const PagedAttentionArgs& a, cudaStream_t str
   p.page_shift = -1;
   for (int s = 0; s <= 20; s++)
     if (a.cache.page_size == (int64_t)1 << s) p.page_shift = s;
+  p.runs = (((uintptr_t)a.q | (uintptr_t)a.out) & 15) == 0 &&
+           ((a.q_stride | a.out_stride | a.cache.hd) * elem_size(a.cache.type)) % 16 == 0;
   p.pairs = (((uintptr_t)a.q | (uintptr_t)a.out) & 3) == 0 && (a.q_stride | a.out_stride) % 2 == 0;
-  p.scale_log2 = a.scale * kLog2e;
-  const int64_t rows = (p.prefix_splits + p.own_splits) * a.n * a.heads;
+  // A scale of 0 is taken as the least normal number: the exponents still come
+  // out equal, and a masked score's minus infinity stays one.
+  p.scale_log2 = a.scale == 0.0f ? 1.17549435e-38f : a.scale * kLog2e;
+  const int64_t rows = p.slices * a.n * a.heads;
   p.ml = static_cast<float2*>(a.workspace);
   p.acc = reinterpret_cast<float*>(p.ml + (rows + 1) / 2 * 2);
   switch (a.cache.type) {

@@ -31,12 +31,14 @@ struct Params {
   int prefix_tiles, prefix_splits;
   int own_slots, own_splits;
   int min_slice;        // keys: slices are not made shorter than this
-  float* acc;           // [prefix_splits + own_splits][n * heads][hd]
-  float2* ml;           // [prefix_splits + own_splits][n * heads]: m, l
+  int prefix_slices, slices;  // results of a row: of the prefix, in all
+  float* acc;           // [slices][n * heads][hd]
+  float2* ml;           // [slices][n * heads]: m, l
   float scale_log2;
   int page_shift;       // log2 of the page size, or -1
   uint32_t* status;     // bounded waits' status word
-  bool pairs;           // rows of q and out are 4-byte aligned
+  bool pairs, runs;     // rows of q and out are 4-byte, 16-byte aligned
+  bool solo;            // each sequence reads the prefix for itself
   bool direct;          // one slice in all: blocks write `out` themselves
 };
 
@@ -92,7 +94,7 @@ __device__ __forceinline__ void sees(const Params& p, const Work& w, int t, int&
   if (w.prefix) {
     high = min(high, (int)p.a.prefix - 1);
   } else {
-    low = max(low, (int)p.a.prefix);
+    if (!p.solo) low = max(low, (int)p.a.prefix);
     high = min(high, (int)(p.a.cache.table_stride * p.a.cache.page_size) - 1);
   }
 }
@@ -169,7 +171,7 @@ __device__ __forceinline__ int entry_of(const Params& p, int pos) {
 __device__ __forceinline__ int page_of(const Params& p, const Work& w, int pos) {
   const int entry = entry_of(p, pos);
   int page;
-  if (w.prefix) {
+  if (w.prefix || (p.solo && pos < (int)p.a.prefix)) {
     if (pos >= (int)p.a.prefix) return -1;
     page = p.a.prefix_pages[entry];
   } else {
@@ -212,8 +214,9 @@ __device__ __forceinline__ int64_t out_index(const Params& p, const Work& w, int
   return (int64_t)token * p.a.heads + head;
 }
 
-__device__ __forceinline__ int slice_index(const Params& p, const Work& w) {
-  return w.prefix ? w.slice : p.prefix_splits + w.slice;
+// Where a block's result (its group's, for a wide block) goes among a row's.
+__device__ __forceinline__ int slice_index(const Params& p, const Work& w, int group = 0) {
+  return w.prefix ? w.slice + group * p.prefix_splits : p.prefix_slices + w.slice + group * p.own_splits;
 }
 
 // Rows of a block by kernel: the f32 one and the thin one (8 or 16), the wide one.
@@ -222,9 +225,22 @@ constexpr int kWideRows = 128;
 constexpr int kWideFrom = 32;  // rows (of the batch, of a sequence on average) from which the wide one runs
 constexpr int kLanes = 32;
 
+// Groups of a wide block, each with results of its own: two outputs of 128
+// columns stand in TMEM beside the scores, of 256 one.
+constexpr int wide_groups(int64_t hd) { return hd <= 128 ? 2 : 1; }
+
 inline dim3 attention_grid(const Params& p) {
   return dim3((unsigned)(p.prefix_tiles * p.prefix_splits + p.own_slots * p.own_splits),
               (unsigned)p.a.cache.kv_heads);
+}
+
+// Dynamic shared memory of a kernel, with the SM's whole split for it: blocks
+// of two kernels stay on one SM only under the same split.
+template <typename K>
+inline cudaError_t allow_smem(K kern, int bytes) {
+  if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes); e != cudaSuccess)
+    return e;
+  return cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
 }
 
 template <typename K, typename... Args>

@@ -78,7 +78,7 @@ struct Shape {
   static constexpr int kPanels = HDP / 64;                // 64 elements wide
   static constexpr int kPanel = kStep * 128;              // bytes of a panel of a step
   static constexpr int kBuf = kPanels * kPanel;           // a step's keys; as many again its values
-  static constexpr int kStages = HDP <= 128 ? 3 : 2;
+  static constexpr int kStages = 2;
   static constexpr int kRing = kStages * 2 * kBuf;        // a warp's
 };
 
@@ -403,10 +403,7 @@ cudaError_t launch_copies(const Params& p, const Maps& maps, cudaStream_t stream
   constexpr int ring = kWarps * Shape<HDP>::kRing;
   constexpr int join = kWarps * 8 * NT * ((HDP + 4) * 4 + 8);
   constexpr int smem = ring > join ? ring : join;
-  if (cudaError_t e = cudaFuncSetAttribute(attention_thin_kernel<T, HDP, NT, TMA>,
-                                           cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-      e != cudaSuccess)
-    return e;
+  if (cudaError_t e = allow_smem(attention_thin_kernel<T, HDP, NT, TMA>, smem); e != cudaSuccess) return e;
   return launch_ex(attention_thin_kernel<T, HDP, NT, TMA>, attention_grid(p), kThreads, smem, stream, pdl, p, maps);
 }
 

@@ -4,16 +4,22 @@
 // 128 rows of one kv head share every key, so the products are the bound:
 // S = Q K^T and O += P V on the 5th-generation tensor cores (tcgen05, f32
 // accumulators in TMEM). A block runs three parts at once:
-//   warp 4 brings tiles of 64 keys and their values by tiled TMA copies;
-//   warp 5 issues the products: S of tile i + 1 while tile i is in softmax;
-//   warps 0 .. 3 hold a row of S each thread: they read it from TMEM, keep the
-//   row's base and sum, and write P (16-bit) over it, which the tensor cores
-//   read from there as the first operand of P V.
-// S is doubled in TMEM so that the tensor cores and the softmax overlap. A
-// base moves only when a score passes it by kSlack (P then stays below 2^8),
-// so O is rescaled in TMEM in the first tiles and hardly ever after. Where rows
-// of the block see different keys of a tile and a value there is not finite,
-// that tile's P V is added term by term instead (0 * infinity would be NaN).
+//   one warp brings tiles of 128 keys and their values by tiled TMA copies;
+//   one warp issues the products;
+//   two groups of 4 warps (one for heads over 128 wide) take the even and the
+//   odd tiles, a row of S each thread: they read it from TMEM 64 keys (a half)
+//   at a time, keep the row's base and sum, and write P (16-bit) over it, which
+//   the tensor cores read from there as the first operand of P V. Each group
+//   has an O of its own, so the groups never wait for one another; the join
+//   adds them.
+// Two tiles of S stand in TMEM: while one group is in softmax the tensor cores
+// serve the other. (With 64-key tiles S took M = 128, N = 64 products, which
+// run at half the rate: 73000 cycles for 2752 keys, the tensor cores the
+// bound.) A base moves only when a score passes it by kSlack (P then stays
+// below 2^8), so O is rescaled in TMEM in the first tiles and hardly ever
+// after. Where rows of the block see different keys of a half and a value
+// there is not finite, that half's P V is added term by term instead
+// (0 * infinity would be NaN).
 #include <type_traits>
 
 #include "dn_tmap.h"
@@ -27,9 +33,11 @@ using namespace paged;
 namespace {
 
 constexpr int kRows = kWideRows;
-constexpr int kKeys = 64;       // of a tile
-constexpr int kRowThreads = 128;
-constexpr int kThreads = 192;
+constexpr int kHalf = 64;         // keys of a half, which one P V takes
+constexpr int kKeys = 2 * kHalf;  // of a tile, which one S takes
+constexpr int kRowThreads = 128;  // of a group
+constexpr int kScores = 2;        // tiles of S in TMEM
+constexpr int kHalves = 2 * kScores;
 constexpr float kSlack = 8.0f;  // log2 units a score may pass the running base
 
 struct alignas(64) Maps {
@@ -39,20 +47,26 @@ struct alignas(64) Maps {
 template <int HDP>
 struct Shape {
   static constexpr int kPanels = HDP / 64;
-  static constexpr int kQPanel = kRows * 128;       // bytes: 64 elements of every row
-  static constexpr int kPanel = kKeys * 128;        // of every key of a tile
-  static constexpr int kTileBytes = kPanels * kPanel;
-  static constexpr int kStages = HDP <= 128 ? 3 : 2;
-  static constexpr int kQ = kPanels * kQPanel;
-  static constexpr int kSmem = kQ + kStages * 2 * kTileBytes;
-  static constexpr uint32_t kCols = HDP <= 128 ? 256 : 512;  // of TMEM: S twice, then O
+  static constexpr int kQPanel = kRows * 128;  // bytes: 64 elements of every row
+  static constexpr int kKPanel = kKeys * 128;  // of every key of a tile
+  static constexpr int kVPanel = kHalf * 128;  // of every value of a half
+  static constexpr int kGroups = wide_groups(HDP);
+  static constexpr int kThreads = kGroups * kRowThreads + 64;
+  static constexpr int kKStages = HDP <= 128 ? 2 : 1, kVStages = HDP <= 128 ? 3 : 2;
+  static constexpr int kK = kPanels * kQPanel;              // where the keys start
+  static constexpr int kV = kK + kKStages * kPanels * kKPanel;
+  static constexpr int kSmem = kV + kVStages * kPanels * kVPanel;
+  static constexpr uint32_t kCols = 512;  // of TMEM: S, then each group's O
+  static_assert(kScores * kKeys + kGroups * HDP <= 512, "TMEM");
 };
 
+// Tile i has barriers i % kScores, half j = 2 i, 2 i + 1 of it j % kHalves
+// (o_done: its P V is done). A thread may pass over phases, and a parity tells
+// two phases in a row apart, not three: S of tile i is there only once P V of
+// half 2 i - 3 is done, so whoever waits for a half of tile i or i - 1 knows
+// the phase before it past.
 struct Bars {
-  uint64_t k_full[3], k_empty[3], v_full[3], v_empty[3], s_full[2], p_full[2];
-  // Of even and odd tiles: a row thread may pass over a tile's, and the parity
-  // of a barrier tells two phases in a row apart, not three.
-  uint64_t o_done[2];
+  uint64_t k_full[2], k_empty[2], v_full[3], v_empty[3], s_full[kScores], p_full[kHalves], o_done[kHalves];
 };
 
 // Shared-memory operand, 128-byte swizzled; `lead` is the stride between
@@ -123,218 +137,237 @@ __device__ __forceinline__ void st32(uint32_t addr, const uint32_t (&v)[32]) {
 }
 __device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// The rows' part. Row `r` of the block is the thread's.
+// A group's part, of tiles group, group + kGroups, ...; `halves` in all of the
+// block; row `r` of the block is the thread's.
 template <typename T, int HDP>
 __device__ __forceinline__ void softmax_rows(const Params& p, const Work& w, char* smem, Bars& bars, uint32_t* skip,
-                                             uint32_t tmem, int begin, int tiles, int low, int high, int all_low,
-                                             int all_high) {
+                                             uint32_t tmem, int begin, int halves, int group, int low, int high,
+                                             int all_low, int all_high) {
   using S = Shape<HDP>;
-  const int r = threadIdx.x, lane = r % kLanes;
+  const int r = threadIdx.x % kRowThreads, lane = r % kLanes;
   const uint32_t mine = tmem + ((uint32_t)(r / kLanes * 32) << 16);
-  const uint32_t out_cols = mine + 2 * kKeys;
-  const int hd = (int)p.a.cache.hd;
+  const uint32_t out_cols = mine + kScores * kKeys + (uint32_t)(group * HDP);
+  const int hd = (int)p.a.cache.hd, tiles = (halves + 1) / 2;
+  const float scale = fabsf(p.scale_log2);
   float m = -INFINITY, l = 0.0f;
-  // Lanes 0 .. 3 know which 16 keys of the next tile have a page.
+  // Lanes 0 .. 7 know which 16 keys of the next tile have a page.
   auto look_up = [&](int tile) {
     return lane < kKeys / 16 && tile < tiles && page_of(p, w, begin + tile * kKeys + 16 * lane) >= 0;
   };
-  bool next_there = look_up(0);
+  bool next_there = look_up(group);
   bool live = true;
-  for (int i = 0; i < tiles; i++) {
-    const unsigned there = __ballot_sync(0xffffffffu, next_there);
-    next_there = look_up(i + 1);
-    const int k0 = begin + i * kKeys;
-    const uint32_t cols = mine + (uint32_t)(i & 1) * kKeys;
-    live = __all_sync(0xffffffffu, mbar_wait_bounded(&bars.s_full[i & 1], (i >> 1) & 1, p.status, kStatusMmaTimeout));
+  auto done = [&](int j) {
+    return __all_sync(0xffffffffu, mbar_wait_bounded(&bars.o_done[j % kHalves], (j / kHalves) & 1, p.status,
+                                                     kStatusMmaTimeout));
+  };
+  int last = -1;  // the group's last half
+  for (int i = group; i < tiles && live; i += S::kGroups) {
+    const unsigned tile_there = __ballot_sync(0xffffffffu, next_there);
+    next_there = look_up(i + S::kGroups);
+    live = __all_sync(0xffffffffu, mbar_wait_bounded(&bars.s_full[i % kScores], (i / kScores) & 1, p.status,
+                                                     kStatusMmaTimeout));
     if (!live) break;
     fence_after();
-    float s[2][32];
-    ld32(cols, s[0]);
-    ld32(cols + 32, s[1]);
-    wait_ld(s[0]);
-    wait_ld(s[1]);
-    const bool all = there == 0xfu && k0 >= all_low && k0 + kKeys - 1 <= all_high;  // the same in every row
-    if (!all) {
-#pragma unroll
-      for (int j = 0; j < kKeys; j++) {
-        const bool seen = (there >> (j / 16) & 1u) != 0 && k0 + j >= low && k0 + j <= high;
-        s[j / 32][j % 32] = seen ? s[j / 32][j % 32] * p.scale_log2 : -INFINITY;
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < kKeys; j++) s[j / 32][j % 32] *= p.scale_log2;
-    }
-    float top4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-    for (int j = 0; j < kKeys; j++) top4[j % 4] = fmaxf(top4[j % 4], s[j / 32][j % 32]);
-    const float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3]));
-    bool waited = false;
-    if (__any_sync(0xffffffffu, top > m + kSlack)) {
-      const float next = fmaxf(m, top);
-      const float keep = next == -INFINITY ? 1.0f : exp2_fast(m - next);
-      m = next;
-      l *= keep;
-      if (i > 0) {
-        live = __all_sync(0xffffffffu, mbar_wait_bounded(&bars.o_done[(i - 1) & 1], ((i - 1) >> 1) & 1, p.status, kStatusMmaTimeout));
-        if (!live) break;
-        waited = true;
-        fence_after();
 #pragma unroll 1
-        for (int c = 0; c < HDP; c += 32) {
-          float o[32];
-          ld32(out_cols + c, o);
-          wait_ld(o);
-          uint32_t u[32];
+    for (int h = 0; h < 2; h++) {
+      const int j = 2 * i + h, k0 = begin + j * kHalf;
+      if (j >= halves) break;
+      const uint32_t cols = mine + (uint32_t)(j % kHalves) * kHalf;
+      const unsigned there = tile_there >> (4 * h) & 0xfu;
+      float s[2][32];
+      ld32(cols, s[0]);
+      ld32(cols + 32, s[1]);
+      wait_ld(s[0]);
+      wait_ld(s[1]);
+      const bool all = there == 0xfu && k0 >= all_low && k0 + kHalf - 1 <= all_high;  // the same in every row
+      if (p.scale_log2 < 0.0f) {
 #pragma unroll
-          for (int e = 0; e < 32; e++) u[e] = __float_as_uint(o[e] * keep);
-          st32(out_cols + c, u);
+        for (int e = 0; e < kHalf; e++) s[e / 32][e % 32] = -s[e / 32][e % 32];
+      }
+      if (!all) {
+#pragma unroll
+        for (int e = 0; e < kHalf; e++) {
+          const bool seen = (there >> (e / 16) & 1u) != 0 && k0 + e >= low && k0 + e <= high;
+          if (!seen) s[e / 32][e % 32] = -INFINITY;
         }
-        wait_st();
       }
-    }
-    const float base = m == -INFINITY ? 0.0f : m;
-    uint32_t pk[32];
-    float sum4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      float top4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-    for (int j = 0; j < kKeys; j += 2) {
-      const float x = exp2_fast(s[j / 32][j % 32] - base), y = exp2_fast(s[j / 32][j % 32 + 1] - base);
-      s[j / 32][j % 32] = x;
-      s[j / 32][j % 32 + 1] = y;
-      sum4[j / 2 % 4] += x + y;
-      pk[j / 2] = Pair<T>::pack(x, y);
-    }
-    l += (sum4[0] + sum4[1]) + (sum4[2] + sum4[3]);
-    if (!all) {
-      // The values have to be looked at, and may have to be added here.
-      char* vals = smem + S::kQ + (i % S::kStages) * 2 * S::kTileBytes + S::kTileBytes;
-      live = __all_sync(0xffffffffu, mbar_wait_bounded(&bars.v_full[i % S::kStages], (i / S::kStages) & 1, p.status,
-                                                       kStatusTmaTimeout));
-      bool bad = false;
-      for (int c = lane; c < S::kTileBytes / 16; c += kLanes) bad = bad || unbounded16<T>(vals + c * 16);
-      bad = __any_sync(0xffffffffu, bad);  // every warp finds the same
-      if (r == 0) skip[i & 1] = bad ? 1u : 0u;
-      if (bad) {
-        if (i > 0 && !waited)
-          live = __all_sync(0xffffffffu, mbar_wait_bounded(&bars.o_done[(i - 1) & 1], ((i - 1) >> 1) & 1, p.status, kStatusMmaTimeout));
-        fence_after();
-        float pr[kKeys];  // indexed at run time: in local memory, here only
-#pragma unroll
-        for (int j = 0; j < kKeys; j++) pr[j] = to_f32<T>(from_f32<T>(s[j / 32][j % 32]));
+      for (int e = 0; e < kHalf; e++) top4[e % 4] = fmaxf(top4[e % 4], s[e / 32][e % 32]);
+      const float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3])) * scale;
+      bool waited = last < 0;
+      if (__any_sync(0xffffffffu, top > m + kSlack)) {
+        const float next = fmaxf(m, top);
+        const float keep = next == -INFINITY ? 1.0f : exp2_fast(m - next);
+        m = next;
+        l *= keep;
+        if (last >= 0) {
+          live = done(last);
+          if (!live) break;
+          waited = true;
+          fence_after();
 #pragma unroll 1
-        for (int c = 0; c < HDP; c += 32) {
-          float o[32];
-          ld32(out_cols + c, o);
-          wait_ld(o);
-          if (i == 0)
+          for (int c = 0; c < HDP; c += 32) {
+            float o[32];
+            ld32(out_cols + c, o);
+            wait_ld(o);
+            uint32_t u[32];
 #pragma unroll
-            for (int e = 0; e < 32; e++) o[e] = 0.0f;
-#pragma unroll 1
-          for (int j = 0; j < kKeys; j++) {
-            if (pr[j] != 0.0f)
-#pragma unroll
-              for (int e = 0; e < 32; e++) {
-                const int d = c + e;
-                const T v = reinterpret_cast<const T*>(vals + d / 64 * S::kPanel + j * 128 +
-                                                       (((d % 64 / 8) ^ (j & 7)) << 4))[d % 8];
-                o[e] = fmaf(pr[j], to_f32<T>(v), o[e]);
-              }
+            for (int e = 0; e < 32; e++) u[e] = __float_as_uint(o[e] * keep);
+            st32(out_cols + c, u);
           }
-          uint32_t u[32];
-#pragma unroll
-          for (int e = 0; e < 32; e++) u[e] = __float_as_uint(o[e]);
-          __syncwarp();
-          st32(out_cols + c, u);
+          wait_st();
         }
       }
-    } else if (r == 0) {
-      skip[i & 1] = 0;
+      const float base = m == -INFINITY ? 0.0f : m;
+      uint32_t pk[32];
+      float sum4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int e = 0; e < kHalf; e += 2) {
+        const float x = exp2_fast(fmaf(s[e / 32][e % 32], scale, -base));
+        const float y = exp2_fast(fmaf(s[e / 32][e % 32 + 1], scale, -base));
+        s[e / 32][e % 32] = x;
+        s[e / 32][e % 32 + 1] = y;
+        sum4[e / 2 % 4] += x + y;
+        pk[e / 2] = Pair<T>::pack(x, y);
+      }
+      l += (sum4[0] + sum4[1]) + (sum4[2] + sum4[3]);
+      if (!all) {
+        // The values have to be looked at, and may have to be added here.
+        char* vals = smem + S::kV + j % S::kVStages * S::kPanels * S::kVPanel;
+        live = __all_sync(0xffffffffu, mbar_wait_bounded(&bars.v_full[j % S::kVStages], (j / S::kVStages) & 1,
+                                                         p.status, kStatusTmaTimeout));
+        if (!live) break;
+        bool bad = false;
+        for (int c = lane; c < S::kPanels * S::kVPanel / 16; c += kLanes) bad = bad || unbounded16<T>(vals + c * 16);
+        bad = __any_sync(0xffffffffu, bad);  // every warp finds the same
+        if (r == 0) skip[j % kHalves] = bad ? 1u : 0u;
+        if (bad) {
+          if (!waited) live = done(last);
+          if (!live) break;
+          fence_after();
+          float pr[kHalf];  // indexed at run time: in local memory, here only
+#pragma unroll
+          for (int e = 0; e < kHalf; e++) pr[e] = to_f32<T>(from_f32<T>(s[e / 32][e % 32]));
+#pragma unroll 1
+          for (int c = 0; c < HDP; c += 32) {
+            float o[32];
+            ld32(out_cols + c, o);
+            wait_ld(o);
+            if (last < 0)
+#pragma unroll
+              for (int e = 0; e < 32; e++) o[e] = 0.0f;
+#pragma unroll 1
+            for (int k = 0; k < kHalf; k++) {
+              if (pr[k] != 0.0f)
+#pragma unroll
+                for (int e = 0; e < 32; e++) {
+                  const int d = c + e;
+                  const T v = reinterpret_cast<const T*>(vals + d / 64 * S::kVPanel + k * 128 +
+                                                         (((d % 64 / 8) ^ (k & 7)) << 4))[d % 8];
+                  o[e] = fmaf(pr[k], to_f32<T>(v), o[e]);
+                }
+            }
+            uint32_t u[32];
+#pragma unroll
+            for (int e = 0; e < 32; e++) u[e] = __float_as_uint(o[e]);
+            __syncwarp();
+            st32(out_cols + c, u);
+          }
+        }
+      } else if (r == 0) {
+        skip[j % kHalves] = 0;
+      }
+      st32(cols, pk);
+      wait_st();
+      fence_before();
+      mbar_arrive(&bars.p_full[j % kHalves]);
+      last = j;
     }
-    st32(cols, pk);
-    wait_st();
-    fence_before();
-    mbar_arrive(&bars.p_full[i & 1]);
   }
-  if (tiles > 0 && live) {
-    live = __all_sync(0xffffffffu,
-                      mbar_wait_bounded(&bars.o_done[(tiles - 1) & 1], ((tiles - 1) >> 1) & 1, p.status, kStatusMmaTimeout));
+  if (last >= 0 && live) {
+    done(last);
     fence_after();
   }
   // The row's result.
   int t = 0, head = 0;
-  const bool there = r < w.rows;
-  const int64_t row = there ? out_index(p, w, r, t, head) : 0;
-  const int64_t to = slice_index(p, w) * (p.a.n * p.a.heads) + row;
+  const bool mine_row = r < w.rows;
+  const int64_t row = mine_row ? out_index(p, w, r, t, head) : 0;
+  const int64_t to = slice_index(p, w, group) * (p.a.n * p.a.heads) + row;
   if (high < low) {  // a row that sees nothing took part unmasked
     m = -INFINITY;
     l = 0.0f;
   }
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  if (there && !p.direct) p.ml[to] = make_float2(m, l);
-  if (tiles == 0 && !p.direct) return;  // the join reads no values of a row with l = 0
+  if (mine_row && !p.direct) p.ml[to] = make_float2(m, l);
+  if (last < 0 && !p.direct) return;  // the join reads no values of a row with l = 0
 #pragma unroll 1
   for (int c = 0; c < HDP; c += 32) {
     float o[32];
-    if (tiles > 0) {
+    if (last >= 0) {
       ld32(out_cols + c, o);
       wait_ld(o);
     } else {
 #pragma unroll
       for (int e = 0; e < 32; e++) o[e] = 0.0f;
     }
-    if (!there) continue;
-    if (p.direct) {
+    if (mine_row && p.direct) {
       T* out = static_cast<T*>(p.a.out) + t * p.a.out_stride + (int64_t)head * hd;
 #pragma unroll
       for (int e = 0; e < 32; e += 2)
         if (c + e < hd)
           store_pair(out + c + e, l == 0.0f ? 0u : Pair<T>::pack(o[e] * inv, o[e + 1] * inv), p.pairs);
-    } else {
+    } else if (mine_row) {
 #pragma unroll
       for (int e = 0; e < 32; e += 4)
         if (c + e < hd)
           *reinterpret_cast<float4*>(p.acc + to * hd + c + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
     }
+    __syncwarp();  // the next load takes whole warps
   }
 }
 
 template <typename T, int HDP>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __maxnreg__(152)
     attention_wide_kernel(const __grid_constant__ Params p, const __grid_constant__ Maps maps, int box) {
   using S = Shape<HDP>;
   pdl_wait();
   pdl_launch_dependents();  // after the wait: what starts now may read this kernel's inputs
   extern __shared__ __align__(1024) char smem[];
   __shared__ Bars bars;
-  __shared__ uint32_t tmem_at, skip[2];
-  __shared__ int span[kRowThreads / kLanes][4];
+  __shared__ uint32_t tmem_at, skip[kHalves];
+  constexpr int kRowWarps = S::kGroups * kRowThreads / kLanes;
+  __shared__ int span[kRowWarps][4];
   Work w;
   if (!find_work(p, w)) return;
   const int tid = threadIdx.x, warp = tid / kLanes, lane = tid % kLanes;
   const int hd = (int)p.a.cache.hd;
-  if (warp == 5) {
+  if (warp == kRowWarps + 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_at)),
                  "r"(S::kCols)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  if (tid == kRowThreads) {
-    for (int i = 0; i < S::kStages; i++) {
+  if (tid == kRowWarps * kLanes) {
+    for (int i = 0; i < S::kKStages; i++) {
       mbar_init(&bars.k_full[i], 1);
       mbar_init(&bars.k_empty[i], 1);
+    }
+    for (int i = 0; i < S::kVStages; i++) {
       mbar_init(&bars.v_full[i], 1);
       mbar_init(&bars.v_empty[i], 1);
     }
-    for (int i = 0; i < 2; i++) {
-      mbar_init(&bars.s_full[i], 1);
+    for (int i = 0; i < kScores; i++) mbar_init(&bars.s_full[i], 1);
+    for (int i = 0; i < kHalves; i++) {
       mbar_init(&bars.p_full[i], kRowThreads);
       mbar_init(&bars.o_done[i], 1);
     }
     fence_mbar_init();
   }
   int low = 0, high = -1;
-  if (tid < kRowThreads) {
-    const bool mine = tid < w.rows;
-    if (mine) sees(p, w, (w.row0 + tid) / p.group, low, high);
+  if (warp < kRowWarps) {
+    const int r = tid % kRowThreads;
+    if (r < w.rows) sees(p, w, (w.row0 + r) / p.group, low, high);
     const bool any = high >= low;
     const int all_lo = __reduce_max_sync(0xffffffffu, any ? low : 0);
     const int all_hi = __reduce_min_sync(0xffffffffu, any ? high : INT32_MAX);
@@ -346,20 +379,25 @@ __global__ void __launch_bounds__(kThreads)
       span[warp][2] = any_lo;
       span[warp][3] = any_hi;
     }
-    // Row tid of Q: chunk c of 8 elements at chunk c ^ (row & 7) of its panel.
-    const T* src = nullptr;
-    if (mine) {
-      int t, head;
-      out_index(p, w, tid, t, head);
-      src = static_cast<const T*>(p.a.q) + t * p.a.q_stride + (int64_t)head * hd;
-    }
+    // Q, a run of lanes for each row: chunk c of 8 elements of row r at chunk
+    // c ^ (r & 7) of its panel.
+    constexpr int kChunks = HDP / 8, kAtOnce = kLanes / kChunks > 0 ? kLanes / kChunks : 1;
 #pragma unroll 4
-    for (int c = 0; c < HDP / 8; c++) {
-      uint32_t v[4];
-#pragma unroll
-      for (int u = 0; u < 4; u++) v[u] = src != nullptr && 8 * c < hd ? load_pair(src + 8 * c + 2 * u, p.pairs) : 0u;
-      *reinterpret_cast<uint4*>(smem + c / 8 * S::kQPanel + tid * 128 + (((c ^ tid) & 7) << 4)) =
-          make_uint4(v[0], v[1], v[2], v[3]);
+    for (int row = warp * kAtOnce + lane / kChunks; row < kRows; row += kRowWarps * kAtOnce) {
+      const int c = lane % kChunks;
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (row < w.rows && 8 * c < hd) {
+        int t, head;
+        out_index(p, w, row, t, head);
+        const T* src = static_cast<const T*>(p.a.q) + t * p.a.q_stride + (int64_t)head * hd + 8 * c;
+        if (p.runs) {
+          v = *reinterpret_cast<const uint4*>(src);
+        } else {
+          v = make_uint4(load_pair(src, p.pairs), load_pair(src + 2, p.pairs), load_pair(src + 4, p.pairs),
+                         load_pair(src + 6, p.pairs));
+        }
+      }
+      *reinterpret_cast<uint4*>(smem + c / 8 * S::kQPanel + row * 128 + (((c ^ row) & 7) << 4)) = v;
     }
     fence_proxy_async_smem();
   }
@@ -369,94 +407,118 @@ __global__ void __launch_bounds__(kThreads)
   const uint32_t tmem = tmem_at;
   int all_low = span[0][0], all_high = span[0][1], any_low = span[0][2], any_high = span[0][3];
 #pragma unroll
-  for (int i = 1; i < kRowThreads / kLanes; i++) {
+  for (int i = 1; i < kRowWarps; i++) {
     all_low = max(all_low, span[i][0]);
     all_high = min(all_high, span[i][1]);
     any_low = min(any_low, span[i][2]);
     any_high = max(any_high, span[i][3]);
   }
   int begin, end;
-  slice_keys(p, w, any_low, any_high, kKeys, begin, end);
-  const int tiles = (end - begin + kKeys - 1) / kKeys;
+  slice_keys(p, w, any_low, any_high, kHalf, begin, end);
+  const int halves = (end - begin + kHalf - 1) / kHalf, tiles = (halves + 1) / 2;
 
-  if (warp < 4) {
-    softmax_rows<T, HDP>(p, w, smem, bars, skip, tmem, begin, tiles, low, high, all_low, all_high);
-  } else if (warp == 4) {
-    const int panels = (hd + 63) / 64, groups = kKeys / box;
+  if (warp < kRowWarps) {
+    softmax_rows<T, HDP>(p, w, smem, bars, skip, tmem, begin, halves, tid / kRowThreads, low, high, all_low, all_high);
+  } else if (warp == kRowWarps) {
+    const int panels = (hd + 63) / 64, groups = kHalf / box;  // groups of keys of one page in a half
+    // Lane g knows the page of group g of the tile; one past the last page
+    // reads as zeros.
     auto look_up = [&](int tile) {
       int page = -1;
-      if (lane < groups && tile < tiles) page = page_of(p, w, begin + tile * kKeys + lane * box);
-      return page >= 0 ? page : (int)p.a.cache.pages;  // one past the last reads as zeros
+      if (lane < 2 * groups && tile < tiles) page = page_of(p, w, begin + tile * kKeys + lane * box);
+      return page >= 0 ? page : (int)p.a.cache.pages;
     };
-    int next = look_up(0);
-    for (int i = 0; i < tiles; i++) {
-      const int s = i % S::kStages, page = next;
-      next = look_up(i + 1);
-      char* kb = smem + S::kQ + s * 2 * S::kTileBytes;
-      bool live = true;
-#pragma unroll
-      for (int kv = 0; kv < 2; kv++) {
-        uint64_t* full = kv ? &bars.v_full[s] : &bars.k_full[s];
-        if (i >= S::kStages)
-          live = live && mbar_wait_bounded(kv ? &bars.v_empty[s] : &bars.k_empty[s], (i / S::kStages - 1) & 1,
-                                           p.status, kStatusMmaTimeout);
-        live = __all_sync(0xffffffffu, live);
-        if (!live) break;
-        if (lane == 0) mbar_arrive_expect_tx(full, (uint32_t)(panels * S::kPanel));
-        for (int g = 0; g < groups; g++) {
-          const int pg = __shfl_sync(0xffffffffu, page, g);
-          const int pos = begin + i * kKeys + g * box, slot = pos - entry_of(p, pos) * (int)p.a.cache.page_size;
-          if (lane == 0)
-            for (int c = 0; c < panels; c++)
-              tma_load_4d(kb + kv * S::kTileBytes + c * S::kPanel + g * box * 128, kv ? &maps.values : &maps.keys,
-                          64 * c, slot, w.head, pg, full);
-        }
+    auto load = [&](const CUtensorMap* map, char* dst, int panel, int j, int page, uint64_t* full) {
+      for (int g = 0; g < groups; g++) {
+        const int pg = __shfl_sync(0xffffffffu, page, (j & 1) * groups + g);
+        const int pos = begin + j * kHalf + g * box, slot = pos - entry_of(p, pos) * (int)p.a.cache.page_size;
+        if (lane == 0)
+          for (int c = 0; c < panels; c++)
+            tma_load_4d(dst + c * panel + g * box * 128, map, 64 * c, slot, w.head, pg, full);
       }
-      if (!live) break;
+    };
+    int ahead = look_up(0), page = 0;
+    bool live = true;
+    for (int i = 0; i <= tiles && live; i++) {  // the keys of tile i, then the values of tile i - 1
+      const int before = page;
+      page = ahead;
+      if (i < tiles) {
+        ahead = look_up(i + 1);
+        const int s = i % S::kKStages;
+        if (i >= S::kKStages)
+          live = __all_sync(0xffffffffu, mbar_wait_bounded(&bars.k_empty[s], (i / S::kKStages - 1) & 1, p.status,
+                                                           kStatusMmaTimeout));
+        if (!live) break;
+        const int parts = min(2, halves - 2 * i);
+        if (lane == 0) mbar_arrive_expect_tx(&bars.k_full[s], (uint32_t)(parts * panels * S::kVPanel));
+        for (int h = 0; h < parts; h++)
+          load(&maps.keys, smem + S::kK + s * S::kPanels * S::kKPanel + h * kHalf * 128, S::kKPanel, 2 * i + h, page,
+               &bars.k_full[s]);
+      }
+      for (int j = max(0, 2 * i - 2); j < min(2 * i, halves) && live; j++) {
+        const int s = j % S::kVStages;
+        if (j >= S::kVStages)
+          live = __all_sync(0xffffffffu, mbar_wait_bounded(&bars.v_empty[s], (j / S::kVStages - 1) & 1, p.status,
+                                                           kStatusMmaTimeout));
+        if (!live) break;
+        if (lane == 0) mbar_arrive_expect_tx(&bars.v_full[s], (uint32_t)(panels * S::kVPanel));
+        load(&maps.values, smem + S::kV + s * S::kPanels * S::kVPanel, S::kVPanel, j, before, &bars.v_full[s]);
+      }
     }
   } else {
     constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
     constexpr uint32_t kQk = idesc(kBf16, kKeys, false), kPv = idesc(kBf16, HDP, true);
+    // Operands' descriptors; the address field counts 16 bytes, so an offset adds.
     const uint32_t q = smem_u32(smem);
+    const uint64_t q_desc = desc(q, 16), k_desc = desc(q + S::kK, 16), v_desc = desc(q + S::kV, S::kVPanel);
     const int steps = (hd + 15) / 16;
-    auto pv = [&](int i) {
-      const int s = i % S::kStages;
-      if (!mbar_wait_bounded(&bars.p_full[i & 1], (i >> 1) & 1, p.status, kStatusMmaTimeout) ||
-          !mbar_wait_bounded(&bars.v_full[s], (i / S::kStages) & 1, p.status, kStatusTmaTimeout))
+    auto pv = [&](int j) {
+      const int s = j % S::kVStages, group = j / 2 % S::kGroups;
+      if (!mbar_wait_bounded(&bars.p_full[j % kHalves], (j / kHalves) & 1, p.status, kStatusMmaTimeout) ||
+          !mbar_wait_bounded(&bars.v_full[s], (j / S::kVStages) & 1, p.status, kStatusTmaTimeout))
         return false;
       fence_after();
-      if (skip[i & 1] == 0) {
-        const uint32_t v = q + S::kQ + s * 2 * S::kTileBytes + S::kTileBytes;
-        for (int k = 0; k < kKeys / 16; k++)
-          mma_ts(tmem + 2 * kKeys, tmem + (uint32_t)(i & 1) * kKeys + 8 * k, desc(v + k * 2048, S::kPanel), kPv,
-                 i > 0 || k > 0 ? 1u : 0u);
+      if (skip[j % kHalves] == 0) {
+        const uint64_t v = v_desc + (uint32_t)(s * S::kPanels * S::kVPanel >> 4);
+        const uint32_t out = tmem + kScores * kKeys + (uint32_t)(group * HDP);
+        const uint32_t pr = tmem + (uint32_t)(j % kHalves) * kHalf;
+#pragma unroll
+        for (int k = 0; k < kHalf / 16; k++)
+          mma_ts(out, pr + 8 * k, v + (uint32_t)(k * 2048 >> 4), kPv, k > 0 || j >= 2 * S::kGroups || j % 2 ? 1u : 0u);
       }
-      commit(&bars.o_done[i & 1]);
+      commit(&bars.o_done[j % kHalves]);
       commit(&bars.v_empty[s]);
       return true;
     };
     if (elect_one()) {
-      for (int i = 0; i < tiles; i++) {
-        const int s = i % S::kStages;
-        // S's buffer is free once the P V of two tiles ago has read P there.
-        if (i >= 2 && !mbar_wait_bounded(&bars.o_done[i & 1], ((i - 2) >> 1) & 1, p.status, kStatusMmaTimeout)) break;
-        if (!mbar_wait_bounded(&bars.k_full[s], (i / S::kStages) & 1, p.status, kStatusTmaTimeout)) break;
-        fence_after();
-        const uint32_t k = q + S::kQ + s * 2 * S::kTileBytes;
-        for (int c = 0; c < steps; c++)
-          mma_ss(tmem + (uint32_t)(i & 1) * kKeys, desc(q + c / 4 * S::kQPanel + c % 4 * 32, 16),
-                 desc(k + c / 4 * S::kPanel + c % 4 * 32, 16), kQk, c > 0 ? 1u : 0u);
-        commit(&bars.s_full[i & 1]);
-        commit(&bars.k_empty[s]);
-        if (i > 0 && !pv(i - 1)) break;
-        if (i == tiles - 1) pv(i);
+      bool live = true;
+      for (int i = 0; i <= tiles && live; i++) {
+        if (i < tiles) {
+          const int s = i % S::kKStages, free = 2 * i - 3;
+          // S's place is free once P V of the tile before the last has read P there.
+          if (free > 0)
+            live = mbar_wait_bounded(&bars.o_done[free % kHalves], (free / kHalves) & 1, p.status, kStatusMmaTimeout);
+          live = live && mbar_wait_bounded(&bars.k_full[s], (i / S::kKStages) & 1, p.status, kStatusTmaTimeout);
+          if (!live) break;
+          fence_after();
+          const uint64_t k = k_desc + (uint32_t)(s * S::kPanels * S::kKPanel >> 4);
+          const uint32_t out = tmem + (uint32_t)(i % kScores) * kKeys;
+#pragma unroll
+          for (int c = 0; c < HDP / 16; c++)
+            if (c < steps)
+              mma_ss(out, q_desc + (uint32_t)((c / 4 * S::kQPanel + c % 4 * 32) >> 4),
+                     k + (uint32_t)((c / 4 * S::kKPanel + c % 4 * 32) >> 4), kQk, c > 0 ? 1u : 0u);
+          commit(&bars.s_full[i % kScores]);
+          commit(&bars.k_empty[s]);
+        }
+        for (int j = max(0, 2 * i - 2); j < min(2 * i, halves) && live; j++) live = pv(j);
       }
     }
     __syncwarp();
   }
   fence_before();
   __syncthreads();
-  if (warp == 5) {
+  if (warp == kRowWarps + 1) {
     fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::kCols) : "memory");
   }
@@ -472,11 +534,8 @@ cudaError_t launch_size(const Params& p, cudaStream_t stream, bool pdl) {
         encode_tmap_pages(&maps.values, c.values, c.type == kBF16, c.hd, c.page_size, c.kv_heads, c.pages,
                           c.page_stride, box)))
     return cudaErrorInvalidValue;
-  if (cudaError_t e = cudaFuncSetAttribute(attention_wide_kernel<T, HDP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                           Shape<HDP>::kSmem);
-      e != cudaSuccess)
-    return e;
-  return launch_ex(attention_wide_kernel<T, HDP>, attention_grid(p), kThreads, Shape<HDP>::kSmem, stream, pdl, p, maps,
+  if (cudaError_t e = allow_smem(attention_wide_kernel<T, HDP>, Shape<HDP>::kSmem); e != cudaSuccess) return e;
+  return launch_ex(attention_wide_kernel<T, HDP>, attention_grid(p), Shape<HDP>::kThreads, Shape<HDP>::kSmem, stream, pdl, p, maps,
                    box);
 }
 
