@@ -62,6 +62,15 @@ __device__ __forceinline__ int seq_start(const Params& p, int s) {
   return v < 0 ? 0 : v > (int)p.a.n ? (int)p.a.n : v;
 }
 
+// A bounded wait that first spins without the clock, whose reading takes
+// longer than most waits here.
+__device__ __forceinline__ bool wait_phase(uint64_t* bar, uint32_t parity, uint32_t* status, uint32_t bits) {
+#pragma unroll 1
+  for (int i = 0; i < 64; i++)
+    if (mbar_try_wait(bar, parity)) return true;
+  return mbar_wait_bounded(bar, parity, status, bits);
+}
+
 // The sequence that token t belongs to, or -1. A batch of one token a
 // sequence is recognized in one round of loads.
 __device__ __forceinline__ int seq_of(const Params& p, int t) {
@@ -84,9 +93,17 @@ __device__ __forceinline__ void sees(const Params& p, const Work& w, int t, int&
   low = 0;
   high = -1;
   if (w.prefix) {
-    const int s = seq_of(p, t);
-    if (s < 0) return;
-    high = p.a.lengths[s] - (seq_start(p, s + 1) - t);
+    // One token a sequence: one round of loads.
+    const int seqs = (int)p.a.cache.sequences, near = min(t, seqs - 1);
+    if (near < 0) return;
+    const int start = seq_start(p, near), end = seq_start(p, near + 1), length = p.a.lengths[near];
+    if (near == t && start == t && end == t + 1) {
+      high = length - 1;
+    } else {
+      const int s = seq_of(p, t);
+      if (s < 0) return;
+      high = p.a.lengths[s] - (seq_start(p, s + 1) - t);
+    }
   } else {
     high = w.length - (w.seq_end - t);
   }
@@ -139,10 +156,12 @@ __device__ __forceinline__ bool find_work(const Params& p, Work& w) {
   const int lane = threadIdx.x % 32;
   int lo = 0, hi = seqs;  // the answer lies in lo .. hi - 1
   const int guess = (int)((int64_t)slot * p.own_rows / (p.own_rows + p.group)) - 16;
-  int at = max(0, min(guess, seqs - 32)), step = 1;
+  int at = max(0, min(guess, seqs - 32)), step = 1, start, ahead, length;
   for (;;) {
     const int s = at + lane * step;
-    const bool under = s < hi && first_slot(p, seq_start(p, s), s) <= slot;
+    start = s < seqs ? seq_start(p, s) : -1;
+    length = s < seqs ? p.a.lengths[s] : 0;
+    const bool under = s < hi && first_slot(p, start, s) <= slot;
     const unsigned votes = __ballot_sync(0xffffffffu, under);
     const int count = __popc(votes);  // monotone: lanes 0 .. count - 1
     if (count > 0) lo = max(lo, at + (count - 1) * step);
@@ -152,9 +171,20 @@ __device__ __forceinline__ bool find_work(const Params& p, Work& w) {
     at = lo;
   }
   w.seq = lo;
-  const int start = seq_start(p, lo);
-  w.seq_end = seq_start(p, lo + 1);
-  w.length = p.a.lengths[lo];
+  // Its start, its end and its length: in a lane as a rule, else loaded.
+  const int from = (lo - at) / step;
+  if (step == 1 && from >= 0 && from < 31) {
+    ahead = __shfl_sync(0xffffffffu, start, from + 1);
+    start = __shfl_sync(0xffffffffu, start, from);
+    length = __shfl_sync(0xffffffffu, length, from);
+    if (ahead < 0) ahead = seq_start(p, lo + 1);
+  } else {
+    start = seq_start(p, lo);
+    ahead = seq_start(p, lo + 1);
+    length = p.a.lengths[lo];
+  }
+  w.seq_end = ahead;
+  w.length = length;
   const int tile = slot - first_slot(p, start, lo);
   w.row0 = start * p.group + tile * p.own_rows;
   w.rows = min(p.own_rows, w.seq_end * p.group - w.row0);

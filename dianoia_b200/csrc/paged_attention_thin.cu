@@ -149,12 +149,12 @@ __device__ __forceinline__ void thin_block(const Params& p, const Maps& maps, co
       const int page = at >= 0 ? (int)at : (int)p.a.cache.pages;
       const int slot = k0 - entry_of(p, k0) * (int)p.a.cache.page_size;
       there[b] = at >= 0 ? 0xffffu : 0u;
-      if (lane == 0) {
-        mbar_arrive_expect_tx(&full[b], (uint32_t)panels * 2 * S::kPanel);
-        for (int i = 0; i < panels; i++) {
-          tma_load_4d(kb + i * S::kPanel, &maps.keys, 64 * i, slot, w.head, page, &full[b]);
-          tma_load_4d(vb + i * S::kPanel, &maps.values, 64 * i, slot, w.head, page, &full[b]);
-        }
+      if (lane == 0) mbar_arrive_expect_tx(&full[b], (uint32_t)panels * 2 * S::kPanel);
+      __syncwarp();
+      if (lane < 2 * panels) {  // a copy a lane: the panels of the keys, then of the values
+        const int c = lane < panels ? lane : lane - panels;
+        tma_load_4d((lane < panels ? kb : vb) + c * S::kPanel, lane < panels ? &maps.keys : &maps.values, 64 * c, slot,
+                    w.head, page, &full[b]);
       }
     } else {
       there[b] = __ballot_sync(0xffffffffu, at >= 0) & 0xffffu;
@@ -215,7 +215,7 @@ __device__ __forceinline__ void thin_block(const Params& p, const Maps& maps, co
     for (int b = 0; b < S::kStages; b++) {
       const int step = base + b;
       if (step >= steps) break;
-      live = __all_sync(0xffffffffu, mbar_wait_bounded(&full[b], (step / S::kStages) & 1, p.status, kStatusTmaTimeout));
+      live = __all_sync(0xffffffffu, wait_phase(&full[b], (step / S::kStages) & 1, p.status, kStatusTmaTimeout));
       if (!live) break;
       issue(step + S::kStages - 1, (b + S::kStages - 1) % S::kStages);
       const char* buf = ring + b * 2 * S::kBuf;

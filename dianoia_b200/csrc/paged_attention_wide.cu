@@ -5,15 +5,15 @@
 // S = Q K^T and O += P V on the 5th-generation tensor cores (tcgen05, f32
 // accumulators in TMEM). A block runs three parts at once:
 //   one warp brings tiles of 128 keys and their values by tiled TMA copies;
-//   one warp issues the products;
+//   a warp for each group issues its products;
 //   two groups of 4 warps (one for heads over 128 wide) take the even and the
 //   odd tiles, a row of S each thread: they read it from TMEM 64 keys (a half)
 //   at a time, keep the row's base and sum, and write P (16-bit) over it, which
 //   the tensor cores read from there as the first operand of P V. Each group
 //   has an O of its own, so the groups never wait for one another; the join
 //   adds them.
-// Two tiles of S stand in TMEM: while one group is in softmax the tensor cores
-// serve the other. (With 64-key tiles S took M = 128, N = 64 products, which
+// A group's S, P and O follow one another; while one group is in softmax the
+// tensor cores serve the other. (With 64-key tiles S took M = 128, N = 64 products, which
 // run at half the rate: 73000 cycles for 2752 keys, the tensor cores the
 // bound.) A base moves only when a score passes it by kSlack (P then stays
 // below 2^8), so O is rescaled in TMEM in the first tiles and hardly ever
@@ -51,8 +51,8 @@ struct Shape {
   static constexpr int kKPanel = kKeys * 128;  // of every key of a tile
   static constexpr int kVPanel = kHalf * 128;  // of every value of a half
   static constexpr int kGroups = wide_groups(HDP);
-  static constexpr int kThreads = kGroups * kRowThreads + 64;
-  static constexpr int kKStages = HDP <= 128 ? 2 : 1, kVStages = HDP <= 128 ? 3 : 2;
+  static constexpr int kThreads = kGroups * (kRowThreads + kLanes) + kLanes;
+  static constexpr int kKStages = HDP <= 128 ? 2 : 1, kVStages = HDP <= 128 ? 4 : 2;
   static constexpr int kK = kPanels * kQPanel;              // where the keys start
   static constexpr int kV = kK + kKStages * kPanels * kKPanel;
   static constexpr int kSmem = kV + kVStages * kPanels * kVPanel;
@@ -62,11 +62,11 @@ struct Shape {
 
 // Tile i has barriers i % kScores, half j = 2 i, 2 i + 1 of it j % kHalves
 // (o_done: its P V is done). A thread may pass over phases, and a parity tells
-// two phases in a row apart, not three: S of tile i is there only once P V of
-// half 2 i - 3 is done, so whoever waits for a half of tile i or i - 1 knows
+// two phases in a row apart, not three: S of a group's tile is there only once
+// P V of its tile before is done, so whoever waits for a half of either knows
 // the phase before it past.
 struct Bars {
-  uint64_t k_full[2], k_empty[2], v_full[3], v_empty[3], s_full[kScores], p_full[kHalves], o_done[kHalves];
+  uint64_t k_full[2], k_empty[2], v_full[4], v_empty[4], s_full[kScores], p_full[kHalves], o_done[kHalves];
 };
 
 // Shared-memory operand, 128-byte swizzled; `lead` is the stride between
@@ -157,14 +157,14 @@ __device__ __forceinline__ void softmax_rows(const Params& p, const Work& w, cha
   bool next_there = look_up(group);
   bool live = true;
   auto done = [&](int j) {
-    return __all_sync(0xffffffffu, mbar_wait_bounded(&bars.o_done[j % kHalves], (j / kHalves) & 1, p.status,
+    return __all_sync(0xffffffffu, wait_phase(&bars.o_done[j % kHalves], (j / kHalves) & 1, p.status,
                                                      kStatusMmaTimeout));
   };
   int last = -1;  // the group's last half
   for (int i = group; i < tiles && live; i += S::kGroups) {
     const unsigned tile_there = __ballot_sync(0xffffffffu, next_there);
     next_there = look_up(i + S::kGroups);
-    live = __all_sync(0xffffffffu, mbar_wait_bounded(&bars.s_full[i % kScores], (i / kScores) & 1, p.status,
+    live = __all_sync(0xffffffffu, wait_phase(&bars.s_full[i % kScores], (i / kScores) & 1, p.status,
                                                      kStatusMmaTimeout));
     if (!live) break;
     fence_after();
@@ -235,7 +235,7 @@ __device__ __forceinline__ void softmax_rows(const Params& p, const Work& w, cha
       if (!all) {
         // The values have to be looked at, and may have to be added here.
         char* vals = smem + S::kV + j % S::kVStages * S::kPanels * S::kVPanel;
-        live = __all_sync(0xffffffffu, mbar_wait_bounded(&bars.v_full[j % S::kVStages], (j / S::kVStages) & 1,
+        live = __all_sync(0xffffffffu, wait_phase(&bars.v_full[j % S::kVStages], (j / S::kVStages) & 1,
                                                          p.status, kStatusTmaTimeout));
         if (!live) break;
         bool bad = false;
@@ -328,7 +328,7 @@ __device__ __forceinline__ void softmax_rows(const Params& p, const Work& w, cha
 }
 
 template <typename T, int HDP>
-__global__ void __maxnreg__(152)
+__global__ void __maxnreg__(136)
     attention_wide_kernel(const __grid_constant__ Params p, const __grid_constant__ Maps maps, int box) {
   using S = Shape<HDP>;
   pdl_wait();
@@ -420,49 +420,49 @@ __global__ void __maxnreg__(152)
   if (warp < kRowWarps) {
     softmax_rows<T, HDP>(p, w, smem, bars, skip, tmem, begin, halves, tid / kRowThreads, low, high, all_low, all_high);
   } else if (warp == kRowWarps) {
-    const int panels = (hd + 63) / 64, groups = kHalf / box;  // groups of keys of one page in a half
-    // Lane g knows the page of group g of the tile; one past the last page
-    // reads as zeros.
+    // One copy a lane: panel c of the keys (values) g * box .. of the tile, all
+    // of one page. (One lane issuing them all took 300 cycles a copy.)
+    const int panels = (hd + 63) / 64, groups = kHalf / box;  // of a half
+    const int g = lane / S::kPanels, c = lane % S::kPanels;
+    const bool mine = g < 2 * groups && c < panels;
+    const uint32_t row0 = (uint32_t)(g % groups * box * 128);
+    // The page of the lane's keys; one past the last reads as zeros.
     auto look_up = [&](int tile) {
-      int page = -1;
-      if (lane < 2 * groups && tile < tiles) page = page_of(p, w, begin + tile * kKeys + lane * box);
+      const int page = mine && tile < tiles ? page_of(p, w, begin + tile * kKeys + g * box) : -1;
       return page >= 0 ? page : (int)p.a.cache.pages;
     };
-    auto load = [&](const CUtensorMap* map, char* dst, int panel, int j, int page, uint64_t* full) {
-      for (int g = 0; g < groups; g++) {
-        const int pg = __shfl_sync(0xffffffffu, page, (j & 1) * groups + g);
-        const int pos = begin + j * kHalf + g * box, slot = pos - entry_of(p, pos) * (int)p.a.cache.page_size;
-        if (lane == 0)
-          for (int c = 0; c < panels; c++)
-            tma_load_4d(dst + c * panel + g * box * 128, map, 64 * c, slot, w.head, pg, full);
-      }
-    };
-    int ahead = look_up(0), page = 0;
+    int ahead = look_up(0), page = 0, slot = 0;
     bool live = true;
     for (int i = 0; i <= tiles && live; i++) {  // the keys of tile i, then the values of tile i - 1
-      const int before = page;
+      const int page_v = page, slot_v = slot;
       page = ahead;
       if (i < tiles) {
+        const int pos = begin + i * kKeys + g * box;
+        slot = pos - entry_of(p, pos) * (int)p.a.cache.page_size;
         ahead = look_up(i + 1);
-        const int s = i % S::kKStages;
+        const int s = i % S::kKStages, parts = min(2, halves - 2 * i);
         if (i >= S::kKStages)
-          live = __all_sync(0xffffffffu, mbar_wait_bounded(&bars.k_empty[s], (i / S::kKStages - 1) & 1, p.status,
-                                                           kStatusMmaTimeout));
+          live = __all_sync(0xffffffffu, wait_phase(&bars.k_empty[s], (i / S::kKStages - 1) & 1, p.status,
+                                                    kStatusMmaTimeout));
         if (!live) break;
-        const int parts = min(2, halves - 2 * i);
         if (lane == 0) mbar_arrive_expect_tx(&bars.k_full[s], (uint32_t)(parts * panels * S::kVPanel));
-        for (int h = 0; h < parts; h++)
-          load(&maps.keys, smem + S::kK + s * S::kPanels * S::kKPanel + h * kHalf * 128, S::kKPanel, 2 * i + h, page,
-               &bars.k_full[s]);
+        __syncwarp();
+        if (mine && g < parts * groups)
+          tma_load_4d(smem + S::kK + s * S::kPanels * S::kKPanel + c * S::kKPanel + g / groups * kHalf * 128 + row0,
+                      &maps.keys, 64 * c, slot, w.head, page, &bars.k_full[s]);
       }
-      for (int j = max(0, 2 * i - 2); j < min(2 * i, halves) && live; j++) {
-        const int s = j % S::kVStages;
+      for (int h = 0; h < 2 && i > 0; h++) {
+        const int j = 2 * i - 2 + h, s = j % S::kVStages;
+        if (j >= halves) break;
         if (j >= S::kVStages)
-          live = __all_sync(0xffffffffu, mbar_wait_bounded(&bars.v_empty[s], (j / S::kVStages - 1) & 1, p.status,
-                                                           kStatusMmaTimeout));
+          live = __all_sync(0xffffffffu, wait_phase(&bars.v_empty[s], (j / S::kVStages - 1) & 1, p.status,
+                                                    kStatusMmaTimeout));
         if (!live) break;
         if (lane == 0) mbar_arrive_expect_tx(&bars.v_full[s], (uint32_t)(panels * S::kVPanel));
-        load(&maps.values, smem + S::kV + s * S::kPanels * S::kVPanel, S::kVPanel, j, before, &bars.v_full[s]);
+        __syncwarp();
+        if (mine && g / groups == h)
+          tma_load_4d(smem + S::kV + s * S::kPanels * S::kVPanel + c * S::kVPanel + row0, &maps.values, 64 * c, slot_v,
+                      w.head, page_v, &bars.v_full[s]);
       }
     }
   } else {
@@ -472,46 +472,43 @@ __global__ void __maxnreg__(152)
     const uint32_t q = smem_u32(smem);
     const uint64_t q_desc = desc(q, 16), k_desc = desc(q + S::kK, 16), v_desc = desc(q + S::kV, S::kVPanel);
     const int steps = (hd + 15) / 16;
-    auto pv = [&](int j) {
-      const int s = j % S::kVStages, group = j / 2 % S::kGroups;
-      if (!mbar_wait_bounded(&bars.p_full[j % kHalves], (j / kHalves) & 1, p.status, kStatusMmaTimeout) ||
-          !mbar_wait_bounded(&bars.v_full[s], (j / S::kVStages) & 1, p.status, kStatusTmaTimeout))
-        return false;
-      fence_after();
-      if (skip[j % kHalves] == 0) {
-        const uint64_t v = v_desc + (uint32_t)(s * S::kPanels * S::kVPanel >> 4);
-        const uint32_t out = tmem + kScores * kKeys + (uint32_t)(group * HDP);
-        const uint32_t pr = tmem + (uint32_t)(j % kHalves) * kHalf;
-#pragma unroll
-        for (int k = 0; k < kHalf / 16; k++)
-          mma_ts(out, pr + 8 * k, v + (uint32_t)(k * 2048 >> 4), kPv, k > 0 || j >= 2 * S::kGroups || j % 2 ? 1u : 0u);
-      }
-      commit(&bars.o_done[j % kHalves]);
-      commit(&bars.v_empty[s]);
-      return true;
-    };
+    const int group = warp - kRowWarps - 1;
+    const uint32_t out = tmem + kScores * kKeys + (uint32_t)(group * HDP);
     if (elect_one()) {
       bool live = true;
-      for (int i = 0; i <= tiles && live; i++) {
-        if (i < tiles) {
-          const int s = i % S::kKStages, free = 2 * i - 3;
-          // S's place is free once P V of the tile before the last has read P there.
-          if (free > 0)
-            live = mbar_wait_bounded(&bars.o_done[free % kHalves], (free / kHalves) & 1, p.status, kStatusMmaTimeout);
-          live = live && mbar_wait_bounded(&bars.k_full[s], (i / S::kKStages) & 1, p.status, kStatusTmaTimeout);
+      int last = -1;  // the group's last half
+      for (int i = group; i < tiles && live; i += S::kGroups) {
+        const int s = i % S::kKStages;
+        // S's place is free once P V of the group's last tile has read P there.
+        if (last >= 0) live = wait_phase(&bars.o_done[last % kHalves], (last / kHalves) & 1, p.status, kStatusMmaTimeout);
+        live = live && wait_phase(&bars.k_full[s], (i / S::kKStages) & 1, p.status, kStatusTmaTimeout);
+        if (!live) break;
+        fence_after();
+        const uint64_t k = k_desc + (uint32_t)(s * S::kPanels * S::kKPanel >> 4);
+#pragma unroll
+        for (int c = 0; c < HDP / 16; c++)
+          if (c < steps)
+            mma_ss(tmem + (uint32_t)(i % kScores) * kKeys, q_desc + (uint32_t)((c / 4 * S::kQPanel + c % 4 * 32) >> 4),
+                   k + (uint32_t)((c / 4 * S::kKPanel + c % 4 * 32) >> 4), kQk, c > 0 ? 1u : 0u);
+        commit(&bars.s_full[i % kScores]);
+        commit(&bars.k_empty[s]);
+        for (int j = 2 * i; j < min(2 * i + 2, halves); j++) {
+          const int vs = j % S::kVStages;
+          live = wait_phase(&bars.v_full[vs], (j / S::kVStages) & 1, p.status, kStatusTmaTimeout) &&
+                 wait_phase(&bars.p_full[j % kHalves], (j / kHalves) & 1, p.status, kStatusMmaTimeout);
           if (!live) break;
           fence_after();
-          const uint64_t k = k_desc + (uint32_t)(s * S::kPanels * S::kKPanel >> 4);
-          const uint32_t out = tmem + (uint32_t)(i % kScores) * kKeys;
+          if (skip[j % kHalves] == 0) {
+            const uint64_t v = v_desc + (uint32_t)(vs * S::kPanels * S::kVPanel >> 4);
+            const uint32_t pr = tmem + (uint32_t)(j % kHalves) * kHalf;
 #pragma unroll
-          for (int c = 0; c < HDP / 16; c++)
-            if (c < steps)
-              mma_ss(out, q_desc + (uint32_t)((c / 4 * S::kQPanel + c % 4 * 32) >> 4),
-                     k + (uint32_t)((c / 4 * S::kKPanel + c % 4 * 32) >> 4), kQk, c > 0 ? 1u : 0u);
-          commit(&bars.s_full[i % kScores]);
-          commit(&bars.k_empty[s]);
+            for (int c = 0; c < kHalf / 16; c++)
+              mma_ts(out, pr + 8 * c, v + (uint32_t)(c * 2048 >> 4), kPv, c > 0 || last >= 0 ? 1u : 0u);
+          }
+          commit(&bars.o_done[j % kHalves]);
+          commit(&bars.v_empty[vs]);
+          last = j;
         }
-        for (int j = max(0, 2 * i - 2); j < min(2 * i, halves) && live; j++) live = pv(j);
       }
     }
     __syncwarp();
