@@ -12,191 +12,166 @@ namespace {
 
 // ------------------------------------------------------- the f32 arithmetic
 //
-// Any type, head size up to 256 and alignment. A block of 4 warps takes 16
-// rows; each tile of 32 keys is brought to shared memory as f32 for all of
-// them. Warp w owns rows 4 w .. 4 w + 3: lane j scores key j for each (f32
-// FMAs along the head), the tile's maximum and sum are warp reductions, and
-// for the values lane j owns dimensions 4 j .. 4 j + 3 (and 128 more on).
+// Any type, head size up to 256 and alignment; f32 caches first of all, whose
+// products the tensor cores would round. Bound by the keys' bytes for the few
+// rows of a decode step, so nothing goes through shared memory: a warp's lanes
+// lie along the head (V dimensions each, 32 V more on), and a step of 32 / RT
+// keys is 32 / RT whole rows loaded at once for RT rows of queries. The 32
+// partial products of a lane are summed over the lanes by halves (31
+// exchanges for 32 sums), which leaves lane l with the score of key l / RT for
+// row l % RT; each probability goes back to all lanes for the values. A block's
+// 4 warps take steps in turn and are joined once at the end.
 constexpr int kSimtThreads = 128;
-constexpr int kSimtKeys = 32;
-constexpr int kWarpRows = 4;
+constexpr int kSimtWarps = kSimtThreads / kLanes;
+constexpr float kSlack = 8.0f;  // log2 units a score may pass the running base
 
-// Floats of a row of keys, values or queries in shared memory: 16-byte
-// aligned, and eight rows apart by 16 bytes of banks.
-__host__ __device__ constexpr int simt_pitch(int hd) { return (hd + 31) / 32 * 32 + 4; }
-
-template <typename T, int V>
+template <typename T, int V, int NU, int RT>
 __global__ void __launch_bounds__(kSimtThreads) attention_simt_kernel(const __grid_constant__ Params p) {
   pdl_launch_dependents();
   pdl_wait();
-  extern __shared__ float smem[];
-  const int hd = (int)p.a.cache.hd, pitch = simt_pitch(hd);
-  float* qs = smem;                            // [kSimtRows][pitch]
-  float* ks = qs + kSimtRows * pitch;          // [kSimtKeys][pitch]
-  float* vs = ks + kSimtKeys * pitch;          // [kSimtKeys][pitch]
-  float* ps = vs + kSimtKeys * pitch;          // [4 warps][kSimtKeys][kWarpRows]
-  __shared__ int row_low[kSimtRows], row_high[kSimtRows], span[2];
-  __shared__ int key_page[kSimtKeys];
+  constexpr int kStep = kLanes / RT;  // keys
+  constexpr int kTile = kSimtWarps * kStep;
+  constexpr int kWidth = kLanes * V * NU;
+  __shared__ float os[kSimtWarps][RT][kWidth];
+  __shared__ float2 ml[kSimtWarps][RT];
   Work w;
   if (!find_work(p, w)) return;
-  const int tid = threadIdx.x, warp = tid / kLanes, lane = tid % kLanes;
-  if (tid < kSimtRows) {
-    int low = 0, high = -1;
-    if (tid < w.rows) {
-      const int t = (w.row0 + tid) / p.group;
-      sees(p, w, t, low, high);
-    }
-    row_low[tid] = low;
-    row_high[tid] = high;
-    const bool any = high >= low;
-    const int lo = __reduce_min_sync(0xffffu, any ? low : INT32_MAX);
-    const int hi = __reduce_max_sync(0xffffu, any ? high : -1);
-    if (tid == 0) {
-      span[0] = lo;
-      span[1] = hi;
-    }
-  }
-  for (int i = tid; i < kSimtRows * pitch; i += kSimtThreads) {
-    const int r = i / pitch, d = i % pitch;
-    float x = 0.0f;
-    if (r < w.rows && d < hd) {
-      int t, head;
-      out_index(p, w, r, t, head);
-      x = to_f32<T>(static_cast<const T*>(p.a.q)[t * p.a.q_stride + (int64_t)head * hd + d]);
-    }
-    qs[i] = x;
-  }
-  __syncthreads();
+  const int warp = threadIdx.x / kLanes, lane = threadIdx.x % kLanes;
+  const int hd = (int)p.a.cache.hd;
+  // What each row sees (lane l: row l % RT).
+  const int my_row = lane % RT;
+  int low = 0, high = -1;
+  if (my_row < w.rows) sees(p, w, (w.row0 + my_row) / p.group, low, high);
+  const bool any = high >= low;
+  const int all_low = __reduce_max_sync(0xffffffffu, any ? low : 0);
+  const int all_high = __reduce_min_sync(0xffffffffu, any ? high : INT32_MAX);
+  const int any_low = __reduce_min_sync(0xffffffffu, any ? low : INT32_MAX);
+  const int any_high = __reduce_max_sync(0xffffffffu, any ? high : -1);
   int begin, end;
-  slice_keys(p, w, span[0], span[1], kSimtKeys, begin, end);
+  slice_keys(p, w, any_low, any_high, kTile, begin, end);
 
-  float m[kWarpRows], l[kWarpRows], acc[kWarpRows][2][4];
+  float q[RT][NU][V], acc[RT][NU][V], m = -INFINITY, l = 0.0f;  // m, l: of row my_row, this lane's keys
 #pragma unroll
-  for (int r = 0; r < kWarpRows; r++) {
-    m[r] = -INFINITY;
-    l[r] = 0.0f;
+  for (int r = 0; r < RT; r++) {
+    int t, head;
+    out_index(p, w, r < w.rows ? r : 0, t, head);
+    const T* src = static_cast<const T*>(p.a.q) + t * p.a.q_stride + (int64_t)head * hd;
 #pragma unroll
-    for (int u = 0; u < 2; u++)
-#pragma unroll
-      for (int e = 0; e < 4; e++) acc[r][u][e] = 0.0f;
-  }
-  const int row_base = warp * kWarpRows;
-  int low[kWarpRows], high[kWarpRows];
-#pragma unroll
-  for (int r = 0; r < kWarpRows; r++) {
-    low[r] = row_low[row_base + r];
-    high[r] = row_high[row_base + r];
-  }
-  for (int k0 = begin; k0 < end; k0 += kSimtKeys) {
-    __syncthreads();  // the last tile is read
-    if (tid < kSimtKeys) key_page[tid] = k0 + tid < end ? page_of(p, w, k0 + tid) : -1;
-    __syncthreads();
-    const int runs = pitch / V;
-    for (int i = tid; i < kSimtKeys * runs; i += kSimtThreads) {
-      const int j = i / runs, d = i % runs * V;
-      float x[V] = {}, y[V] = {};
-      if (key_page[j] >= 0 && d < hd) {
-        const int slot = (k0 + j) % (int)p.a.cache.page_size;
-        const int64_t at = key_page[j] * p.a.cache.page_stride +
-                           ((int64_t)w.head * p.a.cache.page_size + slot) * hd + d;
-        load_run<T, V>(static_cast<const T*>(p.a.cache.keys) + at, x);
-        load_run<T, V>(static_cast<const T*>(p.a.cache.values) + at, y);
-      }
+    for (int u = 0; u < NU; u++)
 #pragma unroll
       for (int e = 0; e < V; e++) {
-        ks[j * pitch + d + e] = x[e];
-        vs[j * pitch + d + e] = y[e];
+        const int d = (u * kLanes + lane) * V + e;
+        q[r][u][e] = r < w.rows && d < hd ? to_f32<T>(src[d]) : 0.0f;
+        acc[r][u][e] = 0.0f;
+      }
+  }
+  const T* keys = static_cast<const T*>(p.a.cache.keys);
+  const T* vals = static_cast<const T*>(p.a.cache.values);
+  for (int k0 = begin + warp * kStep; k0 < end; k0 += kTile) {
+    // Lane k looks key k0 + k up.
+    const int64_t mine = lane < kStep ? row_at(p, w, k0 + lane, any_low, end) : -1;
+    const unsigned there = __ballot_sync(0xffffffffu, mine >= 0);
+    float s[kLanes];
+#pragma unroll
+    for (int i = 0; i < kLanes; i++) s[i] = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kStep; k++) {
+      const int64_t at = __shfl_sync(0xffffffffu, mine, k);
+#pragma unroll
+      for (int u = 0; u < NU; u++) {
+        const int d = (u * kLanes + lane) * V;
+        float x[V] = {};
+        if (at >= 0 && d < hd) load_run<T, V>(keys + at + d, x);
+#pragma unroll
+        for (int r = 0; r < RT; r++)
+#pragma unroll
+          for (int e = 0; e < V; e++) s[k * RT + r] = fmaf(q[r][u][e], x[e], s[k * RT + r]);
       }
     }
-    __syncthreads();
-    // Scores of key `lane` for the warp's rows.
-    float s[kWarpRows] = {};
-    const float4* kv = reinterpret_cast<const float4*>(ks + lane * pitch);
-    for (int d = 0; d < (hd + 3) / 4; d++) {
-      const float4 k = kv[d];
 #pragma unroll
-      for (int r = 0; r < kWarpRows; r++) {
-        const float4 q = reinterpret_cast<const float4*>(qs + (row_base + r) * pitch)[d];
-        s[r] = fmaf(q.x, k.x, s[r]);
-        s[r] = fmaf(q.y, k.y, s[r]);
-        s[r] = fmaf(q.z, k.z, s[r]);
-        s[r] = fmaf(q.w, k.w, s[r]);
+    for (int half = kLanes / 2; half >= 1; half >>= 1) {
+      const bool upper = (lane & half) != 0;
+#pragma unroll
+      for (int i = 0; i < half; i++) {
+        const float keep = upper ? s[i + half] : s[i], give = upper ? s[i] : s[i + half];
+        s[i] = keep + __shfl_xor_sync(0xffffffffu, give, half);
       }
     }
-    const bool there = key_page[lane] >= 0;
-    float pr[kWarpRows];
-    bool all = true;  // every row that sees a key of the tile sees all of it
-#pragma unroll
-    for (int r = 0; r < kWarpRows; r++) {
-      const bool seen = there && k0 + lane >= low[r] && k0 + lane <= high[r];
-      const float x = seen ? s[r] * p.scale_log2 : -INFINITY;
+    const int key = k0 + lane / RT;
+    const bool seen = (there >> (lane / RT) & 1u) != 0 && key >= low && key <= high;
+    const float x = seen ? s[0] * p.scale_log2 : -INFINITY;
+    if (__any_sync(0xffffffffu, x > m + kSlack)) {  // a new base: the row's maximum so far
       float top = x;
 #pragma unroll
-      for (int off = 16; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-      const float next = fmaxf(m[r], top);
-      const float base = next == -INFINITY ? 0.0f : next;
-      const float keep = exp2_fast(m[r] - base);
-      pr[r] = seen ? exp2_fast(x - base) : 0.0f;
-      m[r] = next;
-      l[r] = l[r] * keep + pr[r];  // a lane's share; summed over the lanes at the end
+      for (int off = RT; off < kLanes; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+      const float next = fmaxf(m, top), keep = next == -INFINITY ? 1.0f : exp2_fast(m - next);
+      m = next;
+      l *= keep;
 #pragma unroll
-      for (int u = 0; u < 2; u++)
+      for (int r = 0; r < RT; r++) {
+        const float f = __shfl_sync(0xffffffffu, keep, r);
 #pragma unroll
-        for (int e = 0; e < 4; e++) acc[r][u][e] *= keep;
-      all = all && (seen || high[r] < low[r]);  // (a row that sees nothing has only zeros to add)
-    }
-    float4* pw = reinterpret_cast<float4*>(ps) + warp * kSimtKeys;
-    pw[lane] = make_float4(pr[0], pr[1], pr[2], pr[3]);
-    __syncwarp();
-    const bool fast = __all_sync(0xffffffffu, all);
-    for (int j = 0; j < kSimtKeys; j++) {
-      const float4 q = pw[j];
-      const float pj[kWarpRows] = {q.x, q.y, q.z, q.w};
+        for (int u = 0; u < NU; u++)
 #pragma unroll
-      for (int u = 0; u < 2; u++) {
-        const int d = 4 * lane + 128 * u;
-        if (d >= hd) break;
-        const float4 v = *reinterpret_cast<const float4*>(vs + j * pitch + d);
-        const float ve[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int r = 0; r < kWarpRows; r++)
-#pragma unroll
-          for (int e = 0; e < 4; e++) {
-            // A key that a row does not see adds nothing, infinite or not.
-            if (fast || pj[r] != 0.0f) acc[r][u][e] = fmaf(pj[r], ve[e], acc[r][u][e]);
-          }
+          for (int e = 0; e < V; e++) acc[r][u][e] *= f;
       }
     }
-    __syncwarp();
+    const float pr = seen ? exp2_fast(x - (m == -INFINITY ? 0.0f : m)) : 0.0f;
+    l += pr;
+    const bool all = there == (kStep == 32 ? 0xffffffffu : (1u << kStep) - 1) && k0 >= all_low &&
+                     k0 + kStep - 1 <= all_high;
+#pragma unroll
+    for (int k = 0; k < kStep; k++) {
+      const int64_t at = __shfl_sync(0xffffffffu, mine, k);
+      float y[NU][V] = {};
+#pragma unroll
+      for (int u = 0; u < NU; u++) {
+        const int d = (u * kLanes + lane) * V;
+        if (at >= 0 && d < hd) load_run<T, V>(vals + at + d, y[u]);
+      }
+#pragma unroll
+      for (int r = 0; r < RT; r++) {
+        const float f = __shfl_sync(0xffffffffu, pr, k * RT + r);
+        if (!all && f == 0.0f) continue;  // a key that the row does not see adds nothing, infinite or not
+#pragma unroll
+        for (int u = 0; u < NU; u++)
+#pragma unroll
+          for (int e = 0; e < V; e++) acc[r][u][e] = fmaf(f, y[u][e], acc[r][u][e]);
+      }
+    }
   }
+  // Joined: the lanes' sums of a row, then the warps' results.
 #pragma unroll
-  for (int r = 0; r < kWarpRows; r++) {
-    float sum = l[r];
+  for (int off = RT; off < kLanes; off <<= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
+  if (high < low) l = 0.0f;
+  if (lane < RT) ml[warp][lane] = make_float2(m, l);
 #pragma unroll
-    for (int off = 16; off >= 1; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-    if (row_base + r >= w.rows) continue;
+  for (int r = 0; r < RT; r++)
+#pragma unroll
+    for (int u = 0; u < NU; u++) store_run<float, V>(&os[warp][r][(u * kLanes + lane) * V], acc[r][u]);
+  __syncthreads();
+  for (int i = threadIdx.x; i < w.rows * hd; i += kSimtThreads) {
+    const int r = i / hd, d = i % hd;
+    float top = -INFINITY, sum = 0.0f, o = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kSimtWarps; k++) top = fmaxf(top, ml[k][r].x);
+    const float base = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+    for (int k = 0; k < kSimtWarps; k++) {
+      const float2 part = ml[k][r];
+      if (part.y == 0.0f) continue;
+      const float f = exp2_fast(part.x - base);
+      sum += part.y * f;
+      o += os[k][r][d] * f;
+    }
     int t, head;
-    const int64_t row = out_index(p, w, row_base + r, t, head);
+    const int64_t row = out_index(p, w, r, t, head);
     if (p.direct) {
-      const float inv = sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum;  // NaN stays
-      T* out = static_cast<T*>(p.a.out) + t * p.a.out_stride + (int64_t)head * hd;
-#pragma unroll
-      for (int u = 0; u < 2; u++)
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-          const int d = 4 * lane + 128 * u + e;
-          if (d < hd) out[d] = from_f32<T>(sum == 0.0f ? 0.0f : acc[r][u][e] * inv);
-        }
+      static_cast<T*>(p.a.out)[t * p.a.out_stride + (int64_t)head * hd + d] = from_f32<T>(sum == 0.0f ? 0.0f : o / sum);
     } else {
-      const int64_t at = slice_index(p, w) * (p.a.n * p.a.heads) + row;
-      if (lane == 0) p.ml[at] = make_float2(m[r], sum);
-#pragma unroll
-      for (int u = 0; u < 2; u++)
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-          const int d = 4 * lane + 128 * u + e;
-          if (d < hd) p.acc[at * hd + d] = acc[r][u][e];
-        }
+      const int64_t to = slice_index(p, w) * (p.a.n * p.a.heads) + row;
+      if (d == 0) p.ml[to] = make_float2(top, sum);
+      p.acc[to * hd + d] = o;
     }
   }
 }
@@ -291,18 +266,23 @@ Params plan(const PagedCache& c, int64_t heads, int64_t n, int64_t prefix, int64
   // 8 rows to a thin block where a sequence's rows, and the whole batch's on
   // the prefix, are that few; else 16.
   const bool few = rows <= 8 * seqs && (prefix == 0 || p.prefix_wide || rows <= 8);
-  p.thin_rows = mma_cache(c) ? few ? 8 : 16 : kSimtRows;
+  p.thin_rows = few ? 8 : 16;
+  if (!mma_cache(c)) {
+    // Rows of a block of the f32 kernel: a sequence's, at most 8.
+    const int64_t each = (rows + seqs - 1) / seqs;
+    p.thin_rows = each <= 1 ? 1 : each <= 2 ? 2 : each <= 4 ? 4 : 8;
+  }
   p.prefix_rows = p.prefix_wide ? kWideRows : p.thin_rows;
   p.own_rows = p.own_wide ? kWideRows : p.thin_rows;
   p.own_rows_log2 = 31 - __builtin_clz((unsigned)p.own_rows);
-  p.min_slice = 128;
+  p.min_slice = mma_cache(c) ? 128 : 64;
   const int64_t tiles = (rows + p.prefix_rows - 1) / p.prefix_rows;
   p.prefix_tiles = prefix > 0 ? (int)tiles : 0;
   p.own_slots = (int)(rows / p.own_rows + c.sequences);
   // A part's keys are split as long as blocks are wanting and a slice keeps
-  // min_slice keys: two thin blocks to an SM, one wide.
+  // min_slice keys: four thin or f32 blocks to an SM, one wide.
   auto splits = [&](int64_t blocks, int64_t keys, bool on_wide) {
-    const int64_t want = on_wide ? 148 / (blocks > 0 ? blocks : 1) : (2 * 148 + blocks - 1) / (blocks > 0 ? blocks : 1);
+    const int64_t want = on_wide ? 148 / (blocks > 0 ? blocks : 1) : (4 * 148 + blocks - 1) / (blocks > 0 ? blocks : 1);
     const int64_t most = (keys + p.min_slice - 1) / p.min_slice, least = want < most ? want : most;
     return (int)(least > 1 ? least : 1);
   };
@@ -333,25 +313,30 @@ cudaError_t launch_mma(const Params& p, cudaStream_t stream, bool pdl) {
   return launch_attention_thin(part, stream, pdl || wide);
 }
 
-template <typename T, int V>
+template <typename T, int V, int NU>
+cudaError_t launch_simt_rows(const Params& p, cudaStream_t stream, bool pdl) {
+  const dim3 grid = attention_grid(p);
+  switch (p.own_rows) {
+    case 1: return launch_ex(attention_simt_kernel<T, V, NU, 1>, grid, kSimtThreads, 0, stream, pdl, p);
+    case 2: return launch_ex(attention_simt_kernel<T, V, NU, 2>, grid, kSimtThreads, 0, stream, pdl, p);
+    case 4: return launch_ex(attention_simt_kernel<T, V, NU, 4>, grid, kSimtThreads, 0, stream, pdl, p);
+    default: return launch_ex(attention_simt_kernel<T, V, NU, 8>, grid, kSimtThreads, 0, stream, pdl, p);
+  }
+}
+
+template <typename T>
 cudaError_t launch_simt(const Params& p, cudaStream_t stream, bool pdl) {
-  const size_t smem = ((kSimtRows + 2 * kSimtKeys) * (size_t)simt_pitch((int)p.a.cache.hd) +
-                       kSimtThreads / kLanes * kSimtKeys * kWarpRows) * sizeof(float);
-  if (cudaError_t e = cudaFuncSetAttribute(attention_simt_kernel<T, V>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                           (int)smem);
-      e != cudaSuccess)
-    return e;
-  return launch_ex(attention_simt_kernel<T, V>, attention_grid(p), kSimtThreads, smem, stream, pdl, p);
+  const PagedCache& c = p.a.cache;
+  const bool runs = (((uintptr_t)c.keys | (uintptr_t)c.values) & (4 * sizeof(T) - 1)) == 0 &&
+                    (c.page_stride | c.hd) % 4 == 0;
+  if (!runs) return launch_simt_rows<T, 1, 8>(p, stream, pdl);
+  return c.hd <= 128 ? launch_simt_rows<T, 4, 1>(p, stream, pdl) : launch_simt_rows<T, 4, 2>(p, stream, pdl);
 }
 
 template <typename T>
 cudaError_t launch_type(const Params& p, cudaStream_t stream, bool pdl) {
-  constexpr int V = 16 / sizeof(T);
   const PagedCache& c = p.a.cache;
-  const bool runs = (((uintptr_t)c.keys | (uintptr_t)c.values) & 15) == 0 && (c.page_stride | c.hd) % V == 0;
-  cudaError_t e = mma_cache(c) ? launch_mma(p, stream, pdl)
-                  : runs       ? launch_simt<T, V>(p, stream, pdl)
-                               : launch_simt<T, 1>(p, stream, pdl);
+  const cudaError_t e = mma_cache(c) ? launch_mma(p, stream, pdl) : launch_simt<T>(p, stream, pdl);
   if (e != cudaSuccess || p.direct) return e;
   const int64_t warps = p.a.n * p.a.heads, per = kJoinThreads / kLanes;
   const dim3 grid((unsigned)((warps + per - 1) / per));

@@ -25,7 +25,7 @@ struct Params {
   int group;            // query heads of a kv head
   int prefix_rows, own_rows;  // rows of a block's tile, by the part (a power of two)
   int own_rows_log2;
-  int thin_rows;        // of the thin kernel's tiles: 8 or 16
+  int thin_rows;        // of the tiles of the thin or the f32 kernel
   bool prefix_wide, own_wide;  // which parts the wide kernel takes
   bool beside;          // this launch runs beside the one before it
   int prefix_tiles, prefix_splits;
@@ -249,8 +249,7 @@ __device__ __forceinline__ int slice_index(const Params& p, const Work& w, int g
   return w.prefix ? w.slice + group * p.prefix_splits : p.prefix_slices + w.slice + group * p.own_splits;
 }
 
-// Rows of a block by kernel: the f32 one and the thin one (8 or 16), the wide one.
-constexpr int kSimtRows = 16;
+// Rows of a block of the wide kernel (the thin one: 8 or 16, the f32 one: 1 to 8).
 constexpr int kWideRows = 128;
 constexpr int kWideFrom = 32;  // rows (of the batch, of a sequence on average) from which the wide one runs
 constexpr int kLanes = 32;
