@@ -192,16 +192,18 @@ __global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(const __gr
   constexpr int kRuns = kMaxPagedHd / (kLanes * V);
   const int lane = threadIdx.x % kLanes, hd = (int)p.a.cache.hd;
   const int t = (int)((uint32_t)row / (uint32_t)p.a.heads), head = (int)((uint32_t)row % (uint32_t)p.a.heads);
-  if (p.a.q_start != nullptr && seq_of(p, t) < 0) return;
+  const bool covered = p.a.q_start == nullptr || seq_of(p, t) >= 0;
   const int slices = p.slices;
-  float m = -INFINITY;
-  for (int i = lane; i < slices; i += kLanes) m = fmaxf(m, p.ml[i * rows + row].x);
+  const float2 first = lane < slices ? p.ml[lane * rows + row] : make_float2(-INFINITY, 0.0f);
+  float m = first.x;
+  for (int i = lane + kLanes; i < slices; i += kLanes) m = fmaxf(m, p.ml[i * rows + row].x);
 #pragma unroll
   for (int off = 16; off >= 1; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
   const float base = m == -INFINITY ? 0.0f : m;
   float l = 0.0f, acc[kRuns][V] = {};
   for (int i0 = 0; i0 < slices; i0 += kLanes) {
-    const float2 ml = i0 + lane < slices ? p.ml[(i0 + lane) * rows + row] : make_float2(-INFINITY, 0.0f);
+    float2 ml = first;
+    if (i0 > 0) ml = i0 + lane < slices ? p.ml[(i0 + lane) * rows + row] : make_float2(-INFINITY, 0.0f);
     const float mine = ml.y == 0.0f ? 0.0f : exp2_fast(ml.x - base);
     l += ml.y * mine;
     unsigned left = __ballot_sync(0xffffffffu, ml.y != 0.0f);  // (a slice with l = 0 may hold anything)
@@ -224,6 +226,7 @@ __global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(const __gr
   }
 #pragma unroll
   for (int off = 16; off >= 1; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
+  if (!covered) return;
   T* out = static_cast<T*>(p.a.out) + t * p.a.out_stride + (int64_t)head * hd;
 #pragma unroll
   for (int u = 0; u < kRuns; u++) {

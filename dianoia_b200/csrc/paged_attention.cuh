@@ -155,7 +155,7 @@ __device__ __forceinline__ bool find_work(const Params& p, Work& w) {
   // first of them around where one token a sequence would put it.
   const int lane = threadIdx.x % 32;
   int lo = 0, hi = seqs;  // the answer lies in lo .. hi - 1
-  const int guess = (int)((int64_t)slot * p.own_rows / (p.own_rows + p.group)) - 16;
+  const int guess = (int)((unsigned)(slot * p.own_rows) / (unsigned)(p.own_rows + p.group)) - 16;
   int at = max(0, min(guess, seqs - 32)), step = 1, start, ahead, length;
   for (;;) {
     const int s = at + lane * step;

@@ -176,7 +176,7 @@ __device__ __forceinline__ void thin_block(const Params& p, const Maps& maps, co
   };
   look_up(0);
 #pragma unroll
-  for (int s = 0; s < S::kStages - 1; s++) issue(s, s);
+  for (int s = 0; s < S::kStages; s++) issue(s, s);
 
   int low[NT][2], high[NT][2];
   float m[NT][2], l[NT][2], o[NT][HDP / 16][4];
@@ -217,7 +217,6 @@ __device__ __forceinline__ void thin_block(const Params& p, const Maps& maps, co
       if (step >= steps) break;
       live = __all_sync(0xffffffffu, wait_phase(&full[b], (step / S::kStages) & 1, p.status, kStatusTmaTimeout));
       if (!live) break;
-      issue(step + S::kStages - 1, (b + S::kStages - 1) % S::kStages);
       const char* buf = ring + b * 2 * S::kBuf;
       const uint32_t kb = smem_u32(buf), vb = kb + S::kBuf;
       const int k0 = first + step * kTile;
@@ -315,6 +314,7 @@ __device__ __forceinline__ void thin_block(const Params& p, const Maps& maps, co
         }
       }
       __syncwarp();  // the buffer is read: its next copy may start
+      issue(step + S::kStages, b);
     }
   }
 #pragma unroll
