@@ -77,4 +77,24 @@ __device__ __forceinline__ void store_run(T* p, const float (&x)[V]) {
   }
 }
 
+// A run of V elements as it lies in memory, read once (16 bytes at a time
+// where it has that size: the caller's promise of alignment).
+template <typename T, int V>
+struct Raw {
+  static constexpr int kBytes = V * (int)sizeof(T);
+  T e[V];
+  __device__ __forceinline__ void load(const T* p) {
+    if constexpr (kBytes % 16 == 0) {
+#pragma unroll
+      for (int u = 0; u < kBytes / 16; u++) {
+        const uint4 w = __ldcs(reinterpret_cast<const uint4*>(p) + u);
+        memcpy(reinterpret_cast<char*>(e) + 16 * u, &w, 16);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; i++) e[i] = p[i];
+    }
+  }
+};
+
 }  // namespace dn

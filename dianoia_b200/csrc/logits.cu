@@ -7,11 +7,12 @@
 //   x3 = x2 + the row's biases of v in list order,  y = allowed(v) ? x3 : -inf.
 //
 // Bytes-bound: logits in and out, once. A CTA owns kChunk tokens of one row.
-// It counts the history's tokens that fall into its range in shared memory
+// Its logits are loaded into registers first; while they are on their way it
+// counts the history's tokens that fall into its range in shared memory
 // (integer atomics: their order changes nothing), adds up the biases there
-// (one lane, in list order), and then passes over its logits once, so that
-// there is no count array in memory and one launch. The history is read by
-// every CTA of the row, from L2.
+// (one warp, in list order) and takes its words of the mask. So there is no
+// count array in memory, one launch, and the scan of the history, which every
+// CTA of the row reads from L2, hides behind the logits.
 #include "dn_common.cuh"
 #include "dn_launch.h"
 #include "elem.cuh"
@@ -26,8 +27,10 @@ template <typename T, int V>
 __global__ void __launch_bounds__(kThreads) logits_kernel(const __grid_constant__ LogitsArgs a, int chunks) {
   pdl_launch_dependents();
   pdl_wait();
-  __shared__ uint32_t counts[kChunk];  // 2 * times generated + whether seen
-  __shared__ float biases[kChunk];
+  constexpr int kRuns = kChunk / (kThreads * V);
+  __shared__ __align__(16) uint32_t counts[kChunk];  // 2 * times generated + whether seen
+  __shared__ __align__(16) float biases[kChunk];
+  __shared__ uint32_t words[kChunk / 32 + 2];
   const int tid = threadIdx.x;
   const int64_t row = blockIdx.x / (unsigned)chunks;
   const int chunk = (int)(blockIdx.x % (unsigned)chunks);
@@ -39,82 +42,112 @@ __global__ void __launch_bounds__(kThreads) logits_kernel(const __grid_constant_
   const int base = chunk * kChunk - shift, vocab = (int)a.vocab;
   const LogitRules& r = a.rules;
 
+  Raw<T, V> x[kRuns];
+#pragma unroll
+  for (int i = 0; i < kRuns; i++) {
+    const int v = base + (i * kThreads + tid) * V;
+    if (v >= 0 && v + V <= vocab) {
+      x[i].load(in + v);
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; e++)
+        if (v + e >= 0 && v + e < vocab) x[i].e[e] = in[v + e];
+    }
+  }
   const int64_t h0 = r.history != nullptr ? r.history[row] : 0;
   const int64_t h1 = r.history != nullptr ? r.history[row + 1] : 0;
   const int64_t b0 = r.bias_start != nullptr ? r.bias_start[row] : 0;
   const int64_t b1 = r.bias_start != nullptr ? r.bias_start[row + 1] : 0;
-  const bool counted = h1 > h0, biased = b1 > b0;
-  if (counted)
-    for (int i = tid; i < kChunk; i += kThreads) counts[i] = 0;
-  if (biased)
-    for (int i = tid; i < kChunk; i += kThreads) biases[i] = 0.0f;
-  __syncthreads();
-  if (counted) {
-    const int64_t made = r.generated != nullptr ? h1 - r.generated[row] : h0;
-    for (int64_t i = h0 + tid; i < h1; i += kThreads) {
-      const int v = r.tokens[i];
-      const uint32_t at = (uint32_t)v - (uint32_t)base;
-      if (v >= 0 && v < vocab && at < kChunk) {
-        atomicOr(&counts[at], 1u);
-        if (i >= made) atomicAdd(&counts[at], 2u);
-      }
-    }
-  }
-  if (biased && tid < 32) {
-    for (int64_t i0 = b0; i0 < b1; i0 += 32) {
-      const int64_t i = i0 + tid;
-      const int v = i < b1 ? r.bias_tokens[i] : -1;
-      const uint32_t at = (uint32_t)v - (uint32_t)base;
-      const bool mine = v >= 0 && v < vocab && at < kChunk;
-      const float add = mine ? r.bias[i] : 0.0f;
-      unsigned left = __ballot_sync(0xffffffffu, mine);
-      while (left != 0) {  // in list order
-        const int src = __ffs(left) - 1;
-        left &= left - 1;
-        if (tid == src) biases[at] += add;
-        __syncwarp();
-      }
-    }
-  }
   const float rep = r.repetition != nullptr ? r.repetition[row] : 1.0f;
   const float freq = r.frequency != nullptr ? r.frequency[row] : 0.0f;
   const float pres = r.presence != nullptr ? r.presence[row] : 0.0f;
   const int64_t mrow = r.mask == nullptr ? -1 : r.mask_row != nullptr ? r.mask_row[row] : row;
   const uint32_t* mask = mrow >= 0 && mrow < r.mask_rows ? r.mask + mrow * r.mask_stride : nullptr;
-  const int words = (vocab + 31) / 32;
+  const bool counted = h1 > h0, biased = b1 > b0;
+  const int word0 = (base < 0 ? 0 : base) / 32;  // of words[0]
+  if (counted)
+    for (int i = tid; i < kChunk / 4; i += kThreads) reinterpret_cast<uint4*>(counts)[i] = make_uint4(0, 0, 0, 0);
+  if (biased)
+    for (int i = tid; i < kChunk / 4; i += kThreads)
+      reinterpret_cast<float4*>(biases)[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  if (mask != nullptr)
+    for (int i = tid; i < kChunk / 32 + 2; i += kThreads)
+      words[i] = word0 + i < (vocab + 31) / 32 ? mask[word0 + i] : 0;
   __syncthreads();
-
-  auto rule = [&](float x, int at, bool allowed) {
-    if (counted) {
-      const uint32_t c = counts[at];
-      if (c != 0) {
-        x = x > 0.0f ? x / rep : x * rep;
-        const float times = (float)(c >> 1);
-        x -= times * freq + (times > 0.0f ? pres : 0.0f);
+  if (counted) {
+    const int64_t made = r.generated != nullptr ? h1 - r.generated[row] : h0;
+    constexpr int kAtOnce = 4;
+    for (int64_t i0 = h0 + tid; i0 < h1; i0 += kThreads * kAtOnce) {
+      int v[kAtOnce];
+#pragma unroll
+      for (int k = 0; k < kAtOnce; k++) v[k] = i0 + k * kThreads < h1 ? r.tokens[i0 + k * kThreads] : -1;
+#pragma unroll
+      for (int k = 0; k < kAtOnce; k++) {
+        const uint32_t at = (uint32_t)v[k] - (uint32_t)base;
+        if (v[k] >= 0 && v[k] < vocab && at < kChunk) {
+          atomicOr(&counts[at], 1u);
+          if (i0 + k * kThreads >= made) atomicAdd(&counts[at], 2u);
+        }
       }
     }
-    if (biased) x += biases[at];
-    return allowed ? x : -INFINITY;
-  };
-  for (int at = tid * V; at < kChunk; at += kThreads * V) {
-    const int v = base + at;
+  }
+  if (biased && tid >= kThreads - 32) {
+    const int lane = tid % 32;
+    constexpr int kAtOnce = 4;
+    for (int64_t i0 = b0; i0 < b1; i0 += 32 * kAtOnce) {
+      int v[kAtOnce];
+      float add[kAtOnce];
+#pragma unroll
+      for (int k = 0; k < kAtOnce; k++) {
+        const int64_t i = i0 + 32 * k + lane;
+        v[k] = i < b1 ? r.bias_tokens[i] : -1;
+        add[k] = i < b1 ? r.bias[i] : 0.0f;
+      }
+#pragma unroll
+      for (int k = 0; k < kAtOnce; k++) {
+        const uint32_t at = (uint32_t)v[k] - (uint32_t)base;
+        unsigned left = __ballot_sync(0xffffffffu, v[k] >= 0 && v[k] < vocab && at < kChunk);
+        while (left != 0) {  // in list order
+          const int src = __ffs(left) - 1;
+          left &= left - 1;
+          if (lane == src) biases[at] += add[k];
+          __syncwarp();
+        }
+      }
+    }
+  }
+  __syncthreads();
+
+#pragma unroll
+  for (int i = 0; i < kRuns; i++) {
+    const int at = (i * kThreads + tid) * V, v = base + at;
     if (v >= vocab) break;
-    uint32_t bits = 0xffffffffu;  // of tokens v .. v + V - 1
+    uint32_t allowed = 0xffffffffu;  // of tokens v .. v + V - 1
     if (mask != nullptr) {
-      const int w = v >= 0 ? v / 32 : 0;
-      const uint32_t lo = mask[w], hi = w + 1 < words ? mask[w + 1] : 0;
-      bits = v >= 0 ? __funnelshift_r(lo, hi, v % 32) : lo << -v;
+      const int w = (v < 0 ? 0 : v) / 32 - word0;
+      allowed = v >= 0 ? __funnelshift_r(words[w], words[w + 1], v % 32) : words[w] << -v;
+    }
+    float y[V];
+#pragma unroll
+    for (int e = 0; e < V; e++) {
+      float z = to_f32<T>(x[i].e[e]);
+      if (counted) {
+        const uint32_t c = counts[at + e];
+        if (c != 0) {
+          z = z > 0.0f ? z / rep : z * rep;
+          const float times = (float)(c >> 1);
+          z -= times * freq + (times > 0.0f ? pres : 0.0f);
+        }
+      }
+      if (biased) z += biases[at + e];
+      y[e] = (allowed >> e & 1u) != 0 ? z : -INFINITY;
     }
     if (v >= 0 && v + V <= vocab) {
-      float x[V];
-      load_run<T, V>(in + v, x);
-#pragma unroll
-      for (int e = 0; e < V; e++) x[e] = rule(x[e], at + e, (bits >> e & 1u) != 0);
-      store_run<T, V>(out + v, x);
+      store_run<T, V>(out + v, y);
     } else {
+#pragma unroll
       for (int e = 0; e < V; e++)
-        if (v + e >= 0 && v + e < vocab)
-          out[v + e] = from_f32<T>(rule(to_f32<T>(in[v + e]), at + e, (bits >> e & 1u) != 0));
+        if (v + e >= 0 && v + e < vocab) out[v + e] = from_f32<T>(y[e]);
     }
   }
 }

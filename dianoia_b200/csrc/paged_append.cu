@@ -11,7 +11,9 @@
 // group of G lanes; a lane holds two runs of V values, the two halves of a
 // rotation pair (runs past rot are held two by two), so that the rotation
 // needs no exchange, the norm one shuffle reduction of G lanes, and memory
-// moves in 16-byte accesses. G is the smallest power of two that holds the
+// moves in 16-byte accesses. For long prompts a group takes four heads of a
+// token, whose loads are then in flight together before the chain sequence,
+// position, page is followed, and which share the turns. G is the smallest power of two that holds the
 // head: 8 lanes for 128 values, four heads to a warp.
 #include "dn_common.cuh"
 #include "dn_launch.h"
@@ -22,39 +24,42 @@ namespace {
 
 constexpr int kThreads = 256;
 
-template <typename TI, typename TC, int V, int G, int ITER>
+template <typename TI, typename TC, int V, int G, int ITER, int U>
 __global__ void __launch_bounds__(kThreads) paged_append_kernel(const __grid_constant__ PagedAppendArgs a) {
   pdl_launch_dependents();
   pdl_wait();
   const int hd = (int)a.cache.hd, heads = (int)a.heads, kvh = (int)a.cache.kv_heads;
-  const uint32_t per_token = (uint32_t)(heads + 2 * kvh);
+  const uint32_t slots_all = (uint32_t)(heads + 2 * kvh), per_token = (slots_all + U - 1) / U;
   const int64_t unit = (int64_t)blockIdx.x * (kThreads / G) + threadIdx.x / G;
   if (unit >= a.n * per_token) return;  // whole groups leave together
-  const uint32_t t = (uint32_t)unit / per_token, h = (uint32_t)unit % per_token;
+  const uint32_t t = (uint32_t)unit / per_token, h0 = (uint32_t)unit % per_token * U;
   const int lane = threadIdx.x % G;
   const unsigned group = G == 32 ? 0xffffffffu : ((1u << G) - 1) << (threadIdx.x % 32 / G * G);
-  const bool is_q = (int)h < heads, is_k = !is_q && (int)h < heads + kvh;
-  const int head = is_q ? (int)h : is_k ? (int)h - heads : (int)h - heads - kvh;
-  const TI* src = is_q   ? static_cast<const TI*>(a.q) + (int64_t)t * a.q_stride
-                  : is_k ? static_cast<const TI*>(a.k) + (int64_t)t * a.k_stride
-                         : static_cast<const TI*>(a.v) + (int64_t)t * a.v_stride;
-  src += (int64_t)head * hd;
-  const int rot = is_q || is_k ? (int)a.rot : 0;
 
-  // A slot's two runs: (s, s + rot / 2) for the rotated pairs, then the rest.
-  const int pairs = rot / 2 / V, slots = (hd / V + 1) / 2;
-  int first[ITER], second[ITER];
-  float x[ITER][V], y[ITER][V];
+  // A slot's two runs: (s, s + rot / 2) for the rotated pairs, then the rest;
+  // of a value, which does not turn, runs 2 s and 2 s + 1.
+  const int rot = (int)a.rot, pairs = rot / 2 / V, slots = (hd / V + 1) / 2;
+  auto runs = [&](int s, bool turns, int& first, int& second) {
+    first = turns && s < pairs ? s * V : turns ? rot + 2 * (s - pairs) * V : 2 * s * V;
+    second = turns && s < pairs ? first + rot / 2 : first + V;
+  };
+  Raw<TI, V> x[U][ITER], y[U][ITER];
 #pragma unroll
-  for (int i = 0; i < ITER; i++) {
-    const int s = lane + i * G;
-    first[i] = s < pairs ? s * V : rot + 2 * (s - pairs) * V;
-    second[i] = s < pairs ? first[i] + rot / 2 : first[i] + V;
+  for (int u = 0; u < U; u++) {
+    const int h = (int)h0 + u;
+    if (h >= (int)slots_all) break;
+    const bool is_q = h < heads, is_k = !is_q && h < heads + kvh;
+    const TI* src = is_q   ? static_cast<const TI*>(a.q) + (int64_t)t * a.q_stride + (int64_t)h * hd
+                    : is_k ? static_cast<const TI*>(a.k) + (int64_t)t * a.k_stride + (int64_t)(h - heads) * hd
+                           : static_cast<const TI*>(a.v) + (int64_t)t * a.v_stride + (int64_t)(h - heads - kvh) * hd;
 #pragma unroll
-    for (int e = 0; e < V; e++) x[i][e] = y[i][e] = 0.0f;
-    if (s < slots) {
-      load_run<TI, V>(src + first[i], x[i]);
-      if (second[i] < hd) load_run<TI, V>(src + second[i], y[i]);
+    for (int i = 0; i < ITER; i++) {
+      const int s = lane + i * G;
+      if (s >= slots) break;
+      int first, second;
+      runs(s, is_q || is_k, first, second);
+      x[u][i].load(src + first);
+      if (second < hd) y[u][i].load(src + second);
     }
   }
 
@@ -66,75 +71,90 @@ __global__ void __launch_bounds__(kThreads) paged_append_kernel(const __grid_con
       (a.rot == 0 || pos < a.rope_rows))
     page = a.cache.table[seq * a.cache.table_stride + entry];
   const bool held = page >= 0 && page < a.cache.pages;
-  if (!held) {
-    if (is_q) {
-      const float zero[V] = {};
-      TC* dst = static_cast<TC*>(a.q_out) + (int64_t)t * a.q_out_stride + (int64_t)head * hd;
-#pragma unroll
-      for (int i = 0; i < ITER; i++) {
-        if (lane + i * G >= slots) break;
-        store_run<TC, V>(dst + first[i], zero);
-        if (second[i] < hd) store_run<TC, V>(dst + second[i], zero);
-      }
-    }
-    return;  // the whole group
-  }
-
-  const float* w = is_q ? a.q_norm : is_k ? a.k_norm : nullptr;
-  if (w != nullptr) {
-    float sum = 0.0f;
-#pragma unroll
-    for (int i = 0; i < ITER; i++)
-#pragma unroll
-      for (int e = 0; e < V; e++) sum += x[i][e] * x[i][e] + y[i][e] * y[i][e];
-#pragma unroll
-    for (int off = G / 2; off >= 1; off >>= 1) sum += __shfl_xor_sync(group, sum, off);
-    const float r = 1.0f / sqrtf(sum / (float)hd + a.eps);
+  const int slot = pos - entry * (int)a.cache.page_size;
+  // The token's turns, for every head that this lane holds a part of.
+  float c[ITER][V], n[ITER][V];
+  if (held) {
+    const float* tab = a.rope + (int64_t)pos * rot;
 #pragma unroll
     for (int i = 0; i < ITER; i++) {
-      if (lane + i * G >= slots) break;
-      float wx[V], wy[V] = {};
-      load_run<float, V>(w + first[i], wx);
-      if (second[i] < hd) load_run<float, V>(w + second[i], wy);
-#pragma unroll
-      for (int e = 0; e < V; e++) {
-        x[i][e] *= r * wx[e];
-        y[i][e] *= r * wy[e];
-      }
+      const int s = lane + i * G;
+      if (s >= pairs) break;
+      load_run<float, V>(tab + s * V, c[i]);
+      load_run<float, V>(tab + rot / 2 + s * V, n[i]);
     }
   }
-  const float* tab = a.rope + (int64_t)pos * a.rot;
-  const int slot = pos - entry * (int)a.cache.page_size;
-  TC* dst;
-  if (is_q) {
-    dst = static_cast<TC*>(a.q_out) + (int64_t)t * a.q_out_stride + (int64_t)head * hd;
-  } else {
-    dst = static_cast<TC*>(is_k ? a.cache.keys : a.cache.values) + page * a.cache.page_stride +
-          (head * a.cache.page_size + slot) * hd;
-  }
 #pragma unroll
-  for (int i = 0; i < ITER; i++) {
-    const int s = lane + i * G;
-    if (s >= slots) break;
-    if (s < pairs) {
-      float c[V], n[V];
-      load_run<float, V>(tab + first[i], c);
-      load_run<float, V>(tab + rot / 2 + first[i], n);
+  for (int u = 0; u < U; u++) {
+    const int h = (int)h0 + u;
+    if (h >= (int)slots_all) break;  // whole groups alike
+    const bool is_q = h < heads, is_k = !is_q && h < heads + kvh;
+    if (!held && !is_q) continue;
+    float p[ITER][V], q[ITER][V];
+#pragma unroll
+    for (int i = 0; i < ITER; i++) {
+      const int s = lane + i * G;
+      int first, second;
+      runs(s, is_q || is_k, first, second);
 #pragma unroll
       for (int e = 0; e < V; e++) {
-        const float p = x[i][e], q = y[i][e];
-        x[i][e] = p * c[e] - q * n[e];
-        y[i][e] = q * c[e] + p * n[e];
+        p[i][e] = held && s < slots ? to_f32<TI>(x[u][i].e[e]) : 0.0f;
+        q[i][e] = held && s < slots && second < hd ? to_f32<TI>(y[u][i].e[e]) : 0.0f;
       }
     }
-    store_run<TC, V>(dst + first[i], x[i]);
-    if (second[i] < hd) store_run<TC, V>(dst + second[i], y[i]);
+    const float* w = is_q ? a.q_norm : is_k ? a.k_norm : nullptr;
+    if (held && w != nullptr) {
+      float sum = 0.0f;
+#pragma unroll
+      for (int i = 0; i < ITER; i++)
+#pragma unroll
+        for (int e = 0; e < V; e++) sum += p[i][e] * p[i][e] + q[i][e] * q[i][e];
+#pragma unroll
+      for (int off = G / 2; off >= 1; off >>= 1) sum += __shfl_xor_sync(group, sum, off);
+      const float r = 1.0f / sqrtf(sum / (float)hd + a.eps);
+#pragma unroll
+      for (int i = 0; i < ITER; i++) {
+        const int s = lane + i * G;
+        if (s >= slots) break;
+        int first, second;
+        runs(s, true, first, second);
+        float wx[V], wy[V] = {};
+        load_run<float, V>(w + first, wx);
+        if (second < hd) load_run<float, V>(w + second, wy);
+#pragma unroll
+        for (int e = 0; e < V; e++) {
+          p[i][e] *= r * wx[e];
+          q[i][e] *= r * wy[e];
+        }
+      }
+    }
+    const int head = is_q ? h : is_k ? h - heads : h - heads - kvh;
+    TC* dst = is_q ? static_cast<TC*>(a.q_out) + (int64_t)t * a.q_out_stride + (int64_t)head * hd
+                   : static_cast<TC*>(is_k ? a.cache.keys : a.cache.values) + page * a.cache.page_stride +
+                         ((int64_t)head * a.cache.page_size + slot) * hd;
+#pragma unroll
+    for (int i = 0; i < ITER; i++) {
+      const int s = lane + i * G;
+      if (s >= slots) break;
+      int first, second;
+      runs(s, is_q || is_k, first, second);
+      if (held && (is_q || is_k) && s < pairs) {
+#pragma unroll
+        for (int e = 0; e < V; e++) {
+          const float f = p[i][e], g = q[i][e];
+          p[i][e] = f * c[i][e] - g * n[i][e];
+          q[i][e] = g * c[i][e] + f * n[i][e];
+        }
+      }
+      store_run<TC, V>(dst + first, p[i]);
+      if (second < hd) store_run<TC, V>(dst + second, q[i]);
+    }
   }
 }
 
-template <typename TI, typename TC, int V, int G, int ITER>
-cudaError_t launch_group(const PagedAppendArgs& a, cudaStream_t stream, bool pdl) {
-  const int64_t units = a.n * (a.heads + 2 * a.cache.kv_heads);
+template <typename TI, typename TC, int V, int G, int ITER, int U>
+cudaError_t launch_units(const PagedAppendArgs& a, cudaStream_t stream, bool pdl) {
+  const int64_t units = a.n * ((a.heads + 2 * a.cache.kv_heads + U - 1) / U);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)((units * G + kThreads - 1) / kThreads));
   cfg.blockDim = dim3(kThreads);
@@ -144,7 +164,15 @@ cudaError_t launch_group(const PagedAppendArgs& a, cudaStream_t stream, bool pdl
   attr[0].val.programmaticStreamSerializationAllowed = pdl ? 1 : 0;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, paged_append_kernel<TI, TC, V, G, ITER>, a);
+  return cudaLaunchKernelEx(&cfg, paged_append_kernel<TI, TC, V, G, ITER, U>, a);
+}
+
+template <typename TI, typename TC, int V, int G>
+cudaError_t launch_group(const PagedAppendArgs& a, cudaStream_t stream, bool pdl) {
+  // Four heads a group, once that leaves every SM its 2048 threads twice.
+  const int64_t threads = a.n * (a.heads + 2 * a.cache.kv_heads) * G;
+  return threads >= (int64_t)8 * 148 * 2048 ? launch_units<TI, TC, V, G, 1, 4>(a, stream, pdl)
+                                            : launch_units<TI, TC, V, G, 1, 1>(a, stream, pdl);
 }
 
 template <typename TI, typename TC>
@@ -157,12 +185,12 @@ cudaError_t launch_types(const PagedAppendArgs& a, cudaStream_t stream, bool pdl
                          (uintptr_t)a.q_norm | (uintptr_t)a.k_norm;
   const int64_t step = a.q_stride | a.k_stride | a.v_stride | a.q_out_stride | a.cache.page_stride | a.cache.hd |
                        a.rot / 2;
-  if ((addr & 15) != 0 || step % V != 0) return launch_group<TI, TC, 1, 32, 4>(a, stream, pdl);
+  if ((addr & 15) != 0 || step % V != 0) return launch_units<TI, TC, 1, 32, 4, 1>(a, stream, pdl);
   const int64_t slots = (a.cache.hd / V + 1) / 2;
-  if (slots <= 4) return launch_group<TI, TC, V, 4, 1>(a, stream, pdl);
-  if (slots <= 8) return launch_group<TI, TC, V, 8, 1>(a, stream, pdl);
-  if (slots <= 16) return launch_group<TI, TC, V, 16, 1>(a, stream, pdl);
-  if constexpr (V == 4) return launch_group<TI, TC, V, 32, 1>(a, stream, pdl);
+  if (slots <= 4) return launch_group<TI, TC, V, 4>(a, stream, pdl);
+  if (slots <= 8) return launch_group<TI, TC, V, 8>(a, stream, pdl);
+  if (slots <= 16) return launch_group<TI, TC, V, 16>(a, stream, pdl);
+  if constexpr (V == 4) return launch_group<TI, TC, V, 32>(a, stream, pdl);
   return cudaErrorInvalidValue;  // hd over kMaxPagedHd, which the entry refuses
 }
 
