@@ -22,14 +22,18 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kChunk = 4096;
+constexpr uint32_t kBiased = 1u << 31;
 
 template <typename T, int V>
 __global__ void __launch_bounds__(kThreads) logits_kernel(const __grid_constant__ LogitsArgs a, int chunks) {
   pdl_launch_dependents();
   pdl_wait();
   constexpr int kRuns = kChunk / (kThreads * V);
-  __shared__ __align__(16) uint32_t counts[kChunk];  // 2 * times generated + whether seen
-  __shared__ __align__(16) float biases[kChunk];
+  // Of each token of the range: bit 0 whether seen, bit 31 whether it has a
+  // bias (then biases holds it), between them how often it was generated. A
+  // run of tokens without any of it, nearly all of them, costs one load.
+  __shared__ __align__(16) uint32_t marks[kChunk];
+  __shared__ float biases[kChunk];
   __shared__ uint32_t words[kChunk / 32 + 2];
   const int tid = threadIdx.x;
   const int64_t row = blockIdx.x / (unsigned)chunks;
@@ -65,11 +69,9 @@ __global__ void __launch_bounds__(kThreads) logits_kernel(const __grid_constant_
   const uint32_t* mask = mrow >= 0 && mrow < r.mask_rows ? r.mask + mrow * r.mask_stride : nullptr;
   const bool counted = h1 > h0, biased = b1 > b0;
   const int word0 = (base < 0 ? 0 : base) / 32;  // of words[0]
-  if (counted)
-    for (int i = tid; i < kChunk / 4; i += kThreads) reinterpret_cast<uint4*>(counts)[i] = make_uint4(0, 0, 0, 0);
-  if (biased)
-    for (int i = tid; i < kChunk / 4; i += kThreads)
-      reinterpret_cast<float4*>(biases)[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  const bool marked = counted || biased;
+  if (marked)
+    for (int i = tid; i < kChunk / 4; i += kThreads) reinterpret_cast<uint4*>(marks)[i] = make_uint4(0, 0, 0, 0);
   if (mask != nullptr)
     for (int i = tid; i < kChunk / 32 + 2; i += kThreads)
       words[i] = word0 + i < (vocab + 31) / 32 ? mask[word0 + i] : 0;
@@ -85,8 +87,8 @@ __global__ void __launch_bounds__(kThreads) logits_kernel(const __grid_constant_
       for (int k = 0; k < kAtOnce; k++) {
         const uint32_t at = (uint32_t)v[k] - (uint32_t)base;
         if (v[k] >= 0 && v[k] < vocab && at < kChunk) {
-          atomicOr(&counts[at], 1u);
-          if (i0 + k * kThreads >= made) atomicAdd(&counts[at], 2u);
+          atomicOr(&marks[at], 1u);
+          if (i0 + k * kThreads >= made) atomicAdd(&marks[at], 2u);
         }
       }
     }
@@ -110,7 +112,9 @@ __global__ void __launch_bounds__(kThreads) logits_kernel(const __grid_constant_
         while (left != 0) {  // in list order
           const int src = __ffs(left) - 1;
           left &= left - 1;
-          if (lane == src) biases[at] += add[k];
+          if (lane == src) {
+            biases[at] = (atomicOr(&marks[at], kBiased) & kBiased) != 0 ? biases[at] + add[k] : 0.0f + add[k];
+          }
           __syncwarp();
         }
       }
@@ -128,20 +132,39 @@ __global__ void __launch_bounds__(kThreads) logits_kernel(const __grid_constant_
       allowed = v >= 0 ? __funnelshift_r(words[w], words[w + 1], v % 32) : words[w] << -v;
     }
     float y[V];
+    uint32_t c[V], any = 0;
+    if (marked) {
+      if constexpr (V % 4 == 0) {
 #pragma unroll
-    for (int e = 0; e < V; e++) {
-      float z = to_f32<T>(x[i].e[e]);
-      if (counted) {
-        const uint32_t c = counts[at + e];
-        if (c != 0) {
-          z = z > 0.0f ? z / rep : z * rep;
-          const float times = (float)(c >> 1);
-          z -= times * freq + (times > 0.0f ? pres : 0.0f);
+        for (int e = 0; e < V; e += 4) {
+          const uint4 four = *reinterpret_cast<const uint4*>(&marks[at + e]);
+          c[e] = four.x;
+          c[e + 1] = four.y;
+          c[e + 2] = four.z;
+          c[e + 3] = four.w;
         }
+      } else {
+#pragma unroll
+        for (int e = 0; e < V; e++) c[e] = marks[at + e];
       }
-      if (biased) z += biases[at + e];
-      y[e] = (allowed >> e & 1u) != 0 ? z : -INFINITY;
+#pragma unroll
+      for (int e = 0; e < V; e++) any |= c[e];
     }
+#pragma unroll
+    for (int e = 0; e < V; e++) y[e] = to_f32<T>(x[i].e[e]);
+    if (any != 0) {
+#pragma unroll
+      for (int e = 0; e < V; e++) {
+        if ((c[e] & ~kBiased) != 0) {
+          y[e] = y[e] > 0.0f ? y[e] / rep : y[e] * rep;
+          const float times = (float)((c[e] & ~kBiased) >> 1);
+          y[e] -= times * freq + (times > 0.0f ? pres : 0.0f);
+        }
+        if ((c[e] & kBiased) != 0) y[e] += biases[at + e];
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < V; e++) y[e] = (allowed >> e & 1u) != 0 ? y[e] : -INFINITY;
     if (v >= 0 && v + V <= vocab) {
       store_run<T, V>(out + v, y);
     } else {
