@@ -7,6 +7,8 @@
 #include <cuda_fp16.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 namespace dn {
 
 template <typename T>
@@ -83,6 +85,27 @@ template <typename T, int V>
 struct Raw {
   static constexpr int kBytes = V * (int)sizeof(T);
   T e[V];
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < V; i++) e[i] = from_f32<T>(0.0f);
+  }
+  // The run as elements of TC (the same bits where that is T).
+  template <typename TC>
+  __device__ __forceinline__ void store(TC* p) const {
+    if constexpr (sizeof(T) == sizeof(TC) && kBytes % 16 == 0 && std::is_same<T, TC>::value) {
+#pragma unroll
+      for (int u = 0; u < kBytes / 16; u++) {
+        uint4 w;
+        memcpy(&w, reinterpret_cast<const char*>(e) + 16 * u, 16);
+        reinterpret_cast<uint4*>(p)[u] = w;
+      }
+    } else {
+      float x[V];
+#pragma unroll
+      for (int i = 0; i < V; i++) x[i] = to_f32<T>(e[i]);
+      store_run<TC, V>(p, x);
+    }
+  }
   __device__ __forceinline__ void load(const T* p) {
     if constexpr (kBytes % 16 == 0) {
 #pragma unroll

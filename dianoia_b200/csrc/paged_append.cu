@@ -11,7 +11,7 @@
 // group of G lanes; a lane holds two runs of V values, the two halves of a
 // rotation pair (runs past rot are held two by two), so that the rotation
 // needs no exchange, the norm one shuffle reduction of G lanes, and memory
-// moves in 16-byte accesses. For long prompts a group takes four heads of a
+// moves in 16-byte accesses. For long prompts a group takes six heads of a
 // token, whose loads are then in flight together before the chain sequence,
 // position, page is followed, and which share the turns. G is the smallest power of two that holds the
 // head: 8 lanes for 128 values, four heads to a warp.
@@ -37,29 +37,35 @@ __global__ void __launch_bounds__(kThreads) paged_append_kernel(const __grid_con
   const unsigned group = G == 32 ? 0xffffffffu : ((1u << G) - 1) << (threadIdx.x % 32 / G * G);
 
   // A slot's two runs: (s, s + rot / 2) for the rotated pairs, then the rest;
-  // of a value, which does not turn, runs 2 s and 2 s + 1.
+  // of a value, which does not turn, runs 2 s and 2 s + 1. Runs that are not
+  // there stay zeros.
   const int rot = (int)a.rot, pairs = rot / 2 / V, slots = (hd / V + 1) / 2;
-  auto runs = [&](int s, bool turns, int& first, int& second) {
-    first = turns && s < pairs ? s * V : turns ? rot + 2 * (s - pairs) * V : 2 * s * V;
-    second = turns && s < pairs ? first + rot / 2 : first + V;
-  };
+  int first[2][ITER], second[2][ITER];  // [of a value, of a query or a key]
+#pragma unroll
+  for (int i = 0; i < ITER; i++) {
+    const int s = lane + i * G;
+    first[0][i] = 2 * s * V;
+    second[0][i] = first[0][i] + V;
+    first[1][i] = s < pairs ? s * V : rot + 2 * (s - pairs) * V;
+    second[1][i] = s < pairs ? first[1][i] + rot / 2 : first[1][i] + V;
+  }
+  const TI* tq = static_cast<const TI*>(a.q) + (int64_t)t * a.q_stride;
+  const TI* tk = static_cast<const TI*>(a.k) + (int64_t)t * a.k_stride;
+  const TI* tv = static_cast<const TI*>(a.v) + (int64_t)t * a.v_stride;
   Raw<TI, V> x[U][ITER], y[U][ITER];
 #pragma unroll
   for (int u = 0; u < U; u++) {
     const int h = (int)h0 + u;
-    if (h >= (int)slots_all) break;
-    const bool is_q = h < heads, is_k = !is_q && h < heads + kvh;
-    const TI* src = is_q   ? static_cast<const TI*>(a.q) + (int64_t)t * a.q_stride + (int64_t)h * hd
-                    : is_k ? static_cast<const TI*>(a.k) + (int64_t)t * a.k_stride + (int64_t)(h - heads) * hd
-                           : static_cast<const TI*>(a.v) + (int64_t)t * a.v_stride + (int64_t)(h - heads - kvh) * hd;
+    const bool turns = h < heads + kvh;
+    const TI* src = h < heads ? tq + h * hd : turns ? tk + (h - heads) * hd : tv + (h - heads - kvh) * hd;
 #pragma unroll
     for (int i = 0; i < ITER; i++) {
-      const int s = lane + i * G;
-      if (s >= slots) break;
-      int first, second;
-      runs(s, is_q || is_k, first, second);
-      x[u][i].load(src + first);
-      if (second < hd) y[u][i].load(src + second);
+      x[u][i].clear();
+      y[u][i].clear();
+      if (h >= (int)slots_all || lane + i * G >= slots) continue;
+      x[u][i].load(src + (turns ? first[1][i] : first[0][i]));
+      const int two = turns ? second[1][i] : second[0][i];
+      if (two < hd) y[u][i].load(src + two);
     }
   }
 
@@ -71,39 +77,56 @@ __global__ void __launch_bounds__(kThreads) paged_append_kernel(const __grid_con
       (a.rot == 0 || pos < a.rope_rows))
     page = a.cache.table[seq * a.cache.table_stride + entry];
   const bool held = page >= 0 && page < a.cache.pages;
-  const int slot = pos - entry * (int)a.cache.page_size;
+  TC* out = static_cast<TC*>(a.q_out) + (int64_t)t * a.q_out_stride;
+  if (!held) {  // the whole group
+    const float zero[V] = {};
+#pragma unroll
+    for (int u = 0; u < U; u++)
+#pragma unroll
+      for (int i = 0; i < ITER; i++) {
+        const int h = (int)h0 + u;
+        if (h >= heads || lane + i * G >= slots) continue;
+        store_run<TC, V>(out + h * hd + first[1][i], zero);
+        if (second[1][i] < hd) store_run<TC, V>(out + h * hd + second[1][i], zero);
+      }
+    return;
+  }
+  const int slot = pos - entry * (int)a.cache.page_size, head_step = (int)a.cache.page_size * hd;
+  TC* keys = static_cast<TC*>(a.cache.keys) + page * a.cache.page_stride + slot * hd;
+  TC* vals = static_cast<TC*>(a.cache.values) + page * a.cache.page_stride + slot * hd;
   // The token's turns, for every head that this lane holds a part of.
   float c[ITER][V], n[ITER][V];
-  if (held) {
-    const float* tab = a.rope + (int64_t)pos * rot;
+  const float* tab = a.rope + (int64_t)pos * rot;
 #pragma unroll
-    for (int i = 0; i < ITER; i++) {
-      const int s = lane + i * G;
-      if (s >= pairs) break;
-      load_run<float, V>(tab + s * V, c[i]);
-      load_run<float, V>(tab + rot / 2 + s * V, n[i]);
-    }
+  for (int i = 0; i < ITER; i++) {
+    if (lane + i * G >= pairs) continue;
+    load_run<float, V>(tab + first[1][i], c[i]);
+    load_run<float, V>(tab + rot / 2 + first[1][i], n[i]);
   }
 #pragma unroll
   for (int u = 0; u < U; u++) {
     const int h = (int)h0 + u;
     if (h >= (int)slots_all) break;  // whole groups alike
-    const bool is_q = h < heads, is_k = !is_q && h < heads + kvh;
-    if (!held && !is_q) continue;
+    if (h >= heads + kvh) {          // a value: moved
+      TC* dst = vals + (int64_t)(h - heads - kvh) * head_step;
+#pragma unroll
+      for (int i = 0; i < ITER; i++) {
+        if (lane + i * G >= slots) continue;
+        x[u][i].template store<TC>(dst + first[0][i]);
+        if (second[0][i] < hd) y[u][i].template store<TC>(dst + second[0][i]);
+      }
+      continue;
+    }
     float p[ITER][V], q[ITER][V];
 #pragma unroll
-    for (int i = 0; i < ITER; i++) {
-      const int s = lane + i * G;
-      int first, second;
-      runs(s, is_q || is_k, first, second);
+    for (int i = 0; i < ITER; i++)
 #pragma unroll
       for (int e = 0; e < V; e++) {
-        p[i][e] = held && s < slots ? to_f32<TI>(x[u][i].e[e]) : 0.0f;
-        q[i][e] = held && s < slots && second < hd ? to_f32<TI>(y[u][i].e[e]) : 0.0f;
+        p[i][e] = to_f32<TI>(x[u][i].e[e]);
+        q[i][e] = to_f32<TI>(y[u][i].e[e]);
       }
-    }
-    const float* w = is_q ? a.q_norm : is_k ? a.k_norm : nullptr;
-    if (held && w != nullptr) {
+    const float* w = h < heads ? a.q_norm : a.k_norm;
+    if (w != nullptr) {
       float sum = 0.0f;
 #pragma unroll
       for (int i = 0; i < ITER; i++)
@@ -114,13 +137,10 @@ __global__ void __launch_bounds__(kThreads) paged_append_kernel(const __grid_con
       const float r = 1.0f / sqrtf(sum / (float)hd + a.eps);
 #pragma unroll
       for (int i = 0; i < ITER; i++) {
-        const int s = lane + i * G;
-        if (s >= slots) break;
-        int first, second;
-        runs(s, true, first, second);
+        if (lane + i * G >= slots) continue;
         float wx[V], wy[V] = {};
-        load_run<float, V>(w + first, wx);
-        if (second < hd) load_run<float, V>(w + second, wy);
+        load_run<float, V>(w + first[1][i], wx);
+        if (second[1][i] < hd) load_run<float, V>(w + second[1][i], wy);
 #pragma unroll
         for (int e = 0; e < V; e++) {
           p[i][e] *= r * wx[e];
@@ -128,17 +148,11 @@ __global__ void __launch_bounds__(kThreads) paged_append_kernel(const __grid_con
         }
       }
     }
-    const int head = is_q ? h : is_k ? h - heads : h - heads - kvh;
-    TC* dst = is_q ? static_cast<TC*>(a.q_out) + (int64_t)t * a.q_out_stride + (int64_t)head * hd
-                   : static_cast<TC*>(is_k ? a.cache.keys : a.cache.values) + page * a.cache.page_stride +
-                         ((int64_t)head * a.cache.page_size + slot) * hd;
+    TC* dst = h < heads ? out + h * hd : keys + (int64_t)(h - heads) * head_step;
 #pragma unroll
     for (int i = 0; i < ITER; i++) {
-      const int s = lane + i * G;
-      if (s >= slots) break;
-      int first, second;
-      runs(s, is_q || is_k, first, second);
-      if (held && (is_q || is_k) && s < pairs) {
+      if (lane + i * G >= slots) continue;
+      if (lane + i * G < pairs) {
 #pragma unroll
         for (int e = 0; e < V; e++) {
           const float f = p[i][e], g = q[i][e];
@@ -146,8 +160,8 @@ __global__ void __launch_bounds__(kThreads) paged_append_kernel(const __grid_con
           q[i][e] = g * c[i][e] + f * n[i][e];
         }
       }
-      store_run<TC, V>(dst + first, p[i]);
-      if (second < hd) store_run<TC, V>(dst + second, q[i]);
+      store_run<TC, V>(dst + first[1][i], p[i]);
+      if (second[1][i] < hd) store_run<TC, V>(dst + second[1][i], q[i]);
     }
   }
 }
@@ -169,9 +183,9 @@ cudaError_t launch_units(const PagedAppendArgs& a, cudaStream_t stream, bool pdl
 
 template <typename TI, typename TC, int V, int G>
 cudaError_t launch_group(const PagedAppendArgs& a, cudaStream_t stream, bool pdl) {
-  // Four heads a group, once that leaves every SM its 2048 threads twice.
+  // Six heads a group, once that leaves every SM its 2048 threads twice.
   const int64_t threads = a.n * (a.heads + 2 * a.cache.kv_heads) * G;
-  return threads >= (int64_t)8 * 148 * 2048 ? launch_units<TI, TC, V, G, 1, 4>(a, stream, pdl)
+  return threads >= (int64_t)8 * 148 * 2048 ? launch_units<TI, TC, V, G, 1, 6>(a, stream, pdl)
                                             : launch_units<TI, TC, V, G, 1, 1>(a, stream, pdl);
 }
 
