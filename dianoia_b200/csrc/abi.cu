@@ -765,7 +765,7 @@ int64_t dn_logits_apply(int64_t type, const void* logits, int64_t stride, void* 
     return DN_ERR_ARGS;
   if (vocab > (1 << 30) || n > INT32_MAX || stride > kMaxStride || out_stride > kMaxStride)
     return DN_ERR_TOO_LARGE;
-  if (n > INT32_MAX / (vocab / 4096 + 2)) return DN_ERR_TOO_LARGE;  // the launch's blocks fit 31 bits
+  if (n > INT32_MAX / (vocab / 2048 + 2)) return DN_ERR_TOO_LARGE;  // the launch's blocks fit 31 bits
   const dn_logit_rules& r = *rules;
   if (r.history != nullptr && r.tokens == nullptr) return DN_ERR_ARGS;
   if (r.bias_start != nullptr && (r.bias_tokens == nullptr || r.bias == nullptr)) return DN_ERR_ARGS;
@@ -782,8 +782,9 @@ int64_t dn_logits_apply(int64_t type, const void* logits, int64_t stride, void* 
   if (overlaps(logits, stride, vocab, type, out, out_stride, vocab, type, n) &&
       !(logits == out && stride == out_stride))
     return DN_ERR_ARGS;
-  if (device_state() == nullptr) return DN_ERR_NO_DEVICE;
-  dn::LogitsArgs a{type, logits, out, stride, out_stride, n, vocab, {}};
+  DeviceState* d = device_state();
+  if (d == nullptr) return DN_ERR_NO_DEVICE;
+  dn::LogitsArgs a{type, logits, out, stride, out_stride, n, vocab, {}, d->status_dev};
   memcpy(&a.rules, rules, sizeof a.rules);
   return dn::launch_logits(a, static_cast<cudaStream_t>(stream), (flags & DN_FLAG_PDL) != 0) == cudaSuccess
              ? DN_OK

@@ -267,6 +267,7 @@ struct LogitsArgs {
   void* out;
   int64_t stride, out_stride, n, vocab;
   LogitRules rules;
+  uint32_t* status;
 };
 cudaError_t launch_logits(const LogitsArgs& a, cudaStream_t stream, bool pdl);
 

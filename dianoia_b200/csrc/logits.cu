@@ -6,13 +6,16 @@
 //   x1 = s ? (x > 0 ? x / r : x r) : x,  x2 = x1 - (c f + [c > 0] p),
 //   x3 = x2 + the row's biases of v in list order,  y = allowed(v) ? x3 : -inf.
 //
-// Bytes-bound: logits in and out, once. A CTA owns kChunk tokens of one row.
-// Its logits are loaded into registers first; while they are on their way it
-// counts the history's tokens that fall into its range in shared memory
-// (integer atomics: their order changes nothing), adds up the biases there
-// (one warp, in list order) and takes its words of the mask. So there is no
-// count array in memory, one launch, and the scan of the history, which every
-// CTA of the row reads from L2, hides behind the logits.
+// Bytes-bound: logits in and out, once, and what stands between is latency:
+// the row's rules, its history, the marks. So a CTA's kChunk tokens of one row
+// come to shared memory by one bulk copy, which costs no registers (eleven
+// CTAs to an SM keep 90 KB on the way), and leave by another. Meanwhile the
+// CTA counts the history's tokens that fall into its range (integer atomics:
+// their order changes nothing) and lists them with those that have biases;
+// then the listed tokens, few of the range, are worked out one a thread, the
+// biases added by one warp in list order, and under a mask the range is passed
+// over once. There is no count array in memory and one launch; the history is
+// read by every CTA of the row, from L2.
 #include "dn_common.cuh"
 #include "dn_launch.h"
 #include "elem.cuh"
@@ -20,165 +23,181 @@
 namespace dn {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kChunk = 4096;
+constexpr int kThreads = 128;
+constexpr int kChunk = 2048;
+constexpr int kListed = 512;  // tokens the list holds; with more, all of the range are looked at
 constexpr uint32_t kBiased = 1u << 31;
 
-template <typename T, int V>
+__device__ __forceinline__ void bulk_s2g(void* dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(smem_u32(src)), "r"(bytes)
+               : "memory");
+}
+
+// BULK: rows of out start at the alignment of their rows of logits, so that
+// 16-byte aligned parts of both can be copied whole.
+template <typename T, bool BULK>
 __global__ void __launch_bounds__(kThreads) logits_kernel(const __grid_constant__ LogitsArgs a, int chunks) {
   pdl_launch_dependents();
   pdl_wait();
-  constexpr int kRuns = kChunk / (kThreads * V);
+  constexpr int V = 16 / sizeof(T);
+  __shared__ __align__(128) T x[kChunk];
   // Of each token of the range: bit 0 whether seen, bit 31 whether it has a
-  // bias (then biases holds it), between them how often it was generated. A
-  // run of tokens without any of it, nearly all of them, costs one load.
+  // bias, between them how often it was generated; then, of a listed token,
+  // the bits of its f32 result.
   __shared__ __align__(16) uint32_t marks[kChunk];
-  __shared__ float biases[kChunk];
+  __shared__ uint16_t list[kListed];
   __shared__ uint32_t words[kChunk / 32 + 2];
+  __shared__ int listed;
+  __shared__ uint64_t full;
   const int tid = threadIdx.x;
   const int64_t row = blockIdx.x / (unsigned)chunks;
   const int chunk = (int)(blockIdx.x % (unsigned)chunks);
   const T* in = static_cast<const T*>(a.logits) + row * a.stride;
   T* out = static_cast<T*>(a.out) + row * a.out_stride;
-  // V > 1: ranges start where rows have 16-byte aligned runs, up to V - 1
-  // tokens before the row's first (which are then left out).
-  const int shift = V > 1 ? (int)(((uintptr_t)in & 15) / sizeof(T)) : 0;
+  // Ranges start at 16-byte boundaries: up to V - 1 tokens before the row's
+  // first, which are then left out.
+  const int shift = BULK ? (int)(((uintptr_t)in & 15) / sizeof(T)) : 0;
   const int base = chunk * kChunk - shift, vocab = (int)a.vocab;
+  // The range's tokens of the row, begin .. end - 1 past base; whole 16 bytes
+  // of them, from .. to - 1.
+  const int begin = base < 0 ? -base : 0, end = min(base + kChunk, vocab) - base;
+  const int from = BULK ? begin > 0 ? V : 0 : end, to = BULK && end > from ? from + (end - from) / V * V : from;
   const LogitRules& r = a.rules;
-
-  Raw<T, V> x[kRuns];
-#pragma unroll
-  for (int i = 0; i < kRuns; i++) {
-    const int v = base + (i * kThreads + tid) * V;
-    if (v >= 0 && v + V <= vocab) {
-      x[i].load(in + v);
-    } else {
-#pragma unroll
-      for (int e = 0; e < V; e++)
-        if (v + e >= 0 && v + e < vocab) x[i].e[e] = in[v + e];
+  if (tid == 0) {
+    mbar_init(&full, 1);
+    fence_mbar_init();
+    if (to > from) {
+      mbar_arrive_expect_tx(&full, (uint32_t)((to - from) * sizeof(T)));
+      bulk_g2s(&x[from], in + base + from, (uint32_t)((to - from) * sizeof(T)), &full);
     }
+    listed = 0;
   }
-  const int64_t h0 = r.history != nullptr ? r.history[row] : 0;
-  const int64_t h1 = r.history != nullptr ? r.history[row + 1] : 0;
-  const int64_t b0 = r.bias_start != nullptr ? r.bias_start[row] : 0;
-  const int64_t b1 = r.bias_start != nullptr ? r.bias_start[row + 1] : 0;
-  const float rep = r.repetition != nullptr ? r.repetition[row] : 1.0f;
-  const float freq = r.frequency != nullptr ? r.frequency[row] : 0.0f;
-  const float pres = r.presence != nullptr ? r.presence[row] : 0.0f;
+  // What no bulk copy takes (all of it without BULK).
+  for (int at = begin + tid; at < min(from, end); at += kThreads) x[at] = in[base + at];
+  for (int at = max(to, begin) + tid; BULK && at < end; at += kThreads) x[at] = in[base + at];
+
+  int seen = 0, made = 0, biased = 0;  // tokens of the history, those before the generated ones, biases
+  const int* tokens = nullptr;
+  const int* bias_tokens = nullptr;
+  const float* bias = nullptr;
+  if (r.history != nullptr) {
+    const int64_t h0 = r.history[row], h1 = r.history[row + 1];
+    tokens = r.tokens + h0;
+    seen = (int)min64(h1 - h0, INT32_MAX - 2 * kChunk);
+    made = r.generated != nullptr ? seen - r.generated[row] : 0;
+  }
+  if (r.bias_start != nullptr) {
+    const int64_t b0 = r.bias_start[row], b1 = r.bias_start[row + 1];
+    bias_tokens = r.bias_tokens + b0;
+    bias = r.bias + b0;
+    biased = (int)min64(b1 - b0, INT32_MAX - 2 * kChunk);
+  }
   const int64_t mrow = r.mask == nullptr ? -1 : r.mask_row != nullptr ? r.mask_row[row] : row;
   const uint32_t* mask = mrow >= 0 && mrow < r.mask_rows ? r.mask + mrow * r.mask_stride : nullptr;
-  const bool counted = h1 > h0, biased = b1 > b0;
-  const int word0 = (base < 0 ? 0 : base) / 32;  // of words[0]
-  const bool marked = counted || biased;
-  if (marked)
-    for (int i = tid; i < kChunk / 4; i += kThreads) reinterpret_cast<uint4*>(marks)[i] = make_uint4(0, 0, 0, 0);
-  if (mask != nullptr)
-    for (int i = tid; i < kChunk / 32 + 2; i += kThreads)
-      words[i] = word0 + i < (vocab + 31) / 32 ? mask[word0 + i] : 0;
+  const bool marked = seen > 0 || biased > 0;
+  const int word0 = (base + begin) / 32;  // of words[0]
+  if (marked) {
+#pragma unroll
+    for (int i = 0; i < kChunk / 4 / kThreads; i++)
+      reinterpret_cast<uint4*>(marks)[i * kThreads + tid] = make_uint4(0, 0, 0, 0);
+  }
+  if (mask != nullptr && tid < kChunk / 32 + 2) words[tid] = word0 + tid < (vocab + 31) / 32 ? mask[word0 + tid] : 0;
   __syncthreads();
-  if (counted) {
-    const int64_t made = r.generated != nullptr ? h1 - r.generated[row] : h0;
-    constexpr int kAtOnce = 4;
-    for (int64_t i0 = h0 + tid; i0 < h1; i0 += kThreads * kAtOnce) {
-      int v[kAtOnce];
+  auto add_to_list = [&](uint32_t at) {
+    const int j = atomicAdd(&listed, 1);
+    if (j < kListed) list[j] = (uint16_t)at;
+  };
+  auto mine = [&](uint32_t at) { return at < (uint32_t)end && at >= (uint32_t)begin; };
+  constexpr int kAtOnce = 8;
+  for (int i0 = tid; i0 < seen; i0 += kThreads * kAtOnce) {
+    uint32_t at[kAtOnce];
 #pragma unroll
-      for (int k = 0; k < kAtOnce; k++) v[k] = i0 + k * kThreads < h1 ? r.tokens[i0 + k * kThreads] : -1;
+    for (int k = 0; k < kAtOnce; k++)
+      at[k] = i0 + k * kThreads < seen ? (uint32_t)(tokens[i0 + k * kThreads] - base) : 0xffffffffu;
 #pragma unroll
-      for (int k = 0; k < kAtOnce; k++) {
-        const uint32_t at = (uint32_t)v[k] - (uint32_t)base;
-        if (v[k] >= 0 && v[k] < vocab && at < kChunk) {
-          atomicOr(&marks[at], 1u);
-          if (i0 + k * kThreads >= made) atomicAdd(&marks[at], 2u);
-        }
+    for (int k = 0; k < kAtOnce; k++)
+      if (mine(at[k])) {
+        if (atomicOr(&marks[at[k]], 1u) == 0) add_to_list(at[k]);
+        if (i0 + k * kThreads >= made) atomicAdd(&marks[at[k]], 2u);
       }
-    }
   }
-  if (biased && tid >= kThreads - 32) {
-    const int lane = tid % 32;
-    constexpr int kAtOnce = 4;
-    for (int64_t i0 = b0; i0 < b1; i0 += 32 * kAtOnce) {
-      int v[kAtOnce];
-      float add[kAtOnce];
-#pragma unroll
-      for (int k = 0; k < kAtOnce; k++) {
-        const int64_t i = i0 + 32 * k + lane;
-        v[k] = i < b1 ? r.bias_tokens[i] : -1;
-        add[k] = i < b1 ? r.bias[i] : 0.0f;
-      }
-#pragma unroll
-      for (int k = 0; k < kAtOnce; k++) {
-        const uint32_t at = (uint32_t)v[k] - (uint32_t)base;
-        unsigned left = __ballot_sync(0xffffffffu, v[k] >= 0 && v[k] < vocab && at < kChunk);
-        while (left != 0) {  // in list order
-          const int src = __ffs(left) - 1;
-          left &= left - 1;
-          if (lane == src) {
-            biases[at] = (atomicOr(&marks[at], kBiased) & kBiased) != 0 ? biases[at] + add[k] : 0.0f + add[k];
-          }
-          __syncwarp();
-        }
-      }
-    }
+  for (int i = tid; i < biased; i += kThreads) {
+    const uint32_t at = (uint32_t)(bias_tokens[i] - base);
+    if (mine(at) && atomicOr(&marks[at], kBiased) == 0) add_to_list(at);
   }
+  if (to > from && !mbar_wait_bounded(&full, 0, a.status, kStatusTmaTimeout)) seen = biased = 0;
   __syncthreads();
 
-#pragma unroll
-  for (int i = 0; i < kRuns; i++) {
-    const int at = (i * kThreads + tid) * V, v = base + at;
-    if (v >= vocab) break;
-    uint32_t allowed = 0xffffffffu;  // of tokens v .. v + V - 1
-    if (mask != nullptr) {
-      const int w = (v < 0 ? 0 : v) / 32 - word0;
-      allowed = v >= 0 ? __funnelshift_r(words[w], words[w + 1], v % 32) : words[w] << -v;
-    }
-    float y[V];
-    uint32_t c[V], any = 0;
-    if (marked) {
-      if constexpr (V % 4 == 0) {
-#pragma unroll
-        for (int e = 0; e < V; e += 4) {
-          const uint4 four = *reinterpret_cast<const uint4*>(&marks[at + e]);
-          c[e] = four.x;
-          c[e + 1] = four.y;
-          c[e + 2] = four.z;
-          c[e + 3] = four.w;
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < V; e++) c[e] = marks[at + e];
-      }
-#pragma unroll
-      for (int e = 0; e < V; e++) any |= c[e];
-    }
-#pragma unroll
-    for (int e = 0; e < V; e++) y[e] = to_f32<T>(x[i].e[e]);
-    if (any != 0) {
-#pragma unroll
-      for (int e = 0; e < V; e++) {
-        if ((c[e] & ~kBiased) != 0) {
-          y[e] = y[e] > 0.0f ? y[e] / rep : y[e] * rep;
-          const float times = (float)((c[e] & ~kBiased) >> 1);
-          y[e] -= times * freq + (times > 0.0f ? pres : 0.0f);
-        }
-        if ((c[e] & kBiased) != 0) y[e] += biases[at + e];
-      }
-    }
-#pragma unroll
-    for (int e = 0; e < V; e++) y[e] = (allowed >> e & 1u) != 0 ? y[e] : -INFINITY;
-    if (v >= 0 && v + V <= vocab) {
-      store_run<T, V>(out + v, y);
+  // The marked tokens: f32 results in place of their marks.
+  const int count = marked ? listed : 0;
+  const bool fits = count <= kListed;
+  auto each_marked = [&](auto&& f) {
+    if (fits) {
+      for (int j = tid; j < count; j += kThreads) f((int)list[j]);
     } else {
-#pragma unroll
-      for (int e = 0; e < V; e++)
-        if (v + e >= 0 && v + e < vocab) out[v + e] = from_f32<T>(y[e]);
+      for (int at = begin + tid; at < end; at += kThreads) f(at);
+    }
+  };
+  if (count > 0) {
+    const float rep = r.repetition != nullptr ? r.repetition[row] : 1.0f;
+    const float freq = r.frequency != nullptr ? r.frequency[row] : 0.0f;
+    const float pres = r.presence != nullptr ? r.presence[row] : 0.0f;
+    each_marked([&](int at) {
+      const uint32_t mark = marks[at] & ~kBiased;
+      float z = to_f32<T>(x[at]);
+      if (mark != 0) {
+        z = z > 0.0f ? z / rep : z * rep;
+        const float times = (float)(mark >> 1);
+        z -= times * freq + (times > 0.0f ? pres : 0.0f);
+      }
+      marks[at] = __float_as_uint(z);
+    });
+    __syncthreads();
+    if (biased > 0) {
+      if (tid < 32) {
+        for (int i0 = tid; i0 - tid < biased; i0 += 32) {
+          const uint32_t at = i0 < biased ? (uint32_t)(bias_tokens[i0] - base) : 0xffffffffu;
+          const bool here = mine(at);
+          unsigned left = __ballot_sync(0xffffffffu, here);
+          const float add = here ? bias[i0] : 0.0f;
+          while (left != 0) {  // in list order
+            const int src = __ffs(left) - 1;
+            left &= left - 1;
+            if (tid == src) marks[at] = __float_as_uint(__uint_as_float(marks[at]) + add);
+            __syncwarp();
+          }
+        }
+      }
+      __syncthreads();
+    }
+    each_marked([&](int at) { x[at] = from_f32<T>(__uint_as_float(marks[at])); });
+  }
+  if (mask != nullptr) {
+    if (count > 0) __syncthreads();
+    for (int at = begin + tid; at < end; at += kThreads) {
+      const int v = base + at;
+      if ((words[v / 32 - word0] >> (v % 32) & 1u) == 0) x[at] = from_f32<T>(-INFINITY);
     }
   }
+  if (count > 0 || mask != nullptr) fence_proxy_async_smem();  // the threads' writes, before the bulk copy reads them
+  __syncthreads();
+  if (to > from && tid == 0) {
+    bulk_s2g(out + base + from, &x[from], (uint32_t)((to - from) * sizeof(T)));
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+  }
+  for (int at = begin + tid; at < min(from, end); at += kThreads) out[base + at] = x[at];
+  for (int at = max(to, begin) + tid; BULK && at < end; at += kThreads) out[base + at] = x[at];
+  if (to > from && tid == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
 }
 
-template <typename T, int V>
-cudaError_t launch_run(const LogitsArgs& a, cudaStream_t stream, bool pdl) {
-  const int64_t chunks = (a.vocab + V - 1 + kChunk - 1) / kChunk;
+template <typename T, bool BULK>
+cudaError_t launch_copies(const LogitsArgs& a, cudaStream_t stream, bool pdl) {
+  const int64_t chunks = (a.vocab + 16 / (int64_t)sizeof(T) - 1 + kChunk - 1) / kChunk;
   if (chunks * a.n > 0x7fffffff) return cudaErrorInvalidValue;
+  if (cudaError_t e = cudaFuncSetAttribute(logits_kernel<T, BULK>, cudaFuncAttributePreferredSharedMemoryCarveout,
+                                           cudaSharedmemCarveoutMaxShared);
+      e != cudaSuccess)
+    return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(chunks * a.n));
   cfg.blockDim = dim3(kThreads);
@@ -188,17 +207,15 @@ cudaError_t launch_run(const LogitsArgs& a, cudaStream_t stream, bool pdl) {
   attr[0].val.programmaticStreamSerializationAllowed = pdl ? 1 : 0;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, logits_kernel<T, V>, a, (int)chunks);
+  return cudaLaunchKernelEx(&cfg, logits_kernel<T, BULK>, a, (int)chunks);
 }
 
 template <typename T>
 cudaError_t launch_type(const LogitsArgs& a, cudaStream_t stream, bool pdl) {
-  // 16-byte runs where every row of out starts at the alignment of its row of
-  // logits, whatever that is; else one value at a time.
   constexpr int V = 16 / sizeof(T);
   const bool same = (((uintptr_t)a.logits ^ (uintptr_t)a.out) & 15) == 0 &&
                     (a.n <= 1 || (a.stride - a.out_stride) % V == 0);
-  return same ? launch_run<T, V>(a, stream, pdl) : launch_run<T, 1>(a, stream, pdl);
+  return same ? launch_copies<T, true>(a, stream, pdl) : launch_copies<T, false>(a, stream, pdl);
 }
 
 }  // namespace
