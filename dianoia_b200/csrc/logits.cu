@@ -8,8 +8,8 @@
 //
 // Bytes-bound: logits in and out, once, and what stands between is latency:
 // the row's rules, its history, the marks. So a CTA's kChunk tokens of one row
-// come to shared memory by one bulk copy, which costs no registers (eleven
-// CTAs to an SM keep 90 KB on the way), and leave by another. Meanwhile the
+// come to shared memory by one bulk copy, which costs no registers (six
+// CTAs to an SM keep 96 KB on the way), and leave by another. Meanwhile the
 // CTA counts the history's tokens that fall into its range (integer atomics:
 // their order changes nothing) and lists them with those that have biases;
 // then the listed tokens, few of the range, are worked out one a thread, the
@@ -23,8 +23,8 @@
 namespace dn {
 namespace {
 
-constexpr int kThreads = 128;
-constexpr int kChunk = 2048;
+constexpr int kThreads = 256;
+constexpr int kChunk = 4096;
 constexpr int kListed = 512;  // tokens the list holds; with more, all of the range are looked at
 constexpr uint32_t kBiased = 1u << 31;
 

@@ -67,9 +67,12 @@ __global__ void __launch_bounds__(kSimtThreads) attention_simt_kernel(const __gr
   }
   const T* keys = static_cast<const T*>(p.a.cache.keys);
   const T* vals = static_cast<const T*>(p.a.cache.values);
+  // Lane k looks key k of a step up, a step ahead.
+  auto look_up = [&](int k) { return lane < kStep && k + lane < end ? entry_at(p, w, k + lane) : -1; };
+  int entry = look_up(begin + warp * kStep);
   for (int k0 = begin + warp * kStep; k0 < end; k0 += kTile) {
-    // Lane k looks key k0 + k up.
-    const int64_t mine = lane < kStep ? row_at(p, w, k0 + lane, any_low, end) : -1;
+    const int64_t mine = lane < kStep ? row_at(p, w, entry, k0 + lane, any_low, end) : -1;
+    entry = look_up(k0 + kTile);
     const unsigned there = __ballot_sync(0xffffffffu, mine >= 0);
     float s[kLanes];
 #pragma unroll
@@ -206,21 +209,28 @@ __global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(const __gr
     if (i0 > 0) ml = i0 + lane < slices ? p.ml[(i0 + lane) * rows + row] : make_float2(-INFINITY, 0.0f);
     const float mine = ml.y == 0.0f ? 0.0f : exp2_fast(ml.x - base);
     l += ml.y * mine;
-    unsigned left = __ballot_sync(0xffffffffu, ml.y != 0.0f);  // (a slice with l = 0 may hold anything)
+    const unsigned held = __ballot_sync(0xffffffffu, ml.y != 0.0f);  // (a slice with l = 0 may hold anything)
     const int count = min(kLanes, slices - i0);
-#pragma unroll 4
-    for (int i = 0; i < count; i++) {
-      const float f = __shfl_sync(0xffffffffu, mine, i);
-      const float* a = p.acc + ((i0 + i) * rows + row) * hd;
-      if ((left >> i & 1u) == 0) continue;
+    constexpr int kAtOnce = 8;
+    for (int i = 0; i < count; i += kAtOnce) {
+      float x[kAtOnce][kRuns][V];
 #pragma unroll
-      for (int u = 0; u < kRuns; u++) {
-        const int d = (u * kLanes + lane) * V;
-        if (d >= hd) continue;
-        float x[V];
-        load_run<float, V>(a + d, x);
+      for (int k = 0; k < kAtOnce; k++) {
+        const float* a = p.acc + ((i0 + min(i + k, count - 1)) * rows + row) * hd;
 #pragma unroll
-        for (int e = 0; e < V; e++) acc[u][e] += x[e] * f;
+        for (int u = 0; u < kRuns; u++) {
+          const int d = (u * kLanes + lane) * V;
+          if (d < hd) load_run<float, V>(a + d, x[k][u]);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < kAtOnce; k++) {
+        const float f = __shfl_sync(0xffffffffu, mine, (i + k) % kLanes);
+        if (i + k >= count || (held >> (i + k) & 1u) == 0) continue;
+#pragma unroll
+        for (int u = 0; u < kRuns; u++)
+#pragma unroll
+          for (int e = 0; e < V; e++) acc[u][e] += x[k][u][e] * f;
       }
     }
   }

@@ -197,18 +197,17 @@ __device__ __forceinline__ int entry_of(const Params& p, int pos) {
   return p.page_shift >= 0 ? pos >> p.page_shift : pos / (int)p.a.cache.page_size;
 }
 
-// The page of a position of the part, or -1 where there is none.
-__device__ __forceinline__ int page_of(const Params& p, const Work& w, int pos) {
+// The entry of a position's page as it lies in the list, -1 past its end. Not
+// looked at here, so that the load may be on its way until page_of is called.
+__device__ __forceinline__ int entry_at(const Params& p, const Work& w, int pos) {
   const int entry = entry_of(p, pos);
-  int page;
-  if (w.prefix || (p.solo && pos < (int)p.a.prefix)) {
-    if (pos >= (int)p.a.prefix) return -1;
-    page = p.a.prefix_pages[entry];
-  } else {
-    if (entry >= (int)p.a.cache.table_stride) return -1;
-    page = p.a.cache.table[(int64_t)w.seq * p.a.cache.table_stride + entry];
-  }
-  return page >= 0 && page < (int)p.a.cache.pages ? page : -1;
+  const bool shared = w.prefix || (p.solo && pos < (int)p.a.prefix);
+  const int* list = shared ? p.a.prefix_pages : p.a.cache.table + (int64_t)w.seq * p.a.cache.table_stride;
+  return (shared ? pos < (int)p.a.prefix : entry < (int)p.a.cache.table_stride) ? list[entry] : -1;
+}
+// The page that an entry names, or -1 where that is none.
+__device__ __forceinline__ int page_of(const Params& p, int entry) {
+  return entry >= 0 && entry < (int)p.a.cache.pages ? entry : -1;
 }
 
 // The slice's keys, begin .. end - 1, of the positions low .. high that the
@@ -225,12 +224,11 @@ __device__ __forceinline__ void slice_keys(const Params& p, const Work& w, int l
   end = (int)min((int64_t)high + 1, b + per);
 }
 
-// Element offset, in the pools, of the row of position pos (low <= pos < end)
-// of the block's kv head, or -1.
-__device__ __forceinline__ int64_t row_at(const Params& p, const Work& w, int pos, int low, int end) {
-  if (pos < low || pos >= end) return -1;
-  const int page = page_of(p, w, pos);
-  if (page < 0) return -1;
+// Element offset, in the pools, of the row of position pos of the block's kv
+// head, whose entry is `entry`, or -1; seen are positions low .. end - 1.
+__device__ __forceinline__ int64_t row_at(const Params& p, const Work& w, int entry, int pos, int low, int end) {
+  const int page = page_of(p, entry);
+  if (pos < low || pos >= end || page < 0) return -1;
   const int size = (int)p.a.cache.page_size;
   const int slot = p.page_shift >= 0 ? pos & (size - 1) : pos % size;
   return page * p.a.cache.page_stride + ((int64_t)w.head * size + slot) * p.a.cache.hd;

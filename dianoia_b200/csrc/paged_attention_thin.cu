@@ -129,15 +129,14 @@ __device__ __forceinline__ void thin_block(const Params& p, const Maps& maps, co
     }
   __syncwarp();
 
-  // The page of a step's keys (TMA), or lane l's row of key l % 16, is looked
-  // up one step ahead of the copies.
+  // The entry of a step's page (TMA), or of lane l's key l % 16, is on its way
+  // one step ahead of the copies.
   const int panels = (hd + 63) / 64;
   uint32_t there[S::kStages];  // which of a buffer's keys are there
-  int64_t at = -1;
+  int entry = -1;
   auto look_up = [&](int step) {
-    if (step >= steps) return;
     const int k0 = first + step * kTile;
-    at = TMA ? page_of(p, w, k0) : row_at(p, w, k0 + lane % kStep, any_low, end);
+    if (step < steps) entry = entry_at(p, w, TMA ? k0 : k0 + lane % kStep);
   };
   auto issue = [&](int step, int b) {
     if (step >= steps) return;
@@ -146,9 +145,9 @@ __device__ __forceinline__ void thin_block(const Params& p, const Maps& maps, co
     if constexpr (TMA) {
       const int k0 = first + step * kTile;
       // A page that is not there is one past the last, which reads as zeros.
-      const int page = at >= 0 ? (int)at : (int)p.a.cache.pages;
+      const int found = page_of(p, entry), page = found >= 0 ? found : (int)p.a.cache.pages;
       const int slot = k0 - entry_of(p, k0) * (int)p.a.cache.page_size;
-      there[b] = at >= 0 ? 0xffffu : 0u;
+      there[b] = found >= 0 ? 0xffffu : 0u;
       if (lane == 0) mbar_arrive_expect_tx(&full[b], (uint32_t)panels * 2 * S::kPanel);
       __syncwarp();
       if (lane < 2 * panels) {  // a copy a lane: the panels of the keys, then of the values
@@ -157,6 +156,7 @@ __device__ __forceinline__ void thin_block(const Params& p, const Maps& maps, co
                     w.head, page, &full[b]);
       }
     } else {
+      const int64_t at = row_at(p, w, entry, first + step * kTile + lane % kStep, any_low, end);
       there[b] = __ballot_sync(0xffffffffu, at >= 0) & 0xffffu;
       const T* keys = static_cast<const T*>(p.a.cache.keys);
       const T* vals = static_cast<const T*>(p.a.cache.values);

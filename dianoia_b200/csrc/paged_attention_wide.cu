@@ -152,9 +152,9 @@ __device__ __forceinline__ void softmax_rows(const Params& p, const Work& w, cha
   float m = -INFINITY, l = 0.0f;
   // Lanes 0 .. 7 know which 16 keys of the next tile have a page.
   auto look_up = [&](int tile) {
-    return lane < kKeys / 16 && tile < tiles && page_of(p, w, begin + tile * kKeys + 16 * lane) >= 0;
+    return lane < kKeys / 16 && tile < tiles ? entry_at(p, w, begin + tile * kKeys + 16 * lane) : -1;
   };
-  bool next_there = look_up(group);
+  int next_entry = look_up(group);
   bool live = true;
   auto done = [&](int j) {
     return __all_sync(0xffffffffu, wait_phase(&bars.o_done[j % kHalves], (j / kHalves) & 1, p.status,
@@ -162,8 +162,8 @@ __device__ __forceinline__ void softmax_rows(const Params& p, const Work& w, cha
   };
   int last = -1;  // the group's last half
   for (int i = group; i < tiles && live; i += S::kGroups) {
-    const unsigned tile_there = __ballot_sync(0xffffffffu, next_there);
-    next_there = look_up(i + S::kGroups);
+    const unsigned tile_there = __ballot_sync(0xffffffffu, page_of(p, next_entry) >= 0);
+    next_entry = look_up(i + S::kGroups);
     live = __all_sync(0xffffffffu, wait_phase(&bars.s_full[i % kScores], (i / kScores) & 1, p.status,
                                                      kStatusMmaTimeout));
     if (!live) break;
@@ -426,16 +426,16 @@ __global__ void __maxnreg__(136)
     const int g = lane / S::kPanels, c = lane % S::kPanels;
     const bool mine = g < 2 * groups && c < panels;
     const uint32_t row0 = (uint32_t)(g % groups * box * 128);
-    // The page of the lane's keys; one past the last reads as zeros.
     auto look_up = [&](int tile) {
-      const int page = mine && tile < tiles ? page_of(p, w, begin + tile * kKeys + g * box) : -1;
-      return page >= 0 ? page : (int)p.a.cache.pages;
+      return mine && tile < tiles ? entry_at(p, w, begin + tile * kKeys + g * box) : -1;
     };
     int ahead = look_up(0), page = 0, slot = 0;
     bool live = true;
     for (int i = 0; i <= tiles && live; i++) {  // the keys of tile i, then the values of tile i - 1
       const int page_v = page, slot_v = slot;
-      page = ahead;
+      // The page of the lane's keys; one past the last reads as zeros.
+      page = page_of(p, ahead);
+      page = page >= 0 ? page : (int)p.a.cache.pages;
       if (i < tiles) {
         const int pos = begin + i * kKeys + g * box;
         slot = pos - entry_of(p, pos) * (int)p.a.cache.page_size;
