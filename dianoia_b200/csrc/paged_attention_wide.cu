@@ -4,8 +4,8 @@
 // 128 rows of one kv head share every key, so the products are the bound:
 // S = Q K^T and O += P V on the 5th-generation tensor cores (tcgen05, f32
 // accumulators in TMEM). A block runs three parts at once:
-//   one warp brings tiles of 128 keys and their values by tiled TMA copies;
-//   a warp for each group issues its products;
+//   a warp for each group brings the group's tiles of 128 keys and their values
+//   by tiled TMA copies, a copy a lane, and issues its products;
 //   two groups of 4 warps (one for heads over 128 wide) take the even and the
 //   odd tiles, a row of S each thread: they read it from TMEM 64 keys (a half)
 //   at a time, keep the row's base and sum, and write P (16-bit) over it, which
@@ -51,11 +51,10 @@ struct Shape {
   static constexpr int kKPanel = kKeys * 128;  // of every key of a tile
   static constexpr int kVPanel = kHalf * 128;  // of every value of a half
   static constexpr int kGroups = wide_groups(HDP);
-  static constexpr int kThreads = kGroups * (kRowThreads + kLanes) + kLanes;
-  static constexpr int kKStages = HDP <= 128 ? 2 : 1, kVStages = HDP <= 128 ? 4 : 2;
+  static constexpr int kThreads = kGroups * (kRowThreads + kLanes);
   static constexpr int kK = kPanels * kQPanel;              // where the keys start
-  static constexpr int kV = kK + kKStages * kPanels * kKPanel;
-  static constexpr int kSmem = kV + kVStages * kPanels * kVPanel;
+  static constexpr int kV = kK + kGroups * kPanels * kKPanel;  // one tile of keys a group, and of values
+  static constexpr int kSmem = kV + kGroups * 2 * kPanels * kVPanel;
   static constexpr uint32_t kCols = 512;  // of TMEM: S, then each group's O
   static_assert(kScores * kKeys + kGroups * HDP <= 512, "TMEM");
 };
@@ -66,7 +65,7 @@ struct Shape {
 // P V of its tile before is done, so whoever waits for a half of either knows
 // the phase before it past.
 struct Bars {
-  uint64_t k_full[2], k_empty[2], v_full[4], v_empty[4], s_full[kScores], p_full[kHalves], o_done[kHalves];
+  uint64_t k_full[2], v_full[2], s_full[kScores], p_full[kHalves], o_done[kHalves];  // k, v: a group's
 };
 
 // Shared-memory operand, 128-byte swizzled; `lead` is the stride between
@@ -234,9 +233,9 @@ __device__ __forceinline__ void softmax_rows(const Params& p, const Work& w, cha
       l += (sum4[0] + sum4[1]) + (sum4[2] + sum4[3]);
       if (!all) {
         // The values have to be looked at, and may have to be added here.
-        char* vals = smem + S::kV + j % S::kVStages * S::kPanels * S::kVPanel;
-        live = __all_sync(0xffffffffu, wait_phase(&bars.v_full[j % S::kVStages], (j / S::kVStages) & 1,
-                                                         p.status, kStatusTmaTimeout));
+        char* vals = smem + S::kV + (2 * group + h) * S::kPanels * S::kVPanel;
+        live = __all_sync(0xffffffffu, wait_phase(&bars.v_full[group], (i / S::kGroups) & 1, p.status,
+                                                  kStatusTmaTimeout));
         if (!live) break;
         bool bad = false;
         for (int c = lane; c < S::kPanels * S::kVPanel / 16; c += kLanes) bad = bad || unbounded16<T>(vals + c * 16);
@@ -328,7 +327,7 @@ __device__ __forceinline__ void softmax_rows(const Params& p, const Work& w, cha
 }
 
 template <typename T, int HDP>
-__global__ void __maxnreg__(136)
+__global__ void __maxnreg__(152)
     attention_wide_kernel(const __grid_constant__ Params p, const __grid_constant__ Maps maps, int box) {
   using S = Shape<HDP>;
   pdl_wait();
@@ -342,20 +341,16 @@ __global__ void __maxnreg__(136)
   if (!find_work(p, w)) return;
   const int tid = threadIdx.x, warp = tid / kLanes, lane = tid % kLanes;
   const int hd = (int)p.a.cache.hd;
-  if (warp == kRowWarps + 1) {
+  if (warp == kRowWarps) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_at)),
                  "r"(S::kCols)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   if (tid == kRowWarps * kLanes) {
-    for (int i = 0; i < S::kKStages; i++) {
+    for (int i = 0; i < S::kGroups; i++) {
       mbar_init(&bars.k_full[i], 1);
-      mbar_init(&bars.k_empty[i], 1);
-    }
-    for (int i = 0; i < S::kVStages; i++) {
       mbar_init(&bars.v_full[i], 1);
-      mbar_init(&bars.v_empty[i], 1);
     }
     for (int i = 0; i < kScores; i++) mbar_init(&bars.s_full[i], 1);
     for (int i = 0; i < kHalves; i++) {
@@ -419,103 +414,99 @@ __global__ void __maxnreg__(136)
 
   if (warp < kRowWarps) {
     softmax_rows<T, HDP>(p, w, smem, bars, skip, tmem, begin, halves, tid / kRowThreads, low, high, all_low, all_high);
-  } else if (warp == kRowWarps) {
-    // One copy a lane: panel c of the keys (values) g * box .. of the tile, all
-    // of one page. (One lane issuing them all took 300 cycles a copy.)
+  } else {
+    const int group = warp - kRowWarps;
+    // One copy a lane: panel c of the keys (values) g * box .. of a tile, all
+    // of one page, whose entry is on its way a tile ahead. (One lane issuing
+    // them all took 300 cycles a copy; a third warp for both groups' copies
+    // was the bound, 3300 cycles a tile.)
     const int panels = (hd + 63) / 64, groups = kHalf / box;  // of a half
-    const int g = lane / S::kPanels, c = lane % S::kPanels;
-    const bool mine = g < 2 * groups && c < panels;
+    const int g = lane / S::kPanels, c = lane % S::kPanels, half = g / groups;
     const uint32_t row0 = (uint32_t)(g % groups * box * 128);
+    char* const k_at = smem + S::kK + group * S::kPanels * S::kKPanel + c * S::kKPanel + half * kHalf * 128 + row0;
+    char* const v_at = smem + S::kV + (2 * group + half) * S::kPanels * S::kVPanel + c * S::kVPanel + row0;
+    const bool mine = half < 2 && c < panels;
     auto look_up = [&](int tile) {
       return mine && tile < tiles ? entry_at(p, w, begin + tile * kKeys + g * box) : -1;
     };
-    int ahead = look_up(0), page = 0, slot = 0;
-    bool live = true;
-    for (int i = 0; i <= tiles && live; i++) {  // the keys of tile i, then the values of tile i - 1
-      const int page_v = page, slot_v = slot;
-      // The page of the lane's keys; one past the last reads as zeros.
-      page = page_of(p, ahead);
-      page = page >= 0 ? page : (int)p.a.cache.pages;
-      if (i < tiles) {
-        const int pos = begin + i * kKeys + g * box;
-        slot = pos - entry_of(p, pos) * (int)p.a.cache.page_size;
-        ahead = look_up(i + 1);
-        const int s = i % S::kKStages, parts = min(2, halves - 2 * i);
-        if (i >= S::kKStages)
-          live = __all_sync(0xffffffffu, wait_phase(&bars.k_empty[s], (i / S::kKStages - 1) & 1, p.status,
-                                                    kStatusMmaTimeout));
-        if (!live) break;
-        if (lane == 0) mbar_arrive_expect_tx(&bars.k_full[s], (uint32_t)(parts * panels * S::kVPanel));
-        __syncwarp();
-        if (mine && g < parts * groups)
-          tma_load_4d(smem + S::kK + s * S::kPanels * S::kKPanel + c * S::kKPanel + g / groups * kHalf * 128 + row0,
-                      &maps.keys, 64 * c, slot, w.head, page, &bars.k_full[s]);
-      }
-      for (int h = 0; h < 2 && i > 0; h++) {
-        const int j = 2 * i - 2 + h, s = j % S::kVStages;
-        if (j >= halves) break;
-        if (j >= S::kVStages)
-          live = __all_sync(0xffffffffu, wait_phase(&bars.v_empty[s], (j / S::kVStages - 1) & 1, p.status,
-                                                    kStatusMmaTimeout));
-        if (!live) break;
-        if (lane == 0) mbar_arrive_expect_tx(&bars.v_full[s], (uint32_t)(panels * S::kVPanel));
-        __syncwarp();
-        if (mine && g / groups == h)
-          tma_load_4d(smem + S::kV + s * S::kPanels * S::kVPanel + c * S::kVPanel + row0, &maps.values, 64 * c, slot_v,
-                      w.head, page_v, &bars.v_full[s]);
-      }
-    }
-  } else {
+    // The page of the lane's keys; one past the last reads as zeros.
+    auto page_at = [&](int entry) {
+      const int page = page_of(p, entry);
+      return page >= 0 ? page : (int)p.a.cache.pages;
+    };
+    auto slot_at = [&](int tile) {
+      const int pos = begin + tile * kKeys + g * box;
+      return pos - entry_of(p, pos) * (int)p.a.cache.page_size;
+    };
+    auto load = [&](const CUtensorMap* map, char* dst, int tile, int page, int slot, uint64_t* full) {
+      const int parts = min(2, halves - 2 * tile);
+      if (lane == 0) mbar_arrive_expect_tx(full, (uint32_t)(parts * panels * S::kVPanel));
+      __syncwarp();
+      if (mine && half < parts) tma_load_4d(dst, map, 64 * c, slot, w.head, page, full);
+    };
     constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
     constexpr uint32_t kQk = idesc(kBf16, kKeys, false), kPv = idesc(kBf16, HDP, true);
     // Operands' descriptors; the address field counts 16 bytes, so an offset adds.
     const uint32_t q = smem_u32(smem);
-    const uint64_t q_desc = desc(q, 16), k_desc = desc(q + S::kK, 16), v_desc = desc(q + S::kV, S::kVPanel);
+    const uint64_t q_desc = desc(q, 16), k_desc = desc(q + S::kK + group * S::kPanels * S::kKPanel, 16),
+                   v_desc = desc(q + S::kV + group * 2 * S::kPanels * S::kVPanel, S::kVPanel);
     const int steps = (hd + 15) / 16;
-    const int group = warp - kRowWarps - 1;
     const uint32_t out = tmem + kScores * kKeys + (uint32_t)(group * HDP);
-    if (elect_one()) {
-      bool live = true;
-      int last = -1;  // the group's last half
-      for (int i = group; i < tiles && live; i += S::kGroups) {
-        const int s = i % S::kKStages;
-        // S's place is free once P V of the group's last tile has read P there.
-        if (last >= 0) live = wait_phase(&bars.o_done[last % kHalves], (last / kHalves) & 1, p.status, kStatusMmaTimeout);
-        live = live && wait_phase(&bars.k_full[s], (i / S::kKStages) & 1, p.status, kStatusTmaTimeout);
+    const bool leader = elect_one();
+    auto wait = [&](uint64_t* bar, int phase, uint32_t bits) {
+      return __all_sync(0xffffffffu, wait_phase(bar, phase & 1, p.status, bits));
+    };
+    int page = page_at(look_up(group)), slot = slot_at(group), next = look_up(group + S::kGroups);
+    if (group < tiles) load(&maps.keys, k_at, group, page, slot, &bars.k_full[group]);
+    bool live = true;
+    int last = -1;  // the group's last half
+    for (int i = group; i < tiles && live; i += S::kGroups) {
+      const int turn = i / S::kGroups, page_k = page_at(next), slot_k = slot_at(i + S::kGroups);
+      next = look_up(i + 2 * S::kGroups);
+      // S's place, and the values', are free once P V of the group's last tile is done.
+      if (last >= 0) live = wait(&bars.o_done[last % kHalves], last / kHalves, kStatusMmaTimeout);
+      live = live && wait(&bars.k_full[group], turn, kStatusTmaTimeout);
+      if (!live) break;
+      fence_after();
+      if (leader) {
+#pragma unroll
+        for (int e = 0; e < HDP / 16; e++)
+          if (e < steps)
+            mma_ss(tmem + (uint32_t)(i % kScores) * kKeys, q_desc + (uint32_t)((e / 4 * S::kQPanel + e % 4 * 32) >> 4),
+                   k_desc + (uint32_t)((e / 4 * S::kKPanel + e % 4 * 32) >> 4), kQk, e > 0 ? 1u : 0u);
+        commit(&bars.s_full[i % kScores]);
+      }
+      __syncwarp();
+      load(&maps.values, v_at, i, page, slot, &bars.v_full[group]);
+      page = page_k;
+      slot = slot_k;
+      for (int j = 2 * i; j < min(2 * i + 2, halves); j++) {
+        live = wait(&bars.v_full[group], turn, kStatusTmaTimeout) &&
+               wait(&bars.p_full[j % kHalves], j / kHalves, kStatusMmaTimeout);
         if (!live) break;
         fence_after();
-        const uint64_t k = k_desc + (uint32_t)(s * S::kPanels * S::kKPanel >> 4);
-#pragma unroll
-        for (int c = 0; c < HDP / 16; c++)
-          if (c < steps)
-            mma_ss(tmem + (uint32_t)(i % kScores) * kKeys, q_desc + (uint32_t)((c / 4 * S::kQPanel + c % 4 * 32) >> 4),
-                   k + (uint32_t)((c / 4 * S::kKPanel + c % 4 * 32) >> 4), kQk, c > 0 ? 1u : 0u);
-        commit(&bars.s_full[i % kScores]);
-        commit(&bars.k_empty[s]);
-        for (int j = 2 * i; j < min(2 * i + 2, halves); j++) {
-          const int vs = j % S::kVStages;
-          live = wait_phase(&bars.v_full[vs], (j / S::kVStages) & 1, p.status, kStatusTmaTimeout) &&
-                 wait_phase(&bars.p_full[j % kHalves], (j / kHalves) & 1, p.status, kStatusMmaTimeout);
-          if (!live) break;
-          fence_after();
+        if (leader) {
           if (skip[j % kHalves] == 0) {
-            const uint64_t v = v_desc + (uint32_t)(vs * S::kPanels * S::kVPanel >> 4);
+            const uint64_t v = v_desc + (uint32_t)(j % 2 * S::kPanels * S::kVPanel >> 4);
             const uint32_t pr = tmem + (uint32_t)(j % kHalves) * kHalf;
 #pragma unroll
-            for (int c = 0; c < kHalf / 16; c++)
-              mma_ts(out, pr + 8 * c, v + (uint32_t)(c * 2048 >> 4), kPv, c > 0 || last >= 0 ? 1u : 0u);
+            for (int e = 0; e < kHalf / 16; e++)
+              mma_ts(out, pr + 8 * e, v + (uint32_t)(e * 2048 >> 4), kPv, e > 0 || last >= 0 ? 1u : 0u);
           }
           commit(&bars.o_done[j % kHalves]);
-          commit(&bars.v_empty[vs]);
-          last = j;
         }
+        __syncwarp();
+        last = j;
+        // P is there, so S is: its keys' place is free.
+        if (j == 2 * i && i + S::kGroups < tiles)
+          load(&maps.keys, k_at, i + S::kGroups, page_k, slot_k, &bars.k_full[group]);
       }
     }
     __syncwarp();
   }
   fence_before();
   __syncthreads();
-  if (warp == kRowWarps + 1) {
+  if (warp == kRowWarps) {
     fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::kCols) : "memory");
   }
