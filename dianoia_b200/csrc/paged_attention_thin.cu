@@ -82,6 +82,12 @@ struct Shape {
   static constexpr int kRing = kStages * 2 * kBuf;        // a warp's
 };
 
+// Bytes of a block's rings, which the warps' results take over at the end.
+constexpr int smem_tiles(int hdp, int nt) {
+  const int ring = kWarps * 2 * 2 * kStep * hdp * 2, join = kWarps * 8 * nt * ((hdp + 4) * 4 + 8);
+  return ring > join ? ring : join;
+}
+
 // Byte offset of 16-byte chunk c (8 elements) of key r of a step.
 __device__ __forceinline__ uint32_t chunk_at(int r, int c) {
   return (uint32_t)((c >> 3) * (kStep * 128) + r * 128 + (((c ^ r) & 7) << 4));
@@ -392,7 +398,8 @@ __global__ void __launch_bounds__(kThreads)
   // nothing to wait for but its end, before this grid's: one block does.
   if (!p.beside) pdl_wait();
   extern __shared__ __align__(1024) char smem[];
-  __shared__ uint64_t bars[kWarps * Shape<HDP>::kStages];
+  // (No static shared memory: it would be rounded up to this alignment.)
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + smem_tiles(HDP, NT));
   Work w;
   if (find_work(p, w)) thin_block<T, HDP, NT, TMA>(p, maps, w, smem, bars);
   if (p.beside && blockIdx.x == 0 && blockIdx.y == 0) pdl_wait();
@@ -400,9 +407,8 @@ __global__ void __launch_bounds__(kThreads)
 
 template <typename T, int HDP, int NT, bool TMA>
 cudaError_t launch_copies(const Params& p, const Maps& maps, cudaStream_t stream, bool pdl) {
-  constexpr int ring = kWarps * Shape<HDP>::kRing;
-  constexpr int join = kWarps * 8 * NT * ((HDP + 4) * 4 + 8);
-  constexpr int smem = ring > join ? ring : join;
+  static_assert(smem_tiles(HDP, NT) >= kWarps * Shape<HDP>::kRing, "rings");
+  constexpr int smem = smem_tiles(HDP, NT) + kWarps * Shape<HDP>::kStages * 8;
   if (cudaError_t e = allow_smem(attention_thin_kernel<T, HDP, NT, TMA>, smem); e != cudaSuccess) return e;
   return launch_ex(attention_thin_kernel<T, HDP, NT, TMA>, attention_grid(p), kThreads, smem, stream, pdl, p, maps);
 }

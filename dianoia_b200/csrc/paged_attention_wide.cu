@@ -47,6 +47,9 @@ struct alignas(64) Maps {
 template <int HDP>
 struct Shape {
   static constexpr int kPanels = HDP / 64;
+  // With two groups, three warps to a quarter of the SM: 128 registers leave a
+  // warp of a thin block (128) its place in the quarter's 16384.
+  static constexpr int kRegs = wide_groups(HDP) == 2 ? 128 : 168;
   static constexpr int kQPanel = kRows * 128;  // bytes: 64 elements of every row
   static constexpr int kKPanel = kKeys * 128;  // of every key of a tile
   static constexpr int kVPanel = kHalf * 128;  // of every value of a half
@@ -66,6 +69,14 @@ struct Shape {
 // the phase before it past.
 struct Bars {
   uint64_t k_full[2], v_full[2], s_full[kScores], p_full[kHalves], o_done[kHalves];  // k, v: a group's
+};
+
+// What stands in shared memory behind the tiles.
+template <int HDP>
+struct Control {
+  Bars bars;
+  uint32_t tmem_at, skip[kHalves];
+  int span[Shape<HDP>::kGroups * kRowThreads / kLanes][4];
 };
 
 // Shared-memory operand, 128-byte swizzled; `lead` is the stride between
@@ -327,22 +338,25 @@ __device__ __forceinline__ void softmax_rows(const Params& p, const Work& w, cha
 }
 
 template <typename T, int HDP>
-__global__ void __maxnreg__(152)
+__global__ void __maxnreg__(Shape<HDP>::kRegs)
     attention_wide_kernel(const __grid_constant__ Params p, const __grid_constant__ Maps maps, int box) {
   using S = Shape<HDP>;
   pdl_wait();
   pdl_launch_dependents();  // after the wait: what starts now may read this kernel's inputs
   extern __shared__ __align__(1024) char smem[];
-  __shared__ Bars bars;
-  __shared__ uint32_t tmem_at, skip[kHalves];
+  // No static shared memory: it would be rounded up to the tiles' alignment,
+  // and a thin block would no longer fit beside this one.
+  Control<HDP>& ctl = *reinterpret_cast<Control<HDP>*>(smem + S::kSmem);
+  Bars& bars = ctl.bars;
+  uint32_t* const skip = ctl.skip;
   constexpr int kRowWarps = S::kGroups * kRowThreads / kLanes;
-  __shared__ int span[kRowWarps][4];
+  auto& span = ctl.span;
   Work w;
   if (!find_work(p, w)) return;
   const int tid = threadIdx.x, warp = tid / kLanes, lane = tid % kLanes;
   const int hd = (int)p.a.cache.hd;
   if (warp == kRowWarps) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_at)),
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&ctl.tmem_at)),
                  "r"(S::kCols)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -399,7 +413,7 @@ __global__ void __maxnreg__(152)
   fence_before();
   __syncthreads();
   fence_after();
-  const uint32_t tmem = tmem_at;
+  const uint32_t tmem = ctl.tmem_at;
   int all_low = span[0][0], all_high = span[0][1], any_low = span[0][2], any_high = span[0][3];
 #pragma unroll
   for (int i = 1; i < kRowWarps; i++) {
@@ -478,9 +492,12 @@ __global__ void __maxnreg__(152)
       }
       __syncwarp();
       load(&maps.values, v_at, i, page, slot, &bars.v_full[group]);
+      // S is there: its keys' place is free.
+      live = wait(&bars.s_full[i % kScores], i / kScores, kStatusMmaTimeout);
+      if (live && i + S::kGroups < tiles) load(&maps.keys, k_at, i + S::kGroups, page_k, slot_k, &bars.k_full[group]);
       page = page_k;
       slot = slot_k;
-      for (int j = 2 * i; j < min(2 * i + 2, halves); j++) {
+      for (int j = 2 * i; j < min(2 * i + 2, halves) && live; j++) {
         live = wait(&bars.v_full[group], turn, kStatusTmaTimeout) &&
                wait(&bars.p_full[j % kHalves], j / kHalves, kStatusMmaTimeout);
         if (!live) break;
@@ -497,9 +514,6 @@ __global__ void __maxnreg__(152)
         }
         __syncwarp();
         last = j;
-        // P is there, so S is: its keys' place is free.
-        if (j == 2 * i && i + S::kGroups < tiles)
-          load(&maps.keys, k_at, i + S::kGroups, page_k, slot_k, &bars.k_full[group]);
       }
     }
     __syncwarp();
@@ -522,8 +536,9 @@ cudaError_t launch_size(const Params& p, cudaStream_t stream, bool pdl) {
         encode_tmap_pages(&maps.values, c.values, c.type == kBF16, c.hd, c.page_size, c.kv_heads, c.pages,
                           c.page_stride, box)))
     return cudaErrorInvalidValue;
-  if (cudaError_t e = allow_smem(attention_wide_kernel<T, HDP>, Shape<HDP>::kSmem); e != cudaSuccess) return e;
-  return launch_ex(attention_wide_kernel<T, HDP>, attention_grid(p), Shape<HDP>::kThreads, Shape<HDP>::kSmem, stream, pdl, p, maps,
+  constexpr int smem = Shape<HDP>::kSmem + (int)sizeof(Control<HDP>);
+  if (cudaError_t e = allow_smem(attention_wide_kernel<T, HDP>, smem); e != cudaSuccess) return e;
+  return launch_ex(attention_wide_kernel<T, HDP>, attention_grid(p), Shape<HDP>::kThreads, smem, stream, pdl, p, maps,
                    box);
 }
 
