@@ -19,6 +19,7 @@
 #include "dn_common.cuh"
 #include "dn_launch.h"
 #include "elem.cuh"
+#include "kernel_smem.h"
 
 namespace dn {
 namespace {
@@ -194,10 +195,7 @@ template <typename T, bool BULK>
 cudaError_t launch_copies(const LogitsArgs& a, cudaStream_t stream, bool pdl) {
   const int64_t chunks = (a.vocab + 16 / (int64_t)sizeof(T) - 1 + kChunk - 1) / kChunk;
   if (chunks * a.n > 0x7fffffff) return cudaErrorInvalidValue;
-  if (cudaError_t e = cudaFuncSetAttribute(logits_kernel<T, BULK>, cudaFuncAttributePreferredSharedMemoryCarveout,
-                                           cudaSharedmemCarveoutMaxShared);
-      e != cudaSuccess)
-    return e;
+  if (cudaError_t e = allow_smem<logits_kernel<T, BULK>>(0); e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(chunks * a.n));
   cfg.blockDim = dim3(kThreads);

@@ -14,6 +14,7 @@
 #include "dn_common.cuh"
 #include "dn_launch.h"
 #include "elem.cuh"
+#include "kernel_smem.h"
 
 namespace dn {
 namespace paged {
@@ -259,15 +260,6 @@ constexpr int wide_groups(int64_t hd) { return hd <= 128 ? 2 : 1; }
 inline dim3 attention_grid(const Params& p) {
   return dim3((unsigned)(p.prefix_tiles * p.prefix_splits + p.own_slots * p.own_splits),
               (unsigned)p.a.cache.kv_heads);
-}
-
-// Dynamic shared memory of a kernel, with the SM's whole split for it: blocks
-// of two kernels stay on one SM only under the same split.
-template <typename K>
-inline cudaError_t allow_smem(K kern, int bytes) {
-  if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes); e != cudaSuccess)
-    return e;
-  return cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
 }
 
 template <typename K, typename... Args>

@@ -409,7 +409,7 @@ template <typename T, int HDP, int NT, bool TMA>
 cudaError_t launch_copies(const Params& p, const Maps& maps, cudaStream_t stream, bool pdl) {
   static_assert(smem_tiles(HDP, NT) >= kWarps * Shape<HDP>::kRing, "rings");
   constexpr int smem = smem_tiles(HDP, NT) + kWarps * Shape<HDP>::kStages * 8;
-  if (cudaError_t e = allow_smem(attention_thin_kernel<T, HDP, NT, TMA>, smem); e != cudaSuccess) return e;
+  if (cudaError_t e = allow_smem<attention_thin_kernel<T, HDP, NT, TMA>>(smem); e != cudaSuccess) return e;
   return launch_ex(attention_thin_kernel<T, HDP, NT, TMA>, attention_grid(p), kThreads, smem, stream, pdl, p, maps);
 }
 

@@ -537,7 +537,7 @@ cudaError_t launch_size(const Params& p, cudaStream_t stream, bool pdl) {
                           c.page_stride, box)))
     return cudaErrorInvalidValue;
   constexpr int smem = Shape<HDP>::kSmem + (int)sizeof(Control<HDP>);
-  if (cudaError_t e = allow_smem(attention_wide_kernel<T, HDP>, smem); e != cudaSuccess) return e;
+  if (cudaError_t e = allow_smem<attention_wide_kernel<T, HDP>>(smem); e != cudaSuccess) return e;
   return launch_ex(attention_wide_kernel<T, HDP>, attention_grid(p), Shape<HDP>::kThreads, smem, stream, pdl, p, maps,
                    box);
 }
