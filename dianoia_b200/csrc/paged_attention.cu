@@ -195,7 +195,8 @@ __global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(const __gr
   constexpr int kRuns = kMaxPagedHd / (kLanes * V);
   const int lane = threadIdx.x % kLanes, hd = (int)p.a.cache.hd;
   const int t = (int)((uint32_t)row / (uint32_t)p.a.heads), head = (int)((uint32_t)row % (uint32_t)p.a.heads);
-  const bool covered = p.a.q_start == nullptr || seq_of(p, t) >= 0;
+  // Whether the token belongs to a sequence.
+  const bool covered = t >= seq_start(p, 0) && t < seq_start(p, (int)p.a.cache.sequences);
   const int slices = p.slices;
   const float2 first = lane < slices ? p.ml[lane * rows + row] : make_float2(-INFINITY, 0.0f);
   float m = first.x;
@@ -264,6 +265,11 @@ bool mma_cache(const PagedCache& c) {
 constexpr int64_t kSoloKeys = 512;    // of the longest sequence
 constexpr int64_t kSoloReads = 8192;  // keys of the prefix, once for each sequence
 
+// Least keys of a slice: of the thin kernel, the f32 one, and a wide block of
+// two groups and of one (24 ragged sequences on 2048 keys: 28 us with 512, 29
+// with 256, 33 with 1024; with 256-wide heads 29 us with 128, 32 with 256).
+constexpr int kThinLeast = 256, kSimtLeast = 128, kWide2Least = 512, kWide1Least = 128;
+
 // How the work is divided, from sizes that the host knows.
 Params plan(const PagedCache& c, int64_t heads, int64_t n, int64_t prefix, int64_t max_length) {
   Params p{};
@@ -288,20 +294,23 @@ Params plan(const PagedCache& c, int64_t heads, int64_t n, int64_t prefix, int64
   p.prefix_rows = p.prefix_wide ? kWideRows : p.thin_rows;
   p.own_rows = p.own_wide ? kWideRows : p.thin_rows;
   p.own_rows_log2 = 31 - __builtin_clz((unsigned)p.own_rows);
-  p.min_slice = mma_cache(c) ? 128 : 64;
   const int64_t tiles = (rows + p.prefix_rows - 1) / p.prefix_rows;
   p.prefix_tiles = prefix > 0 ? (int)tiles : 0;
   p.own_slots = (int)(rows / p.own_rows + c.sequences);
-  // A part's keys are split as long as blocks are wanting and a slice keeps
-  // min_slice keys: four thin or f32 blocks to an SM, one wide.
-  auto splits = [&](int64_t blocks, int64_t keys, bool on_wide) {
+  // A part's keys are split as long as blocks are wanting (four thin or f32
+  // blocks to an SM, one wide) and a slice keeps its least keys: shorter ones
+  // cost the join more than they save the slices.
+  const int wide_least = wide_groups(c.hd) == 2 ? kWide2Least : kWide1Least;
+  p.prefix_least = p.prefix_wide ? wide_least : mma_cache(c) ? kThinLeast : kSimtLeast;
+  p.own_least = p.own_wide ? wide_least : mma_cache(c) ? kThinLeast : kSimtLeast;
+  auto splits = [&](int64_t blocks, int64_t keys, bool on_wide, int64_t least_keys) {
     const int64_t want = on_wide ? 148 / (blocks > 0 ? blocks : 1) : (4 * 148 + blocks - 1) / (blocks > 0 ? blocks : 1);
-    const int64_t most = (keys + p.min_slice - 1) / p.min_slice, least = want < most ? want : most;
+    const int64_t most = (keys + least_keys - 1) / least_keys, least = want < most ? want : most;
     return (int)(least > 1 ? least : 1);
   };
-  p.prefix_splits = prefix > 0 ? splits(tiles * c.kv_heads, prefix, p.prefix_wide) : 0;
+  p.prefix_splits = prefix > 0 ? splits(tiles * c.kv_heads, prefix, p.prefix_wide, p.prefix_least) : 0;
   const int64_t own = max_length > prefix ? max_length - prefix : 1;
-  p.own_splits = splits((int64_t)p.own_slots * c.kv_heads, own, p.own_wide);
+  p.own_splits = splits((int64_t)p.own_slots * c.kv_heads, own, p.own_wide, p.own_least);
   p.prefix_slices = p.prefix_splits * (p.prefix_wide ? wide_groups(c.hd) : 1);
   p.slices = p.prefix_slices + p.own_splits * (p.own_wide ? wide_groups(c.hd) : 1);
   p.direct = p.slices == 1;

@@ -31,7 +31,7 @@ struct Params {
   bool beside;          // this launch runs beside the one before it
   int prefix_tiles, prefix_splits;
   int own_slots, own_splits;
-  int min_slice;        // keys: slices are not made shorter than this
+  int prefix_least, own_least;  // keys: slices are not made shorter than this
   int prefix_slices, slices;  // results of a row: of the prefix, in all
   float* acc;           // [slices][n * heads][hd]
   float2* ml;           // [slices][n * heads]: m, l
@@ -218,7 +218,7 @@ __device__ __forceinline__ void slice_keys(const Params& p, const Work& w, int l
   begin = end = 0;
   if (high < low) return;
   const int lo = low / tile * tile, keys = high - lo + 1;
-  int per = max((keys + w.splits - 1) / w.splits, p.min_slice);
+  int per = max((keys + w.splits - 1) / w.splits, w.prefix ? p.prefix_least : p.own_least);
   per = (per + tile - 1) / tile * tile;
   const int64_t b = lo + (int64_t)w.slice * per;
   begin = (int)min((int64_t)high + 1, b);
