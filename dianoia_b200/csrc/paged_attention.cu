@@ -21,6 +21,9 @@ namespace {
 // exchanges for 32 sums), which leaves lane l with the score of key l / RT for
 // row l % RT; each probability goes back to all lanes for the values. A block's
 // 4 warps take steps in turn and are joined once at the end.
+// Measured: 7 sequences of 680 keys, 8 kv heads of 128, 2 heads a group, window
+// 600: 12.5 us with the join (46 us with tiles in shared memory, where a block's
+// 16 rows were mostly empty).
 constexpr int kSimtThreads = 128;
 constexpr int kSimtWarps = kSimtThreads / kLanes;
 constexpr float kSlack = 8.0f;  // log2 units a score may pass the running base

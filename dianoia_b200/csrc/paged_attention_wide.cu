@@ -20,6 +20,10 @@
 // after. Where rows of the block see different keys of a half and a value
 // there is not finite, that half's P V is added term by term instead
 // (0 * infinity would be NaN).
+// Measured: 768 rows on 8192 keys of 8 kv heads of 128, bf16, in 50 us alone
+// (520 TFLOP/s); a group's tile takes some 5800 cycles, 3600 of them softmax
+// (the exponentials' unit for half of that, with both groups in step) and 2150
+// the way from the last P through P V, its commit and the next S.
 #include <type_traits>
 
 #include "dn_tmap.h"

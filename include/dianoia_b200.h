@@ -489,7 +489,8 @@ typedef struct dn_logit_rules {
   /* Penalties for repeated tokens (history NULL: none). Row r's tokens so far
    * are tokens[history[r]] .. tokens[history[r + 1] - 1]; its last
    * generated[r] of them were generated (generated NULL: all). Ids outside
-   * [0, vocab) are ignored. NULL penalties are neutral. */
+   * [0, vocab) are ignored. NULL penalties are neutral. A row has fewer than
+   * 2^31 tokens, and biases. */
   const int32_t* tokens;
   const int64_t* history;   /* [n + 1] */
   const int32_t* generated; /* [n] */
