@@ -151,6 +151,29 @@ __device__ __forceinline__ void st32(uint32_t addr, const uint32_t (&v)[32]) {
 }
 __device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+// Two f32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+      "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "add.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+
 // A group's part, of tiles group, group + kGroups, ...; `halves` in all of the
 // block; row `r` of the block is the thread's.
 template <typename T, int HDP>
@@ -207,7 +230,8 @@ __device__ __forceinline__ void softmax_rows(const Params& p, const Work& w, cha
       }
       float top4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int e = 0; e < kHalf; e++) top4[e % 4] = fmaxf(top4[e % 4], s[e / 32][e % 32]);
+      for (int e = 0; e < kHalf; e += 2)
+        top4[e / 2 % 4] = max3(top4[e / 2 % 4], s[e / 32][e % 32], s[e / 32][e % 32 + 1]);
       const float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3])) * scale;
       bool waited = last < 0;
       if (__any_sync(0xffffffffu, top > m + kSlack)) {
@@ -235,17 +259,19 @@ __device__ __forceinline__ void softmax_rows(const Params& p, const Work& w, cha
       }
       const float base = m == -INFINITY ? 0.0f : m;
       uint32_t pk[32];
-      float sum4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      float2 sums[2] = {};
 #pragma unroll
       for (int e = 0; e < kHalf; e += 2) {
-        const float x = exp2_fast(fmaf(s[e / 32][e % 32], scale, -base));
-        const float y = exp2_fast(fmaf(s[e / 32][e % 32 + 1], scale, -base));
-        s[e / 32][e % 32] = x;
-        s[e / 32][e % 32 + 1] = y;
-        sum4[e / 2 % 4] += x + y;
-        pk[e / 2] = Pair<T>::pack(x, y);
+        float2 x = fma2(make_float2(s[e / 32][e % 32], s[e / 32][e % 32 + 1]), make_float2(scale, scale),
+                        make_float2(-base, -base));
+        x.x = exp2_fast(x.x);
+        x.y = exp2_fast(x.y);
+        s[e / 32][e % 32] = x.x;
+        s[e / 32][e % 32 + 1] = x.y;
+        sums[e / 2 % 2] = add2(sums[e / 2 % 2], x);
+        pk[e / 2] = Pair<T>::pack(x.x, x.y);
       }
-      l += (sum4[0] + sum4[1]) + (sum4[2] + sum4[3]);
+      l += (sums[0].x + sums[0].y) + (sums[1].x + sums[1].y);
       if (!all) {
         // The values have to be looked at, and may have to be added here.
         char* vals = smem + S::kV + (2 * group + h) * S::kPanels * S::kVPanel;
