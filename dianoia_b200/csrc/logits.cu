@@ -12,9 +12,9 @@
 // CTAs to an SM keep 96 KB on the way), and leave by another. Meanwhile the
 // CTA counts the history's tokens that fall into its range (integer atomics:
 // their order changes nothing) and lists them with those that have biases;
-// then the listed tokens, few of the range, are worked out one a thread, the
-// biases added by one warp in list order, and under a mask the range is passed
-// over once. There is no count array in memory and one launch; the history is
+// then the listed tokens, few of the range, are worked out one a thread, which
+// adds the token's biases in list order (one warp does where a range has more
+// than kFew of them), and under a mask the range is passed over once. There is no count array in memory and one launch; the history is
 // read by every CTA of the row, from L2.
 // Measured: 256 rows of 151936 f32 logits in 66 us (4.8 TB/s of logits in and
 // out; holding them in registers 83 us, chunks of 2048 67 us); 64 rows behind
@@ -30,6 +30,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kChunk = 4096;
 constexpr int kListed = 512;  // tokens the list holds; with more, all of the range are looked at
+constexpr int kFew = 32;       // biases of a range that their tokens' threads add themselves
 constexpr uint32_t kBiased = 1u << 31;
 
 __device__ __forceinline__ void bulk_s2g(void* dst, const void* src, uint32_t bytes) {
@@ -46,12 +47,13 @@ __global__ void __launch_bounds__(kThreads) logits_kernel(const __grid_constant_
   constexpr int V = 16 / sizeof(T);
   __shared__ __align__(128) T x[kChunk];
   // Of each token of the range: bit 0 whether seen, bit 31 whether it has a
-  // bias, between them how often it was generated; then, of a listed token,
-  // the bits of its f32 result.
+  // bias, between them how often it was generated.
   __shared__ __align__(16) uint32_t marks[kChunk];
   __shared__ uint16_t list[kListed];
   __shared__ uint32_t words[kChunk / 32 + 2];
-  __shared__ int listed;
+  __shared__ int listed, few;  // tokens listed; biases of the range
+  __shared__ int few_at[kFew], few_order[kFew];
+  __shared__ float few_add[kFew];
   __shared__ uint64_t full;
   const int tid = threadIdx.x;
   const int64_t row = blockIdx.x / (unsigned)chunks;
@@ -74,7 +76,7 @@ __global__ void __launch_bounds__(kThreads) logits_kernel(const __grid_constant_
       mbar_arrive_expect_tx(&full, (uint32_t)((to - from) * sizeof(T)));
       bulk_g2s(&x[from], in + base + from, (uint32_t)((to - from) * sizeof(T)), &full);
     }
-    listed = 0;
+    listed = few = 0;
   }
   // What no bulk copy takes (all of it without BULK).
   for (int at = begin + tid; at < min(from, end); at += kThreads) x[at] = in[base + at];
@@ -99,6 +101,15 @@ __global__ void __launch_bounds__(kThreads) logits_kernel(const __grid_constant_
   const int64_t mrow = r.mask == nullptr ? -1 : r.mask_row != nullptr ? r.mask_row[row] : row;
   const uint32_t* mask = mrow >= 0 && mrow < r.mask_rows ? r.mask + mrow * r.mask_stride : nullptr;
   const bool marked = seen > 0 || biased > 0;
+  // The first tokens and biases are on their way while the marks are cleared.
+  constexpr int kAtOnce = 8;
+  uint32_t at[kAtOnce], first_bias = tid < biased ? (uint32_t)(bias_tokens[tid] - base) : 0xffffffffu;
+  auto load_tokens = [&](int i0) {
+#pragma unroll
+    for (int k = 0; k < kAtOnce; k++)
+      at[k] = i0 + k * kThreads < seen ? (uint32_t)(tokens[i0 + k * kThreads] - base) : 0xffffffffu;
+  };
+  load_tokens(tid);
   const int word0 = (base + begin) / 32;  // of words[0]
   if (marked) {
 #pragma unroll
@@ -112,12 +123,8 @@ __global__ void __launch_bounds__(kThreads) logits_kernel(const __grid_constant_
     if (j < kListed) list[j] = (uint16_t)at;
   };
   auto mine = [&](uint32_t at) { return at < (uint32_t)end && at >= (uint32_t)begin; };
-  constexpr int kAtOnce = 8;
   for (int i0 = tid; i0 < seen; i0 += kThreads * kAtOnce) {
-    uint32_t at[kAtOnce];
-#pragma unroll
-    for (int k = 0; k < kAtOnce; k++)
-      at[k] = i0 + k * kThreads < seen ? (uint32_t)(tokens[i0 + k * kThreads] - base) : 0xffffffffu;
+    if (i0 != tid) load_tokens(i0);
 #pragma unroll
     for (int k = 0; k < kAtOnce; k++)
       if (mine(at[k])) {
@@ -126,13 +133,20 @@ __global__ void __launch_bounds__(kThreads) logits_kernel(const __grid_constant_
       }
   }
   for (int i = tid; i < biased; i += kThreads) {
-    const uint32_t at = (uint32_t)(bias_tokens[i] - base);
-    if (mine(at) && atomicOr(&marks[at], kBiased) == 0) add_to_list(at);
+    const uint32_t v = i == tid ? first_bias : (uint32_t)(bias_tokens[i] - base);
+    if (!mine(v)) continue;
+    const int j = atomicAdd(&few, 1);
+    if (j < kFew) {
+      few_at[j] = (int)v;
+      few_order[j] = i;
+      few_add[j] = bias[i];
+    }
+    if (atomicOr(&marks[v], kBiased) == 0) add_to_list(v);
   }
   if (to > from && !mbar_wait_bounded(&full, 0, a.status, kStatusTmaTimeout)) seen = biased = 0;
   __syncthreads();
 
-  // The marked tokens: f32 results in place of their marks.
+  // The marked tokens.
   const int count = marked ? listed : 0;
   const bool fits = count <= kListed;
   auto each_marked = [&](auto&& f) {
@@ -146,18 +160,40 @@ __global__ void __launch_bounds__(kThreads) logits_kernel(const __grid_constant_
     const float rep = r.repetition != nullptr ? r.repetition[row] : 1.0f;
     const float freq = r.frequency != nullptr ? r.frequency[row] : 0.0f;
     const float pres = r.presence != nullptr ? r.presence[row] : 0.0f;
-    each_marked([&](int at) {
-      const uint32_t mark = marks[at] & ~kBiased;
+    auto penalized = [&](int at, uint32_t mark) {
       float z = to_f32<T>(x[at]);
       if (mark != 0) {
         z = z > 0.0f ? z / rep : z * rep;
         const float times = (float)(mark >> 1);
         z -= times * freq + (times > 0.0f ? pres : 0.0f);
       }
-      marks[at] = __float_as_uint(z);
-    });
-    __syncthreads();
-    if (biased > 0) {
+      return z;
+    };
+    const int adds = few;
+    if (adds <= kFew) {
+      each_marked([&](int at) {
+        const uint32_t mark = marks[at];
+        if (mark == 0) return;
+        float z = penalized(at, mark & ~kBiased);
+        if ((mark & kBiased) != 0) {
+          for (int last = -1;;) {  // its biases in list order
+            int next = INT32_MAX, from = 0;
+            for (int j = 0; j < adds; j++)
+              if (few_at[j] == at && few_order[j] > last && few_order[j] < next) {
+                next = few_order[j];
+                from = j;
+              }
+            if (next == INT32_MAX) break;
+            z += few_add[from];
+            last = next;
+          }
+        }
+        x[at] = from_f32<T>(z);
+      });
+    } else {
+      // f32 results in place of the marks; one warp adds the biases to them.
+      each_marked([&](int at) { marks[at] = __float_as_uint(penalized(at, marks[at] & ~kBiased)); });
+      __syncthreads();
       if (tid < 32) {
         for (int i0 = tid; i0 - tid < biased; i0 += 32) {
           const uint32_t at = i0 < biased ? (uint32_t)(bias_tokens[i0] - base) : 0xffffffffu;
@@ -173,8 +209,8 @@ __global__ void __launch_bounds__(kThreads) logits_kernel(const __grid_constant_
         }
       }
       __syncthreads();
+      each_marked([&](int at) { x[at] = from_f32<T>(__uint_as_float(marks[at])); });
     }
-    each_marked([&](int at) { x[at] = from_f32<T>(__uint_as_float(marks[at])); });
   }
   if (mask != nullptr) {
     if (count > 0) __syncthreads();

@@ -187,3 +187,25 @@ def test_refusals(cuda_lib):
     assert (y == 5).all()
     assert call(n=0) == 0 and call(vocab=0) == 0
     assert call() == 0
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("repeats,others", [(2, 3), (20, 0), (30, 30)])
+def test_repeated_biases_and_penalties_on_one_token(cuda_lib, kind, repeats, others):
+    """A token that is seen, generated and biased several times, few or many biases in its range."""
+    dt, _, u = ref.TYPES[kind]
+    vocab = 5000
+    g = torch.Generator(device="cuda").manual_seed(repeats)
+    ids = [4090] * repeats + [4091 + i for i in range(others)]
+    rules = {"bias_start": ints([0, len(ids)], torch.int64), "bias_tokens": ints(ids),
+             "bias": torch.randn(len(ids), generator=g, device="cuda"),
+             "history": ints([0, 5], torch.int64), "tokens": ints([4090, 7, 4090, 4092, 4090]), "generated": ints([3]),
+             "repetition": ints([1.5], torch.float32), "frequency": ints([0.25], torch.float32),
+             "presence": ints([0.5], torch.float32)}
+    x = (torch.randn((1, vocab), generator=g, device="cuda") * 3).to(dt)
+    out = torch.empty_like(x)
+    assert apply(cuda_lib, kind, x, out, vocab, rules) == 0
+    want, tol = ref.logits(x, rules, vocab)
+    # Each bias rounds once more: the running sum is at most the terms' magnitudes.
+    tol = tol + len(ids) * ref.U32 * (x[:1].double().abs() * 1.5 + 2 + rules["bias"].double().abs().sum())
+    ref.check(out, want, tol, u, "biases")
