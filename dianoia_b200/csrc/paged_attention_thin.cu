@@ -14,9 +14,9 @@
 // of kStages buffers, so that no block barrier stands in the loop; the warps'
 // results are joined once at the end. Where 16 keys lie in one page (page
 // sizes that are multiples of 16) one lane brings them by tiled TMA copies of
-// 16 x 64 elements (one bulk copy a row, which needs no tensor map, was
-// limited by the copy engine's rate: 2.4 TB/s); for other page sizes the lanes
-// copy 16 bytes each. Both leave chunk c of key r's 64 elements at chunk
+// 16 x 64 elements (one bulk copy a row, which needs no tensor map, brought 3.1
+// TB/s where these brought 4.3); for other page sizes the lanes copy 16 bytes
+// each. Both leave chunk c of key r's 64 elements at chunk
 // c ^ (r & 7), which the fragment loads read without a bank conflict.
 // Measured: 192 sequences of 540 keys on average, 8 kv heads of 128, 4 heads a
 // group, bf16: 69 us, 5.9 TB/s of keys and values. Two buffers a warp and three

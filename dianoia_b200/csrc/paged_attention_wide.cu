@@ -1,9 +1,9 @@
 // The paged attention's kernel for many rows of queries on 16-bit caches: the
 // whole batch on the shared prefix, long chunks of a sequence's queries.
 //
-// 128 rows of one kv head share every key, so the products are the bound:
-// S = Q K^T and O += P V on the 5th-generation tensor cores (tcgen05, f32
-// accumulators in TMEM). A block runs three parts at once:
+// 128 rows of one kv head share every key, so operations are the bound, not
+// bytes: S = Q K^T and O += P V go to the 5th-generation tensor cores (tcgen05,
+// f32 accumulators in TMEM). A block runs two parts at once:
 //   a warp for each group brings the group's tiles of 128 keys and their values
 //   by tiled TMA copies, a copy a lane, and issues its products;
 //   two groups of 4 warps (one for heads over 128 wide) take the even and the
@@ -13,15 +13,15 @@
 //   has an O of its own, so the groups never wait for one another; the join
 //   adds them.
 // A group's S, P and O follow one another; while one group is in softmax the
-// tensor cores serve the other. (With 64-key tiles S took M = 128, N = 64 products, which
-// run at half the rate: 73000 cycles for 2752 keys, the tensor cores the
-// bound.) A base moves only when a score passes it by kSlack (P then stays
-// below 2^8), so O is rescaled in TMEM in the first tiles and hardly ever
-// after. Where rows of the block see different keys of a half and a value
-// there is not finite, that half's P V is added term by term instead
-// (0 * infinity would be NaN).
-// Measured: 768 rows on 8192 keys of 8 kv heads of 128, bf16, in 50 us alone
-// (520 TFLOP/s); a group's tile takes some 5800 cycles, 3600 of them softmax
+// tensor cores serve the other. (S by halves, one ahead, leaves a group no gap
+// between them but takes products of N = 64 and twice the commits: 121 us
+// where whole tiles take 117, on 192 sequences behind 8192 keys.) A base moves
+// only when a score passes it by kSlack (P then stays below 2^8), so O is
+// rescaled in TMEM in the first tiles and hardly ever after. Where rows of the
+// block see different keys of a half and a value there is not finite, that
+// half's P V is added term by term instead (0 * infinity would be NaN).
+// Measured: 768 rows on 8192 keys of 8 kv heads of 128, bf16, in 48 us alone
+// (540 TFLOP/s); a group's tile takes some 5500 cycles, 3300 of them softmax
 // (the exponentials' unit for half of that, with both groups in step) and 2150
 // the way from the last P through P V, its commit and the next S.
 #include <type_traits>

@@ -449,3 +449,42 @@ def test_attention_refusals(cuda_lib):
     for args in [(3, 2, 16, 32), (4, -1, 16, 32), (4, 2, -1, 32), (4, 2, 16, -1)]:
         assert L.dn_paged_attention_workspace(pool.c, *args) == -1, args
     assert call(n=0) == 0
+
+
+@pytest.mark.parametrize("own", [1, 120])
+def test_both_kernels_at_once_repeat_and_replay(cuda_lib, own):
+    """Many rows on the prefix beside each sequence's own: the same bits every time, back to back, with programmatic launch and in a graph."""
+    L = cuda_lib
+    seqs, heads = 100, 8
+    b = Batch("bf16", heads, 2, 128, 16, 1200, [1 + (own * (i % 7)) // 6 for i in range(seqs)], [1] * seqs, seed=own)
+    first = b.check(L).clone()
+    starts, lens = ints(b.starts), ints(b.lengths)
+    most = max(b.lengths)
+    need = L.dn_paged_attention_workspace(b.pool.c, heads, b.n, b.prefix, most)
+    ws = torch.full((need,), 255, dtype=torch.uint8, device="cuda")
+    outs = [torch.zeros_like(b.q) for _ in range(8)]
+
+    def call(out, flags):
+        assert L.dn_paged_attention(b.pool.c, b.q.data_ptr(), b.q.stride(0), starts.data_ptr(), lens.data_ptr(),
+                                    b.prefix_pages.data_ptr(), b.prefix, most, 128 ** -0.5, 0, out.data_ptr(), out.stride(0), heads,
+                                    b.n, ws.data_ptr(), need, flags, stream()) == 0
+
+    for flags in (0, 1):
+        for out in outs:
+            out.zero_()
+        torch.cuda.synchronize()
+        for out in outs:
+            call(out, flags)
+        torch.cuda.synchronize()
+        assert all(torch.equal(out, first) for out in outs)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        for i, out in enumerate(outs):
+            call(out, i % 2)
+    for _ in range(3):
+        for out in outs:
+            out.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(out, first) for out in outs)
+    assert L.dn_device_status(1) == 0
