@@ -314,8 +314,7 @@ Params plan(const PagedCache& c, int64_t heads, int64_t n, int64_t prefix, int64
   p.prefix_splits = prefix > 0 ? splits(tiles * c.kv_heads, prefix, p.prefix_wide, p.prefix_least) : 0;
   const int64_t own = max_length > prefix ? max_length - prefix : 1;
   p.own_splits = splits((int64_t)p.own_slots * c.kv_heads, own, p.own_wide, p.own_least);
-  p.prefix_slices = p.prefix_splits * (p.prefix_wide ? wide_groups(c.hd) : 1);
-  p.slices = p.prefix_slices + p.own_splits * (p.own_wide ? wide_groups(c.hd) : 1);
+  p.slices = p.prefix_splits + p.own_splits;
   p.direct = p.slices == 1;
   return p;
 }

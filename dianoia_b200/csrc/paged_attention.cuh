@@ -32,7 +32,7 @@ struct Params {
   int prefix_tiles, prefix_splits;
   int own_slots, own_splits;
   int prefix_least, own_least;  // keys: slices are not made shorter than this
-  int prefix_slices, slices;  // results of a row: of the prefix, in all
+  int slices;           // results of a row
   float* acc;           // [slices][n * heads][hd]
   float2* ml;           // [slices][n * heads]: m, l
   float scale_log2;
@@ -243,9 +243,9 @@ __device__ __forceinline__ int64_t out_index(const Params& p, const Work& w, int
   return (int64_t)token * p.a.heads + head;
 }
 
-// Where a block's result (its group's, for a wide block) goes among a row's.
-__device__ __forceinline__ int slice_index(const Params& p, const Work& w, int group = 0) {
-  return w.prefix ? w.slice + group * p.prefix_splits : p.prefix_slices + w.slice + group * p.own_splits;
+// Where a block's result goes among a row's.
+__device__ __forceinline__ int slice_index(const Params& p, const Work& w) {
+  return w.prefix ? w.slice : p.prefix_splits + w.slice;
 }
 
 // Rows of a block of the wide kernel (the thin one: 8 or 16, the f32 one: 1 to 8).
@@ -253,8 +253,8 @@ constexpr int kWideRows = 128;
 constexpr int kWideFrom = 32;  // rows (of the batch, of a sequence on average) from which the wide one runs
 constexpr int kLanes = 32;
 
-// Groups of a wide block, each with results of its own: two outputs of 128
-// columns stand in TMEM beside the scores, of 256 one.
+// Groups of a wide block: two outputs of 128 columns stand in TMEM beside the
+// scores, of 256 one.
 constexpr int wide_groups(int64_t hd) { return hd <= 128 ? 2 : 1; }
 
 inline dim3 attention_grid(const Params& p) {

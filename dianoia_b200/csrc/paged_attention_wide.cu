@@ -10,8 +10,8 @@
 //   odd tiles, a row of S each thread: they read it from TMEM 64 keys (a half)
 //   at a time, keep the row's base and sum, and write P (16-bit) over it, which
 //   the tensor cores read from there as the first operand of P V. Each group
-//   has an O of its own, so the groups never wait for one another; the join
-//   adds them.
+//   has an O of its own, so the groups do not wait for one another until the
+//   first takes the second's result in, through shared memory, at the end.
 // A group's S, P and O follow one another; while one group is in softmax the
 // tensor cores serve the other. (S by halves, one ahead, leaves a group no gap
 // between them but takes products of N = 64 and twice the commits: 121 us
@@ -73,6 +73,7 @@ struct Shape {
 // the phase before it past.
 struct Bars {
   uint64_t k_full[2], v_full[2], s_full[kScores], p_full[kHalves], o_done[kHalves];  // k, v: a group's
+  uint64_t second;  // the second group's results are in shared memory
 };
 
 // What stands in shared memory behind the tiles.
@@ -81,6 +82,7 @@ struct Control {
   Bars bars;
   uint32_t tmem_at, skip[kHalves];
   int span[Shape<HDP>::kGroups * kRowThreads / kLanes][4];
+  float2 second[Shape<HDP>::kGroups == 2 ? kRowThreads : 1];  // its rows' m and l
 };
 
 // Shared-memory operand, 128-byte swizzled; `lead` is the stride between
@@ -177,7 +179,7 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
 // A group's part, of tiles group, group + kGroups, ...; `halves` in all of the
 // block; row `r` of the block is the thread's.
 template <typename T, int HDP>
-__device__ __forceinline__ void softmax_rows(const Params& p, const Work& w, char* smem, Bars& bars, uint32_t* skip,
+__device__ __forceinline__ void softmax_rows(const Params& p, const Work& w, char* smem, Bars& bars, float2* second, uint32_t* skip,
                                              uint32_t tmem, int begin, int halves, int group, int low, int high,
                                              int all_low, int all_high) {
   using S = Shape<HDP>;
@@ -329,15 +331,49 @@ __device__ __forceinline__ void softmax_rows(const Params& p, const Work& w, cha
     done(last);
     fence_after();
   }
-  // The row's result.
-  int t = 0, head = 0;
-  const bool mine_row = r < w.rows;
-  const int64_t row = mine_row ? out_index(p, w, r, t, head) : 0;
-  const int64_t to = slice_index(p, w, group) * (p.a.n * p.a.heads) + row;
   if (high < low) {  // a row that sees nothing took part unmasked
     m = -INFINITY;
     l = 0.0f;
   }
+  // The second group's result goes to the first through the second's own keys'
+  // and values' places: 4 columns at a time, chunk c of row r at c ^ r.
+  constexpr int kPart = HDP / 8;  // chunks in the keys' place; as many in the values'
+  auto place = [&](int chunk) {
+    char* at = smem + (chunk < kPart ? S::kK + S::kPanels * S::kKPanel : S::kV + 2 * S::kPanels * S::kVPanel);
+    return reinterpret_cast<float4*>(at + r * (kPart * 16) + ((chunk ^ r) & (kPart - 1)) * 16);
+  };
+  float keep_first = 1.0f, keep_second = 0.0f;
+  if constexpr (S::kGroups == 2) {
+    if (group == 1) {
+      if (last >= 0) {
+#pragma unroll 1
+        for (int c = 0; c < HDP; c += 32) {
+          float o[32];
+          ld32(out_cols + c, o);
+          wait_ld(o);
+#pragma unroll
+          for (int e = 0; e < 32; e += 4) *place((c + e) / 4) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+        }
+      }
+      second[r] = make_float2(m, l);
+      mbar_arrive(&bars.second);
+      return;
+    }
+    live = __all_sync(0xffffffffu, wait_phase(&bars.second, 0, p.status, kStatusMmaTimeout));
+    const float2 other = second[r];
+    if (live && other.y != 0.0f) {
+      const float top = fmaxf(m, other.x), base = top == -INFINITY ? 0.0f : top;
+      keep_first = exp2_fast(m - base);
+      keep_second = exp2_fast(other.x - base);
+      l = (l == 0.0f ? 0.0f : l * keep_first) + other.y * keep_second;
+      m = top;
+    }
+  }
+  // The row's result.
+  int t = 0, head = 0;
+  const bool mine_row = r < w.rows;
+  const int64_t row = mine_row ? out_index(p, w, r, t, head) : 0;
+  const int64_t to = slice_index(p, w) * (p.a.n * p.a.heads) + row;
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   if (mine_row && !p.direct) p.ml[to] = make_float2(m, l);
   if (last < 0 && !p.direct) return;  // the join reads no values of a row with l = 0
@@ -350,6 +386,16 @@ __device__ __forceinline__ void softmax_rows(const Params& p, const Work& w, cha
     } else {
 #pragma unroll
       for (int e = 0; e < 32; e++) o[e] = 0.0f;
+    }
+    if (keep_second != 0.0f) {
+#pragma unroll
+      for (int e = 0; e < 32; e += 4) {
+        const float4 v = *place((c + e) / 4);
+        o[e] = o[e] * keep_first + v.x * keep_second;
+        o[e + 1] = o[e + 1] * keep_first + v.y * keep_second;
+        o[e + 2] = o[e + 2] * keep_first + v.z * keep_second;
+        o[e + 3] = o[e + 3] * keep_first + v.w * keep_second;
+      }
     }
     if (mine_row && p.direct) {
       T* out = static_cast<T*>(p.a.out) + t * p.a.out_stride + (int64_t)head * hd;
@@ -397,6 +443,7 @@ __global__ void __maxnreg__(Shape<HDP>::kRegs)
       mbar_init(&bars.v_full[i], 1);
     }
     for (int i = 0; i < kScores; i++) mbar_init(&bars.s_full[i], 1);
+    mbar_init(&bars.second, kRowThreads);
     for (int i = 0; i < kHalves; i++) {
       mbar_init(&bars.p_full[i], kRowThreads);
       mbar_init(&bars.o_done[i], 1);
@@ -457,7 +504,7 @@ __global__ void __maxnreg__(Shape<HDP>::kRegs)
   const int halves = (end - begin + kHalf - 1) / kHalf, tiles = (halves + 1) / 2;
 
   if (warp < kRowWarps) {
-    softmax_rows<T, HDP>(p, w, smem, bars, skip, tmem, begin, halves, tid / kRowThreads, low, high, all_low, all_high);
+    softmax_rows<T, HDP>(p, w, smem, bars, ctl.second, skip, tmem, begin, halves, tid / kRowThreads, low, high, all_low, all_high);
   } else {
     const int group = warp - kRowWarps;
     // One copy a lane: panel c of the keys (values) g * box .. of a tile, all
