@@ -269,9 +269,10 @@ constexpr int64_t kSoloKeys = 512;    // of the longest sequence
 constexpr int64_t kSoloReads = 8192;  // keys of the prefix, once for each sequence
 
 // Least keys of a slice: of the thin kernel, the f32 one, and a wide block of
-// two groups and of one (24 ragged sequences on 2048 keys: 28 us with 512, 29
-// with 256, 33 with 1024, before the wide softmax was packed; with 256-wide heads 29 us with 128, 32 with 256).
-constexpr int kThinLeast = 256, kSimtLeast = 128, kWide2Least = 512, kWide1Least = 128;
+// two groups and of one (32 chat sequences and 24 of drafts: 23 and 22 us with
+// 384, 22 and 27 with 256, 25 and 23 with 512; with 256-wide heads 29 us with
+// 128, 32 with 256).
+constexpr int kThinLeast = 256, kSimtLeast = 128, kWide2Least = 384, kWide1Least = 128;
 
 // How the work is divided, from sizes that the host knows.
 Params plan(const PagedCache& c, int64_t heads, int64_t n, int64_t prefix, int64_t max_length) {

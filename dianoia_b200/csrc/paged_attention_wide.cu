@@ -15,7 +15,8 @@
 // A group's S, P and O follow one another; while one group is in softmax the
 // tensor cores serve the other. (S by halves, one ahead, leaves a group no gap
 // between them but takes products of N = 64 and twice the commits: 121 us
-// where whole tiles take 117, on 192 sequences behind 8192 keys.) A base moves
+// where whole tiles took 117, on 192 sequences behind 8192 keys; joining the
+// groups here instead of in the join kernel made that 113.) A base moves
 // only when a score passes it by kSlack (P then stays below 2^8), so O is
 // rescaled in TMEM in the first tiles and hardly ever after. Where rows of the
 // block see different keys of a half and a value there is not finite, that
