@@ -65,8 +65,11 @@ __global__ void __launch_bounds__(kThreads) logits_kernel(const __grid_constant_
   // first, which are then left out.
   const int shift = BULK ? (int)(((uintptr_t)in & 15) / sizeof(T)) : 0;
   const int base = chunk * kChunk - shift, vocab = (int)a.vocab;
-  // The range's tokens of the row, begin .. end - 1 past base; whole 16 bytes
-  // of them, from .. to - 1.
+  // The chunks are counted for the largest shift: a row of a smaller one may
+  // have no token left for its last.
+  if (base >= vocab) return;
+  // The range's tokens of the row, begin .. end - 1 past base (one at least);
+  // whole 16 bytes of them, from .. to - 1.
   const int begin = base < 0 ? -base : 0, end = min(base + kChunk, vocab) - base;
   const int from = BULK ? begin > 0 ? V : 0 : end, to = BULK && end > from ? from + (end - from) / V * V : from;
   const LogitRules& r = a.rules;
@@ -104,11 +107,11 @@ __global__ void __launch_bounds__(kThreads) logits_kernel(const __grid_constant_
   const bool marked = seen > 0 || biased > 0;
   // The first tokens and biases are on their way while the marks are cleared.
   constexpr int kAtOnce = 8;
-  uint32_t at[kAtOnce], first_bias = tid < biased ? (uint32_t)(bias_tokens[tid] - base) : 0xffffffffu;
+  uint32_t at[kAtOnce], first_bias = tid < biased ? (uint32_t)bias_tokens[tid] - (uint32_t)base : 0xffffffffu;
   auto load_tokens = [&](int i0) {
 #pragma unroll
     for (int k = 0; k < kAtOnce; k++)
-      at[k] = i0 + k * kThreads < seen ? (uint32_t)(tokens[i0 + k * kThreads] - base) : 0xffffffffu;
+      at[k] = i0 + k * kThreads < seen ? (uint32_t)tokens[i0 + k * kThreads] - (uint32_t)base : 0xffffffffu;
   };
   load_tokens(tid);
   const int word0 = (base + begin) / 32;  // of words[0]
@@ -123,7 +126,7 @@ __global__ void __launch_bounds__(kThreads) logits_kernel(const __grid_constant_
     const int j = atomicAdd(&listed, 1);
     if (j < kListed) list[j] = (uint16_t)at;
   };
-  auto mine = [&](uint32_t at) { return at < (uint32_t)end && at >= (uint32_t)begin; };
+  auto mine = [&](uint32_t at) { return at - (uint32_t)begin < (uint32_t)(end - begin); };
   for (int i0 = tid; i0 < seen; i0 += kThreads * kAtOnce) {
     if (i0 != tid) load_tokens(i0);
 #pragma unroll
@@ -134,7 +137,7 @@ __global__ void __launch_bounds__(kThreads) logits_kernel(const __grid_constant_
       }
   }
   for (int i = tid; i < biased; i += kThreads) {
-    const uint32_t v = i == tid ? first_bias : (uint32_t)(bias_tokens[i] - base);
+    const uint32_t v = i == tid ? first_bias : (uint32_t)bias_tokens[i] - (uint32_t)base;
     if (!mine(v)) continue;
     const int j = atomicAdd(&few, 1);
     if (j < kFew) {
@@ -197,7 +200,7 @@ __global__ void __launch_bounds__(kThreads) logits_kernel(const __grid_constant_
       __syncthreads();
       if (tid < 32) {
         for (int i0 = tid; i0 - tid < biased; i0 += 32) {
-          const uint32_t at = i0 < biased ? (uint32_t)(bias_tokens[i0] - base) : 0xffffffffu;
+          const uint32_t at = i0 < biased ? (uint32_t)bias_tokens[i0] - (uint32_t)base : 0xffffffffu;
           const bool here = mine(at);
           unsigned left = __ballot_sync(0xffffffffu, here);
           const float add = here ? bias[i0] : 0.0f;

@@ -209,3 +209,34 @@ def test_repeated_biases_and_penalties_on_one_token(cuda_lib, kind, repeats, oth
     # Each bias rounds once more: the running sum is at most the terms' magnitudes.
     tol = tol + len(ids) * ref.U32 * (x[:1].double().abs() * 1.5 + 2 + rules["bias"].double().abs().sum())
     ref.check(out, want, tol, u, "biases")
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("vocab", [*range(4089, 4099), *range(8185, 8195), 32766, 65535])
+def test_vocabularies_around_whole_ranges(cuda_lib, kind, vocab):
+    """Vocabularies that end just before, at and after a multiple of a CTA's 4096 tokens, rows at every alignment,
+    copied whole and element by element: a last CTA without tokens leaves everything alone."""
+    dt, _, u = ref.TYPES[kind]
+    n, whole = 3, 16 // dt.itemsize
+    rules = make_rules(n, vocab, ALL, seed=vocab, history=300, biases=90)
+    x = (torch.randn((n, vocab), device="cuda") * 4).to(dt)
+    want, tol = ref.logits(x, rules, vocab)
+    tol = tol * (6 + 90) / 6  # one more rounding for each of up to 90 biases of a token
+    stride = -(-vocab // whole) * whole + whole  # every row at the alignment of the first
+    first = None
+    for off_in in range(whole):
+        for off_out in (off_in, (off_in + 1) % whole):
+            a = torch.full((n * stride + whole,), 5.0, device="cuda", dtype=dt)
+            b = torch.full_like(a, 6.0)
+            rows_in = a[off_in:off_in + n * stride].view(n, stride)
+            rows_out = b[off_out:off_out + n * stride].view(n, stride)
+            rows_in[:, :vocab] = x
+            assert apply(cuda_lib, kind, rows_in, rows_out, vocab, rules) == 0
+            got = rows_out[:, :vocab].clone()
+            if first is None:
+                first = got
+                ref.check(first, want, tol, u, "logits")
+            assert torch.equal(got, first)
+            rows_out[:, :vocab] = 6.0
+            assert (b == 6).all()
+    assert cuda_lib.dn_device_status(1) == 0
