@@ -239,6 +239,9 @@ __device__ __forceinline__ void thin_block(const Params& p, const Maps& maps, co
         for (int e = 0; e < 4; e++) s[n][e] = s2[n][e] = 0.0f;
 #pragma unroll
       for (int k = 0; k < HDP / 16; k++) {
+        // Heads of 129 to 192 have a panel that no copy writes: what stands there
+        // may be NaN, which the queries' zeros would pass on.
+        if (HDP > 128 && 16 * k >= hd) continue;
         uint32_t a[4];
         ldsm4(a, kb + chunk_at(lane & 15, 2 * k + (lane >> 4)));
 #pragma unroll
@@ -317,6 +320,7 @@ __device__ __forceinline__ void thin_block(const Params& p, const Maps& maps, co
       } else {
 #pragma unroll
         for (int k = 0; k < HDP / 16; k++) {
+          if (HDP > 128 && 16 * k >= hd) continue;
           uint32_t a[4];
           ldsm4_t(a, vb + chunk_at((lane & 7) + (lane >> 4) * 8, 2 * k + ((lane >> 3) & 1)));
 #pragma unroll

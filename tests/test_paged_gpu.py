@@ -488,3 +488,30 @@ def test_both_kernels_at_once_repeat_and_replay(cuda_lib, own):
         torch.cuda.synchronize()
         assert all(torch.equal(out, first) for out in outs)
     assert L.dn_device_status(1) == 0
+
+
+# ---- heads between two panel counts, after other heads have used the same shared memory
+
+
+def spoil(L, kind, hd, wide, value):
+    """A pass over keys and values of `value` that fills the kernel's shared memory on every SM."""
+    seqs, q = (40, 40) if wide else (500, 1)
+    b = Batch(kind, 4, 2, hd, 16, 0, [64] * seqs, [q] * seqs, seed=1)
+    b.pool.keys.fill_(value), b.pool.values.fill_(value)
+    b.run(L)
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("hd", [136, 160, 192, 200])
+@pytest.mark.parametrize("page", [16, 7])
+@pytest.mark.parametrize("group,q", [(2, 1), (12, 1), (2, 40)])
+def test_heads_whose_last_panel_is_not_copied(cuda_lib, kind, hd, page, group, q):
+    """Heads of 129 to 192 elements fill three of the four panels of their kernel: what another call left in the
+    fourth, NaN and large values, does not reach a score. Thin blocks of 8 and of 16 rows, and wide ones."""
+    own = [70, 45, 130, 64]
+    b = Batch(kind, group * 2, 2, hd, page, 48, [max(k, q) for k in own], [q] * 4, seed=hd + q)
+    for value in (float("nan"), 6e4, 1.0):
+        spoil(cuda_lib, kind, 256, q > 1, value)
+        b.check(cuda_lib, max_length=4096)
+        spoil(cuda_lib, kind, 256, q > 1, value)
+        b.check(cuda_lib)
