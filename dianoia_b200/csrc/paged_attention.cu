@@ -281,11 +281,13 @@ Params plan(const PagedCache& c, int64_t heads, int64_t n, int64_t prefix, int64
   const int64_t rows = n * p.group, seqs = c.sequences > 1 ? c.sequences : 1;
   const bool wide = mma_cache(c) && c.page_size % 16 == 0 && c.pages > 0;
   // Short sequences in all: each reads the prefix for itself, from L2, which
-  // saves the second launch that joins two parts.
-  p.solo = prefix > 0 && prefix % 16 == 0 && max_length <= kSoloKeys && c.sequences * prefix <= kSoloReads;
+  // saves the second launch that joins two parts. The page list then changes at
+  // `prefix`, which no copy may span: 16 keys of a thin block, a wide one's box.
+  p.own_wide = wide && rows > kWideFrom * seqs;
+  p.solo = prefix > 0 && prefix % (p.own_wide ? wide_box(c.page_size) : 16) == 0 && max_length <= kSoloKeys &&
+           c.sequences * prefix <= kSoloReads;
   if (p.solo) prefix = 0;
   p.prefix_wide = wide && prefix > 0 && rows > kWideFrom;
-  p.own_wide = wide && rows > kWideFrom * seqs;
   // 8 rows to a thin block where a sequence's rows, and the whole batch's on
   // the prefix, are that few; else 16.
   const bool few = rows <= 8 * seqs && (prefix == 0 || p.prefix_wide || rows <= 8);

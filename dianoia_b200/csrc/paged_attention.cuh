@@ -257,6 +257,9 @@ constexpr int kLanes = 32;
 // scores, of 256 one.
 constexpr int wide_groups(int64_t hd) { return hd <= 128 ? 2 : 1; }
 
+// Keys of a wide block's copy, all of one page: the box must divide the page.
+inline int wide_box(int64_t page_size) { return page_size % 64 == 0 ? 64 : page_size % 32 == 0 ? 32 : 16; }
+
 inline dim3 attention_grid(const Params& p) {
   return dim3((unsigned)(p.prefix_tiles * p.prefix_splits + p.own_slots * p.own_splits),
               (unsigned)p.a.cache.kv_heads);

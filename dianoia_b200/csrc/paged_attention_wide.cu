@@ -607,7 +607,7 @@ __global__ void __maxnreg__(Shape<HDP>::kRegs)
 template <typename T, int HDP>
 cudaError_t launch_size(const Params& p, cudaStream_t stream, bool pdl) {
   const PagedCache& c = p.a.cache;
-  const int box = c.page_size % 64 == 0 ? 64 : c.page_size % 32 == 0 ? 32 : 16;
+  const int box = wide_box(c.page_size);
   Maps maps{};
   if (!(encode_tmap_pages(&maps.keys, c.keys, c.type == kBF16, c.hd, c.page_size, c.kv_heads, c.pages, c.page_stride,
                           box) &&

@@ -515,3 +515,21 @@ def test_heads_whose_last_panel_is_not_copied(cuda_lib, kind, hd, page, group, q
         b.check(cuda_lib, max_length=4096)
         spoil(cuda_lib, kind, 256, q > 1, value)
         b.check(cuda_lib)
+
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("page", [32, 64, 96])
+@pytest.mark.parametrize("prefix", [16, 48, 96, 208])
+@pytest.mark.parametrize("shape", ["queries", "heads"])
+def test_short_sequences_of_many_rows_behind_a_prefix_inside_a_page(cuda_lib, kind, page, prefix, shape):
+    """Short sequences that read the prefix themselves, with rows enough for the wide kernel: keys after the prefix's
+    end come from the sequence's own page, also where one page's worth of copies spans the end."""
+    if shape == "queries":
+        b = Batch(kind, 4, 2, 64, page, prefix, [112, 60, 45], [40] * 3, seed=prefix)
+    else:
+        b = Batch(kind, 40, 1, 128, page, prefix, [30, 1], [1, 1], seed=prefix)
+    assert max(b.lengths) <= 512 and len(b.lengths) * prefix <= 8192
+    b.check(cuda_lib)
+    b.check(cuda_lib, window=70)
+    b.check(cuda_lib, max_length=5000)
