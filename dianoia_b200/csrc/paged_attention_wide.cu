@@ -282,7 +282,8 @@ __device__ __forceinline__ void softmax_rows(const Params& p, const Work& w, cha
                                                   kStatusTmaTimeout));
         if (!live) break;
         bool bad = false;
-        for (int c = lane; c < S::kPanels * S::kVPanel / 16; c += kLanes) bad = bad || unbounded16<T>(vals + c * 16);
+        const int copied = (hd + 63) / 64 * S::kVPanel;  // the head's panels: nothing writes the others
+        for (int c = lane; c < copied / 16; c += kLanes) bad = bad || unbounded16<T>(vals + c * 16);
         bad = __any_sync(0xffffffffu, bad);  // every warp finds the same
         if (r == 0) skip[j % kHalves] = bad ? 1u : 0u;
         if (bad) {
@@ -293,7 +294,7 @@ __device__ __forceinline__ void softmax_rows(const Params& p, const Work& w, cha
 #pragma unroll
           for (int e = 0; e < kHalf; e++) pr[e] = to_f32<T>(from_f32<T>(s[e / 32][e % 32]));
 #pragma unroll 1
-          for (int c = 0; c < HDP; c += 32) {
+          for (int c = 0; c < hd; c += 32) {
             float o[32];
             ld32(out_cols + c, o);
             wait_ld(o);

@@ -533,3 +533,16 @@ def test_short_sequences_of_many_rows_behind_a_prefix_inside_a_page(cuda_lib, ki
     b.check(cuda_lib)
     b.check(cuda_lib, window=70)
     b.check(cuda_lib, max_length=5000)
+
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("hd", [136, 160, 192])
+def test_result_does_not_depend_on_what_ran_before(cuda_lib, kind, hd):
+    """Many rows with a window (tiles whose values are looked at): the same bits after any other call."""
+    b = Batch(kind, 4, 2, hd, 16, 0, [300, 211], [90, 90], seed=hd)
+    outs = []
+    for value in (0.0, float("nan"), 6e4, float("inf"), 0.0):
+        spoil(cuda_lib, kind, 256, True, value)
+        outs.append(b.check(cuda_lib, window=50).clone())
+    assert all(torch.equal(o, outs[0]) for o in outs)
