@@ -380,7 +380,7 @@ int64_t paged_attention_workspace(const PagedCache& c, int64_t heads, int64_t n,
 }
 
 cudaError_t launch_paged_attention(const PagedAttentionArgs& a, cudaStream_t stream, bool pdl) {
-  if (a.n <= 0) return cudaSuccess;
+  if (a.n <= 0 || a.cache.sequences <= 0) return cudaSuccess;  // no sequence: no token belongs to one
   Params p = plan(a.cache, a.heads, a.n, a.prefix, a.max_length);
   p.a = a;
   p.status = a.status;

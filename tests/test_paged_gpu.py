@@ -546,3 +546,24 @@ def test_result_does_not_depend_on_what_ran_before(cuda_lib, kind, hd):
         spoil(cuda_lib, kind, 256, True, value)
         outs.append(b.check(cuda_lib, window=50).clone())
     assert all(torch.equal(o, outs[0]) for o in outs)
+
+
+
+@pytest.mark.parametrize("kind,hd", [("f32", 64), ("bf16", 64), ("f16", 33)])
+@pytest.mark.parametrize("prefix", [0, 32])
+@pytest.mark.parametrize("n", [1, 3, 100])
+def test_tokens_without_sequences_are_left_alone(cuda_lib, kind, hd, prefix, n):
+    """A batch of no sequences: every token lies past q_start[0]."""
+    from dianoia_b200 import _lib
+    L = cuda_lib
+    dt, code, _ = ref.TYPES[kind]
+    pool = ref.Pool(kind, 4, 16, 2, hd, 1, 2, fill=1.0)
+    c = changed(pool.c, sequences=0)
+    q, out = torch.ones((n, 4, hd), device="cuda", dtype=dt), torch.full((n, 4, hd), 7.0, device="cuda", dtype=dt)
+    starts, lens, pages = ints([0]), ints([0]), ints([0, 1])
+    need = L.dn_paged_attention_workspace(c, 4, n, prefix, 64)
+    ws = torch.full((need,), 255, dtype=torch.uint8, device="cuda")
+    assert L.dn_paged_attention(c, q.data_ptr(), 4 * hd, starts.data_ptr(), lens.data_ptr(), pages.data_ptr(), prefix, 64, 0.125, 0,
+                                out.data_ptr(), 4 * hd, 4, n, ws.data_ptr(), need, 0, stream()) == _lib.DN_OK
+    torch.cuda.synchronize()
+    assert (out == 7).all()
