@@ -113,7 +113,8 @@ __device__ __forceinline__ void sees(const Params& p, const Work& w, int t, int&
     high = min(high, (int)p.a.prefix - 1);
   } else {
     if (!p.solo) low = max(low, (int)p.a.prefix);
-    high = min(high, (int)(p.a.cache.table_stride * p.a.cache.page_size) - 1);
+    const int held = (int)(p.a.cache.table_stride * p.a.cache.page_size);  // (the prefix needs no table)
+    high = min(high, (p.solo ? max(held, (int)p.a.prefix) : held) - 1);
   }
 }
 

@@ -420,7 +420,8 @@ int64_t dn_linear_qa(int64_t format, const void* qs, const void* scales, const u
  * time. hd is at most 256. A table entry outside [0, pages) names no page:
  * nothing is written through it, and no query sees its positions (a window's
  * freed pages may be marked -1). A position past the table's table_stride
- * pages does not exist. */
+ * pages does not exist (those of a shared prefix, which dn_paged_attention
+ * reads through a list of their own, need no entry). */
 typedef struct dn_paged_cache {
   void* keys;
   void* values;

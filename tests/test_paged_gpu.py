@@ -567,3 +567,21 @@ def test_tokens_without_sequences_are_left_alone(cuda_lib, kind, hd, prefix, n):
                                 out.data_ptr(), 4 * hd, 4, n, ws.data_ptr(), need, 0, stream()) == _lib.DN_OK
     torch.cuda.synchronize()
     assert (out == 7).all()
+
+
+
+@pytest.mark.parametrize("kind,page", [("f32", 16), ("bf16", 16), ("bf16", 7), ("f16", 64)])
+@pytest.mark.parametrize("q", [1, 40])
+def test_prefix_needs_no_table(cuda_lib, kind, page, q):
+    """Sequences that lie in the prefix altogether, behind tables that end before it: the prefix is read through its
+    own pages, whatever length the batch is said to have."""
+    prefix = 128
+    b = Batch(kind, 4, 2, 64, page, prefix, [0, 0, 0], [q] * 3, seed=q)
+    b.lengths = [128, 100, 40]
+    b.pool.table = b.pool.table[:, :1].contiguous()
+    b.pool.c.table, b.pool.c.table_stride = b.pool.table.data_ptr(), 1
+    b.check(cuda_lib)
+    b.check(cuda_lib, max_length=5000)
+    b.check(cuda_lib, window=30)
+    b.lengths[0] = 140  # its last positions have no page
+    b.check(cuda_lib)
