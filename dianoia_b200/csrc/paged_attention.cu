@@ -122,7 +122,8 @@ __global__ void __launch_bounds__(kSimtThreads) attention_simt_kernel(const __gr
           for (int e = 0; e < V; e++) acc[r][u][e] *= f;
       }
     }
-    const float pr = seen ? exp2_fast(x - (m == -INFINITY ? 0.0f : m)) : 0.0f;
+    // -0: not seen. (A key that is seen counts, however small its weight.)
+    const float pr = seen ? exp2_fast(x - (m == -INFINITY ? 0.0f : m)) : -0.0f;
     l += pr;
     const bool all = there == (kStep == 32 ? 0xffffffffu : (1u << kStep) - 1) && k0 >= all_low &&
                      k0 + kStep - 1 <= all_high;
@@ -138,7 +139,7 @@ __global__ void __launch_bounds__(kSimtThreads) attention_simt_kernel(const __gr
 #pragma unroll
       for (int r = 0; r < RT; r++) {
         const float f = __shfl_sync(0xffffffffu, pr, k * RT + r);
-        if (!all && f == 0.0f) continue;  // a key that the row does not see adds nothing, infinite or not
+        if (!all && __float_as_int(f) < 0) continue;  // a key that the row does not see adds nothing, infinite or not
 #pragma unroll
         for (int u = 0; u < NU; u++)
 #pragma unroll

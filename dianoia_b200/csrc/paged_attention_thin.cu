@@ -307,7 +307,8 @@ __device__ __forceinline__ void thin_block(const Params& p, const Maps& maps, co
             for (int h = 0; h < 2; h++) {
               const float x = __shfl_sync(0xffffffffu, j < 8 ? s[n][h] : s[n][2 + h], j % 8 * 4 + lane % 4);
               const float r = to_f32<T>(from_f32<T>(x));
-              if (x == 0.0f) continue;
+              // (A key that the row sees counts, however small its weight.)
+              if ((there[b] >> j & 1u) == 0 || k0 + j < low[n][h] || k0 + j > high[n][h]) continue;
 #pragma unroll
               for (int k = 0; k < HDP / 16; k++)
 #pragma unroll

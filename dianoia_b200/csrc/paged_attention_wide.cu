@@ -292,7 +292,11 @@ __device__ __forceinline__ void softmax_rows(const Params& p, const Work& w, cha
           fence_after();
           float pr[kHalf];  // indexed at run time: in local memory, here only
 #pragma unroll
-          for (int e = 0; e < kHalf; e++) pr[e] = to_f32<T>(from_f32<T>(s[e / 32][e % 32]));
+          for (int e = 0; e < kHalf; e++) {
+            // -0: not seen. (A key that is seen counts, however small its weight.)
+            const bool seen = (there >> (e / 16) & 1u) != 0 && k0 + e >= low && k0 + e <= high;
+            pr[e] = seen ? to_f32<T>(from_f32<T>(s[e / 32][e % 32])) : -0.0f;
+          }
 #pragma unroll 1
           for (int c = 0; c < hd; c += 32) {
             float o[32];
@@ -303,7 +307,7 @@ __device__ __forceinline__ void softmax_rows(const Params& p, const Work& w, cha
               for (int e = 0; e < 32; e++) o[e] = 0.0f;
 #pragma unroll 1
             for (int k = 0; k < kHalf; k++) {
-              if (pr[k] != 0.0f)
+              if (__float_as_int(pr[k]) >= 0)
 #pragma unroll
                 for (int e = 0; e < 32; e++) {
                   const int d = c + e;

@@ -585,3 +585,23 @@ def test_prefix_needs_no_table(cuda_lib, kind, page, q):
     b.check(cuda_lib, window=30)
     b.lengths[0] = 140  # its last positions have no page
     b.check(cuda_lib)
+
+
+
+@pytest.mark.parametrize("kind,hd", [("f32", 64), ("f16", 64), ("bf16", 128), ("bf16", 20)])
+@pytest.mark.parametrize("q", [6, 40])
+def test_seen_infinities_count_however_small_their_weight(cuda_lib, kind, hd, q):
+    """A value that is not finite, at a key that a query sees with a weight below every type's least: the query's output
+    is not finite, whether the rows beside it see the same keys or not."""
+    b = Batch(kind, 4, 2, hd, 16, 0, [90, 90], [q, q], seed=hd)
+    b.q.fill_(1.0)
+    b.pool.keys[torch.isfinite(b.pool.keys)] = 0.0
+    for at, value in ((3, float("inf")), (90 - 4, float("nan"))):  # seen by all, by the last four queries
+        pg, slot = b.pool.where(0, 90)
+        b.pool.keys[pg[at], :, slot[at]] = -60.0  # a score of -60 hd
+        b.pool.values[pg[at], :, slot[at]] = value
+    out = b.run(cuda_lib, scale=1.0)
+    assert not torch.isfinite(out[:q]).any()
+    assert torch.isfinite(out[q:]).all()
+    out = b.run(cuda_lib, scale=1.0, window=40)  # now position 3 is behind every window
+    assert torch.isfinite(out[:q - 4]).all() and not torch.isfinite(out[q - 4:q]).any()
