@@ -6,9 +6,10 @@
 // S^T = K Q^T (16 keys x 8 rows) and O^T = V^T P^T (16 dimensions x 8 rows)
 // with m16n8k16 and f32 accumulators, so that 8 rows cost 8 rows' work, and a
 // step of 16 keys of 128 dimensions takes 16 products. P^T comes from S^T's
-// layout by an 8 x 8 transpose in registers. The softmax keeps the maximum it
-// has until a score passes it by kSlack (2^8 fits every type here), so most
-// steps exchange nothing between lanes; what is stored is exact for any base.
+// layout by an 8 x 8 transpose in registers. The softmax keeps the base it has
+// (kLift below the maximum of the time, pair16.cuh) until a score passes that
+// maximum by kSlack, so most steps exchange nothing between lanes; what is
+// stored is exact for any base.
 //
 // Each of a block's 4 warps streams its own 16 keys of every 64 through a ring
 // of kStages buffers, so that no block barrier stands in the loop; the warps'
@@ -36,7 +37,6 @@ constexpr int kThreads = 128;
 constexpr int kWarps = kThreads / kLanes;
 constexpr int kStep = 16;             // keys of a warp's step
 constexpr int kTile = kWarps * kStep;  // keys of the block's
-constexpr float kSlack = 8.0f;        // log2 units a score may pass the running base
 
 __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __half) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -106,6 +106,7 @@ __device__ __forceinline__ void thin_block(const Params& p, const Maps& maps, co
                                            uint64_t* bars) {
   using S = Shape<HDP>;
   constexpr int kRows = 8 * NT;
+  constexpr float kLift = Pair<T>::kLift, kSlack = Pair<T>::kSlack;
   const int warp = threadIdx.x / kLanes, lane = threadIdx.x % kLanes;
   const int hd = (int)p.a.cache.hd;
   char* ring = smem + warp * S::kRing;
@@ -260,9 +261,12 @@ __device__ __forceinline__ void thin_block(const Params& p, const Maps& maps, co
             x = seen ? x : -INFINITY;
           }
           s[n][e] = x;
-          past = past || x > m[n][e & 1] + kSlack;
         }
-      if (__any_sync(0xffffffffu, past)) {  // new bases: the rows' maxima so far
+#pragma unroll
+      for (int n = 0; n < NT; n++)
+#pragma unroll
+        for (int h = 0; h < 2; h++) past = past || fmaxf(s[n][h], s[n][2 + h]) - m[n][h] > kSlack + kLift;
+      if (__any_sync(0xffffffffu, past)) {  // new bases: kLift below the rows' maxima so far
 #pragma unroll
         for (int n = 0; n < NT; n++)
 #pragma unroll
@@ -270,7 +274,7 @@ __device__ __forceinline__ void thin_block(const Params& p, const Maps& maps, co
             float top = fmaxf(s[n][h], s[n][2 + h]);
 #pragma unroll
             for (int off = 4; off <= 16; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-            const float next = fmaxf(m[n][h], top);
+            const float next = fmaxf(m[n][h], top - kLift);
             const float keep = next == -INFINITY ? 1.0f : exp2_fast(m[n][h] - next);
             m[n][h] = next;
             l[n][h] *= keep;

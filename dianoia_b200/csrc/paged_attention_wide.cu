@@ -16,11 +16,12 @@
 // tensor cores serve the other. (S by halves, one ahead, leaves a group no gap
 // between them but takes products of N = 64 and twice the commits: 121 us
 // where whole tiles took 117, on 192 sequences behind 8192 keys; joining the
-// groups here instead of in the join kernel made that 113.) A base moves
-// only when a score passes it by kSlack (P then stays below 2^8), so O is
-// rescaled in TMEM in the first tiles and hardly ever after. Where rows of the
-// block see different keys of a half and a value there is not finite, that
-// half's P V is added term by term instead (0 * infinity would be NaN).
+// groups here instead of in the join kernel made that 113.) A base, set
+// kLift below a maximum, moves only when a score passes that by kSlack (both
+// pair16.cuh), so O is rescaled in TMEM in the first tiles and hardly ever
+// after. Where rows of the block see different keys of a half and a value there
+// is not finite, that half's P V is added term by term instead (0 * infinity
+// would be NaN).
 // Measured: 768 rows on 8192 keys of 8 kv heads of 128, bf16, in 48 us alone
 // (540 TFLOP/s); a group's tile takes some 5500 cycles, 3300 of them softmax
 // (the exponentials' unit for half of that, with both groups in step) and 2150
@@ -43,7 +44,6 @@ constexpr int kKeys = 2 * kHalf;  // of a tile, which one S takes
 constexpr int kRowThreads = 128;  // of a group
 constexpr int kScores = 2;        // tiles of S in TMEM
 constexpr int kHalves = 2 * kScores;
-constexpr float kSlack = 8.0f;  // log2 units a score may pass the running base
 
 struct alignas(64) Maps {
   CUtensorMap keys, values;
@@ -184,6 +184,7 @@ __device__ __forceinline__ void softmax_rows(const Params& p, const Work& w, cha
                                              uint32_t tmem, int begin, int halves, int group, int low, int high,
                                              int all_low, int all_high) {
   using S = Shape<HDP>;
+  constexpr float kLift = Pair<T>::kLift, kSlack = Pair<T>::kSlack;
   const int r = threadIdx.x % kRowThreads, lane = r % kLanes;
   const uint32_t mine = tmem + ((uint32_t)(r / kLanes * 32) << 16);
   const uint32_t out_cols = mine + kScores * kKeys + (uint32_t)(group * HDP);
@@ -237,8 +238,8 @@ __device__ __forceinline__ void softmax_rows(const Params& p, const Work& w, cha
         top4[e / 2 % 4] = max3(top4[e / 2 % 4], s[e / 32][e % 32], s[e / 32][e % 32 + 1]);
       const float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3])) * scale;
       bool waited = last < 0;
-      if (__any_sync(0xffffffffu, top > m + kSlack)) {
-        const float next = fmaxf(m, top);
+      if (__any_sync(0xffffffffu, top - m > kSlack + kLift)) {
+        const float next = fmaxf(m, top - kLift);
         const float keep = next == -INFINITY ? 1.0f : exp2_fast(m - next);
         m = next;
         l *= keep;

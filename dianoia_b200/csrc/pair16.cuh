@@ -7,8 +7,16 @@ namespace dn {
 
 template <typename T>
 struct Pair;
+// A softmax's base stands kLift (log2) below the largest score of the time it
+// was set, and stays until a score passes that by kSlack: weights reach
+// 2^(kLift + kSlack). bf16 has f32's exponents. f16's least number is 2^-24,
+// and a weight below half of that would count in the sum and not among the
+// values (128k keys of weight e^-18 beside one of 1 are 0.2% of the whole):
+// raised by 2^7, weights are kept down to 2^-32 of the largest. 2^12 leaves
+// room below f16's 2^16 for scores so large that they are rounded to units.
 template <>
 struct Pair<__half> {
+  static constexpr float kLift = 7.0f, kSlack = 5.0f;
   static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
     uint32_t u;
@@ -22,6 +30,7 @@ struct Pair<__half> {
 };
 template <>
 struct Pair<__nv_bfloat16> {
+  static constexpr float kLift = 0.0f, kSlack = 8.0f;
   static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
     uint32_t u;

@@ -470,7 +470,8 @@ int64_t dn_paged_append(const dn_paged_cache* cache, int64_t type, const void* q
  * and what lies in positions that a query does not see (infinities and NaN
  * too) does not reach its output. Scores, softmax and sums are in f32; for
  * 16-bit types the probabilities are rounded to that type before they multiply
- * the values, as the tensor cores take them. out may be q (the same address
+ * the values, as the tensor cores take them (in f16 those below 2^-32 of a
+ * row's largest come out as 0). out may be q (the same address
  * and stride). Tokens at and past q_start[sequences] are left alone.
  * max_length is the longest length the batch may have: a hint that sizes the
  * split of long sequences, any lengths are computed right. `workspace`

@@ -605,3 +605,40 @@ def test_seen_infinities_count_however_small_their_weight(cuda_lib, kind, hd, q)
     assert torch.isfinite(out[q:]).all()
     out = b.run(cuda_lib, scale=1.0, window=40)  # now position 3 is behind every window
     assert torch.isfinite(out[:q - 4]).all() and not torch.isfinite(out[q - 4:q]).any()
+
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("shared", [False, True])
+def test_many_small_probabilities_beside_a_large_one(cuda_lib, kind, shared):
+    """One key of weight near 1 and value 0 (where attention goes that has nowhere to go), and 131071 of weight e^-18
+    and value 1 behind it: their sum reaches the output. Batches large enough that no slice is short."""
+    L = cuda_lib
+    dt, code, u = ref.TYPES[kind]
+    from dianoia_b200 import _lib
+    keys, page, hd = 1 << 17, 64, 64
+    seqs, heads = (75, 128) if shared else (600, 4)
+    pages = keys // page
+    pool = ref.Pool(kind, pages, page, 1, hd, seqs, pages + 1, fill=0.0)
+    pool.table[:, :pages] = torch.arange(pages, device="cuda", dtype=torch.int32)  # one sequence's pages for all
+    pool.values.fill_(1.0)
+    pool.keys[0, 0, 3, 0], pool.values[0, 0, 3] = 4.0, 0.0
+    q = torch.zeros((seqs, heads, hd), device="cuda", dtype=dt)
+    q[:, :, 0] = 4.5
+    out = torch.full_like(q, 7.0)
+    prefix = keys if shared else 0
+    lens = ints([keys] * seqs)
+    need = L.dn_paged_attention_workspace(pool.c, heads, seqs, prefix, keys)
+    ws = torch.full((need,), 255, dtype=torch.uint8, device="cuda")
+    assert L.dn_paged_attention(pool.c, q.data_ptr(), heads * hd, None, lens.data_ptr(), pool.table[0].data_ptr(), prefix, keys, 1.0, 0,
+                                out.data_ptr(), heads * hd, heads, seqs, ws.data_ptr(), need, 0, stream()) == 0
+    torch.cuda.synchronize()
+    import math
+    tail = (keys - 1) * math.exp(-18.0)
+    want = torch.full_like(out, tail / (1 + tail), dtype=torch.float64)
+    # The probabilities' rounding: u of each, and in f16, whose numbers end at 2^-24, half of that for each key against
+    # a largest probability of 2^7 at least; scores and sums in f32 as in the reference's bound (mag 18).
+    a = want[0, 0, 0].item()
+    small = keys * 2.0 ** -25 * 2.0 ** -7 if kind == "f16" else 0.0
+    tol = small + a * (u + 2 * (hd + 8) * ref.U32 * 18 + (keys + 64) * ref.U32) * (1 + u)
+    ref.check(out, want, torch.full_like(want, tol), u, "small probabilities")
