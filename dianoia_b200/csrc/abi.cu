@@ -671,8 +671,11 @@ int64_t dn_paged_append(const dn_paged_cache* cache, int64_t type, const void* q
   if ((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v) & es) != 0 || ((uintptr_t)q_out & cs) != 0 ||
       (((uintptr_t)seq | (uintptr_t)pos | (uintptr_t)rope | (uintptr_t)q_norm | (uintptr_t)k_norm) & 3) != 0)
     return DN_ERR_ARGS;
-  if (heads > 0 && overlaps(q, q_stride, qd, type, q_out, q_out_stride, qd, cache->type, n) &&
-      !(q == q_out && type == cache->type && q_stride == q_out_stride))
+  const bool in_place = q == q_out && type == cache->type && q_stride == q_out_stride;
+  if (heads > 0 && !in_place &&
+      (overlaps(q, q_stride, qd, type, q_out, q_out_stride, qd, cache->type, n) ||
+       overlaps(k, k_stride, kv, type, q_out, q_out_stride, qd, cache->type, n) ||
+       overlaps(v, v_stride, kv, type, q_out, q_out_stride, qd, cache->type, n)))
     return DN_ERR_ARGS;
   if (device_state() == nullptr) return DN_ERR_NO_DEVICE;
   dn::PagedAppendArgs a{};

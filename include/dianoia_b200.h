@@ -443,7 +443,7 @@ typedef struct dn_paged_cache {
  * each result is rounded once, to the cache's type: keys and values into the
  * token's slot, queries to q_out (`heads` rows of hd at t * q_out_stride).
  * heads 0 (q and q_out may be NULL) appends without queries. q_out must not
- * overlap q unless it has the same address, type and stride.
+ * overlap q, k or v, except that it may have q's address, type and stride.
  * A token is skipped - nothing appended, its q_out row zeros - where seq[t] is
  * outside [0, sequences), pos[t] is negative, past the table or (rot > 0) past
  * the rope_rows rows of `rope`, or its table entry names no page. Two tokens

@@ -93,3 +93,17 @@ def test_interleaved_rows_are_no_overlap(L):
         assert L.dn_paged_append(*args.values()) == _lib.DN_ERR_NO_DEVICE
         args["qo"] += 2
         assert L.dn_paged_append(*args.values()) == _lib.DN_ERR_ARGS
+
+
+def test_rotated_queries_apart_from_keys_and_values(L):
+    """Rotated queries over keys or values that other threads still read are refused, as over other queries."""
+    args = dict(c=cache(), t=2, q=A, qs=512, k=A + 2 * 128, ks=512, v=A + 2 * 256, vs=512, seq=A, pos=A, rope=A, rows=64, rot=64,
+                qn=None, kn=None, eps=1e-6, qo=A, qos=512, h=2, n=5, f=0, s=None)
+    call = lambda **kw: L.dn_paged_append(*{**args, **kw}.values())
+    for kw in (dict(qo=A + 2 * 128), dict(qo=A + 2 * 256), dict(qo=A + 2 * 383), dict(qo=A + 2 * 4 * 512 + 2 * 300),
+               dict(qo=A + 2 * 256, qos=256), dict(q=A + 2 * 384, qo=A + 2 * 129)):
+        assert call(**kw) == _lib.DN_ERR_ARGS, kw
+    if not has_gpu():
+        assert call() == _lib.DN_ERR_NO_DEVICE  # in place, beside its keys and values
+        assert call(qo=A + 2 * 384) == _lib.DN_ERR_NO_DEVICE  # after them in the same rows
+        assert call(h=0, q=None, qo=None) == _lib.DN_ERR_NO_DEVICE
