@@ -250,6 +250,16 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint64_t* bar, uint32_t parity
   }
 }
 
+// Lets what is in flight towards `bar` land before its shared or tensor memory
+// goes, where a bounded wait has run out: at most kWaitLimitNs more, whatever
+// dn_set_wait_limit_ns says (a limit shorter than a copy takes must not end a
+// CTA under it).
+__device__ __forceinline__ void mbar_land(uint64_t* bar, uint32_t parity) {
+  const uint64_t start = globaltimer_ns();
+  while (!mbar_try_wait(bar, parity) && globaltimer_ns() - start <= kWaitLimitNs) {
+  }
+}
+
 // 1-D bulk copy global -> shared (TMA engine), completing on `bar` with
 // `bytes` transaction bytes. dst, src and bytes must be multiples of 16.
 __device__ __forceinline__ void bulk_g2s(void* dst, const void* src, uint32_t bytes,

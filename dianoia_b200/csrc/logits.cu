@@ -147,8 +147,9 @@ __global__ void __launch_bounds__(kThreads) logits_kernel(const __grid_constant_
     }
     if (atomicOr(&marks[v], kBiased) == 0) add_to_list(v);
   }
-  if (to > from && !mbar_wait_bounded(&full, 0, a.status, kStatusTmaTimeout)) seen = biased = 0;
-  __syncthreads();
+  const bool landed = to <= from || mbar_wait_bounded(&full, 0, a.status, kStatusTmaTimeout);
+  if (!landed) mbar_land(&full, 0);
+  if (!__syncthreads_and(landed)) return;
 
   // The marked tokens.
   const int count = marked ? listed : 0;

@@ -221,10 +221,11 @@ __device__ __forceinline__ void thin_block(const Params& p, const Maps& maps, co
   }
 
   bool live = true;
+  int step = 0;
   for (int base = 0; base < steps && live; base += S::kStages) {
 #pragma unroll
     for (int b = 0; b < S::kStages; b++) {
-      const int step = base + b;
+      step = base + b;
       if (step >= steps) break;
       live = __all_sync(0xffffffffu, wait_phase(&full[b], (step / S::kStages) & 1, p.status, kStatusTmaTimeout));
       if (!live) break;
@@ -336,6 +337,8 @@ __device__ __forceinline__ void thin_block(const Params& p, const Maps& maps, co
       issue(step + S::kStages, b);
     }
   }
+  if (!live)  // copies on their way into this step's buffer and the ones after it
+    for (int i = step; i < min(steps, step + S::kStages); i++) mbar_land(&full[i % S::kStages], (i / S::kStages) & 1);
 #pragma unroll
   for (int n = 0; n < NT; n++)
 #pragma unroll

@@ -558,6 +558,7 @@ __global__ void __maxnreg__(Shape<HDP>::kRegs)
     if (group < tiles) load(&maps.keys, k_at, group, page, slot, &bars.k_full[group]);
     bool live = true;
     int last = -1;  // the group's last half
+    int keys = group, tile = -1;  // the last tiles whose keys, and whose S and values, were asked for
     for (int i = group; i < tiles && live; i += S::kGroups) {
       const int turn = i / S::kGroups, page_k = page_at(next), slot_k = slot_at(i + S::kGroups);
       next = look_up(i + 2 * S::kGroups);
@@ -578,7 +579,10 @@ __global__ void __maxnreg__(Shape<HDP>::kRegs)
       load(&maps.values, v_at, i, page, slot, &bars.v_full[group]);
       // S is there: its keys' place is free.
       live = wait(&bars.s_full[i % kScores], i / kScores, kStatusMmaTimeout);
-      if (live && i + S::kGroups < tiles) load(&maps.keys, k_at, i + S::kGroups, page_k, slot_k, &bars.k_full[group]);
+      if (live && i + S::kGroups < tiles) {
+        keys = i + S::kGroups;
+        load(&maps.keys, k_at, keys, page_k, slot_k, &bars.k_full[group]);
+      }
       page = page_k;
       slot = slot_k;
       for (int j = 2 * i; j < min(2 * i + 2, halves) && live; j++) {
@@ -600,6 +604,15 @@ __global__ void __maxnreg__(Shape<HDP>::kRegs)
         last = j;
       }
     }
+    // Nothing is in flight when the block goes, given up or not.
+    if (!live) {
+      mbar_land(&bars.k_full[group], keys / S::kGroups & 1);
+      if (tile >= 0) {
+        mbar_land(&bars.v_full[group], tile / S::kGroups & 1);
+        mbar_land(&bars.s_full[tile % kScores], tile / kScores & 1);
+      }
+    }
+    if (last >= 0) mbar_land(&bars.o_done[last % kHalves], last / kHalves & 1);
     __syncwarp();
   }
   fence_before();

@@ -240,3 +240,22 @@ def test_vocabularies_around_whole_ranges(cuda_lib, kind, vocab):
             rows_out[:, :vocab] = 6.0
             assert (b == 6).all()
     assert cuda_lib.dn_device_status(1) == 0
+
+
+def test_a_wait_that_runs_out_leaves_nothing_in_flight(cuda_lib):
+    """With a wait limit shorter than a copy takes, calls come back, their status bit a copy's alone; the next one is right."""
+    L, vocab = cuda_lib, 50257
+    rules = make_rules(20, vocab, ALL, seed=9)
+    x = torch.randn((20, vocab), device="cuda")
+    first, out = torch.empty_like(x), torch.empty_like(x)
+    assert apply(L, "f32", x, first, vocab, rules) == 0
+    assert L.dn_set_wait_limit_ns(1) == 0
+    try:
+        for _ in range(3):
+            assert apply(L, "f32", x, out, vocab, rules) == 0
+    finally:
+        torch.cuda.synchronize()
+        assert L.dn_set_wait_limit_ns(0) == 0
+    assert L.dn_device_status(1) & ~1 == 0
+    assert apply(L, "f32", x, out, vocab, rules) == 0
+    assert torch.equal(out, first) and L.dn_device_status(1) == 0

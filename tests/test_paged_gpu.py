@@ -642,3 +642,28 @@ def test_many_small_probabilities_beside_a_large_one(cuda_lib, kind, shared):
     small = keys * 2.0 ** -25 * 2.0 ** -7 if kind == "f16" else 0.0
     tol = small + a * (u + 2 * (hd + 8) * ref.U32 * 18 + (keys + 64) * ref.U32) * (1 + u)
     ref.check(out, want, torch.full_like(want, tol), u, "small probabilities")
+
+
+def test_waits_that_run_out_leave_nothing_in_flight(cuda_lib):
+    """With a wait limit far shorter than a copy takes, calls come back (their outputs may be incomplete, and the status
+    word says so with the bits of a copy or of a product alone) and the next ones with the usual limit are right."""
+    L = cuda_lib
+    batches = [Batch("bf16", 4, 2, 64, 16, 48, [300, 64, 77], [1, 1, 1], seed=1),  # copied by tiles
+               Batch("f16", 4, 2, 96, 7, 0, [300, 64, 77], [1, 9, 1], seed=2),  # by the lanes
+               Batch("bf16", 8, 2, 128, 16, 1200, [40] * 60, [1] * 60, seed=3),  # wide blocks beside thin ones
+               Batch("f16", 4, 1, 192, 32, 0, [500, 90], [90, 90], seed=4)]
+    firsts = [b.check(L).clone() for b in batches]
+    assert L.dn_device_status(1) == 0
+    torch.cuda.synchronize()
+    assert L.dn_set_wait_limit_ns(1) == 0
+    try:
+        for b in batches:
+            for _ in range(3):
+                b.run(L)
+    finally:
+        torch.cuda.synchronize()
+        assert L.dn_set_wait_limit_ns(0) == 0
+    assert L.dn_device_status(1) & ~(1 | 4) == 0
+    for b, first in zip(batches, firsts):
+        assert torch.equal(b.run(L), first)
+    assert L.dn_device_status(1) == 0
