@@ -18,7 +18,6 @@ _i64 = ctypes.c_int64
 _p = ctypes.c_void_p
 
 
-
 class PagedCache(ctypes.Structure):
     """dn_paged_cache (include/dianoia_b200.h)."""
     _fields_ = [("keys", _p), ("values", _p), ("table", _p), ("type", _i64), ("pages", _i64),

@@ -14,7 +14,8 @@ namespace {
 //
 // Any type, head size up to 256 and alignment; f32 caches first of all, whose
 // products the tensor cores would round. Bound by the keys' bytes for the few
-// rows of a decode step, so nothing goes through shared memory: a warp's lanes
+// rows of a decode step (a block holds a sequence's rows, at most 8, and reads
+// its keys for them, the prefix's too), so nothing goes through shared memory: a warp's lanes
 // lie along the head (V dimensions each, 32 V more on), and a step of 32 / RT
 // keys is 32 / RT whole rows loaded at once for RT rows of queries. The 32
 // partial products of a lane are summed over the lanes by halves (31
@@ -22,8 +23,11 @@ namespace {
 // row l % RT; each probability goes back to all lanes for the values. A block's
 // 4 warps take steps in turn and are joined once at the end.
 // Measured: 7 sequences of 680 keys, 8 kv heads of 128, 2 heads a group, window
-// 600: 12.5 us with the join (46 us with tiles in shared memory, where a block's
-// 16 rows were mostly empty).
+// 600: 12.6 us with the join (46 us with tiles in shared memory, where a block's
+// 16 rows were mostly empty). What it costs where rows are many or a 16-bit cache
+// is not the tensor cores': a prompt of 2048 f32 tokens (16 heads of 128) 884 us;
+// 32 chat sequences of a bf16 cache that starts 8 bytes off a 16-byte boundary
+// 80 us, 2 bytes off (element by element) 278 us, where the tensor cores take 24.
 constexpr int kSimtThreads = 128;
 constexpr int kSimtWarps = kSimtThreads / kLanes;
 constexpr float kSlack = 8.0f;  // log2 units a score may pass the running base
@@ -266,13 +270,23 @@ bool mma_cache(const PagedCache& c) {
   return c.type != kF32 && (((uintptr_t)c.keys | (uintptr_t)c.values) & 15) == 0 && (c.page_stride | c.hd) % 8 == 0;
 }
 
-constexpr int64_t kSoloKeys = 512;    // of the longest sequence
-constexpr int64_t kSoloReads = 8192;  // keys of the prefix, once for each sequence
+// Limits up to which sequences read the prefix for themselves: keys of the
+// longest, and of the prefix, once for each sequence. Measured with and without
+// (us; 8 kv heads of 128, 2 heads a group, bf16, 16 own keys): 2 sequences
+// behind 64 keys 6.7 and 8.2, 8 behind 256 10.8 and 13.5, 16 behind 512 12.3
+// and 13.8, 32 behind 256 15.8 and 17.1; past the limits 16 behind 1024 18.1
+// and 14.4, 32 behind 512 19.5 and 19.2, though 8 behind 1024 11.6 and 13.8.
+// One or two sequences of 320 to 512 keys lose 0.1 to 0.8 by it.
+constexpr int64_t kSoloKeys = 512;
+constexpr int64_t kSoloReads = 8192;
 
 // Least keys of a slice: of the thin kernel, the f32 one, and a wide block of
-// two groups and of one (32 chat sequences and 24 of drafts: 23 and 22 us with
-// 384, 22 and 27 with 256, 25 and 23 with 512; with 256-wide heads 29 us with
-// 128, 32 with 256).
+// two groups and of one. Over 35 batches (16 to 192 sequences behind 700 to 8192
+// keys, heads of 64 and 128) a least of 384 takes the same time as 512, 1% more
+// than 256, and 2% and 7% less than 128 and 768, in the geometric mean; single
+// batches differ more (32 chat sequences and 24 of drafts: 23.6 and 22.1 us with
+// 384, 21.9 and 27.3 with 256, 24.8 and 23.1 with 512). With 256-wide heads 29 us
+// with 128, 32 with 256.
 constexpr int kThinLeast = 256, kSimtLeast = 128, kWide2Least = 384, kWide1Least = 128;
 
 // How the work is divided, from sizes that the host knows.

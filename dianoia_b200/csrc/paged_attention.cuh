@@ -251,7 +251,15 @@ __device__ __forceinline__ int slice_index(const Params& p, const Work& w) {
 
 // Rows of a block of the wide kernel (the thin one: 8 or 16, the f32 one: 1 to 8).
 constexpr int kWideRows = 128;
-constexpr int kWideFrom = 32;  // rows (of the batch, of a sequence on average) from which the wide one runs
+// Rows (of the batch on the prefix, of a sequence on average) past which the
+// wide one runs. Measured, thin and wide (us, whole calls; 8 kv heads of 128, 2
+// heads a group, bf16): on a prefix of 8192 keys 16 rows 22 and 24, 32 rows 32
+// and 26, 64 rows 39 and 29, 128 rows 57 and 33; of 1024 keys 40 rows 14.7 and
+// 18.5, 64 rows 15 and 19, 96 rows 21 and 20, 128 rows 22 and 22; rows of 16
+// sequences of up to 1024 own keys, 24 rows on average 28 and 28, 32 rows 33 and
+// 28, 48 rows 44 and 33; of one sequence of 2048 keys, at most 96 rows, 14 and
+// 18. A middle: the long prefix gains from some 20 rows on, the short one from 96.
+constexpr int kWideFrom = 32;
 constexpr int kLanes = 32;
 
 // Groups of a wide block: two outputs of 128 columns stand in TMEM beside the

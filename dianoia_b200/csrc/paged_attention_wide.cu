@@ -22,8 +22,8 @@
 // after. Where rows of the block see different keys of a half and a value there
 // is not finite, that half's P V is added term by term instead (0 * infinity
 // would be NaN).
-// Measured: 768 rows on 8192 keys of 8 kv heads of 128, bf16, in 48 us alone
-// (540 TFLOP/s); a group's tile takes some 5500 cycles, 3300 of them softmax
+// Measured: 768 rows on 8192 keys of 8 kv heads of 128, bf16, in 45 us alone
+// (570 TFLOP/s); a group's tile takes some 5500 cycles, 3300 of them softmax
 // (the exponentials' unit for half of that, with both groups in step) and 2150
 // the way from the last P through P V, its commit and the next S.
 #include <type_traits>
@@ -53,7 +53,9 @@ template <int HDP>
 struct Shape {
   static constexpr int kPanels = HDP / 64;
   // With two groups, three warps to a quarter of the SM: 128 registers leave a
-  // warp of a thin block (128) its place in the quarter's 16384.
+  // warp of an 8-row thin block (128) its place in the quarter's 16384 (not of a
+  // 16-row one, which takes 168 of heads of 65 to 128 and waits for wide blocks
+  // to end).
   static constexpr int kRegs = wide_groups(HDP) == 2 ? 128 : 168;
   static constexpr int kQPanel = kRows * 128;  // bytes: 64 elements of every row
   static constexpr int kKPanel = kKeys * 128;  // of every key of a tile

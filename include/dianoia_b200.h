@@ -456,9 +456,13 @@ int64_t dn_paged_append(const dn_paged_cache* cache, int64_t type, const void* q
 
 /* Causal grouped-query attention of a batch over a paged cache whose
  * sequences share their first `prefix` positions: those keys and values are
- * read once, through prefix_pages (the ceil(prefix / page_size) pages that
- * hold them; NULL with prefix 0), for every query of the batch; positions from
- * `prefix` on are read through each sequence's own table row. Queries are
+ * read through prefix_pages (the ceil(prefix / page_size) pages that hold
+ * them; NULL with prefix 0), positions from `prefix` on through each sequence's
+ * own table row. Where 16-bit caches go to the tensor cores (aligned as above,
+ * hd a multiple of 8), the prefix is read once for the rows (query heads of a
+ * kv head, of any sequences) of a tile: 128 rows where there are more than 32
+ * and pages are multiples of 16, else 8 or 16; short batches (sequences of 512
+ * keys at most) and f32 arithmetic read it once for each sequence. Queries are
  * ragged: sequence s has tokens q_start[s] .. q_start[s + 1] - 1 of q (n =
  * q_start[sequences]; q_start NULL is one token for each sequence), its last
  * ones, so that token t is at position lengths[s] - (q_start[s + 1] - t) and
@@ -492,7 +496,7 @@ typedef struct dn_logit_rules {
    * are tokens[history[r]] .. tokens[history[r + 1] - 1]; its last
    * generated[r] of them were generated (generated NULL: all). Ids outside
    * [0, vocab) are ignored. NULL penalties are neutral. A row has fewer than
-   * 2^31 tokens, and biases. */
+   * 2^30 tokens, and biases. */
   const int32_t* tokens;
   const int64_t* history;   /* [n + 1] */
   const int32_t* generated; /* [n] */
