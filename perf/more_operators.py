@@ -300,9 +300,9 @@ def run(state):
 
 def _kept(state, make):
     """The descriptors that a user's program makes once for its cache or its batch and passes to every call."""
-    if "kept" not in state:
-        state["kept"] = make(state)
-    return state["kept"]
+    if "handle" not in state:
+        state["handle"] = make(state)
+    return state["handle"]
 
 
 def _stream():
