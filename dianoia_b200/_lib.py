@@ -32,7 +32,21 @@ class LogitRules(ctypes.Structure):
                 ("mask_row", _p), ("mask_rows", _i64), ("mask_stride", _i64)]
 
 
+class PagedQ8Cache(ctypes.Structure):
+    """dn_paged_q8_cache (include/dianoia_b200.h)."""
+    _fields_ = [("keys", _p), ("values", _p), ("key_scales", _p), ("value_scales", _p), ("table", _p), ("pages", _i64),
+                ("page_size", _i64), ("kv_heads", _i64), ("hd", _i64), ("sequences", _i64), ("table_stride", _i64),
+                ("page_stride", _i64), ("scale_stride", _i64)]
+
+
+class Sampling(ctypes.Structure):
+    """dn_sampling (include/dianoia_b200.h)."""
+    _fields_ = [("temperature", _p), ("top_k", _p), ("top_p", _p), ("min_p", _p), ("uniform", _p)]
+
+
 _cache_p = ctypes.POINTER(PagedCache)
+_q8_cache_p = ctypes.POINTER(PagedQ8Cache)
+_sampling_p = ctypes.POINTER(Sampling)
 _rules_p = ctypes.POINTER(LogitRules)
 
 # Every exported function with its ctypes signature (restype, argtypes).
@@ -102,6 +116,15 @@ SIGNATURES = {
     "dn_paged_attention": (_i64, [_cache_p, _p, _i64, _p, _p, _p, _i64, _i64, ctypes.c_double, _i64, _p, _i64, _i64,
                                   _i64, _p, _i64, _i64, _p]),
     "dn_logits_apply": (_i64, [_i64, _p, _i64, _p, _i64, _i64, _i64, _rules_p, _i64, _p]),
+    "dn_paged_q8_append": (_i64, [_q8_cache_p, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _p, _p, _i64, _i64, _p, _p,
+                                  ctypes.c_double, _i64, _p, _i64, _i64, _i64, _i64, _p]),
+    "dn_paged_q8_read": (_i64, [_q8_cache_p, _i64, _p, _p, _p, _i64, _p, _i64, _i64, _i64, _p]),
+    "dn_paged_q8_attention_workspace": (_i64, [_q8_cache_p, _i64, _i64, _i64]),
+    "dn_paged_q8_attention": (_i64, [_q8_cache_p, _i64, _p, _i64, _p, _p, _i64, ctypes.c_double, _i64, _p, _i64, _i64, _i64,
+                                     _p, _i64, _i64, _p]),
+    "dn_residual_norm": (_i64, [_i64, _p, _i64, _p, _p, _i64, ctypes.c_double, _i64, _p, _i64, _p, _i64, _p, ctypes.c_double,
+                                _p, _i64, _p, _i64, _i64, _i64, _i64, _p]),
+    "dn_sample": (_i64, [_i64, _p, _i64, _i64, _i64, _sampling_p, _p, _p, _p, _i64, _p]),
     "dn_linear_qa": (_i64, [_i64, _p, _p, _p, _i64, _p, _i64, _p, _i64, _i64, _i64, _i64, _i64, _p]),
     "dn_linear_allgather": (_i64, [_i64, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _p, _p, _i64, _p]),
     "dn_linear_qa_allgather": (_i64, [_i64, _p, _p, _p, _i64, _i64, _i64, _p, _p, _i64, _i64, _p]),

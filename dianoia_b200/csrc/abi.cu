@@ -438,6 +438,57 @@ int64_t check_attention(const dn_paged_cache* c, int64_t heads, int64_t n, int64
   return DN_OK;
 }
 
+// Whether two runs of bytes share one.
+bool runs_meet(const void* a, int64_t abytes, const void* b, int64_t bbytes) {
+  const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+  return a != nullptr && b != nullptr && abytes > 0 && bbytes > 0 && x < y + (uintptr_t)bbytes &&
+         y < x + (uintptr_t)abytes;
+}
+
+int64_t rows_bytes(int64_t rows, int64_t stride, int64_t cols, int64_t size) {
+  return rows <= 0 || cols <= 0 ? 0 : ((rows - 1) * stride + cols) * size;
+}
+
+int64_t check_q8_cache(const dn_paged_q8_cache* c) {
+  static_assert(sizeof(dn_paged_q8_cache) == sizeof(dn::PagedQ8Cache), "cache layouts differ");
+  static_assert(sizeof(dn_sampling) == sizeof(dn::Sampling), "sampling layouts differ");
+  if (c == nullptr || c->pages < 0 || c->page_size < 1 || c->kv_heads < 1 || c->hd < 16 || c->hd % 16 != 0 ||
+      c->sequences < 0 || c->table_stride < 0)
+    return DN_ERR_ARGS;
+  if (c->hd > dn::kMaxPagedHd || c->page_size > (1 << 20) || c->kv_heads > 65535 || c->pages > INT32_MAX ||
+      c->sequences > (1 << 24) || c->table_stride > INT32_MAX || c->page_stride > kMaxStride ||
+      c->scale_stride > kMaxStride)
+    return DN_ERR_TOO_LARGE;
+  if (c->page_stride < c->kv_heads * c->page_size * c->hd || c->scale_stride < c->kv_heads * c->page_size ||
+      c->page_stride % 16 != 0)
+    return DN_ERR_ARGS;
+  // Positions are int32.
+  if (c->table_stride * c->page_size > (int64_t)1 << 30) return DN_ERR_TOO_LARGE;
+  if (c->pages > 0 && (c->keys == nullptr || c->values == nullptr || c->key_scales == nullptr ||
+                       c->value_scales == nullptr))
+    return DN_ERR_ARGS;
+  if (c->sequences > 0 && c->table_stride > 0 && c->table == nullptr) return DN_ERR_ARGS;
+  if ((((uintptr_t)c->keys | (uintptr_t)c->values) & 15) != 0 ||
+      (((uintptr_t)c->key_scales | (uintptr_t)c->value_scales | (uintptr_t)c->table) & 3) != 0)
+    return DN_ERR_ARGS;
+  return DN_OK;
+}
+
+// Whether a run of bytes meets the cache's rows or scales.
+bool meets_q8_cache(const dn_paged_q8_cache* c, const void* p, int64_t bytes) {
+  const int64_t rows = rows_bytes(c->pages, c->page_stride, c->kv_heads * c->page_size * c->hd, 1);
+  const int64_t scales = rows_bytes(c->pages, c->scale_stride, c->kv_heads * c->page_size, 4);
+  return runs_meet(p, bytes, c->keys, rows) || runs_meet(p, bytes, c->values, rows) ||
+         runs_meet(p, bytes, c->key_scales, scales) || runs_meet(p, bytes, c->value_scales, scales);
+}
+
+int64_t check_q8_attention(const dn_paged_q8_cache* c, int64_t heads, int64_t n, int64_t max_length) {
+  if (heads < 1 || heads % c->kv_heads != 0 || n < 0 || max_length < 0) return DN_ERR_ARGS;
+  if (heads > (1 << 20) || n > (int64_t)1 << 24 || n * heads > (int64_t)1 << 30 || max_length > (int64_t)1 << 30)
+    return DN_ERR_TOO_LARGE;
+  return DN_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -790,6 +841,247 @@ int64_t dn_logits_apply(int64_t type, const void* logits, int64_t stride, void* 
   dn::LogitsArgs a{type, logits, out, stride, out_stride, n, vocab, {}, d->status_dev};
   memcpy(&a.rules, rules, sizeof a.rules);
   return dn::launch_logits(a, static_cast<cudaStream_t>(stream), (flags & DN_FLAG_PDL) != 0) == cudaSuccess
+             ? DN_OK
+             : launch_failed();
+}
+
+int64_t dn_paged_q8_append(const dn_paged_q8_cache* cache, int64_t type, const void* q, int64_t q_stride,
+                           const void* k, int64_t k_stride, const void* v, int64_t v_stride,
+                           const int32_t* seq, const int32_t* pos, const float* rope, int64_t rope_rows,
+                           int64_t rot, const float* q_norm, const float* k_norm, double eps,
+                           int64_t out_type, void* q_out, int64_t q_out_stride, int64_t heads, int64_t n,
+                           int64_t flags, void* stream) {
+  if (int64_t rc = check_q8_cache(cache); rc != DN_OK) return rc;
+  if (!elem_type(type) || !elem_type(out_type) || n < 0 || heads < 0 || rot < 0 || rot % 2 != 0 || rot > cache->hd ||
+      rope_rows < 0)
+    return DN_ERR_ARGS;
+  const int64_t kv = cache->kv_heads * cache->hd, qd = heads * cache->hd;
+  if (heads > (1 << 20) || q_stride > kMaxStride || k_stride > kMaxStride || v_stride > kMaxStride ||
+      q_out_stride > kMaxStride)
+    return DN_ERR_TOO_LARGE;
+  if (k_stride < kv || v_stride < kv || q_stride < qd || q_out_stride < qd) return DN_ERR_ARGS;
+  // A group of lanes for each (token, head): the launch's block count fits 31 bits.
+  if (n > (int64_t)0x7fffffff / (heads + 2 * cache->kv_heads)) return DN_ERR_TOO_LARGE;
+  if (n == 0) return DN_OK;
+  if (k == nullptr || v == nullptr || seq == nullptr || pos == nullptr || (rot > 0 && rope == nullptr) ||
+      (heads > 0 && (q == nullptr || q_out == nullptr)))
+    return DN_ERR_ARGS;
+  const int64_t size = dn::elem_size(type), out_size = dn::elem_size(out_type);
+  if ((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v) & (uintptr_t)(size - 1)) != 0 ||
+      ((uintptr_t)q_out & (uintptr_t)(out_size - 1)) != 0 ||
+      (((uintptr_t)seq | (uintptr_t)pos | (uintptr_t)rope | (uintptr_t)q_norm | (uintptr_t)k_norm) & 3) != 0)
+    return DN_ERR_ARGS;
+  const bool in_place = q == q_out && type == out_type && q_stride == q_out_stride;
+  if (heads > 0 && ((!in_place && overlaps(q, q_stride, qd, type, q_out, q_out_stride, qd, out_type, n)) ||
+                    overlaps(k, k_stride, kv, type, q_out, q_out_stride, qd, out_type, n) ||
+                    overlaps(v, v_stride, kv, type, q_out, q_out_stride, qd, out_type, n) ||
+                    meets_q8_cache(cache, q, rows_bytes(n, q_stride, qd, size)) ||
+                    meets_q8_cache(cache, q_out, rows_bytes(n, q_out_stride, qd, out_size))))
+    return DN_ERR_ARGS;
+  if (meets_q8_cache(cache, k, rows_bytes(n, k_stride, kv, size)) ||
+      meets_q8_cache(cache, v, rows_bytes(n, v_stride, kv, size)))
+    return DN_ERR_ARGS;
+  if (device_state() == nullptr) return DN_ERR_NO_DEVICE;
+  dn::PagedQ8AppendArgs a{};
+  memcpy(&a.cache, cache, sizeof a.cache);
+  a.type = type;
+  a.out_type = out_type;
+  a.q = q;
+  a.k = k;
+  a.v = v;
+  a.q_stride = q_stride;
+  a.k_stride = k_stride;
+  a.v_stride = v_stride;
+  a.seq = seq;
+  a.pos = pos;
+  a.rope = rope;
+  a.rope_rows = rope_rows;
+  a.rot = rot;
+  a.q_norm = q_norm;
+  a.k_norm = k_norm;
+  a.eps = (float)eps;
+  a.q_out = q_out;
+  a.q_out_stride = q_out_stride;
+  a.heads = heads;
+  a.n = n;
+  return dn::launch_paged_q8_append(a, static_cast<cudaStream_t>(stream), (flags & DN_FLAG_PDL) != 0) == cudaSuccess
+             ? DN_OK
+             : launch_failed();
+}
+
+int64_t dn_paged_q8_read(const dn_paged_q8_cache* cache, int64_t type, const int32_t* seq, const int32_t* pos,
+                         void* k_out, int64_t k_stride, void* v_out, int64_t v_stride, int64_t n,
+                         int64_t flags, void* stream) {
+  if (int64_t rc = check_q8_cache(cache); rc != DN_OK) return rc;
+  if (!elem_type(type) || n < 0) return DN_ERR_ARGS;
+  const int64_t kv = cache->kv_heads * cache->hd, size = dn::elem_size(type);
+  if (k_stride > kMaxStride || v_stride > kMaxStride || n > (int64_t)0x7fffffff / (2 * cache->kv_heads))
+    return DN_ERR_TOO_LARGE;
+  if ((k_out != nullptr && k_stride < kv) || (v_out != nullptr && v_stride < kv)) return DN_ERR_ARGS;
+  if (n == 0 || (k_out == nullptr && v_out == nullptr)) return DN_OK;
+  if (seq == nullptr || pos == nullptr || (((uintptr_t)seq | (uintptr_t)pos) & 3) != 0 ||
+      (((uintptr_t)k_out | (uintptr_t)v_out) & (uintptr_t)(size - 1)) != 0)
+    return DN_ERR_ARGS;
+  if (k_out != nullptr && v_out != nullptr && overlaps(k_out, k_stride, kv, type, v_out, v_stride, kv, type, n))
+    return DN_ERR_ARGS;
+  if (meets_q8_cache(cache, k_out, rows_bytes(n, k_stride, kv, size)) ||
+      meets_q8_cache(cache, v_out, rows_bytes(n, v_stride, kv, size)))
+    return DN_ERR_ARGS;
+  if (device_state() == nullptr) return DN_ERR_NO_DEVICE;
+  dn::PagedQ8ReadArgs a{};
+  memcpy(&a.cache, cache, sizeof a.cache);
+  a.type = type;
+  a.seq = seq;
+  a.pos = pos;
+  a.k_out = k_out;
+  a.v_out = v_out;
+  a.k_stride = k_stride;
+  a.v_stride = v_stride;
+  a.n = n;
+  return dn::launch_paged_q8_read(a, static_cast<cudaStream_t>(stream), (flags & DN_FLAG_PDL) != 0) == cudaSuccess
+             ? DN_OK
+             : launch_failed();
+}
+
+int64_t dn_paged_q8_attention_workspace(const dn_paged_q8_cache* cache, int64_t heads, int64_t n,
+                                        int64_t max_length) {
+  if (int64_t rc = check_q8_cache(cache); rc != DN_OK) return rc;
+  if (int64_t rc = check_q8_attention(cache, heads, n, max_length); rc != DN_OK) return rc;
+  dn::PagedQ8Cache c;
+  memcpy(&c, cache, sizeof c);
+  return dn::paged_q8_attention_workspace(c, heads, n, max_length);
+}
+
+int64_t dn_paged_q8_attention(const dn_paged_q8_cache* cache, int64_t type, const void* q, int64_t q_stride,
+                              const int32_t* q_start, const int32_t* lengths, int64_t max_length,
+                              double scale, int64_t window, void* out, int64_t out_stride, int64_t heads,
+                              int64_t n, void* workspace, int64_t workspace_bytes, int64_t flags,
+                              void* stream) {
+  if (int64_t rc = check_q8_cache(cache); rc != DN_OK) return rc;
+  if (int64_t rc = check_q8_attention(cache, heads, n, max_length); rc != DN_OK) return rc;
+  const int64_t row = heads * cache->hd;
+  if (!elem_type(type) || window < 0 || window > INT32_MAX || q_stride < row || out_stride < row ||
+      workspace_bytes < 0)
+    return DN_ERR_ARGS;
+  if (q_stride > kMaxStride || out_stride > kMaxStride) return DN_ERR_TOO_LARGE;
+  if (q_start == nullptr && n != cache->sequences) return DN_ERR_ARGS;
+  if (n == 0) return DN_OK;
+  if (q == nullptr || lengths == nullptr || out == nullptr || workspace == nullptr) return DN_ERR_ARGS;
+  const int64_t size = dn::elem_size(type);
+  if ((((uintptr_t)q | (uintptr_t)out) & (uintptr_t)(size - 1)) != 0 || ((uintptr_t)workspace & 15) != 0 ||
+      (((uintptr_t)q_start | (uintptr_t)lengths) & 3) != 0)
+    return DN_ERR_ARGS;
+  if (overlaps(q, q_stride, row, type, out, out_stride, row, type, n) && !(q == out && q_stride == out_stride))
+    return DN_ERR_ARGS;
+  const int64_t q_bytes = rows_bytes(n, q_stride, row, size), out_bytes = rows_bytes(n, out_stride, row, size);
+  if (meets_q8_cache(cache, out, out_bytes) || meets_q8_cache(cache, workspace, workspace_bytes) ||
+      runs_meet(workspace, workspace_bytes, q, q_bytes) || runs_meet(workspace, workspace_bytes, out, out_bytes))
+    return DN_ERR_ARGS;
+  dn::PagedQ8AttentionArgs a{};
+  memcpy(&a.cache, cache, sizeof a.cache);
+  if (workspace_bytes < dn::paged_q8_attention_workspace(a.cache, heads, n, max_length)) return DN_ERR_ARGS;
+  if (device_state() == nullptr) return DN_ERR_NO_DEVICE;
+  a.type = type;
+  a.q = q;
+  a.q_stride = q_stride;
+  a.q_start = q_start;
+  a.lengths = lengths;
+  a.max_length = max_length;
+  a.scale = (float)scale;
+  a.window = window;
+  a.out = out;
+  a.out_stride = out_stride;
+  a.heads = heads;
+  a.n = n;
+  a.workspace = workspace;
+  return dn::launch_paged_q8_attention(a, static_cast<cudaStream_t>(stream), (flags & DN_FLAG_PDL) != 0) ==
+                 cudaSuccess
+             ? DN_OK
+             : launch_failed();
+}
+
+int64_t dn_residual_norm(int64_t type, const void* y, int64_t y_stride, const float* post, const void* gate,
+                         int64_t gate_stride, double scale, int64_t x_type, const void* x, int64_t x_stride,
+                         void* x_out, int64_t x_out_stride, const float* pre, double eps, void* h,
+                         int64_t h_stride, uint8_t* qa, int64_t qa_stride, int64_t rows, int64_t cols,
+                         int64_t flags, void* stream) {
+  if (!elem_type(type) || !elem_type(x_type) || rows < 0 || cols < 0) return DN_ERR_ARGS;
+  if (rows > INT32_MAX || cols > dn::kMaxResidualCols || y_stride > kMaxStride || gate_stride > kMaxStride ||
+      x_stride > kMaxStride || x_out_stride > kMaxStride || h_stride > kMaxStride || qa_stride > kMaxStride)
+    return DN_ERR_TOO_LARGE;
+  if (y_stride < cols || x_stride < cols || x_out_stride < cols || (h != nullptr && h_stride < cols) ||
+      (gate != nullptr && gate_stride != 0 && gate_stride < cols))
+    return DN_ERR_ARGS;
+  const int64_t qa_cols = cols / 32 * dn::kQABytes;
+  if (pre == nullptr && (h != nullptr || qa != nullptr)) return DN_ERR_ARGS;
+  if (qa != nullptr && (cols % 32 != 0 || qa_stride < qa_cols || ((uintptr_t)qa & 3) != 0 || (qa_stride & 3) != 0))
+    return DN_ERR_ARGS;
+  if (rows == 0 || cols == 0) return DN_OK;
+  if (y == nullptr || x == nullptr || x_out == nullptr) return DN_ERR_ARGS;
+  const int64_t size = dn::elem_size(type), x_size = dn::elem_size(x_type);
+  if ((((uintptr_t)y | (uintptr_t)gate | (uintptr_t)h) & (uintptr_t)(size - 1)) != 0 ||
+      (((uintptr_t)x | (uintptr_t)x_out) & (uintptr_t)(x_size - 1)) != 0 ||
+      (((uintptr_t)post | (uintptr_t)pre) & 3) != 0)
+    return DN_ERR_ARGS;
+  // Every output apart from every input and from the other outputs, but for x_out on x and h on y.
+  struct Rows {
+    const void* p;
+    int64_t stride, cols, type;  // of bytes where type is -1
+  };
+  auto meet = [&](const Rows& a, const Rows& b) {
+    if (a.p == nullptr || b.p == nullptr) return false;
+    if (a.stride == 0 || b.stride == 0 || a.type < 0 || b.type < 0) {
+      const int64_t as = a.type < 0 ? 1 : dn::elem_size(a.type), bs = b.type < 0 ? 1 : dn::elem_size(b.type);
+      return runs_meet(a.p, rows_bytes(rows, a.stride, a.cols, as), b.p, rows_bytes(rows, b.stride, b.cols, bs));
+    }
+    return overlaps(a.p, a.stride, a.cols, a.type, b.p, b.stride, b.cols, b.type, rows);
+  };
+  const Rows ry{y, y_stride, cols, type}, rg{gate, gate_stride, cols, type}, rx{x, x_stride, cols, x_type};
+  const Rows rpost{post, 0, cols, DN_F32}, rpre{pre, 0, cols, DN_F32};
+  const Rows rxo{x_out, x_out_stride, cols, x_type}, rh{h, h_stride, cols, type}, rqa{qa, qa_stride, qa_cols, -1};
+  for (const Rows* o : {&rxo, &rh, &rqa})
+    for (const Rows* i : {&ry, &rg, &rx, &rpost, &rpre, &rxo, &rh, &rqa}) {
+      if (i == o || (o == &rxo && i == &rx && x_out == x && x_out_stride == x_stride) ||
+          (o == &rh && i == &ry && h == y && h_stride == y_stride))
+        continue;
+      if (meet(*o, *i)) return DN_ERR_ARGS;
+    }
+  if (device_state() == nullptr) return DN_ERR_NO_DEVICE;
+  const dn::ResidualNormArgs a{type,     x_type,      y,        post,         gate,     x,
+                               x_out,    pre,         h,        qa,           y_stride, gate_stride,
+                               x_stride, x_out_stride, h_stride, qa_stride,   rows,     cols,
+                               (float)scale, (float)eps};
+  return dn::launch_residual_norm(a, static_cast<cudaStream_t>(stream), (flags & DN_FLAG_PDL) != 0) == cudaSuccess
+             ? DN_OK
+             : launch_failed();
+}
+
+int64_t dn_sample(int64_t type, const void* logits, int64_t stride, int64_t n, int64_t vocab,
+                  const dn_sampling* how, int32_t* tokens, float* logprobs, int32_t* kept, int64_t flags,
+                  void* stream) {
+  if (!elem_type(type) || n < 0 || vocab < 0 || stride < vocab || how == nullptr) return DN_ERR_ARGS;
+  if (vocab > dn::kMaxSampleVocab || n > (1 << 24) || stride > kMaxStride) return DN_ERR_TOO_LARGE;
+  if ((((uintptr_t)how->temperature | (uintptr_t)how->top_k | (uintptr_t)how->top_p | (uintptr_t)how->min_p |
+        (uintptr_t)how->uniform | (uintptr_t)tokens | (uintptr_t)logprobs | (uintptr_t)kept) & 3) != 0)
+    return DN_ERR_ARGS;
+  if (n == 0) return DN_OK;
+  if (how->uniform == nullptr || tokens == nullptr || (vocab > 0 && logits == nullptr) ||
+      ((uintptr_t)logits & (uintptr_t)(dn::elem_size(type) - 1)) != 0)
+    return DN_ERR_ARGS;
+  const int64_t in_bytes = rows_bytes(n, stride, vocab, dn::elem_size(type));
+  const void* outs[] = {tokens, logprobs, kept};
+  const void* ins[] = {how->temperature, how->top_k, how->top_p, how->min_p, how->uniform};
+  for (int i = 0; i < 3; i++) {
+    if (runs_meet(outs[i], n * 4, logits, in_bytes)) return DN_ERR_ARGS;
+    for (int j = i + 1; j < 3; j++)
+      if (runs_meet(outs[i], n * 4, outs[j], n * 4)) return DN_ERR_ARGS;
+    for (const void* in : ins)
+      if (runs_meet(outs[i], n * 4, in, n * 4)) return DN_ERR_ARGS;
+  }
+  if (device_state() == nullptr) return DN_ERR_NO_DEVICE;
+  dn::SampleArgs a{type, logits, stride, n, vocab, {}, tokens, logprobs, kept};
+  memcpy(&a.how, how, sizeof a.how);
+  return dn::launch_sample(a, static_cast<cudaStream_t>(stream), (flags & DN_FLAG_PDL) != 0) == cudaSuccess
              ? DN_OK
              : launch_failed();
 }

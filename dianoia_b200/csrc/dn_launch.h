@@ -271,6 +271,101 @@ struct LogitsArgs {
 };
 cudaError_t launch_logits(const LogitsArgs& a, cudaStream_t stream, bool pdl);
 
+// A paged cache in 8 bits (dn_paged_q8_cache, whose layout this is).
+struct PagedQ8Cache {
+  int8_t* keys;
+  int8_t* values;
+  float* key_scales;
+  float* value_scales;
+  const int32_t* table;
+  int64_t pages, page_size, kv_heads, hd, sequences, table_stride, page_stride, scale_stride;
+};
+
+// A step's keys and values quantized into the cache, its queries rotated
+// (paged_q8_cache.cu). The fields of PagedAppendArgs.
+struct PagedQ8AppendArgs {
+  PagedQ8Cache cache;
+  int64_t type, out_type;
+  const void* q;
+  const void* k;
+  const void* v;
+  int64_t q_stride, k_stride, v_stride;
+  const int32_t* seq;
+  const int32_t* pos;
+  const float* rope;
+  int64_t rope_rows, rot;
+  const float* q_norm;
+  const float* k_norm;
+  float eps;
+  void* q_out;
+  int64_t q_out_stride, heads, n;
+};
+cudaError_t launch_paged_q8_append(const PagedQ8AppendArgs& a, cudaStream_t stream, bool pdl);
+
+// Rows read back from it (paged_q8_cache.cu).
+struct PagedQ8ReadArgs {
+  PagedQ8Cache cache;
+  int64_t type;
+  const int32_t* seq;
+  const int32_t* pos;
+  void* k_out;
+  void* v_out;
+  int64_t k_stride, v_stride, n;
+};
+cudaError_t launch_paged_q8_read(const PagedQ8ReadArgs& a, cudaStream_t stream, bool pdl);
+
+// Attention over it (paged_q8_attention.cu).
+struct PagedQ8AttentionArgs {
+  PagedQ8Cache cache;
+  int64_t type;
+  const void* q;
+  const int32_t* q_start;  // [sequences + 1], or null: one token for each sequence
+  const int32_t* lengths;
+  void* out;
+  int64_t q_stride, out_stride, max_length, window, heads, n;
+  float scale;
+  void* workspace;
+};
+int64_t paged_q8_attention_workspace(const PagedQ8Cache& c, int64_t heads, int64_t n, int64_t max_length);
+cudaError_t launch_paged_q8_attention(const PagedQ8AttentionArgs& a, cudaStream_t stream, bool pdl);
+
+// What stands between two blocks of a layer (residual_norm.cu).
+constexpr int64_t kMaxResidualCols = 32768;
+struct ResidualNormArgs {
+  int64_t type, x_type;
+  const void* y;
+  const float* post;
+  const void* gate;
+  const void* x;
+  void* x_out;
+  const float* pre;
+  void* h;
+  uint8_t* qa;
+  int64_t y_stride, gate_stride, x_stride, x_out_stride, h_stride, qa_stride, rows, cols;
+  float scale, eps;
+};
+cudaError_t launch_residual_norm(const ResidualNormArgs& a, cudaStream_t stream, bool pdl);
+
+// How tokens are chosen (dn_sampling, whose layout this is; sample.cu).
+struct Sampling {
+  const float* temperature;
+  const int32_t* top_k;
+  const float* top_p;
+  const float* min_p;
+  const float* uniform;
+};
+constexpr int64_t kMaxSampleVocab = 1 << 19;
+struct SampleArgs {
+  int64_t type;
+  const void* logits;
+  int64_t stride, n, vocab;
+  Sampling how;
+  int32_t* tokens;
+  float* logprobs;
+  int32_t* kept;
+};
+cudaError_t launch_sample(const SampleArgs& a, cudaStream_t stream, bool pdl);
+
 // The decode GEMV on either activation form (gemv.cu).
 int64_t launch_gemv_ex(const GemvArgs& g, cudaStream_t stream, bool pdl);
 bool gemv_ex_supported(const GemvArgs& g);

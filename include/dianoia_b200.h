@@ -526,6 +526,119 @@ typedef struct dn_logit_rules {
 int64_t dn_logits_apply(int64_t type, const void* logits, int64_t stride, void* out, int64_t out_stride,
                         int64_t n, int64_t vocab, const dn_logit_rules* rules, int64_t flags, void* stream);
 
+/* A paged cache in 8 bits: a position's row of hd values of a kv head is kept
+ * as int8 with one f32 scale, value = int8 * scale: half a 16-bit cache's
+ * bytes, and the scale stays out of the sums that attention takes over a row.
+ * Pages, table and positions are as in dn_paged_cache; page i's rows start at
+ * byte i * page_stride of `keys` and of `values` ([kv_heads, page_size, hd]),
+ * its scales at element i * scale_stride of key_scales and value_scales
+ * ([kv_heads, page_size]). hd is a multiple of 16, at most 256; keys and
+ * values are 16-byte aligned and page_stride a multiple of 16. */
+typedef struct dn_paged_q8_cache {
+  int8_t* keys;
+  int8_t* values;
+  float* key_scales;
+  float* value_scales;
+  const int32_t* table;
+  int64_t pages, page_size, kv_heads, hd, sequences, table_stride, page_stride, scale_stride;
+} dn_paged_q8_cache;
+
+/* dn_paged_append into an 8-bit cache: the same norms, rotation, skipped
+ * tokens and argument rules, in f32; a row is then kept with scale = amax /
+ * 127 (amax its largest magnitude) as its values times 1 / scale, rounded half
+ * away from zero, as lab_quantize_q8 rounds a block. A row whose scale would
+ * be less than the smallest normal f32 (2^-126) is kept as zeros; one that
+ * holds an infinity or a NaN is kept with a NaN scale and reads back as NaN.
+ * Rotated queries go to q_out as elements of `out_type`, rounded once. q_out
+ * may be q (the same address, type and stride). The cache's own memory must
+ * not overlap q, k, v or q_out. Two tokens of one call in the same slot leave
+ * a mixture of the two there (and nothing wrong elsewhere). */
+int64_t dn_paged_q8_append(const dn_paged_q8_cache* cache, int64_t type, const void* q, int64_t q_stride,
+                           const void* k, int64_t k_stride, const void* v, int64_t v_stride,
+                           const int32_t* seq, const int32_t* pos, const float* rope, int64_t rope_rows,
+                           int64_t rot, const float* q_norm, const float* k_norm, double eps,
+                           int64_t out_type, void* q_out, int64_t q_out_stride, int64_t heads, int64_t n,
+                           int64_t flags, void* stream);
+
+/* Reads positions of an 8-bit cache back: row t of k_out and of v_out
+ * (kv_heads * hd elements of `type` at t * k_stride and t * v_stride) receives
+ * position pos[t] of sequence seq[t], int8 times scale in f32, rounded to
+ * `type`; zeros where the cache holds no such position (as dn_paged_append
+ * skips). Either of k_out and v_out may be NULL. With the rows of a whole
+ * sequence a prompt's attention, or dn_paged_append into another cache, reads
+ * what the 8-bit one holds. k_out and v_out must not overlap each other or
+ * the cache. */
+int64_t dn_paged_q8_read(const dn_paged_q8_cache* cache, int64_t type, const int32_t* seq, const int32_t* pos,
+                         void* k_out, int64_t k_stride, void* v_out, int64_t v_stride, int64_t n,
+                         int64_t flags, void* stream);
+
+/* Causal grouped-query attention of a batch over an 8-bit cache: queries,
+ * positions, window, outputs and the rows that see nothing as for
+ * dn_paged_attention, every position read through its sequence's table row
+ * (there is no shared prefix; sequences may name the same pages). q and out
+ * are elements of `type`. It is made for decode steps, one to a few tokens a
+ * sequence: a sequence's keys are split over the GPU by length and joined, and
+ * read once for up to 32 rows (tokens times heads of a kv head; fewer for
+ * heads over 128). Any number of tokens is computed right. Scores, softmax and
+ * sums are in f32; the int8 values enter the tensor cores as they are, the
+ * queries and each weight (probability times its value's scale) as one (bf16),
+ * two (f16) or three (f32) bf16 parts, 8 bits each. max_length and
+ * `workspace` as for dn_paged_attention. */
+int64_t dn_paged_q8_attention_workspace(const dn_paged_q8_cache* cache, int64_t heads, int64_t n,
+                                        int64_t max_length);
+int64_t dn_paged_q8_attention(const dn_paged_q8_cache* cache, int64_t type, const void* q, int64_t q_stride,
+                              const int32_t* q_start, const int32_t* lengths, int64_t max_length,
+                              double scale, int64_t window, void* out, int64_t out_stride, int64_t heads,
+                              int64_t n, void* workspace, int64_t workspace_bytes, int64_t flags,
+                              void* stream);
+
+/* What stands between two blocks of a layer, in one pass over `rows` rows of
+ * `cols` values (at most 32768):
+ *   b = y, or with post (cols f32 weights) post * y / sqrt(mean(y^2) + eps),
+ *   x' = x + scale * g * b, with g the row's gate (1 where gate is NULL),
+ *   h = pre * x' / sqrt(mean(x'^2) + eps).
+ * y (a block's output), gate and h are elements of `type`, the residual stream
+ * x and x_out of `x_type`; row r starts at element r * stride of each
+ * (gate_stride 0: one row of gates for all). pre NULL leaves h out; h may be
+ * NULL. With qa not NULL (cols % 32 == 0; pre not NULL) h also goes out as QA
+ * blocks, row r at qa + r * qa_stride, for dn_linear_qa. Arithmetic is in f32,
+ * from the sums on to each result, which is rounded once (h follows the f32
+ * x', not its rounding to x_type; QA blocks the f32 h). x_out may be x and h
+ * may be y (the same address, type and stride); no output may overlap
+ * anything else. */
+int64_t dn_residual_norm(int64_t type, const void* y, int64_t y_stride, const float* post, const void* gate,
+                         int64_t gate_stride, double scale, int64_t x_type, const void* x, int64_t x_stride,
+                         void* x_out, int64_t x_out_stride, const float* pre, double eps, void* h,
+                         int64_t h_stride, uint8_t* qa, int64_t qa_stride, int64_t rows, int64_t cols,
+                         int64_t flags, void* stream);
+
+/* How a batch's tokens are chosen; each array [n] or NULL. */
+typedef struct dn_sampling {
+  const float* temperature; /* NULL: 1; a row whose temperature is not > 0 takes its largest logit */
+  const int32_t* top_k;     /* at most so many tokens; NULL, or not > 0: any number */
+  const float* top_p;       /* the likeliest with this share of what top_k leaves; NULL, or not < 1: all */
+  const float* min_p;       /* at least this share of the likeliest token's probability; NULL: 0 */
+  const float* uniform;     /* the random number, in [0, 1) (values outside count as its ends); not NULL */
+} dn_sampling;
+
+/* Chooses a token for each of n rows of `vocab` logits of `type` (at most
+ * 524288, row r at r * stride), such as dn_logits_apply leaves them. With
+ * w = exp((x - max) / temperature) and the row's tokens ordered by logit,
+ * equal ones by index, these are kept: the first top_k; of those the first few
+ * whose w sum to at least top_p of their sum; of those the ones with w >=
+ * min_p (the first token always). tokens[r] is then, in index order, the first
+ * kept token up to which the kept w sum to more than uniform[r] times their
+ * sum; logprobs[r] (NULL: not wanted) the logarithm of its share of that sum,
+ * kept[r] (NULL: not wanted) how many were kept. Logits of minus infinity and
+ * NaN are no tokens; a row of nothing else gives token -1, logprob minus
+ * infinity and 0 kept. Where the largest is plus infinity only its equals have
+ * weight. Weights are computed in f64 and summed in whole steps of 2^-44 of
+ * the largest, so that no order of summation changes a choice: equal inputs
+ * give equal tokens, alone or in any batch. */
+int64_t dn_sample(int64_t type, const void* logits, int64_t stride, int64_t n, int64_t vocab,
+                  const dn_sampling* how, int32_t* tokens, float* logprobs, int32_t* kept, int64_t flags,
+                  void* stream);
+
 /* A decode chain: the quantized products of one token (or any sequence of
  * GEMVs on QA activations) run by ONE persistent kernel, so HBM keeps
  * streaming weights across the dependencies between them. Op i reads QA
