@@ -484,7 +484,8 @@ bool meets_q8_cache(const dn_paged_q8_cache* c, const void* p, int64_t bytes) {
 
 int64_t check_q8_attention(const dn_paged_q8_cache* c, int64_t heads, int64_t n, int64_t max_length) {
   if (heads < 1 || heads % c->kv_heads != 0 || n < 0 || max_length < 0) return DN_ERR_ARGS;
-  if (heads > (1 << 20) || n > (int64_t)1 << 24 || n * heads > (int64_t)1 << 30 || max_length > (int64_t)1 << 30)
+  if (heads > (1 << 20) || n > (int64_t)1 << 24 || n * heads > (int64_t)1 << 30 || max_length > (int64_t)1 << 30 ||
+      c->sequences * c->kv_heads > (int64_t)1 << 26)
     return DN_ERR_TOO_LARGE;
   return DN_OK;
 }

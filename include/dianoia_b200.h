@@ -581,8 +581,9 @@ int64_t dn_paged_q8_read(const dn_paged_q8_cache* cache, int64_t type, const int
  * read once for up to 32 rows (tokens times heads of a kv head; fewer for
  * heads over 128). Any number of tokens is computed right. Scores, softmax and
  * sums are in f32; the int8 values enter the tensor cores as they are, the
- * queries and each weight (probability times its value's scale) as one (bf16),
- * two (f16) or three (f32) bf16 parts, 8 bits each. max_length and
+ * queries and each weight (probability times its value's scale) as bf16 parts
+ * of 8 bits each: one and two of them (bf16), two (f16) or three (f32).
+ * max_length and
  * `workspace` as for dn_paged_attention. */
 int64_t dn_paged_q8_attention_workspace(const dn_paged_q8_cache* cache, int64_t heads, int64_t n,
                                         int64_t max_length);

@@ -53,8 +53,8 @@ def attention(pool, kind, q, q_start, lengths, scale, window, heads):
     """out [n, heads, hd] in f64 and the bound on each value's error.
 
     With p the softmax and A = sum p s |v|: rounding the result (u |out|); each
-    weight p s in one, two or three bf16 parts, 2^-8 of what the parts before
-    leave (A times 2^-8, 2^-16 or 2^-24); each score's f32 sum and scaling, at
+    weight p s in two or three bf16 parts, 2^-8 of what the parts before leave
+    (A times 2^-16 or 2^-24); each score's f32 sum and scaling, at
     most (hd + 8) 2^-24 of scale sum |q| s |k|, which moves a probability by
     that much relatively, twice over through the normalization; and the f32
     sums over the keys with the exponential's, the products' and the joins'
@@ -62,7 +62,7 @@ def attention(pool, kind, q, q_start, lengths, scale, window, heads):
     """
     n, hd, group = q.shape[0], pool.hd, heads // pool.kv_heads
     u = TYPES[kind][2]
-    parts = {"bf16": 2.0 ** -8, "f16": 2.0 ** -16, "f32": 2.0 ** -24}[kind]
+    parts = {"bf16": 2.0 ** -16, "f16": 2.0 ** -16, "f32": 2.0 ** -24}[kind]
     out = torch.zeros((n, heads, hd), dtype=torch.float64, device="cuda")
     tol = torch.zeros_like(out)
     for s in range(len(lengths)):
