@@ -151,6 +151,12 @@ __device__ __forceinline__ uint32_t widened(uint32_t x) {
   return y;
 }
 
+__device__ __forceinline__ float power2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 __device__ __forceinline__ float2 unpacked(uint32_t x) {
   return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));
 }
@@ -167,15 +173,14 @@ __device__ __forceinline__ void load_words(const uint8_t* p, uint32_t (&w)[WORDS
   }
 }
 
-// Where 16-byte part `part` of row `row` lies in a chunk of keys or of values:
-// in lines of 128 bytes, turned so that the eight lanes that read at once
-// (keys: two rows' four parts; values: four even or odd rows' two parts) meet
-// eight different places of the line.
-template <int HD, bool VALUES>
+// Where 16-byte part `part` of row `row` lies in a chunk: in lines of 128 bytes,
+// turned so that the eight lanes that read at once (keys: two rows' four parts;
+// values: four even or odd rows' two parts) meet eight different places of the
+// line.
+template <int HD>
 __device__ __forceinline__ int place(int row, int part) {
-  const int at = row * (HD / 16) + part;
-  const int turn = VALUES ? row & 6 : HD == 64 ? 0 : (row & 1) << 2;
-  return (at ^ turn) * 16;
+  const int turn = HD == 64 ? row & 6 : (row & 6) ^ (row & 1) << 2;
+  return ((row * (HD / 16) + part) ^ turn) * 16;
 }
 
 template <int HD>
@@ -229,32 +234,58 @@ __global__ void __launch_bounds__(kThreads, BLOCKS)
     __syncwarp();
   }
   const int32_t* table = c.table + (int64_t)w.seq * c.table_stride;
-  const int row = lane % kKeys;
+  // Pages of whole chunks: a chunk's rows are one run of bytes, and every lane
+  // follows its first. Else a lane follows a row.
+  const bool whole_pages = page_size % kKeys == 0;
+  const int row = whole_pages ? 0 : lane % kKeys;
   int pos = begin + warp * kKeys + row;  // of the next chunk to issue
   int entry = pos / page_size, slot = pos - entry * page_size;
   const int entry_step = kWarps * kKeys / page_size, slot_step = kWarps * kKeys - entry_step * page_size;
-  auto page_at = [&]() { return pos < end ? (int64_t)table[entry] : (int64_t)-1; };
-  int64_t page = page_at();
+  auto page_at = [&]() { return pos < end ? table[entry] : -1; };
+  int page = page_at();
   constexpr int COPIES = HD / 32;  // 16-byte parts a lane brings, of the keys and of the values
   const int parts = hd / 16;
+  const uint32_t per_part = 65536u / (uint32_t)parts + 1;  // x per_part / 65536 is x / parts, for x below 512
+  int to[COPIES];  // where they go
+#pragma unroll
+  for (int i = 0; i < COPIES; i++) {
+    const int which = lane + 32 * i, r = (int)(which * per_part >> 16);
+    to[i] = place<HD>(r % kKeys, which - r * parts);
+  }
+  const int copies = (kKeys * parts - lane + 31) / 32;  // of this lane
   auto issue = [&](int stage) {
     const bool there = page >= 0 && page < c.pages;
+    const int64_t row_at = there ? page * c.scale_stride + (int64_t)kv * page_size + slot : 0;
     const int64_t at = there ? page * c.page_stride + ((int64_t)kv * page_size + slot) * hd : -1;
-    const int64_t scale_at = there ? page * c.scale_stride + (int64_t)kv * page_size + slot : 0;
-    const uint32_t mask = __ballot_sync(0xffffffffu, there) & 0xffffu;
     uint8_t* keys = ring + stage * 2 * S::kChunk;
     uint8_t* values = keys + S::kChunk;
+    uint32_t mask;
+    if (whole_pages) {
+      const int8_t* from_keys = c.keys + (there ? at : 0) + lane * 16;
+      const int8_t* from_values = c.values + (there ? at : 0) + lane * 16;
 #pragma unroll
-    for (int i = 0; i < COPIES; i++) {
-      const int which = lane + 32 * i, r = which / parts, part = which - r * parts;
-      const int64_t from = __shfl_sync(0xffffffffu, at, r % kKeys);
-      if (r < kKeys) {
-        const int64_t src = from >= 0 ? from + part * 16 : 0;
-        cp16(keys + place<HD, false>(r, part), c.keys + src, from >= 0);
-        cp16(values + place<HD, true>(r, part), c.values + src, from >= 0);
+      for (int i = 0; i < COPIES; i++)
+        if (i < copies) {
+          cp16(keys + to[i], from_keys + i * 512, there);
+          cp16(values + to[i], from_values + i * 512, there);
+        }
+      const int left = end - pos;
+      mask = there ? left >= kKeys ? 0xffffu : (1u << left) - 1 : 0;
+      cp4(scales + stage * 2 * kKeys + lane, (lane < kKeys ? c.key_scales : c.value_scales - kKeys) + (row_at + lane), there);
+    } else {
+      mask = __ballot_sync(0xffffffffu, there) & 0xffffu;
+#pragma unroll
+      for (int i = 0; i < COPIES; i++) {
+        const int which = lane + 32 * i, r = (int)(which * per_part >> 16), part = which - r * parts;
+        const int64_t from = __shfl_sync(0xffffffffu, at, r % kKeys);
+        if (r < kKeys) {
+          const int64_t src = from >= 0 ? from + part * 16 : 0;
+          cp16(keys + to[i], c.keys + src, from >= 0);
+          cp16(values + to[i], c.values + src, from >= 0);
+        }
       }
+      cp4(scales + stage * 2 * kKeys + lane, (lane < kKeys ? c.key_scales : c.value_scales) + row_at, there);
     }
-    cp4(scales + stage * 2 * kKeys + lane, (lane < kKeys ? c.key_scales : c.value_scales) + scale_at, there);
     if (lane == 0) masks[stage] = mask;
     pos += kWarps * kKeys;
     entry += entry_step;
@@ -273,7 +304,8 @@ __global__ void __launch_bounds__(kThreads, BLOCKS)
   }
 
   // ---- the queries, as the products take them: of step i lane (g, t) holds
-  // row g's dims 64 (i / 4) + 16 t + 4 (i % 4) .. + 3
+  // row g's dims 64 (i / 4) + 16 t + 4 (i % 4) .. + 3, the even ones first as
+  // the keys' words give them
   uint2* queries = reinterpret_cast<uint2*>(smem + S::kQueries);
   for (int at = tid; at < NT * STEPS * 32; at += kThreads) {
     const int l = at % 32, i = at / 32 % STEPS, nt = at / 32 / STEPS, r = nt * 8 + l / 4;
@@ -287,10 +319,10 @@ __global__ void __launch_bounds__(kThreads, BLOCKS)
     }
 #pragma unroll
     for (int p = 0; p < PARTS; p++) {
-      const uint2 b = make_uint2(Pair<__nv_bfloat16>::pack(x[0], x[1]), Pair<__nv_bfloat16>::pack(x[2], x[3]));
+      const uint2 b = make_uint2(Pair<__nv_bfloat16>::pack(x[0], x[2]), Pair<__nv_bfloat16>::pack(x[1], x[3]));
       queries[(p * NT + nt) * STEPS * 32 + i * 32 + l] = b;
       const float2 lo = unpacked(b.x), hi = unpacked(b.y);
-      x[0] -= lo.x, x[1] -= lo.y, x[2] -= hi.x, x[3] -= hi.y;
+      x[0] -= lo.x, x[2] -= lo.y, x[1] -= hi.x, x[3] -= hi.y;
     }
   }
   __syncthreads();
@@ -320,6 +352,11 @@ __global__ void __launch_bounds__(kThreads, BLOCKS)
     for (int i = 0; i < STEPS; i++) acc[nt][i][0] = acc[nt][i][1] = acc[nt][i][2] = acc[nt][i][3] = 0.0f;
   }
 
+  // Where this lane's words lie: its two keys' parts (the second 8 rows on), its values' (keys 2 t and 2 t + 1; 8 rows on).
+  const int key_at[2] = {place<HD>(g, t), place<HD>(g, (t + 4) % (HD / 16))};
+  const int value_at[2] = {HD == 64 ? place<HD>(2 * t, g / 2) + g % 2 * 8 : place<HD>(2 * t, g),
+                           HD == 64 ? place<HD>(2 * t + 1, g / 2) + g % 2 * 8 : place<HD>(2 * t + 1, g)};
+
   int stage = 0;
   for (int chunk = 0; chunk < chunks; chunk++) {
     asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
@@ -338,12 +375,11 @@ __global__ void __launch_bounds__(kThreads, BLOCKS)
 #pragma unroll
     for (int block = 0; block < HD / 64; block++) {
       uint32_t k0[4], k1[4];
-      load_words<4>(keys + place<HD, false>(g, block * 4 + t), k0);
-      load_words<4>(keys + place<HD, false>(g + 8, block * 4 + t), k1);
+      load_words<4>(keys + key_at[block % 2] + block / 2 * 128, k0);
+      load_words<4>(keys + key_at[block % 2] + block / 2 * 128 + 8 * HD, k1);
 #pragma unroll
       for (int j = 0; j < 4; j++) {
-        const uint32_t f[4] = {widened(__byte_perm(k0[j], 0, 0x1100)), widened(__byte_perm(k1[j], 0, 0x1100)),
-                               widened(__byte_perm(k0[j], 0, 0x3322)), widened(__byte_perm(k1[j], 0, 0x3322))};
+        const uint32_t f[4] = {widened(k0[j]), widened(k1[j]), widened(k0[j] >> 8), widened(k1[j] >> 8)};
         const int i = block * 4 + j;
 #pragma unroll
         for (int p = 0; p < PARTS; p++)
@@ -386,7 +422,7 @@ __global__ void __launch_bounds__(kThreads, BLOCKS)
           for (int off = 4; off <= 16; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
           if (!(top > m[nt][e])) continue;  // the same in the row's lanes
           top += kSlack;
-          const float fade = exp2f(m[nt][e] - top);
+          const float fade = power2(m[nt][e] - top);
           m[nt][e] = top;
           sum[nt][e] *= fade;
 #pragma unroll
@@ -401,7 +437,7 @@ __global__ void __launch_bounds__(kThreads, BLOCKS)
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
       const float m0 = m[nt][0] == -INFINITY ? 0.0f : m[nt][0], m1 = m[nt][1] == -INFINITY ? 0.0f : m[nt][1];
-      const float p0 = exp2f(s[nt][0] - m0), p1 = exp2f(s[nt][1] - m1), p2 = exp2f(s[nt][2] - m0), p3 = exp2f(s[nt][3] - m1);
+      const float p0 = power2(s[nt][0] - m0), p1 = power2(s[nt][1] - m1), p2 = power2(s[nt][2] - m0), p3 = power2(s[nt][3] - m1);
       sum[nt][0] += p0 + p2;
       sum[nt][1] += p1 + p3;
       float x0 = p0 * vs0, x1 = p1 * vs0, x2 = p2 * vs1, x3 = p3 * vs1;
@@ -427,11 +463,7 @@ __global__ void __launch_bounds__(kThreads, BLOCKS)
       uint32_t v[4][WORDS];
 #pragma unroll
       for (int j = 0; j < 4; j++) {
-        const int key = 2 * t + (j & 1) + (j >> 1) * 8;
-        if constexpr (HD == 64)
-          load_words<2>(values + place<HD, true>(key, g / 2) + g % 2 * 8, v[j]);
-        else
-          load_words<4>(values + place<HD, true>(key, half * 8 + g), v[j]);
+        load_words<WORDS>(values + value_at[j % 2] + j / 2 * 8 * HD + half * 128, v[j]);
       }
 #pragma unroll
       for (int word = 0; word < WORDS; word++)
@@ -493,7 +525,7 @@ __global__ void __launch_bounds__(kThreads, BLOCKS)
     float o[4] = {};
 #pragma unroll
     for (int i = 0; i < kWarps; i++) {
-      const float fade = exp2f(stats[(i * R + r) * 2] - base);
+      const float fade = power2(stats[(i * R + r) * 2] - base);
       total += stats[(i * R + r) * 2 + 1] * fade;
       const float4 v = *reinterpret_cast<const float4*>(sums + (i * R + r) * HD + dim);
       o[0] += v.x * fade, o[1] += v.y * fade, o[2] += v.z * fade, o[3] += v.w * fade;
@@ -537,7 +569,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32)
 #pragma unroll 8
   for (int i = warp; i < w.slices; i += kJoinWarps) {
     const float2 st = stats[i * step / 2];
-    const float fade = exp2f(st.x - base);
+    const float fade = power2(st.x - base);
     total += st.y * fade;
 #pragma unroll
     for (int j = 0; j < N; j++) {
