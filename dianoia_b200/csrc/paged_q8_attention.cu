@@ -139,9 +139,14 @@ __device__ __forceinline__ uint32_t transposed(uint32_t x) {
   return y;
 }
 
-// Bytes 0 and 2 of x, as int8, to bf16; bytes 1 and 3 do not count.
-__device__ __forceinline__ uint32_t widened(uint32_t x) {
-  const uint32_t low = (x & 0x007f007fu) | 0x43004300u, sign = (x & 0x00800080u) | 0x43004300u;
+// Bytes 0 and 2 of x, as int8, to bf16; bytes 1 and 3 do not count. `bits` is
+// kExponent in a register: with two literals the compiler takes two operations
+// for each of these.
+constexpr uint32_t kExponent = 0x43004300u;
+__device__ __forceinline__ uint32_t widened(uint32_t x, uint32_t bits) {
+  uint32_t low, sign;
+  asm("lop3.b32 %0, %1, 0x007f007f, %2, 0xea;" : "=r"(low) : "r"(x), "r"(bits));   // x & mask | bits
+  asm("lop3.b32 %0, %1, 0x00800080, %2, 0xea;" : "=r"(sign) : "r"(x), "r"(bits));
   __nv_bfloat162 l, s;
   memcpy(&l, &low, 4);
   memcpy(&s, &sign, 4);
@@ -357,6 +362,8 @@ __global__ void __launch_bounds__(kThreads, BLOCKS)
   const int value_at[2] = {HD == 64 ? place<HD>(2 * t, g / 2) + g % 2 * 8 : place<HD>(2 * t, g),
                            HD == 64 ? place<HD>(2 * t + 1, g / 2) + g % 2 * 8 : place<HD>(2 * t + 1, g)};
 
+  uint32_t bits;
+  asm volatile("mov.b32 %0, %1;" : "=r"(bits) : "n"(kExponent));
   int stage = 0;
   for (int chunk = 0; chunk < chunks; chunk++) {
     asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
@@ -379,7 +386,8 @@ __global__ void __launch_bounds__(kThreads, BLOCKS)
       load_words<4>(keys + key_at[block % 2] + block / 2 * 128 + 8 * HD, k1);
 #pragma unroll
       for (int j = 0; j < 4; j++) {
-        const uint32_t f[4] = {widened(k0[j]), widened(k1[j]), widened(k0[j] >> 8), widened(k1[j] >> 8)};
+        const uint32_t f[4] = {widened(k0[j], bits), widened(k1[j], bits), widened(k0[j] >> 8, bits),
+                               widened(k1[j] >> 8, bits)};
         const int i = block * 4 + j;
 #pragma unroll
         for (int p = 0; p < PARTS; p++)
@@ -470,8 +478,9 @@ __global__ void __launch_bounds__(kThreads, BLOCKS)
 #pragma unroll
         for (int two = 0; two < 2; two++) {  // dims 2 two and 2 two + 1 of the word: rows g and g + 8
           const uint32_t s0 = two == 0 ? 0x4400u : 0x6622u, s1 = two == 0 ? 0x5511u : 0x7733u;
-          const uint32_t f[4] = {widened(__byte_perm(v[0][word], v[1][word], s0)), widened(__byte_perm(v[0][word], v[1][word], s1)),
-                                 widened(__byte_perm(v[2][word], v[3][word], s0)), widened(__byte_perm(v[2][word], v[3][word], s1))};
+          const uint32_t f[4] = {
+              widened(__byte_perm(v[0][word], v[1][word], s0), bits), widened(__byte_perm(v[0][word], v[1][word], s1), bits),
+              widened(__byte_perm(v[2][word], v[3][word], s0), bits), widened(__byte_perm(v[2][word], v[3][word], s1), bits)};
           const int i = half * 8 + word * 2 + two;
 #pragma unroll
           for (int nt = 0; nt < NT; nt++) {
