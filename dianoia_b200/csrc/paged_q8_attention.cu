@@ -36,7 +36,7 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
-constexpr int kKeys = 16;  // of a chunk
+constexpr int kRun = 16;  // keys of a product; pages of whole runs are copied as such
 constexpr float kSlack = 8.0f;
 constexpr int kJoinWarps = 8;
 
@@ -60,7 +60,7 @@ struct Parts<__nv_bfloat16> {
 struct Split {
   int rows;      // of a tile: 8, 16 or 32
   int slices;    // of a tile, at most
-  int slice;     // keys of each but the last, a multiple of kWarps * kKeys
+  int slice;     // keys of each but the last, a multiple of 64
   int most;      // slices that a call with a window may have at most
   int64_t tiles;
 };
@@ -68,7 +68,7 @@ struct Split {
 struct Work {
   int seq, first, count;  // the sequence, its first token, its tokens
   int row0, rows;         // the tile's first row of the sequence's, rows left from there
-  int begin, end;         // keys that some row may see, begin a multiple of kKeys
+  int begin, end;         // keys that some row may see, begin a multiple of kRun
   int slices;             // in use
   int length;
 };
@@ -113,7 +113,7 @@ __device__ __forceinline__ Work find_work(const PagedQ8AttentionArgs& a, const S
   const int64_t most = a.cache.table_stride * a.cache.page_size;
   w.end = (int)(last + 1 < 0 ? 0 : min64(last + 1, most));
   const int64_t low = a.window > 0 ? first - a.window + 1 : 0;
-  w.begin = low > 0 ? (int)(min64(low, most) / kKeys * kKeys) : 0;
+  w.begin = low > 0 ? (int)(min64(low, most) / kRun * kRun) : 0;
   if (w.end > w.begin) w.slices = min(d.slices, (w.end - w.begin + d.slice - 1) / d.slice);
   return w;
 }
@@ -183,19 +183,18 @@ __device__ __forceinline__ void load_words(const uint8_t* p, uint32_t (&w)[WORDS
 // values: four even or odd rows' two parts) meet eight different places of the
 // line.
 template <int HD>
-__device__ __forceinline__ int place(int row, int part) {
-  const int turn = HD == 64 ? row & 6 : (row & 6) ^ (row & 1) << 2;
-  return ((row * (HD / 16) + part) ^ turn) * 16;
+__host__ __device__ constexpr int turn_of(int row) {
+  return HD == 64 ? row & 6 : (row & 6) ^ (row & 1) << 2;
 }
-
 template <int HD>
-constexpr int ring_stages() {
-  return HD == 256 ? 3 : 4;
+__device__ __forceinline__ int place(int row, int part) {
+  return ((row * (HD / 16) + part) ^ turn_of<HD>(row)) * 16;
 }
 
 template <int HD, int NT, int PARTS>
 struct Smem {
-  static constexpr int kStages = ring_stages<HD>();
+  // A warp's ring: chunks of kKeys keys and values, kStages of them.
+  static constexpr int kKeys = HD == 256 ? 16 : 32, kStages = HD == 64 ? 4 : HD == 128 ? 2 : 3;
   static constexpr int kChunk = kKeys * HD;  // bytes of a chunk's keys, or values
   static constexpr int kRing = kWarps * kStages * 2 * kChunk;
   static constexpr int kJoin = kWarps * NT * 8 * HD * 4;  // the warps' sums, over the ring
@@ -214,7 +213,7 @@ __global__ void __launch_bounds__(kThreads, BLOCKS)
   // results would show: there each chunk's sums begin at 0 and are added here.
   constexpr bool kFine = std::is_same<T, float>::value;
   using S = Smem<HD, NT, PARTS>;
-  constexpr int STAGES = S::kStages, STEPS = HD / 16;
+  constexpr int STAGES = S::kStages, KEYS = S::kKeys, STEPS = HD / 16;
   extern __shared__ __align__(128) uint8_t smem[];
   pdl_launch_dependents();
   pdl_wait();
@@ -231,7 +230,7 @@ __global__ void __launch_bounds__(kThreads, BLOCKS)
 
   // ---- the ring: this lane's row of a chunk, its page a chunk ahead
   uint8_t* ring = smem + warp * STAGES * 2 * S::kChunk;
-  float* scales = reinterpret_cast<float*>(smem + S::kScales) + warp * STAGES * 2 * kKeys;
+  float* scales = reinterpret_cast<float*>(smem + S::kScales) + warp * STAGES * 2 * KEYS;
   uint32_t* masks = reinterpret_cast<uint32_t*>(smem + S::kMasks) + warp * STAGES;
   if (hd != HD) {  // parts that no copy writes
     for (int at = lane * 16; at < STAGES * 2 * S::kChunk; at += 32 * 16)
@@ -239,60 +238,69 @@ __global__ void __launch_bounds__(kThreads, BLOCKS)
     __syncwarp();
   }
   const int32_t* table = c.table + (int64_t)w.seq * c.table_stride;
-  // Pages of whole chunks: a chunk's rows are one run of bytes, and every lane
-  // follows its first. Else a lane follows a row.
-  const bool whole_pages = page_size % kKeys == 0;
-  const int row = whole_pages ? 0 : lane % kKeys;
-  int pos = begin + warp * kKeys + row;  // of the next chunk to issue
+  // Pages of whole runs of 16: LANES lanes copy a run, as one run of bytes. Else
+  // a row's parts are copied from where the lane that follows it says.
+  const bool runs = page_size % kRun == 0;
+  constexpr int LANES = KEYS == 32 ? 16 : 32, COPIES = KEYS * HD / 16 / 32;
+  const int row = lane % KEYS, in_run = row % kRun;
+  int pos = begin + warp * KEYS + row;  // of the next chunk to issue
   int entry = pos / page_size, slot = pos - entry * page_size;
-  const int entry_step = kWarps * kKeys / page_size, slot_step = kWarps * kKeys - entry_step * page_size;
-  auto page_at = [&]() { return pos < end ? table[entry] : -1; };
+  const int entry_step = kWarps * KEYS / page_size, slot_step = kWarps * KEYS - entry_step * page_size;
+  auto page_at = [&]() { return pos - (runs ? in_run : 0) < end ? table[entry] : -1; };
   int page = page_at();
-  constexpr int COPIES = HD / 32;  // 16-byte parts a lane brings, of the keys and of the values
   const int parts = hd / 16;
   const uint32_t per_part = 65536u / (uint32_t)parts + 1;  // x per_part / 65536 is x / parts, for x below 512
-  int to[COPIES];  // where they go
-#pragma unroll
-  for (int i = 0; i < COPIES; i++) {
-    const int which = lane + 32 * i, r = (int)(which * per_part >> 16);
-    to[i] = place<HD>(r % kKeys, which - r * parts);
-  }
-  const int copies = (kKeys * parts - lane + 31) / 32;  // of this lane
+  const int first_to = place<HD>(lane / 16 * (KEYS == 32 ? kRun : 1) + lane % 16 / (HD / 16), lane % LANES % (HD / 16));
   auto issue = [&](int stage) {
-    const bool there = page >= 0 && page < c.pages;
-    const int64_t row_at = there ? page * c.scale_stride + (int64_t)kv * page_size + slot : 0;
-    const int64_t at = there ? page * c.page_stride + ((int64_t)kv * page_size + slot) * hd : -1;
+    const bool held = page >= 0 && page < c.pages, there = held && pos < end;
+    const int64_t scale_at = there ? page * c.scale_stride + (int64_t)kv * page_size + slot : 0;
+    const uint32_t mask = __ballot_sync(0xffffffffu, there);
     uint8_t* keys = ring + stage * 2 * S::kChunk;
     uint8_t* values = keys + S::kChunk;
-    uint32_t mask;
-    if (whole_pages) {
-      const int8_t* from_keys = c.keys + (there ? at : 0) + lane * 16;
-      const int8_t* from_values = c.values + (there ? at : 0) + lane * 16;
+    if (runs) {
+      const int64_t at = held ? page * c.page_stride + ((int64_t)kv * page_size + (slot - in_run)) * hd : 0;
+      const int8_t* from_keys = c.keys + at + lane % LANES * 16;
+      const int8_t* from_values = c.values + at + lane % LANES * 16;
+      if (hd == HD) {
 #pragma unroll
-      for (int i = 0; i < COPIES; i++)
-        if (i < copies) {
-          cp16(keys + to[i], from_keys + i * 512, there);
-          cp16(values + to[i], from_values + i * 512, there);
+        for (int i = 0; i < COPIES; i++) {  // LANES * 16 / HD rows on each time
+          const int to = (first_to ^ turn_of<HD>(i * (LANES * 16 / HD)) * 16) + i * LANES * 16;
+          cp16(keys + to, from_keys + i * LANES * 16, held);
+          cp16(values + to, from_values + i * LANES * 16, held);
         }
-      const int left = end - pos;
-      mask = there ? left >= kKeys ? 0xffffu : (1u << left) - 1 : 0;
-      cp4(scales + stage * 2 * kKeys + lane, (lane < kKeys ? c.key_scales : c.value_scales - kKeys) + (row_at + lane), there);
+      } else {
+#pragma unroll
+        for (int i = 0; i < COPIES; i++) {
+          const int which = lane % LANES + i * LANES, r = (int)(which * per_part >> 16);
+          if (r < kRun) {
+            const int to = place<HD>(r + (KEYS == 32 ? lane / 16 * kRun : 0), which - r * parts);
+            cp16(keys + to, from_keys + i * LANES * 16, held);
+            cp16(values + to, from_values + i * LANES * 16, held);
+          }
+        }
+      }
     } else {
-      mask = __ballot_sync(0xffffffffu, there) & 0xffffu;
+      const int64_t at = there ? page * c.page_stride + ((int64_t)kv * page_size + slot) * hd : -1;
 #pragma unroll
       for (int i = 0; i < COPIES; i++) {
         const int which = lane + 32 * i, r = (int)(which * per_part >> 16), part = which - r * parts;
-        const int64_t from = __shfl_sync(0xffffffffu, at, r % kKeys);
-        if (r < kKeys) {
+        const int64_t from = __shfl_sync(0xffffffffu, at, r % KEYS);
+        if (r < KEYS) {
+          const int to = place<HD>(r, part);
           const int64_t src = from >= 0 ? from + part * 16 : 0;
-          cp16(keys + to[i], c.keys + src, from >= 0);
-          cp16(values + to[i], c.values + src, from >= 0);
+          cp16(keys + to, c.keys + src, from >= 0);
+          cp16(values + to, c.values + src, from >= 0);
         }
       }
-      cp4(scales + stage * 2 * kKeys + lane, (lane < kKeys ? c.key_scales : c.value_scales) + row_at, there);
+    }
+    if constexpr (KEYS == 32) {
+      cp4(scales + stage * 2 * KEYS + lane, c.key_scales + scale_at, there);
+      cp4(scales + stage * 2 * KEYS + KEYS + lane, c.value_scales + scale_at, there);
+    } else {
+      cp4(scales + stage * 2 * KEYS + lane, (lane < KEYS ? c.key_scales : c.value_scales) + scale_at, there);
     }
     if (lane == 0) masks[stage] = mask;
-    pos += kWarps * kKeys;
+    pos += kWarps * KEYS;
     entry += entry_step;
     slot += slot_step;
     if (slot >= page_size) {
@@ -301,9 +309,9 @@ __global__ void __launch_bounds__(kThreads, BLOCKS)
     }
     page = page_at();
   };
-  const int chunks = end > begin + warp * kKeys ? (end - begin - warp * kKeys + kWarps * kKeys - 1) / (kWarps * kKeys) : 0;
+  const int mine = end - begin - warp * KEYS, chunks = mine > 0 ? (mine + kWarps * KEYS - 1) / (kWarps * KEYS) : 0;
 #pragma unroll
-  for (int s = 0; s < STAGES - 1; s++) {
+  for (int s = 0; s < STAGES; s++) {
     if (s < chunks) issue(s);
     asm volatile("cp.async.commit_group;" ::: "memory");
   }
@@ -366,134 +374,137 @@ __global__ void __launch_bounds__(kThreads, BLOCKS)
   asm volatile("mov.b32 %0, %1;" : "=r"(bits) : "n"(kExponent));
   int stage = 0;
   for (int chunk = 0; chunk < chunks; chunk++) {
-    asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
+    asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
     __syncwarp();
-    if (chunk + STAGES - 1 < chunks) issue(stage == 0 ? STAGES - 1 : stage - 1);
-    asm volatile("cp.async.commit_group;" ::: "memory");
-    const uint8_t* keys = ring + stage * 2 * S::kChunk;
-    const uint8_t* values = keys + S::kChunk;
+#pragma unroll 1
+    for (int run = 0; run < KEYS / kRun; run++) {
+      const uint8_t* keys = ring + stage * 2 * S::kChunk + run * kRun * HD;
+      const uint8_t* values = keys + S::kChunk;
 
-    // Scores: rows 2 t, 2 t + 1 of keys g (0, 1) and g + 8 (2, 3).
-    float s[NT][4], less[NT][4];  // `less`: of the queries' parts but the first
-#pragma unroll
-    for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-      for (int e = 0; e < 4; e++) s[nt][e] = less[nt][e] = 0.0f;
-#pragma unroll
-    for (int block = 0; block < HD / 64; block++) {
-      uint32_t k0[4], k1[4];
-      load_words<4>(keys + key_at[block % 2] + block / 2 * 128, k0);
-      load_words<4>(keys + key_at[block % 2] + block / 2 * 128 + 8 * HD, k1);
-#pragma unroll
-      for (int j = 0; j < 4; j++) {
-        const uint32_t f[4] = {widened(k0[j], bits), widened(k1[j], bits), widened(k0[j] >> 8, bits),
-                               widened(k1[j] >> 8, bits)};
-        const int i = block * 4 + j;
-#pragma unroll
-        for (int p = 0; p < PARTS; p++)
-#pragma unroll
-          for (int nt = 0; nt < NT; nt++) {
-            const int at = (p * NT + nt) * STEPS + i;
-            uint2 b;
-            if constexpr (kHeld) b = held[at]; else b = queries[at * 32 + lane];
-            mma16816(p == 0 ? s[nt] : less[nt], f, b.x, b.y);
-          }
-      }
-    }
-    const float* sc = scales + stage * 2 * kKeys;
-    const float ks0 = sc[g] * factor, ks1 = sc[g + 8] * factor, vs0 = sc[kKeys + g], vs1 = sc[kKeys + g + 8];
-    const int first = begin + (chunk * kWarps + warp) * kKeys;
-    const uint32_t mask = masks[stage];
-    const bool whole = mask == 0xffffu && first + kKeys - 1 <= all_high && first >= all_low;
-    bool past = false;
-#pragma unroll
-    for (int nt = 0; nt < NT; nt++) {
-#pragma unroll
-      for (int e = 0; e < 4; e++) s[nt][e] = (PARTS > 1 ? s[nt][e] + less[nt][e] : s[nt][e]) * (e < 2 ? ks0 : ks1);
-      if (!whole) {
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-          const int key = g + (e >= 2 ? 8 : 0), at = first + key, hi = high[nt][e & 1];
-          const bool sees = (mask >> key & 1u) != 0 && at <= hi && (window == 0 || (int64_t)at > hi - window);
-          s[nt][e] = sees ? s[nt][e] : -INFINITY;
-        }
-      }
-      past |= fmaxf(s[nt][0], s[nt][2]) > m[nt][0] || fmaxf(s[nt][1], s[nt][3]) > m[nt][1];
-    }
-    if (__any_sync(0xffffffffu, past)) {
+      // Scores: rows 2 t, 2 t + 1 of keys g (0, 1) and g + 8 (2, 3).
+      float s[NT][4], less[NT][4];  // `less`: of the queries' parts but the first
 #pragma unroll
       for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-        for (int e = 0; e < 2; e++) {
-          float top = fmaxf(s[nt][e], s[nt][e + 2]);
+        for (int e = 0; e < 4; e++) s[nt][e] = less[nt][e] = 0.0f;
 #pragma unroll
-          for (int off = 4; off <= 16; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-          if (!(top > m[nt][e])) continue;  // the same in the row's lanes
-          top += kSlack;
-          const float fade = power2(m[nt][e] - top);
-          m[nt][e] = top;
-          sum[nt][e] *= fade;
+      for (int block = 0; block < HD / 64; block++) {
+        uint32_t k0[4], k1[4];
+        load_words<4>(keys + key_at[block % 2] + block / 2 * 128, k0);
+        load_words<4>(keys + key_at[block % 2] + block / 2 * 128 + 8 * HD, k1);
 #pragma unroll
-          for (int i = 0; i < STEPS; i++) {
-            acc[nt][i][e] *= fade;
-            acc[nt][i][e + 2] *= fade;
+        for (int j = 0; j < 4; j++) {
+          const uint32_t f[4] = {widened(k0[j], bits), widened(k1[j], bits), widened(k0[j] >> 8, bits),
+                                 widened(k1[j] >> 8, bits)};
+          const int i = block * 4 + j;
+#pragma unroll
+          for (int p = 0; p < PARTS; p++)
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) {
+              const int at = (p * NT + nt) * STEPS + i;
+              uint2 b;
+              if constexpr (kHeld) b = held[at]; else b = queries[at * 32 + lane];
+              mma16816(p == 0 ? s[nt] : less[nt], f, b.x, b.y);
+            }
+        }
+      }
+      const float* sc = scales + stage * 2 * KEYS + run * kRun;
+      const float ks0 = sc[g] * factor, ks1 = sc[g + 8] * factor, vs0 = sc[KEYS + g], vs1 = sc[KEYS + g + 8];
+      const int first = begin + (chunk * kWarps + warp) * KEYS + run * kRun;
+      const uint32_t mask = masks[stage] >> run * kRun & 0xffffu;
+      const bool whole = mask == 0xffffu && first + kRun - 1 <= all_high && first >= all_low;
+      bool past = false;
+#pragma unroll
+      for (int nt = 0; nt < NT; nt++) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) s[nt][e] = (PARTS > 1 ? s[nt][e] + less[nt][e] : s[nt][e]) * (e < 2 ? ks0 : ks1);
+        if (!whole) {
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            const int key = g + (e >= 2 ? 8 : 0), at = first + key, hi = high[nt][e & 1];
+            const bool sees = (mask >> key & 1u) != 0 && at <= hi && (window == 0 || (int64_t)at > hi - window);
+            s[nt][e] = sees ? s[nt][e] : -INFINITY;
           }
         }
-    }
-    // Weights, as the second product takes them: keys down, rows across.
-    uint32_t b[WPARTS][NT][2];
-#pragma unroll
-    for (int nt = 0; nt < NT; nt++) {
-      const float m0 = m[nt][0] == -INFINITY ? 0.0f : m[nt][0], m1 = m[nt][1] == -INFINITY ? 0.0f : m[nt][1];
-      const float p0 = power2(s[nt][0] - m0), p1 = power2(s[nt][1] - m1), p2 = power2(s[nt][2] - m0), p3 = power2(s[nt][3] - m1);
-      sum[nt][0] += p0 + p2;
-      sum[nt][1] += p1 + p3;
-      float x0 = p0 * vs0, x1 = p1 * vs0, x2 = p2 * vs1, x3 = p3 * vs1;
-      if (!whole) {  // an unseen value's scale does not count, whatever it is
-        x0 = s[nt][0] == -INFINITY ? 0.0f : x0;
-        x1 = s[nt][1] == -INFINITY ? 0.0f : x1;
-        x2 = s[nt][2] == -INFINITY ? 0.0f : x2;
-        x3 = s[nt][3] == -INFINITY ? 0.0f : x3;
+        past |= fmaxf(s[nt][0], s[nt][2]) > m[nt][0] || fmaxf(s[nt][1], s[nt][3]) > m[nt][1];
       }
+      if (__any_sync(0xffffffffu, past)) {
 #pragma unroll
-      for (int p = 0; p < WPARTS; p++) {
-        const uint32_t lo = Pair<__nv_bfloat16>::pack(x0, x1), hi = Pair<__nv_bfloat16>::pack(x2, x3);
-        b[p][nt][0] = transposed(lo);
-        b[p][nt][1] = transposed(hi);
-        const float2 l = unpacked(lo), h = unpacked(hi);
-        x0 -= l.x, x1 -= l.y, x2 -= h.x, x3 -= h.y;
-      }
-    }
-    // Values: lane (g, t) holds dims HD / 8 g .. of keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9.
-    constexpr int WORDS = HD == 64 ? 2 : 4;
+        for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-    for (int half = 0; half < (HD == 256 ? 2 : 1); half++) {
-      uint32_t v[4][WORDS];
+          for (int e = 0; e < 2; e++) {
+            float top = fmaxf(s[nt][e], s[nt][e + 2]);
 #pragma unroll
-      for (int j = 0; j < 4; j++) {
-        load_words<WORDS>(values + value_at[j % 2] + j / 2 * 8 * HD + half * 128, v[j]);
-      }
+            for (int off = 4; off <= 16; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+            if (!(top > m[nt][e])) continue;  // the same in the row's lanes
+            top += kSlack;
+            const float fade = power2(m[nt][e] - top);
+            m[nt][e] = top;
+            sum[nt][e] *= fade;
 #pragma unroll
-      for (int word = 0; word < WORDS; word++)
-#pragma unroll
-        for (int two = 0; two < 2; two++) {  // dims 2 two and 2 two + 1 of the word: rows g and g + 8
-          const uint32_t s0 = two == 0 ? 0x4400u : 0x6622u, s1 = two == 0 ? 0x5511u : 0x7733u;
-          const uint32_t f[4] = {
-              widened(__byte_perm(v[0][word], v[1][word], s0), bits), widened(__byte_perm(v[0][word], v[1][word], s1), bits),
-              widened(__byte_perm(v[2][word], v[3][word], s0), bits), widened(__byte_perm(v[2][word], v[3][word], s1), bits)};
-          const int i = half * 8 + word * 2 + two;
-#pragma unroll
-          for (int nt = 0; nt < NT; nt++) {
-            float fresh[4] = {};
-#pragma unroll
-            for (int p = WPARTS - 1; p >= 0; p--) mma16816(kFine ? fresh : acc[nt][i], f, b[p][nt][0], b[p][nt][1]);
-            if constexpr (kFine)
-#pragma unroll
-              for (int e = 0; e < 4; e++) acc[nt][i][e] += fresh[e];
+            for (int i = 0; i < STEPS; i++) {
+              acc[nt][i][e] *= fade;
+              acc[nt][i][e + 2] *= fade;
+            }
           }
+      }
+      // Weights, as the second product takes them: keys down, rows across.
+      uint32_t b[WPARTS][NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; nt++) {
+        const float m0 = m[nt][0] == -INFINITY ? 0.0f : m[nt][0], m1 = m[nt][1] == -INFINITY ? 0.0f : m[nt][1];
+        const float p0 = power2(s[nt][0] - m0), p1 = power2(s[nt][1] - m1), p2 = power2(s[nt][2] - m0), p3 = power2(s[nt][3] - m1);
+        sum[nt][0] += p0 + p2;
+        sum[nt][1] += p1 + p3;
+        float x0 = p0 * vs0, x1 = p1 * vs0, x2 = p2 * vs1, x3 = p3 * vs1;
+        if (!whole) {  // an unseen value's scale does not count, whatever it is
+          x0 = s[nt][0] == -INFINITY ? 0.0f : x0;
+          x1 = s[nt][1] == -INFINITY ? 0.0f : x1;
+          x2 = s[nt][2] == -INFINITY ? 0.0f : x2;
+          x3 = s[nt][3] == -INFINITY ? 0.0f : x3;
         }
+#pragma unroll
+        for (int p = 0; p < WPARTS; p++) {
+          const uint32_t lo = Pair<__nv_bfloat16>::pack(x0, x1), hi = Pair<__nv_bfloat16>::pack(x2, x3);
+          b[p][nt][0] = transposed(lo);
+          b[p][nt][1] = transposed(hi);
+          const float2 l = unpacked(lo), h = unpacked(hi);
+          x0 -= l.x, x1 -= l.y, x2 -= h.x, x3 -= h.y;
+        }
+      }
+      // Values: lane (g, t) holds dims HD / 8 g .. of keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9.
+      constexpr int WORDS = HD == 64 ? 2 : 4;
+#pragma unroll
+      for (int half = 0; half < (HD == 256 ? 2 : 1); half++) {
+        uint32_t v[4][WORDS];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          load_words<WORDS>(values + value_at[j % 2] + j / 2 * 8 * HD + half * 128, v[j]);
+        }
+#pragma unroll
+        for (int word = 0; word < WORDS; word++)
+#pragma unroll
+          for (int two = 0; two < 2; two++) {  // dims 2 two and 2 two + 1 of the word: rows g and g + 8
+            const uint32_t s0 = two == 0 ? 0x4400u : 0x6622u, s1 = two == 0 ? 0x5511u : 0x7733u;
+            const uint32_t f[4] = {
+                widened(__byte_perm(v[0][word], v[1][word], s0), bits), widened(__byte_perm(v[0][word], v[1][word], s1), bits),
+                widened(__byte_perm(v[2][word], v[3][word], s0), bits), widened(__byte_perm(v[2][word], v[3][word], s1), bits)};
+            const int i = half * 8 + word * 2 + two;
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) {
+              float fresh[4] = {};
+#pragma unroll
+              for (int p = WPARTS - 1; p >= 0; p--) mma16816(kFine ? fresh : acc[nt][i], f, b[p][nt][0], b[p][nt][1]);
+              if constexpr (kFine)
+#pragma unroll
+                for (int e = 0; e < 4; e++) acc[nt][i][e] += fresh[e];
+            }
+          }
+      }
     }
     __syncwarp();
+    if (chunk + STAGES < chunks) issue(stage);
+    asm volatile("cp.async.commit_group;" ::: "memory");
     stage = stage + 1 == STAGES ? 0 : stage + 1;
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -630,7 +641,7 @@ Split split_of(const PagedQ8Cache& c, int64_t heads, int64_t n, int64_t max_leng
   const int64_t most = (keys + kMinSlice - 1) / kMinSlice;
   slices = slices < most ? slices : most;
   d.most = (int)slices;
-  const int64_t step = kWarps * kKeys, slice = ((keys + slices - 1) / slices + step - 1) / step * step;
+  const int64_t step = 64, slice = ((keys + slices - 1) / slices + step - 1) / step * step;
   d.slice = (int)slice;
   d.slices = (int)((keys + slice - 1) / slice);
   return d;
