@@ -63,6 +63,13 @@ struct Parts<__nv_bfloat16> {
 };
 
 constexpr int kUnit = 64;  // keys
+// What a pair costs beside its keys, in units: its queries, the first copies'
+// way through the page table, the join. It comes before the keys. A border
+// between two blocks that would leave the first of them fewer than kLeast units
+// of keys, or the second, is at the pair's begin or end instead.
+// 32 sequences of up to 4096 keys: 67 us without it (short sequences' pairs fill
+// some blocks and keep the others waiting).
+constexpr int kCost = 4, kLeast = 2;
 
 // A sequence's share of the batch: `tiles` tiles of its rows, each of them with
 // every kv head `units` units (as many as its longest tile needs).
@@ -81,8 +88,13 @@ __device__ __forceinline__ Share share_of(const PagedQ8AttentionArgs& a, int seq
   int64_t keys = min64(s.length, a.cache.table_stride * a.cache.page_size);
   // A tile's window and its other tokens, from a multiple of kRun on.
   if (a.window > 0) keys = min64(keys, a.window + (R - 1) / group + 1 + kRun);
-  s.units = keys <= kUnit ? 1 : (keys + kUnit - 1) / kUnit;
+  s.units = kCost + (keys <= 0 ? 0 : (keys + kUnit - 1) / kUnit);
   return s;
+}
+
+// Where a border at unit `at` of a pair of `units` comes to be.
+__device__ __forceinline__ int64_t border_at(int64_t at, int64_t units) {
+  return at < kCost + kLeast ? 0 : units - at < kLeast ? units : at;
 }
 
 // A pair that is split: its parts are what block `block` left in its second
@@ -192,6 +204,8 @@ __global__ void __launch_bounds__(kThreads, BLOCKS)
   constexpr bool kFine = std::is_same<T, float>::value;
   using S = Smem<HD, NT, PARTS>;
   constexpr int STAGES = S::kStages, KEYS = S::kKeys, STEPS = HD / 16;
+  constexpr int RUNS = NT == 1 ? KEYS / kRun : 1;  // taken together: independent products while others are under way
+  constexpr uint32_t kAll = RUNS == 2 ? 0xffffffffu : 0xffffu;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int64_t sums_of[kWarps + 1], found_at;
   __shared__ int found;
@@ -224,12 +238,12 @@ __global__ void __launch_bounds__(kThreads, BLOCKS)
   }
   before -= own;
   const int64_t blocks = min64(gridDim.x, total), block = blockIdx.x;
+  Cut* cut = &cuts_of(a, R, HD)[block];
   if (block >= blocks) {
-    if (split != 0 && tid == 0) cuts_of(a, R, HD)[block].rows = 0;
+    if (split != 0 && tid == 0) cut->rows = 0;
     return;
   }
-  int64_t at = block * total / blocks;
-  const int64_t stop = (block + 1) * total / blocks;
+  int64_t at = block * total / blocks, stop = (block + 1) * total / blocks;
   if (at >= before && at < before + own) {
     int64_t start = before;
     int i = tid * each;
@@ -245,7 +259,7 @@ __global__ void __launch_bounds__(kThreads, BLOCKS)
   __syncthreads();
   int seq = found;
   int64_t seq_at = found_at;
-  bool opening = true;  // the block's first part
+  bool opening = true;  // the block's first pair
   while (at < stop) {
     const Share sh = share_of<R>(a, seq, group);
     const int64_t pair_units = sh.units, seq_units = sh.tiles * pair_units * kvh;
@@ -254,32 +268,35 @@ __global__ void __launch_bounds__(kThreads, BLOCKS)
       seq++;
       continue;
     }
-    const int64_t pair = (at - seq_at) / pair_units, from = (at - seq_at) - pair * pair_units;
+    const int64_t pair = (at - seq_at) / pair_units, pair_at = seq_at + pair * pair_units;
     const int kv = (int)(pair % kvh);
-    const int64_t row0_ = pair / kvh * R;
-    const int row0 = (int)row0_, rows = (int)min64((int64_t)sh.count * group - row0_, R);
-    const int64_t pair_at = at - from;
-    if (opening && split != 0 && tid == 0) {
-      // The first border inside a pair tells the second launch of it.
-      Cut* cut = &cuts_of(a, R, HD)[block];
-      const bool first_border = from > 0 && (block - 1) * total / blocks <= pair_at;
-      cut->rows = first_border ? rows : 0;
-      cut->first = sh.first;
-      cut->row0 = row0;
-      cut->kv = kv;
-      cut->last = (int)(((pair_at + pair_units) * blocks - 1) / total);
+    const int row0 = (int)(pair / kvh * R), rows = (int)min64((int64_t)sh.count * group - row0, R);
+    int64_t from = 0, to = pair_units;
+    if (split != 0) {
+      if (opening) {
+        from = border_at(at - pair_at, pair_units);
+        // The first border inside a pair tells the second launch of it.
+        const bool inside = from > 0 && from < pair_units;
+        const bool first_border = inside && border_at((block - 1) * total / blocks - pair_at, pair_units) == 0;
+        if (tid == 0) {
+          cut->rows = first_border ? rows : 0;
+          if (first_border) {
+            const int64_t pair_end = pair_at + pair_units, last = (pair_end * blocks - 1) / total;
+            cut->first = sh.first;
+            cut->row0 = row0;
+            cut->kv = kv;
+            cut->last = (int)(border_at(last * total / blocks - pair_at, pair_units) == pair_units ? last - 1 : last);
+          }
+        }
+      }
+      if (stop < pair_at + pair_units) to = border_at(stop - pair_at, pair_units);
+    } else if (at > pair_at) {  // a pair belongs to the block that its first unit falls to
+      from = to;
     }
     opening = false;
-    int64_t units = min64(pair_units - from, stop - at);
-    if (split == 0) {  // a pair belongs to the block that its first unit falls to
-      if (from > 0) {
-        at += pair_units - from;
-        continue;
-      }
-      units = pair_units;
-    }
-    const bool alone = units == pair_units;
-    at += units;
+    at = pair_at + pair_units;
+    if (from >= to) continue;
+    const bool alone = from == 0 && to == pair_units;
 
     // Positions of the tile's first and last tokens, and the keys of this part.
     const int64_t first_pos = (int64_t)sh.length - sh.count + row0 / group;
@@ -288,8 +305,8 @@ __global__ void __launch_bounds__(kThreads, BLOCKS)
     const int64_t low = a.window > 0 ? first_pos - a.window + 1 : 0;
     const int64_t pair_begin = low > 0 ? min64(low, most) / kRun * kRun : 0;
     const int64_t pair_end = last_pos + 1 < 0 ? 0 : min64(last_pos + 1, most);
-    const int begin = (int)min64(pair_begin + from * kUnit, most);
-    const int end = (int)min64(pair_end, pair_begin + (from + units) * kUnit);
+    const int begin = (int)min64(pair_begin + (from > 0 ? from - kCost : 0) * kUnit, most);
+    const int end = (int)min64(pair_end, pair_begin + (to - kCost) * kUnit);
     __syncthreads();  // the part before has left shared memory
 
     // ---- the ring: this lane's row of a chunk, its page a chunk ahead
@@ -441,63 +458,78 @@ __global__ void __launch_bounds__(kThreads, BLOCKS)
       asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
       __syncwarp();
 #pragma unroll 1
-      for (int run = 0; run < KEYS / kRun; run++) {
-        const uint8_t* keys = ring + stage * 2 * S::kChunk + run * kRun * HD;
+      for (int run0 = 0; run0 < KEYS / kRun; run0 += RUNS) {
+        const uint8_t* keys = ring + stage * 2 * S::kChunk + run0 * kRun * HD;
         const uint8_t* values = keys + S::kChunk;
 
-        // Scores: rows 2 t, 2 t + 1 of keys g (0, 1) and g + 8 (2, 3).
-        float s[NT][4], less[NT][4];  // `less`: of the queries' parts but the first
+        // Scores: rows 2 t, 2 t + 1 of keys g (0, 1) and g + 8 (2, 3). `less`:
+        // of the queries' parts but the first; of bf16, of every other step,
+        // which leaves a chain of products half as long.
+        float s[RUNS][NT][4], less[RUNS][NT][4];
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++)
+        for (int run = 0; run < RUNS; run++)
 #pragma unroll
-          for (int e = 0; e < 4; e++) s[nt][e] = less[nt][e] = 0.0f;
+          for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) s[run][nt][e] = less[run][nt][e] = 0.0f;
 #pragma unroll
         for (int block = 0; block < HD / 64; block++) {
-          uint32_t k0[4], k1[4];
-          load_words<4>(keys + key_at[block % 2] + block / 2 * 128, k0);
-          load_words<4>(keys + key_at[block % 2] + block / 2 * 128 + 8 * HD, k1);
+          uint32_t k[RUNS][2][4];
 #pragma unroll
-          for (int j = 0; j < 4; j++) {
-            const uint32_t f[4] = {widened(k0[j], bits), widened(k1[j], bits), widened(k0[j] >> 8, bits),
-                                   widened(k1[j] >> 8, bits)};
-            const int i = block * 4 + j;
+          for (int run = 0; run < RUNS; run++)
 #pragma unroll
-            for (int p = 0; p < PARTS; p++)
+            for (int e = 0; e < 2; e++)
+              load_words<4>(keys + key_at[block % 2] + block / 2 * 128 + (run * kRun + e * 8) * HD, k[run][e]);
 #pragma unroll
-              for (int nt = 0; nt < NT; nt++) {
-                const int at = (p * NT + nt) * STEPS + i;
-                uint2 b;
-                if constexpr (kHeld) b = held[at]; else b = queries[at * 32 + lane];
-                mma16816(p == 0 ? s[nt] : less[nt], f, b.x, b.y);
-              }
-          }
+          for (int j = 0; j < 4; j++)
+#pragma unroll
+            for (int run = 0; run < RUNS; run++) {
+              const uint32_t k0 = k[run][0][j], k1 = k[run][1][j];
+              const uint32_t f[4] = {widened(k0, bits), widened(k1, bits), widened(k0 >> 8, bits), widened(k1 >> 8, bits)};
+              const int i = block * 4 + j;
+#pragma unroll
+              for (int p = 0; p < PARTS; p++)
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) {
+                  const int at = (p * NT + nt) * STEPS + i;
+                  uint2 b;
+                  if constexpr (kHeld) b = held[at]; else b = queries[at * 32 + lane];
+                  mma16816((PARTS > 1 ? p > 0 : i % 2 != 0) ? less[run][nt] : s[run][nt], f, b.x, b.y);
+                }
+            }
         }
-        const float* sc = scales + stage * 2 * KEYS + run * kRun;
-        const float ks0 = sc[g] * factor, ks1 = sc[g + 8] * factor, vs0 = sc[KEYS + g], vs1 = sc[KEYS + g + 8];
-        const int first = begin + (chunk * kWarps + warp) * KEYS + run * kRun;
-        const uint32_t mask = masks[stage] >> run * kRun & 0xffffu;
-        const bool whole = mask == 0xffffu && first + kRun - 1 <= all_high && first >= all_low;
+        const float* sc = scales + stage * 2 * KEYS + run0 * kRun;
+        const int first = begin + (chunk * kWarps + warp) * KEYS + run0 * kRun;
+        const uint32_t mask = masks[stage] >> run0 * kRun & kAll;
+        const bool whole = mask == kAll && first + RUNS * kRun - 1 <= all_high && first >= all_low;
         bool past = false;
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++) {
+        for (int run = 0; run < RUNS; run++) {
+          const float ks[2] = {sc[run * kRun + g] * factor, sc[run * kRun + g + 8] * factor};
 #pragma unroll
-          for (int e = 0; e < 4; e++) s[nt][e] = (PARTS > 1 ? s[nt][e] + less[nt][e] : s[nt][e]) * (e < 2 ? ks0 : ks1);
-          if (!whole) {
+          for (int nt = 0; nt < NT; nt++) {
+            float(&x)[4] = s[run][nt];
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-              const int key = g + (e >= 2 ? 8 : 0), at = first + key, hi = high[nt][e & 1];
-              const bool sees = (mask >> key & 1u) != 0 && at <= hi && (window == 0 || (int64_t)at > hi - window);
-              s[nt][e] = sees ? s[nt][e] : -INFINITY;
+            for (int e = 0; e < 4; e++) x[e] = (x[e] + less[run][nt][e]) * ks[e / 2];
+            if (!whole) {
+#pragma unroll
+              for (int e = 0; e < 4; e++) {
+                const int key = run * kRun + g + e / 2 * 8, at = first + key, hi = high[nt][e & 1];
+                const bool sees = (mask >> key & 1u) != 0 && at <= hi && (window == 0 || (int64_t)at > hi - window);
+                x[e] = sees ? x[e] : -INFINITY;
+              }
             }
+            past |= fmaxf(x[0], x[2]) > m[nt][0] || fmaxf(x[1], x[3]) > m[nt][1];
           }
-          past |= fmaxf(s[nt][0], s[nt][2]) > m[nt][0] || fmaxf(s[nt][1], s[nt][3]) > m[nt][1];
         }
         if (__any_sync(0xffffffffu, past)) {
 #pragma unroll
           for (int nt = 0; nt < NT; nt++)
 #pragma unroll
             for (int e = 0; e < 2; e++) {
-              float top = fmaxf(s[nt][e], s[nt][e + 2]);
+              float top = fmaxf(s[0][nt][e], s[0][nt][e + 2]);
+#pragma unroll
+              for (int run = 1; run < RUNS; run++) top = fmaxf(top, fmaxf(s[run][nt][e], s[run][nt][e + 2]));
 #pragma unroll
               for (int off = 4; off <= 16; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
               if (!(top > m[nt][e])) continue;  // the same in the row's lanes
@@ -513,58 +545,63 @@ __global__ void __launch_bounds__(kThreads, BLOCKS)
             }
         }
         // Weights, as the second product takes them: keys down, rows across.
-        uint32_t b[WPARTS][NT][2];
+        uint32_t b[RUNS][WPARTS][NT][2];
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++) {
-          const float m0 = m[nt][0] == -INFINITY ? 0.0f : m[nt][0], m1 = m[nt][1] == -INFINITY ? 0.0f : m[nt][1];
-          const float p0 = power2(s[nt][0] - m0), p1 = power2(s[nt][1] - m1), p2 = power2(s[nt][2] - m0), p3 = power2(s[nt][3] - m1);
-          sum[nt][0] += p0 + p2;
-          sum[nt][1] += p1 + p3;
-          float x0 = p0 * vs0, x1 = p1 * vs0, x2 = p2 * vs1, x3 = p3 * vs1;
-          if (!whole) {  // an unseen value's scale does not count, whatever it is
-            x0 = s[nt][0] == -INFINITY ? 0.0f : x0;
-            x1 = s[nt][1] == -INFINITY ? 0.0f : x1;
-            x2 = s[nt][2] == -INFINITY ? 0.0f : x2;
-            x3 = s[nt][3] == -INFINITY ? 0.0f : x3;
-          }
+        for (int run = 0; run < RUNS; run++) {
+          const float vs[2] = {sc[KEYS + run * kRun + g], sc[KEYS + run * kRun + g + 8]};
 #pragma unroll
-          for (int p = 0; p < WPARTS; p++) {
-            const uint32_t lo = Pair<__nv_bfloat16>::pack(x0, x1), hi = Pair<__nv_bfloat16>::pack(x2, x3);
-            b[p][nt][0] = transposed(lo);
-            b[p][nt][1] = transposed(hi);
-            const float2 l = unpacked(lo), h = unpacked(hi);
-            x0 -= l.x, x1 -= l.y, x2 -= h.x, x3 -= h.y;
+          for (int nt = 0; nt < NT; nt++) {
+            float x[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+              const float base = m[nt][e & 1] == -INFINITY ? 0.0f : m[nt][e & 1];
+              const float p = power2(s[run][nt][e] - base);
+              sum[nt][e & 1] += p;
+              x[e] = p * vs[e / 2];
+              // An unseen value's scale does not count, whatever it is.
+              if (!whole) x[e] = s[run][nt][e] == -INFINITY ? 0.0f : x[e];
+            }
+#pragma unroll
+            for (int p = 0; p < WPARTS; p++) {
+              const uint32_t lo = Pair<__nv_bfloat16>::pack(x[0], x[1]), hi = Pair<__nv_bfloat16>::pack(x[2], x[3]);
+              b[run][p][nt][0] = transposed(lo);
+              b[run][p][nt][1] = transposed(hi);
+              const float2 l = unpacked(lo), h = unpacked(hi);
+              x[0] -= l.x, x[1] -= l.y, x[2] -= h.x, x[3] -= h.y;
+            }
           }
         }
         // Values: lane (g, t) holds dims HD / 8 g .. of keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9.
         constexpr int WORDS = HD == 64 ? 2 : 4;
 #pragma unroll
-        for (int half = 0; half < (HD == 256 ? 2 : 1); half++) {
-          uint32_t v[4][WORDS];
+        for (int half = 0; half < (HD == 256 ? 2 : 1); half++)
 #pragma unroll
-          for (int j = 0; j < 4; j++) {
-            load_words<WORDS>(values + value_at[j % 2] + j / 2 * 8 * HD + half * 128, v[j]);
-          }
+          for (int run = 0; run < RUNS; run++) {
+            uint32_t v[4][WORDS];
 #pragma unroll
-          for (int word = 0; word < WORDS; word++)
+            for (int j = 0; j < 4; j++)
+              load_words<WORDS>(values + value_at[j % 2] + (run * kRun + j / 2 * 8) * HD + half * 128, v[j]);
 #pragma unroll
-            for (int two = 0; two < 2; two++) {  // dims 2 two and 2 two + 1 of the word: rows g and g + 8
-              const uint32_t s0 = two == 0 ? 0x4400u : 0x6622u, s1 = two == 0 ? 0x5511u : 0x7733u;
-              const uint32_t f[4] = {
-                  widened(__byte_perm(v[0][word], v[1][word], s0), bits), widened(__byte_perm(v[0][word], v[1][word], s1), bits),
-                  widened(__byte_perm(v[2][word], v[3][word], s0), bits), widened(__byte_perm(v[2][word], v[3][word], s1), bits)};
-              const int i = half * 8 + word * 2 + two;
+            for (int word = 0; word < WORDS; word++)
 #pragma unroll
-              for (int nt = 0; nt < NT; nt++) {
-                float fresh[4] = {};
+              for (int two = 0; two < 2; two++) {  // dims 2 two and 2 two + 1 of the word: rows g and g + 8
+                const uint32_t s0 = two == 0 ? 0x4400u : 0x6622u, s1 = two == 0 ? 0x5511u : 0x7733u;
+                const uint32_t f[4] = {
+                    widened(__byte_perm(v[0][word], v[1][word], s0), bits), widened(__byte_perm(v[0][word], v[1][word], s1), bits),
+                    widened(__byte_perm(v[2][word], v[3][word], s0), bits), widened(__byte_perm(v[2][word], v[3][word], s1), bits)};
+                const int i = half * 8 + word * 2 + two;
 #pragma unroll
-                for (int p = WPARTS - 1; p >= 0; p--) mma16816(kFine ? fresh : acc[nt][i], f, b[p][nt][0], b[p][nt][1]);
-                if constexpr (kFine)
+                for (int nt = 0; nt < NT; nt++) {
+                  float fresh[4] = {};
 #pragma unroll
-                  for (int e = 0; e < 4; e++) acc[nt][i][e] += fresh[e];
+                  for (int p = WPARTS - 1; p >= 0; p--)
+                    mma16816(kFine ? fresh : acc[nt][i], f, b[run][p][nt][0], b[run][p][nt][1]);
+                  if constexpr (kFine)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) acc[nt][i][e] += fresh[e];
+                }
               }
-            }
-        }
+          }
       }
       __syncwarp();
       if (chunk + STAGES < chunks) issue(stage);
