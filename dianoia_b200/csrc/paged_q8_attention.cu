@@ -20,14 +20,16 @@
 // (a tile of rows, a kv head) is a row of units of 64 keys, the pairs of all
 // sequences one after another, and every block of one turn of the GPU takes an
 // equal share of the units, whole pairs and parts of them. A block's four warps
-// take every fourth chunk of 32 keys and bring them themselves, by 16-byte
+// take every fourth chunk of 32 keys and bring it themselves, by 16-byte
 // asynchronous copies into a ring of their own, the rows found through the page
-// table a chunk ahead. The base m of a row's softmax is set kSlack (log2) above
-// its largest score so far and stands until a score passes it, which keeps the
-// common path free of reductions: weights stay at most 1, and bf16 weights and
-// f32 sums lose nothing by being 2^-kSlack of that. The warps join in shared
-// memory, the parts of a pair through the workspace in a second launch that is
-// already waiting (programmatic launch).
+// table a chunk ahead. (Warps that each took a share of their own were slower:
+// one sequence of 131072 keys 58 us against 41, everyone at another place of the
+// code and many more parts to join.) The base m of a row's softmax is set kSlack (log2)
+// above its largest score so far and stands until a score passes it, which keeps
+// the common path free of reductions: weights stay at most 1, and bf16 weights
+// and f32 sums lose nothing by being 2^-kSlack of that. The parts of a pair join
+// through the workspace in a second launch that is already waiting (programmatic
+// launch).
 #include "dn_common.cuh"
 #include "dn_launch.h"
 #include "elem.cuh"
@@ -42,8 +44,8 @@ constexpr int kThreads = kWarps * 32;
 constexpr int kRun = 16;  // keys of a product; pages of whole runs are copied as such
 constexpr float kSlack = 8.0f;
 constexpr int kJoinWarps = 8;
+constexpr int kCuts = 4;  // that a block of the second launch looks at
 constexpr int kSms = 148;
-constexpr int64_t kMaxBlocks = kSms * 3;
 constexpr int64_t kWhole = 256;  // batches whose sequences are said to be no longer are not split
 
 // Parts of a query, and of a weight (bf16's one part alone would be the
@@ -97,16 +99,31 @@ __device__ __forceinline__ int64_t border_at(int64_t at, int64_t units) {
   return at < kCost + kLeast ? 0 : units - at < kLeast ? units : at;
 }
 
-// A pair that is split: its parts are what block `block` left in its second
-// place and the blocks up to `last` in their first.
+// A pair that is split: its parts are what the block before left in its second
+// place, and this block and those up to `last` in their first.
 struct Cut {
   int rows;  // 0: no pair begins to be split here
   int first, row0, kv, last;
 };
 
+constexpr int64_t kMaxBlocks = kSms * 4;
+
 // Behind the parts: two places a block, [row][dim] sums and [row] base and total.
 __device__ __forceinline__ Cut* cuts_of(const PagedQ8AttentionArgs& a, int rows, int hd) {
   return reinterpret_cast<Cut*>(static_cast<float*>(a.workspace) + kMaxBlocks * 2 * rows * (hd + 2));
+}
+
+// The dim at place p of a row of sums, which lie as the products' lanes hold
+// them: step p / 16's pair of dims of lane group p % 16 / 2.
+template <int HD>
+__device__ __forceinline__ int dim_of(int p) {
+  const int i = p / 16, g = p % 16 / 2;
+  return (HD == 64 ? g * 8 + i * 2 : i / 8 * 128 + g * 16 + i % 8 * 2) + p % 2;
+}
+
+// a / b for a >= 0, b > 0, by the short division where that is enough.
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+  return ((a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
 }
 
 __device__ __forceinline__ void cp16(void* dst, const void* src, bool there) {
@@ -187,7 +204,8 @@ struct Smem {
   static constexpr int kKeys = HD == 256 ? 16 : 32, kStages = HD == 64 ? 4 : HD == 128 ? 2 : 3;
   static constexpr int kChunk = kKeys * HD;  // bytes of a chunk's keys, or values
   static constexpr int kRing = kWarps * kStages * 2 * kChunk;
-  static constexpr int kJoin = kWarps * NT * 8 * HD * 4;  // the warps' sums, over the ring
+  static constexpr int kRow = HD + 4;                      // floats: the lanes' pairs meet all banks
+  static constexpr int kJoin = kWarps * NT * 8 * kRow * 4;  // the warps' sums, over the ring
   static constexpr int kScales = kRing > kJoin ? kRing : kJoin;
   static constexpr int kMasks = kScales + kWarps * kStages * 2 * kKeys * 4;
   static constexpr int kStats = kMasks + kWarps * kStages * 4;
@@ -195,7 +213,8 @@ struct Smem {
   static constexpr int kBytes = kQueries + PARTS * NT * (HD / 16) * 32 * 8;
 };
 
-template <typename T, int HD, int NT, int BLOCKS>
+// EXACT: rows of HD values in pages of whole runs.
+template <typename T, int HD, int NT, int BLOCKS, bool EXACT>
 __global__ void __launch_bounds__(kThreads, BLOCKS)
     paged_q8_attention_kernel(const __grid_constant__ PagedQ8AttentionArgs a, const int split) {
   constexpr int PARTS = Parts<T>::query, WPARTS = Parts<T>::weight, R = NT * 8;
@@ -207,15 +226,15 @@ __global__ void __launch_bounds__(kThreads, BLOCKS)
   constexpr int RUNS = NT == 1 ? KEYS / kRun : 1;  // taken together: independent products while others are under way
   constexpr uint32_t kAll = RUNS == 2 ? 0xffffffffu : 0xffffu;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ int64_t sums_of[kWarps + 1], found_at;
+  __shared__ int64_t sums_of[kWarps], found_at;
   __shared__ int found;
   pdl_launch_dependents();
   pdl_wait();
   const PagedQ8Cache& c = a.cache;
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32, g = lane / 4, t = lane % 4;
-  const int hd = (int)c.hd, page_size = (int)c.page_size, group = (int)(a.heads / c.kv_heads), kvh = (int)c.kv_heads;
+  const int hd = EXACT ? HD : (int)c.hd, page_size = (int)c.page_size, group = (int)(a.heads / c.kv_heads), kvh = (int)c.kv_heads;
 
-  // ---- this block's units, and the sequence that the first one belongs to
+  // ---- the block's units, and the sequence that the first one belongs to
   const int seqs = (int)c.sequences, each = (seqs + kThreads - 1) / kThreads;
   int64_t own = 0;
   for (int i = tid * each; i < min(seqs, (tid + 1) * each); i++) {
@@ -243,22 +262,25 @@ __global__ void __launch_bounds__(kThreads, BLOCKS)
     if (split != 0 && tid == 0) cut->rows = 0;
     return;
   }
-  int64_t at = block * total / blocks, stop = (block + 1) * total / blocks;
+  int64_t at = quotient(block * total, blocks);
+  const int64_t stop = quotient((block + 1) * total, blocks);
   if (at >= before && at < before + own) {
     int64_t start = before;
-    int i = tid * each;
-    for (;; i++) {
-      const Share s = share_of<R>(a, i, group);
+    int seq = tid * each;
+    for (;; seq++) {
+      const Share s = share_of<R>(a, seq, group);
       const int64_t size = s.tiles * s.units * kvh;
       if (at < start + size) break;
       start += size;
     }
-    found = i;
+    found = seq;
     found_at = start;
   }
   __syncthreads();
   int seq = found;
   int64_t seq_at = found_at;
+  // Four values of a query at once.
+  const bool wide_q = ((uintptr_t)a.q & (4 * sizeof(T) - 1)) == 0 && a.q_stride % 4 == 0;
   bool opening = true;  // the block's first pair
   while (at < stop) {
     const Share sh = share_of<R>(a, seq, group);
@@ -268,16 +290,17 @@ __global__ void __launch_bounds__(kThreads, BLOCKS)
       seq++;
       continue;
     }
-    const int64_t pair = (at - seq_at) / pair_units, pair_at = seq_at + pair * pair_units;
-    const int kv = (int)(pair % kvh);
-    const int row0 = (int)(pair / kvh * R), rows = (int)min64((int64_t)sh.count * group - row0, R);
+    const int64_t pair = quotient(at - seq_at, pair_units), pair_at = seq_at + pair * pair_units;
+    const int64_t tile = quotient(pair, kvh);
+    const int kv = (int)(pair - tile * kvh);
+    const int row0 = (int)(tile * R), rows = (int)min64((int64_t)sh.count * group - row0, R);
     int64_t from = 0, to = pair_units;
     if (split != 0) {
       if (opening) {
         from = border_at(at - pair_at, pair_units);
         // The first border inside a pair tells the second launch of it.
         const bool inside = from > 0 && from < pair_units;
-        const bool first_border = inside && border_at((block - 1) * total / blocks - pair_at, pair_units) == 0;
+        const bool first_border = inside && border_at(quotient((block - 1) * total, blocks) - pair_at, pair_units) == 0;
         if (tid == 0) {
           cut->rows = first_border ? rows : 0;
           if (first_border) {
@@ -285,7 +308,7 @@ __global__ void __launch_bounds__(kThreads, BLOCKS)
             cut->first = sh.first;
             cut->row0 = row0;
             cut->kv = kv;
-            cut->last = (int)(border_at(last * total / blocks - pair_at, pair_units) == pair_units ? last - 1 : last);
+            cut->last = (int)(border_at(quotient(last * total, blocks) - pair_at, pair_units) == pair_units ? last - 1 : last);
           }
         }
       }
@@ -319,15 +342,15 @@ __global__ void __launch_bounds__(kThreads, BLOCKS)
       __syncwarp();
     }
     const int32_t* table = c.table + (int64_t)seq * c.table_stride;
-    // Pages of whole runs of 16: LANES lanes copy a run, as one run of bytes. Else
-    // a row's parts are copied from where the lane that follows it says.
-    const bool runs = page_size % kRun == 0;
+    // Where pages have whole runs of 16 rows of HD values, LANES lanes copy a run,
+    // as one run of bytes. Else a row's parts are copied from where the lane that
+    // follows it says.
     constexpr int LANES = KEYS == 32 ? 16 : 32, COPIES = KEYS * HD / 16 / 32;
     const int row = lane % KEYS, in_run = row % kRun;
     int pos = begin + warp * KEYS + row;  // of the next chunk to issue
     int entry = pos / page_size, slot = pos - entry * page_size;
     const int entry_step = kWarps * KEYS / page_size, slot_step = kWarps * KEYS - entry_step * page_size;
-    auto page_at = [&]() { return pos - (runs ? in_run : 0) < end ? table[entry] : -1; };
+    auto page_at = [&]() { return pos - (EXACT ? in_run : 0) < end ? table[entry] : -1; };
     int page = page_at();
     const int parts = hd / 16;
     const uint32_t per_part = 65536u / (uint32_t)parts + 1;  // x per_part / 65536 is x / parts, for x below 512
@@ -338,27 +361,15 @@ __global__ void __launch_bounds__(kThreads, BLOCKS)
       const uint32_t mask = __ballot_sync(0xffffffffu, there);
       uint8_t* keys = ring + stage * 2 * S::kChunk;
       uint8_t* values = keys + S::kChunk;
-      if (runs) {
+      if constexpr (EXACT) {
         const int64_t at = held ? page * c.page_stride + ((int64_t)kv * page_size + (slot - in_run)) * hd : 0;
         const int8_t* from_keys = c.keys + at + lane % LANES * 16;
         const int8_t* from_values = c.values + at + lane % LANES * 16;
-        if (hd == HD) {
 #pragma unroll
-          for (int i = 0; i < COPIES; i++) {  // LANES * 16 / HD rows on each time
-            const int to = (first_to ^ turn_of<HD>(i * (LANES * 16 / HD)) * 16) + i * LANES * 16;
-            cp16(keys + to, from_keys + i * LANES * 16, held);
-            cp16(values + to, from_values + i * LANES * 16, held);
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < COPIES; i++) {
-            const int which = lane % LANES + i * LANES, r = (int)(which * per_part >> 16);
-            if (r < kRun) {
-              const int to = place<HD>(r + (KEYS == 32 ? lane / 16 * kRun : 0), which - r * parts);
-              cp16(keys + to, from_keys + i * LANES * 16, held);
-              cp16(values + to, from_values + i * LANES * 16, held);
-            }
-          }
+        for (int i = 0; i < COPIES; i++) {  // LANES * 16 / HD rows on each time
+          const int to = (first_to ^ turn_of<HD>(i * (LANES * 16 / HD)) * 16) + i * LANES * 16;
+          cp16(keys + to, from_keys + i * LANES * 16, held);
+          cp16(values + to, from_values + i * LANES * 16, held);
         }
       } else {
         const int64_t at = there ? page * c.page_stride + ((int64_t)kv * page_size + slot) * hd : -1;
@@ -391,33 +402,35 @@ __global__ void __launch_bounds__(kThreads, BLOCKS)
       page = page_at();
     };
     const int mine = end - begin - warp * KEYS, chunks = mine > 0 ? (mine + kWarps * KEYS - 1) / (kWarps * KEYS) : 0;
-#pragma unroll
-    for (int s = 0; s < STAGES; s++) {
-      if (s < chunks) issue(s);
-      asm volatile("cp.async.commit_group;" ::: "memory");
-    }
-
     // ---- the queries, as the products take them: of step i lane (g, t) holds
     // row g's dims 64 (i / 4) + 16 t + 4 (i % 4) .. + 3, the even ones first as
     // the keys' words give them
-    uint2* queries = reinterpret_cast<uint2*>(smem + S::kQueries);
-    for (int at = tid; at < NT * STEPS * 32; at += kThreads) {
-      const int l = at % 32, i = at / 32 % STEPS, nt = at / 32 / STEPS, r = nt * 8 + l / 4;
-      const int dim = i / 4 * 64 + l % 4 * 16 + i % 4 * 4;
+    auto load_query = [&](int nt, int i, int l, uint2(&to)[PARTS]) {
+      const int r = nt * 8 + l / 4, dim = i / 4 * 64 + l % 4 * 16 + i % 4 * 4;
       const int token = sh.first + (row0 + r) / group, head = kv * group + (row0 + r) % group;
       float x[4] = {};
       if (r < rows && dim < hd && token >= 0 && token < a.n) {
         const T* src = static_cast<const T*>(a.q) + (int64_t)token * a.q_stride + (int64_t)head * hd + dim;
+        if (wide_q) {
+          load_run<T, 4>(src, x);
+        } else {
 #pragma unroll
-        for (int e = 0; e < 4; e++) x[e] = to_f32<T>(src[e]);
+          for (int e = 0; e < 4; e++) x[e] = to_f32<T>(src[e]);
+        }
       }
 #pragma unroll
       for (int p = 0; p < PARTS; p++) {
-        const uint2 b = make_uint2(Pair<__nv_bfloat16>::pack(x[0], x[2]), Pair<__nv_bfloat16>::pack(x[1], x[3]));
-        queries[(p * NT + nt) * STEPS * 32 + i * 32 + l] = b;
-        const float2 lo = unpacked(b.x), hi = unpacked(b.y);
+        to[p] = make_uint2(Pair<__nv_bfloat16>::pack(x[0], x[2]), Pair<__nv_bfloat16>::pack(x[1], x[3]));
+        const float2 lo = unpacked(to[p].x), hi = unpacked(to[p].y);
         x[0] -= lo.x, x[2] -= lo.y, x[1] -= hi.x, x[3] -= hi.y;
       }
+    };
+    uint2* queries = reinterpret_cast<uint2*>(smem + S::kQueries);
+    for (int at = tid; at < NT * STEPS * 32; at += kThreads) {
+      uint2 x[PARTS];
+      load_query(at / 32 / STEPS, at / 32 % STEPS, at % 32, x);
+#pragma unroll
+      for (int p = 0; p < PARTS; p++) queries[p * NT * STEPS * 32 + at] = x[p];
     }
     __syncthreads();
     constexpr bool kHeld = PARTS * NT * STEPS * 2 <= 32;  // in registers
@@ -454,7 +467,11 @@ __global__ void __launch_bounds__(kThreads, BLOCKS)
     uint32_t bits;
     asm volatile("mov.b32 %0, %1;" : "=r"(bits) : "n"(kExponent));
     int stage = 0;
-    for (int chunk = 0; chunk < chunks; chunk++) {
+    // The first STAGES turns only fill the ring: `issue` and what follows are in
+    // the code once, which the instruction cache needs with every warp elsewhere.
+#pragma unroll 1
+    for (int chunk = -STAGES; chunk < chunks; chunk++) {
+     if (chunk >= 0) {
       asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
       __syncwarp();
 #pragma unroll 1
@@ -604,41 +621,46 @@ __global__ void __launch_bounds__(kThreads, BLOCKS)
           }
       }
       __syncwarp();
+     }
       if (chunk + STAGES < chunks) issue(stage);
       asm volatile("cp.async.commit_group;" ::: "memory");
       stage = stage + 1 == STAGES ? 0 : stage + 1;
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
 
-    // ---- the warps join
+    // ---- out, or to this part's place
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+      for (int e = 0; e < 2; e++)
+#pragma unroll
+        for (int off = 4; off <= 16; off <<= 1) sum[nt][e] += __shfl_xor_sync(0xffffffffu, sum[nt][e], off);
+    float* part = static_cast<float*>(a.workspace) + (block * 2 + (from == 0 ? 1 : 0)) * (int64_t)(R * (HD + 2));
+    auto out_row = [&](int r) -> T* {
+      const int token = sh.first + (row0 + r) / group, head = kv * group + (row0 + r) % group;
+      return token < 0 || token >= a.n ? nullptr : static_cast<T*>(a.out) + (int64_t)token * a.out_stride + (int64_t)head * hd;
+    };
     float* stats = reinterpret_cast<float*>(smem + S::kStats);  // [warp][row][base, sum]
-    float* sums = reinterpret_cast<float*>(smem);               // [warp][row][dim], over the ring
+    float* sums = reinterpret_cast<float*>(smem);               // [warp][row][place], over the ring
     __syncthreads();
 #pragma unroll
     for (int nt = 0; nt < NT; nt++)
 #pragma unroll
       for (int e = 0; e < 2; e++) {
-        float total = sum[nt][e];
-#pragma unroll
-        for (int off = 4; off <= 16; off <<= 1) total += __shfl_xor_sync(0xffffffffu, total, off);
         const int r = nt * 8 + 2 * t + e;
         if (g == 0) {
           stats[(warp * R + r) * 2] = m[nt][e];
-          stats[(warp * R + r) * 2 + 1] = total;
+          stats[(warp * R + r) * 2 + 1] = sum[nt][e];
         }
-        float* to = sums + (warp * R + r) * HD;
+        float* to = sums + (warp * R + r) * S::kRow + g * 2;
 #pragma unroll
-        for (int i = 0; i < STEPS; i++) {
-          // Step i's dims: two of this lane's run of 16 (8 where HD is 64) in its half.
-          const int dim = HD == 64 ? g * 8 + i * 2 : i / 8 * 128 + g * 16 + i % 8 * 2;
-          *reinterpret_cast<float2*>(to + dim) = make_float2(acc[nt][i][e], acc[nt][i][e + 2]);
-        }
+        for (int i = 0; i < STEPS; i++)
+          *reinterpret_cast<float2*>(to + i * 16) = make_float2(acc[nt][i][e], acc[nt][i][e + 2]);
       }
     __syncthreads();
-    float* part = static_cast<float*>(a.workspace) + (block * 2 + (from == 0 ? 1 : 0)) * (int64_t)(R * (HD + 2));
     for (int at = tid; at < rows * (HD / 4); at += kThreads) {
-      const int r = at / (HD / 4), dim = at % (HD / 4) * 4;
-      float top = -INFINITY, total = 0.0f;
+      const int r = at / (HD / 4), p = at % (HD / 4) * 4;
+      float top = -INFINITY, whole_sum = 0.0f;
 #pragma unroll
       for (int i = 0; i < kWarps; i++) top = fmaxf(top, stats[(i * R + r) * 2]);
       const float base = top == -INFINITY ? 0.0f : top;
@@ -646,82 +668,104 @@ __global__ void __launch_bounds__(kThreads, BLOCKS)
 #pragma unroll
       for (int i = 0; i < kWarps; i++) {
         const float fade = power2(stats[(i * R + r) * 2] - base);
-        total += stats[(i * R + r) * 2 + 1] * fade;
-        const float4 v = *reinterpret_cast<const float4*>(sums + (i * R + r) * HD + dim);
+        whole_sum += stats[(i * R + r) * 2 + 1] * fade;
+        const float4 v = *reinterpret_cast<const float4*>(sums + (i * R + r) * S::kRow + p);
         o[0] += v.x * fade, o[1] += v.y * fade, o[2] += v.z * fade, o[3] += v.w * fade;
       }
       if (!alone) {
-        if (dim == 0) *reinterpret_cast<float2*>(part + R * HD + r * 2) = make_float2(top, total);
-        *reinterpret_cast<float4*>(part + r * HD + dim) = make_float4(o[0], o[1], o[2], o[3]);
-      } else if (dim < hd) {
-        const int token = sh.first + (row0 + r) / group, head = kv * group + (row0 + r) % group;
-        if (token < 0 || token >= a.n) continue;
-        T* out = static_cast<T*>(a.out) + (int64_t)token * a.out_stride + (int64_t)head * hd + dim;
+        if (p == 0) *reinterpret_cast<float2*>(part + R * HD + r * 2) = make_float2(top, whole_sum);
+        *reinterpret_cast<float4*>(part + r * HD + p) = make_float4(o[0], o[1], o[2], o[3]);
+      } else if (T* out = out_row(r); out != nullptr) {
+        const float inv = whole_sum == 0.0f ? 0.0f : 1.0f / whole_sum;
 #pragma unroll
-        for (int e = 0; e < 4; e++) out[e] = from_f32<T>(total == 0.0f ? 0.0f : o[e] / total);
+        for (int e = 0; e < 4; e++)
+          if (const int dim = dim_of<HD>(p + e); dim < hd) out[dim] = from_f32<T>(o[e] * inv);
       }
     }
   }
 }
 
-// The parts of a split pair's row, a block: its warps take every kJoinWarps-th.
+// A row of the pairs that kCuts blocks begin to split: a warp to a pair of few
+// parts, all of the block to one of many.
 template <typename T, int HD>
 __global__ void __launch_bounds__(kJoinWarps * 32)
     paged_q8_join_kernel(const __grid_constant__ PagedQ8AttentionArgs a, const int tile_rows) {
   pdl_launch_dependents();
+  constexpr int N = HD > 128 ? HD / 128 : 1, kFew = 8;
   __shared__ float sums[kJoinWarps][HD], totals[kJoinWarps];
-  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, r = (int)blockIdx.y;
   const int group = (int)(a.heads / a.cache.kv_heads), hd = (int)a.cache.hd;
-  const int r = (int)(blockIdx.x % (unsigned)tile_rows);
-  const int64_t block = blockIdx.x / (unsigned)tile_rows;
+  const int64_t block0 = (int64_t)blockIdx.x * kCuts, step = 2 * tile_rows * (HD + 2);
   pdl_wait();
-  const Cut cut = cuts_of(a, tile_rows, HD)[block];
-  if (r >= cut.rows) return;
-  const int64_t step = 2 * tile_rows * (HD + 2);
-  // Part 0 lies in the second place of the block before; part i in block + i - 1's first.
-  const float* parts = static_cast<const float*>(a.workspace) + (block - 1) * step;
-  const int count = (int)(cut.last - block) + 2;
-  auto part = [&](int i) { return parts + i * step + (i == 0 ? step / 2 : 0); };
-  auto stats = [&](int i) { return *reinterpret_cast<const float2*>(part(i) + tile_rows * HD + r * 2); };
-  float top = -INFINITY;
-  for (int i = lane; i < count; i += 32) top = fmaxf(top, stats(i).x);
+  const Cut* cuts = cuts_of(a, tile_rows, HD) + block0;
+  // Sums of every `by`-th part from `i0` on, under the base of all.
+  auto sum_parts = [&](const Cut& cut, int64_t block, int i0, int by, float(&o)[N][4], float& total) {
+    // Part 0 lies in the second place of the block before; part i in block + i - 1's first.
+    const float* parts = static_cast<const float*>(a.workspace) + (block - 1) * step;
+    const int count = (int)(cut.last - block) + 2;
+    auto part = [&](int i) { return parts + i * step + (i == 0 ? step / 2 : 0); };
+    auto stats = [&](int i) { return *reinterpret_cast<const float2*>(part(i) + tile_rows * HD + r * 2); };
+    float top = -INFINITY;
+    for (int i = lane; i < count; i += 32) top = fmaxf(top, stats(i).x);
 #pragma unroll
-  for (int off = 16; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-  const float base = top == -INFINITY ? 0.0f : top;
-  constexpr int N = HD > 128 ? HD / 128 : 1;
-  float o[N][4] = {}, total = 0.0f;
+    for (int off = 16; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+    const float base = top == -INFINITY ? 0.0f : top;
 #pragma unroll 4
-  for (int i = warp; i < count; i += kJoinWarps) {
-    const float2 st = stats(i);
-    const float fade = power2(st.x - base);
-    total += st.y * fade;
+    for (int i = i0; i < count; i += by) {
+      const float2 st = stats(i);
+      const float fade = power2(st.x - base);
+      total += st.y * fade;
 #pragma unroll
-    for (int j = 0; j < N; j++) {
-      const int dim = (j * 32 + lane) * 4;
-      if (dim < HD) {
-        const float4 v = *reinterpret_cast<const float4*>(part(i) + r * HD + dim);
-        o[j][0] += v.x * fade, o[j][1] += v.y * fade, o[j][2] += v.z * fade, o[j][3] += v.w * fade;
+      for (int j = 0; j < N; j++) {
+        const int p = (j * 32 + lane) * 4;
+        if (p < HD) {
+          const float4 v = *reinterpret_cast<const float4*>(part(i) + r * HD + p);
+          o[j][0] += v.x * fade, o[j][1] += v.y * fade, o[j][2] += v.z * fade, o[j][3] += v.w * fade;
+        }
       }
     }
-  }
+  };
+  auto out_row = [&](const Cut& cut) -> T* {
+    const int token = cut.first + (cut.row0 + r) / group, head = cut.kv * group + (cut.row0 + r) % group;
+    return token < 0 || token >= a.n ? nullptr : static_cast<T*>(a.out) + (int64_t)token * a.out_stride + (int64_t)head * hd;
+  };
+  if (const Cut cut = cuts[warp % kCuts]; warp < kCuts && r < cut.rows && cut.last - (block0 + warp) + 2 <= kFew) {
+    float o[N][4] = {}, total = 0.0f;
+    sum_parts(cut, block0 + warp, 0, 1, o, total);
+    if (T* out = out_row(cut); out != nullptr) {
+      const float inv = total == 0.0f ? 0.0f : 1.0f / total;
 #pragma unroll
-  for (int j = 0; j < N; j++) {
-    const int dim = (j * 32 + lane) * 4;
-    if (dim < HD) *reinterpret_cast<float4*>(&sums[warp][dim]) = make_float4(o[j][0], o[j][1], o[j][2], o[j][3]);
-  }
-  if (lane == 0) totals[warp] = total;
-  __syncthreads();
-  const int token = cut.first + (cut.row0 + r) / group, head = cut.kv * group + (cut.row0 + r) % group;
-  if (token < 0 || token >= a.n) return;
-  T* out = static_cast<T*>(a.out) + (int64_t)token * a.out_stride + (int64_t)head * hd;
-  for (int dim = threadIdx.x; dim < hd; dim += kJoinWarps * 32) {
-    float x = 0.0f, all = 0.0f;
+      for (int j = 0; j < N; j++)
 #pragma unroll
-    for (int i = 0; i < kJoinWarps; i++) {
-      x += sums[i][dim];
-      all += totals[i];
+        for (int e = 0; e < 4; e++) {
+          const int p = (j * 32 + lane) * 4 + e;
+          if (const int dim = dim_of<HD>(p); p < HD && dim < hd) out[dim] = from_f32<T>(o[j][e] * inv);
+        }
     }
-    out[dim] = from_f32<T>(all == 0.0f ? 0.0f : x / all);
+  }
+  for (int i = 0; i < kCuts; i++) {
+    const Cut cut = cuts[i];
+    if (r >= cut.rows || cut.last - (block0 + i) + 2 <= kFew) continue;  // the same in all threads
+    float o[N][4] = {}, total = 0.0f;
+    sum_parts(cut, block0 + i, warp, kJoinWarps, o, total);
+    __syncthreads();  // the pair before has been read
+#pragma unroll
+    for (int j = 0; j < N; j++) {
+      const int p = (j * 32 + lane) * 4;
+      if (p < HD) *reinterpret_cast<float4*>(&sums[warp][p]) = make_float4(o[j][0], o[j][1], o[j][2], o[j][3]);
+    }
+    if (lane == 0) totals[warp] = total;
+    __syncthreads();
+    T* out = out_row(cut);
+    for (int p = threadIdx.x; p < HD; p += kJoinWarps * 32) {
+      float x = 0.0f, all = 0.0f;
+#pragma unroll
+      for (int j = 0; j < kJoinWarps; j++) {
+        x += sums[j][p];
+        all += totals[j];
+      }
+      if (const int dim = dim_of<HD>(p); out != nullptr && dim < hd) out[dim] = from_f32<T>(all == 0.0f ? 0.0f : x * (1.0f / all));
+    }
   }
 }
 
@@ -736,9 +780,9 @@ int tile_rows(const PagedQ8Cache& c, int64_t heads, int64_t n) {
 }
 
 template <auto KERNEL>
-cudaError_t launch(int64_t blocks, int threads, int smem, const PagedQ8AttentionArgs& a, int arg, cudaStream_t stream, bool pdl) {
+cudaError_t launch(dim3 grid, int threads, int smem, const PagedQ8AttentionArgs& a, int arg, cudaStream_t stream, bool pdl) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)blocks);
+  cfg.gridDim = grid;
   cfg.blockDim = dim3((unsigned)threads);
   cfg.dynamicSmemBytes = (size_t)smem;
   cfg.stream = stream;
@@ -750,34 +794,36 @@ cudaError_t launch(int64_t blocks, int threads, int smem, const PagedQ8Attention
   return cudaLaunchKernelEx(&cfg, KERNEL, a, arg);
 }
 
-template <typename T, int HD, int NT, int BLOCKS>
+template <typename T, int HD, int NT, int BLOCKS, bool EXACT>
 cudaError_t launch_tile(const PagedQ8AttentionArgs& a, cudaStream_t stream, bool pdl) {
-  constexpr int smem = Smem<HD, NT, Parts<T>::query>::kBytes, blocks = kSms * BLOCKS;
-  static_assert(blocks <= kMaxBlocks, "the workspace has places for so many");
-  if (cudaError_t e = allow_smem<paged_q8_attention_kernel<T, HD, NT, BLOCKS>>(smem); e != cudaSuccess) return e;
+  using S = Smem<HD, NT, Parts<T>::query>;
+  constexpr int blocks = kSms * BLOCKS;
+  static_assert(blocks <= kMaxBlocks && blocks % kCuts == 0, "the workspace has places for so many");
+  if (cudaError_t e = allow_smem<paged_q8_attention_kernel<T, HD, NT, BLOCKS, EXACT>>(S::kBytes); e != cudaSuccess) return e;
   const bool split = a.max_length > kWhole;
-  if (cudaError_t e = launch<paged_q8_attention_kernel<T, HD, NT, BLOCKS>>(blocks, kThreads, smem, a, split ? 1 : 0, stream, pdl);
+  if (cudaError_t e = launch<paged_q8_attention_kernel<T, HD, NT, BLOCKS, EXACT>>(dim3(blocks), kThreads, S::kBytes, a,
+                                                                           split ? 1 : 0, stream, pdl);
       e != cudaSuccess || !split)
     return e;
-  return launch<paged_q8_join_kernel<T, HD>>((int64_t)blocks * NT * 8, kJoinWarps * 32, 0, a, NT * 8, stream, true);
+  return launch<paged_q8_join_kernel<T, HD>>(dim3(blocks / kCuts, NT * 8), kJoinWarps * 32, 0, a, NT * 8, stream, true);
 }
 
-template <typename T>
+template <typename T, bool EXACT>
 cudaError_t launch_type(const PagedQ8AttentionArgs& a, cudaStream_t stream, bool pdl) {
-  // f32's three parts leave registers for 16 rows.
-  constexpr int most = std::is_same<T, float>::value ? 2 : 4;
+  // Queries of two and three parts leave registers for 16 rows.
+  constexpr int most = Parts<T>::query == 1 ? 4 : 2;
   const int rows = tile_rows(a.cache, a.heads, a.n);
   switch (padded_hd(a.cache.hd)) {
     case 64:
-      return rows == 8    ? launch_tile<T, 64, 1, 3>(a, stream, pdl)
-             : rows == 16 ? launch_tile<T, 64, 2, 3>(a, stream, pdl)
-                          : launch_tile<T, 64, most, 2>(a, stream, pdl);
+      return rows == 8    ? launch_tile<T, 64, 1, 3, EXACT>(a, stream, pdl)
+             : rows == 16 ? launch_tile<T, 64, 2, 3, EXACT>(a, stream, pdl)
+                          : launch_tile<T, 64, most, 2, EXACT>(a, stream, pdl);
     case 128:
-      return rows == 8    ? launch_tile<T, 128, 1, 3>(a, stream, pdl)
-             : rows == 16 ? launch_tile<T, 128, 2, 2>(a, stream, pdl)
-                          : launch_tile<T, 128, most, 2>(a, stream, pdl);
+      return rows == 8    ? launch_tile<T, 128, 1, 3, EXACT>(a, stream, pdl)
+             : rows == 16 ? launch_tile<T, 128, 2, 2, EXACT>(a, stream, pdl)
+                          : launch_tile<T, 128, most, 2, EXACT>(a, stream, pdl);
     default:
-      return rows == 8 ? launch_tile<T, 256, 1, 2>(a, stream, pdl) : launch_tile<T, 256, 2, 2>(a, stream, pdl);
+      return rows == 8 ? launch_tile<T, 256, 1, 2, EXACT>(a, stream, pdl) : launch_tile<T, 256, 2, 2, EXACT>(a, stream, pdl);
   }
 }
 
@@ -790,10 +836,12 @@ int64_t paged_q8_attention_workspace(const PagedQ8Cache& c, int64_t heads, int64
 
 cudaError_t launch_paged_q8_attention(const PagedQ8AttentionArgs& a, cudaStream_t stream, bool pdl) {
   if (a.n <= 0 || a.cache.sequences <= 0) return cudaSuccess;
+  const bool exact = a.cache.hd == padded_hd(a.cache.hd) && a.cache.page_size % kRun == 0;
   switch (a.type) {
-    case kF32: return launch_type<float>(a, stream, pdl);
-    case kF16: return launch_type<__half>(a, stream, pdl);
-    default: return launch_type<__nv_bfloat16>(a, stream, pdl);
+    case kF32: return exact ? launch_type<float, true>(a, stream, pdl) : launch_type<float, false>(a, stream, pdl);
+    case kF16: return exact ? launch_type<__half, true>(a, stream, pdl) : launch_type<__half, false>(a, stream, pdl);
+    default:
+      return exact ? launch_type<__nv_bfloat16, true>(a, stream, pdl) : launch_type<__nv_bfloat16, false>(a, stream, pdl);
   }
 }
 
