@@ -15,10 +15,11 @@
 //    histogram of their distance from the largest one: at least k tokens are as
 //    near as the k-th of these;
 //  - min_p: the weight says it;
-//  - top_p: weights of 2^-16 and more; the rest only adds to the sum, from f32
-//    exponentials in the same steps.
-// Their weights (f64) and keys go to the first block, which sorts them and
-// decides alone while the others leave. Where more tokens matter than its
+//  - top_p: the weights by their log2, roughly, in a histogram: as many of the
+//    largest as hold that share. The rest only adds to the sum (below 2^-20 from
+//    f32 exponentials, in the same steps).
+// Their weights (f64) and keys go to the first block's shared memory, which sorts
+// them and decides alone while the others leave. Where more tokens matter than its
 // lists hold (flat distributions, many ties, thousands of top_k) the border is
 // found eight bits of the key at a time over all of the row in the cluster's
 // shared memory; without a rule but the temperature every token has its f64
@@ -43,7 +44,8 @@ constexpr int kSorted = 2048;   // that the first one sorts, over its part of th
 constexpr int kMostK = 1536;    // top_k up to which the histogram is asked
 constexpr int kBins = 256;
 constexpr double kOne = 17592186044416.0;  // 2^44, the largest weight
-constexpr float kHead = -16.0f;            // log2 of the weights that top_p lists
+constexpr int kLevels = 24;      // log2 of the weights that top_p may list
+constexpr float kExact = -20.0f;  // log2 of the weights that count in f64
 
 // Ordered as the floats are, -0 as +0; 0 for what is no token.
 __device__ __forceinline__ uint32_t key_of(float x) {
@@ -58,6 +60,7 @@ __device__ __forceinline__ float value_of(uint32_t key) {
 // What the blocks of a cluster read of one another.
 struct Shared {
   uint64_t hist[kBins];
+  uint32_t near[kBins];
   uint64_t list_weight[kListed];
   uint32_t list_key[kListed];
   uint16_t list_at[kListed];
@@ -69,6 +72,27 @@ struct Shared {
   int border_bin;  // of this block alone
   uint64_t border_above;
 };
+
+// The sum over the cluster's blocks of f(what a block shares), the same in every
+// lane; the blocks before `upto` in `before`. A lane asks a block.
+template <typename F>
+__device__ __forceinline__ uint64_t over_blocks(cg::cluster_group& cluster, Shared& sh, F&& f, int upto, uint64_t& before) {
+  const int lane = threadIdx.x % 32;
+  uint64_t v = lane < (int)cluster.num_blocks() ? (uint64_t)f(*cluster.map_shared_rank(&sh, lane)) : 0;
+  uint64_t b = lane < upto ? v : 0;
+#pragma unroll
+  for (int off = 8; off >= 1; off >>= 1) {
+    v += __shfl_xor_sync(0xffffffffu, v, off);
+    b += __shfl_xor_sync(0xffffffffu, b, off);
+  }
+  before = __shfl_sync(0xffffffffu, b, 0);
+  return __shfl_sync(0xffffffffu, v, 0);
+}
+template <typename F>
+__device__ __forceinline__ uint64_t over_blocks(cg::cluster_group& cluster, Shared& sh, F&& f) {
+  uint64_t before;
+  return over_blocks(cluster, sh, f, 0, before);
+}
 
 template <typename T>
 struct Row {
@@ -175,7 +199,8 @@ __device__ uint32_t border_of(cg::cluster_group& cluster, Shared& sh, const Row<
     // Thread t has bin 255 - t: the sums before it are those above it.
     const int bin = 255 - tid;
     uint64_t own = 0;
-    for (int b = 0; b < blocks; b++) own += cluster.map_shared_rank(&sh, b)->hist[bin];
+#pragma unroll
+    for (int b = 0; b < kMaxBlocks; b++) own += b < blocks ? cluster.map_shared_rank(&sh, b)->hist[bin] : 0;
     if (less != 0 && (shift == 24 || at_key >> (shift + 8) == prefix) && (int)(at_key >> shift & 255) == bin) own -= less;
     uint64_t all;
     const uint64_t before = above + scan_block(own, sh.scan, all);
@@ -194,22 +219,10 @@ __device__ uint32_t border_of(cg::cluster_group& cluster, Shared& sh, const Row<
 template <typename T>
 __device__ void choose_over_row(cg::cluster_group& cluster, Shared& sh, const SampleArgs& a, int64_t row, const Row<T>& r,
                                 int top_k, float top_p, float min_p, float u) {
-  const int tid = threadIdx.x, blocks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+  const int tid = threadIdx.x, rank = (int)cluster.block_rank();
   uint32_t border = 1;       // tokens below it are out,
   uint64_t ties = ~0ull;     // of those at it the first so many are in
   auto one = [](uint32_t) -> uint64_t { return 1; };
-  // Tokens at `key`, in the cluster.
-  auto count_at = [&](uint32_t key) {
-    uint64_t own = 0, all;
-    for (int at = tid; at < r.n; at += kThreads) own += r.key(at) == key;
-    scan_block(own, sh.scan, all);
-    if (tid == 0) sh.mass = all;
-    cluster.sync();
-    all = 0;
-    for (int b = 0; b < blocks; b++) all += cluster.map_shared_rank(&sh, b)->mass;
-    cluster.sync();
-    return all;
-  };
   // The sum of f over the cluster's tokens.
   auto sum_of = [&](auto&& f) {
     uint64_t own = 0, all;
@@ -217,8 +230,7 @@ __device__ void choose_over_row(cg::cluster_group& cluster, Shared& sh, const Sa
     scan_block(own, sh.scan, all);
     if (tid == 0) sh.mass = all;
     cluster.sync();
-    all = 0;
-    for (int b = 0; b < blocks; b++) all += cluster.map_shared_rank(&sh, b)->mass;
+    all = over_blocks(cluster, sh, [](const Shared& o) { return o.mass; });
     cluster.sync();
     return all;
   };
@@ -228,7 +240,7 @@ __device__ void choose_over_row(cg::cluster_group& cluster, Shared& sh, const Sa
     ties = (uint64_t)top_k - above;
   }
   if (top_p < 1.0f) {
-    const uint64_t each = r.weight(border == 1 ? 0 : border), tied = border == 1 ? 0 : count_at(border);
+    const uint64_t each = r.weight(border == 1 ? 0 : border), tied = border == 1 ? 0 : sum_of([&](uint32_t key) -> uint64_t { return key == border; });
     const uint64_t less = tied > ties ? (tied - ties) * each : 0;
     auto weight = [&](uint32_t key) { return key >= border ? r.weight(key) : 0; };
     const uint64_t total = sum_of(weight) - less, want = wanted_of(top_p, total);
@@ -247,7 +259,8 @@ __device__ void choose_over_row(cg::cluster_group& cluster, Shared& sh, const Sa
     tie0 = scan_block(own, sh.scan, all);
     if (tid == 0) sh.ties = (int)all;
     cluster.sync();
-    for (int b = 0; b < rank; b++) tie0 += (uint64_t)cluster.map_shared_rank(&sh, b)->ties;
+    over_blocks(cluster, sh, [](const Shared& o) { return o.ties; }, rank, all);
+    tie0 += all;
   }
   // Calls f(at, weight) for this thread's kept tokens.
   auto each_kept = [&](auto&& f) {
@@ -273,12 +286,10 @@ __device__ void choose_over_row(cg::cluster_group& cluster, Shared& sh, const Sa
     sh.count = (int)count;
   }
   cluster.sync();
-  mass = count = 0;
-  for (int b = 0; b < blocks; b++) {
-    if (b == rank) before += mass;
-    mass += cluster.map_shared_rank(&sh, b)->mass;
-    count += (uint64_t)cluster.map_shared_rank(&sh, b)->count;
-  }
+  uint64_t blocks_before;
+  mass = over_blocks(cluster, sh, [](const Shared& o) { return o.mass; }, rank, blocks_before);
+  before += blocks_before;
+  count = over_blocks(cluster, sh, [](const Shared& o) { return o.count; });
   cluster.sync();  // the others have read this block's
   const uint64_t target = target_of(u, mass);
   if (before <= target && target < before + own)
@@ -291,7 +302,7 @@ __device__ void choose_over_row(cg::cluster_group& cluster, Shared& sh, const Sa
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant__ SampleArgs a, int block_vecs) {
+__global__ void __launch_bounds__(kThreads, 4) sample_kernel(const __grid_constant__ SampleArgs a, int block_vecs) {
   pdl_launch_dependents();
   pdl_wait();
   constexpr int V = 16 / sizeof(T);
@@ -315,7 +326,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
     sh.head = sh.tail = 0;
     sh.first = INT32_MAX;
   }
-  sh.hist[tid] = 0;
+  sh.near[tid] = 0;
   float own = -INFINITY;  // this thread's largest
   constexpr int kAtOnce = 10;
   for (int v0 = tid; v0 < r.n / V; v0 += kThreads * kAtOnce) {
@@ -391,11 +402,13 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
     constexpr int kBase = (127 - 16) * 8;
     if (own > -INFINITY) {
       const int bin = (int)(__float_as_uint(r.largest - own) >> 20) - kBase;
-      atomicAdd(reinterpret_cast<unsigned long long*>(&sh.hist[min(max(bin, 0), kBins - 1)]), 1ull);
+      atomicAdd(&sh.near[min(max(bin, 0), kBins - 1)], 1u);
     }
     cluster.sync();
-    uint64_t bin_own = 0, all;
-    for (int b = 0; b < blocks; b++) bin_own += cluster.map_shared_rank(&sh, b)->hist[tid];
+    uint32_t bin_own = 0;
+#pragma unroll
+    for (int b = 0; b < kMaxBlocks; b++) bin_own += b < blocks ? cluster.map_shared_rank(&sh, b)->near[tid] : 0;
+    uint64_t all;
     const uint64_t before = scan_block(bin_own, sh.scan, all);
     if (tid == 0) sh.border_bin = kBins - 1;
     __syncthreads();
@@ -403,31 +416,57 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
     __syncthreads();
     if (sh.border_bin < kBins - 1) far = __uint_as_float((uint32_t)(sh.border_bin + kBase + 1) << 20);
   }
+  auto log2_weight = [&](float z) { return (z - r.largest) * per; };
+  // Calls f(place, logit) for this thread's tokens.
+  auto each_token = [&](auto&& f) {
+    for (int v = tid; v < r.n / V; v += kThreads) {
+      T e[V];
+      const uint4 raw = *reinterpret_cast<const uint4*>(x + v * V);
+      memcpy(e, &raw, 16);
+#pragma unroll
+      for (int j = 0; j < V; j++)
+        if (const float z = to_f32<T>(e[j]); z > -INFINITY) f(v * V + j, z);
+    }
+  };
   // min_p's cut may not touch what top_p sums. The margin is what f32 may be off by.
   float low = -INFINITY;  // log2 of a weight
   if (m && !p) low = log2f(min_p) * 1.00001f - 0.001f;
-  if (p && top_k == 0) low = kHead;
   const bool sums = p && top_k == 0;  // the rest of the row counts in top_p's sum
-  uint64_t tail = 0;
-  for (int v = tid; v < r.n / V; v += kThreads) {
-    T e[V];
-    const uint4 raw = *reinterpret_cast<const uint4*>(x + v * V);
-    memcpy(e, &raw, 16);
+  if (sums) {
+    // Weights in steps of 2^-16 by their log2, the small ones in the last bin.
+    each_token([&](int, float z) {
+      const float l = log2_weight(z);
+      const uint32_t w = __float2uint_rn(exp2f(l + 16.0f));
+      if (w != 0) atomicAdd(&sh.near[(int)min(-l, (float)(kLevels - 1))], w);
+    });
+    cluster.sync();
+    // A lane has a bin: enough are those that hold the share and a little more.
+    float bin_own = 0.0f;
 #pragma unroll
-    for (int j = 0; j < V; j++) {
-      const float z = to_f32<T>(e[j]), d = r.largest - z, log2w = -d * per;
-      if (!(z > -INFINITY)) continue;
-      if (!(d >= far) && !(log2w < low)) {
-        const int at = atomicAdd(&sh.listed, 1);
-        if (at < kListed) sh.list_at[at] = (uint16_t)(v * V + j);
-      } else if (sums) {
-        tail += __float2uint_rn(exp2f(log2w + 44.0f));
-      }
+    for (int b = 0; b < kMaxBlocks; b++)
+      if (b < blocks && lane < kLevels) bin_own += (float)cluster.map_shared_rank(&sh, b)->near[lane];
+    float upto = bin_own;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const float y = __shfl_up_sync(0xffffffffu, upto, off);
+      if (lane >= off) upto += y;
     }
+    const float whole = __shfl_sync(0xffffffffu, upto, 31);
+    const unsigned enough = __ballot_sync(0xffffffffu, upto >= (top_p + 0.002f) * whole);
+    low = -(float)min(enough != 0 ? __ffs(enough) : kLevels, kLevels - 1);
   }
+  uint64_t head = 0, tail = 0;
+  each_token([&](int place, float z) {
+    const float l = log2_weight(z);
+    if (!(r.largest - z >= far) && !(l < low)) {
+      const int at = atomicAdd(&sh.listed, 1);
+      if (at < kListed) sh.list_at[at] = (uint16_t)place;
+    } else if (sums) {
+      tail += l < kExact ? __float2uint_rn(exp2f(l + 44.0f)) : r.weight(key_of(z));
+    }
+  });
   __syncthreads();
   const int listed = min(sh.listed, kListed);
-  uint64_t head = 0;
   for (int i = tid; i < listed; i += kThreads) {
     const uint32_t key = r.key(sh.list_at[i]);
     const uint64_t w = r.weight(key);
@@ -444,16 +483,12 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
   }
   cluster.sync();
   // ---- whether the lists hold what matters
-  int total = 0, before_block = 0;
-  bool over = false;
-  head = tail = 0;
-  for (int b = 0; b < blocks; b++) {
-    const Shared* other = cluster.map_shared_rank(&sh, b);
-    const int count = other->listed;
-    if (count > kListed) over = true;
-    total += count;
-    head += other->head;
-    tail += other->tail;
+  uint64_t before_block;
+  const int total = (int)over_blocks(cluster, sh, [](const Shared& o) { return o.listed; }, rank, before_block);
+  const bool over = over_blocks(cluster, sh, [](const Shared& o) { return o.listed > kListed; }) != 0;
+  if (sums) {
+    head = over_blocks(cluster, sh, [](const Shared& o) { return o.head; });
+    tail = over_blocks(cluster, sh, [](const Shared& o) { return o.tail; });
   }
   if (over || total > kSorted || (sums && head < wanted_of(top_p, head + tail))) {
     cluster.sync();  // the lists have been read
@@ -461,23 +496,19 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
     return;
   }
   // ---- the first block sorts and decides, over its part of the row
-  uint64_t* by = reinterpret_cast<uint64_t*>(smem);
+  uint64_t* by = reinterpret_cast<uint64_t*>(cluster.map_shared_rank(smem, 0));
   uint64_t* with = by + kSorted;
   const int n2 = power_of_two(total);
-  if (rank == 0) {
-    for (int b = 0; b < blocks; b++) {
-      const Shared* other = cluster.map_shared_rank(&sh, b);
-      const int count = other->listed, token0 = b * block_vecs * V - shift;
-      for (int i = tid; i < count; i += kThreads) {
-        by[before_block + i] = (uint64_t)other->list_key[i] << 32 | (uint32_t)~(token0 + other->list_at[i]);
-        with[before_block + i] = other->list_weight[i];
-      }
-      before_block += count;
-    }
-    for (int i = total + tid; i < n2; i += kThreads) by[i] = with[i] = 0;
+  for (int i = tid; i < listed; i += kThreads) {
+    by[before_block + i] = (uint64_t)sh.list_key[i] << 32 | (uint32_t)~(r.first + (int)sh.list_at[i]);
+    with[before_block + i] = sh.list_weight[i];
   }
+  if (rank == 0)
+    for (int i = total + tid; i < n2; i += kThreads) by[i] = with[i] = 0;
   cluster.sync();
   if (rank != 0) return;
+  by = reinterpret_cast<uint64_t*>(smem);
+  with = by + kSorted;
   sort_block(by, with, n2);
   int kept = top_k > 0 ? min(top_k, total) : total;
   // Threads have contiguous places; `upto` is what lies before a thread's.
