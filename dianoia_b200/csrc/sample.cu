@@ -15,15 +15,14 @@
 //    histogram of their distance from the largest one: at least k tokens are as
 //    near as the k-th of these;
 //  - min_p: the weight says it;
-//  - top_p: the weights by their log2, roughly, in a histogram: as many of the
-//    largest as hold that share. The rest only adds to the sum (below 2^-20 from
-//    f32 exponentials, in the same steps).
-// Their weights (f64) and keys go to the first block's shared memory, which sorts
-// them and decides alone while the others leave. Where more tokens matter than its
-// lists hold (flat distributions, many ties, thousands of top_k) the border is
-// found eight bits of the key at a time over all of the row in the cluster's
-// shared memory; without a rule but the temperature every token has its f64
-// weight and the block that the random number falls to looks for the token.
+// Their weights and keys go to the first block's shared memory, which sorts them
+// and decides alone while the others leave. top_p alone may keep any number of
+// tokens: all weights go into a histogram by their log2, whose border bin's
+// tokens are the ones that are sorted; without a rule but the temperature there
+// is nothing to sort. Then every block knows what it keeps, and the one that the
+// random number falls to looks for the token. Where more tokens matter than the
+// lists hold (thousands of top_k, many ties) the border is found eight bits of the
+// key at a time over all of the row in the cluster's shared memory.
 #include <cooperative_groups.h>
 
 #include "dn_common.cuh"
@@ -43,9 +42,17 @@ constexpr int kListed = 512;    // tokens that a block lists
 constexpr int kSorted = 2048;   // that the first one sorts, over its part of the row
 constexpr int kMostK = 1536;    // top_k up to which the histogram is asked
 constexpr int kBins = 256;
-constexpr double kOne = 17592186044416.0;  // 2^44, the largest weight
-constexpr int kLevels = 24;      // log2 of the weights that top_p may list
-constexpr float kExact = -20.0f;  // log2 of the weights that count in f64
+constexpr int kSteps = 1024;      // bins of top_p's histogram,
+constexpr float kPerOctave = 32;  // so many to an octave of weights
+
+// The cluster's barrier counts whole warps: lanes that leave a loop a turn late
+// would be counted as there, their additions still to come (seen as sums that
+// lacked a few tokens). The block's own barrier waits for every thread.
+__device__ __forceinline__ void sync_all(cg::cluster_group& cluster) {
+  __syncthreads();
+  __syncwarp();
+  cluster.sync();
+}
 
 // Ordered as the floats are, -0 as +0; 0 for what is no token.
 __device__ __forceinline__ uint32_t key_of(float x) {
@@ -59,19 +66,32 @@ __device__ __forceinline__ float value_of(uint32_t key) {
 
 // What the blocks of a cluster read of one another.
 struct Shared {
-  uint64_t hist[kBins];
+  // A histogram's sums in three parts of 15 bits, which shared memory adds by
+  // itself (64-bit additions are loops there); the share's border tokens over it.
+  union {
+    uint32_t part[3][kSteps];
+    uint64_t sorted[kSteps];
+  };
   uint32_t near[kBins];
-  uint64_t list_weight[kListed];
   uint32_t list_key[kListed];
   uint16_t list_at[kListed];
   uint64_t scan[kWarps];  // of this block alone, as the next two
-  uint64_t head, tail;    // sums of the listed weights, and of the others
-  uint64_t mass;
-  uint32_t top;
+  uint64_t mass, border, rest;
+  uint32_t top, most, least;
   int listed, ties, count, first;
   int border_bin;  // of this block alone
   uint64_t border_above;
 };
+
+__device__ __forceinline__ void add_to_bin(Shared& sh, int bin, uint64_t w) {
+  const uint32_t low = (uint32_t)w & 0x7fff, mid = (uint32_t)(w >> 15) & 0x7fff, high = (uint32_t)(w >> 30);
+  if (low != 0) atomicAdd(&sh.part[0][bin], low);
+  if (mid != 0) atomicAdd(&sh.part[1][bin], mid);
+  if (high != 0) atomicAdd(&sh.part[2][bin], high);
+}
+__device__ __forceinline__ uint64_t bin_sum(const Shared& sh, int bin) {
+  return sh.part[0][bin] + ((uint64_t)sh.part[1][bin] << 15) + ((uint64_t)sh.part[2][bin] << 30);
+}
 
 // The sum over the cluster's blocks of f(what a block shares), the same in every
 // lane; the blocks before `upto` in `before`. A lane asks a block.
@@ -99,7 +119,7 @@ struct Row {
   const T* x;     // this block's part of the row
   int n, first;   // its elements (some before the row's begin or past its end hold -inf), the token of the first
   float largest;
-  double inv;     // 1 / temperature
+  double inv, per;  // 1 / temperature; of a logit, in log2 of a weight
   uint32_t top;
 
   __device__ __forceinline__ uint32_t key(int at) const { return key_of(to_f32<T>(x[at])); }
@@ -109,7 +129,31 @@ struct Row {
     if (key == 0 || isinf(largest)) return 0.0;
     return exp(((double)value_of(key) - (double)largest) * inv);
   }
-  __device__ __forceinline__ uint64_t weight(uint32_t key) const { return (uint64_t)__double2ull_rn(share(key) * kOne); }
+  // The same in steps of 2^-44, from the power series of 2^f about 0: |f| <= 1/2
+  // leaves (ln2 / 2)^12 / 12! = 2^-47 of it out. Half of exp's time, which it is
+  // all of (17 f64 operations a token).
+  __device__ __forceinline__ uint64_t weight(uint32_t key) const {
+    if (key == top) return (uint64_t)1 << 44;
+    const double t = ((double)value_of(key) - (double)largest) * per;  // log2
+    if (!(t > -46.0) || key == 0) return 0;
+    const double n = t + 6755399441055744.0;  // 1.5 2^52: the whole part lands in the low bits
+    const double f = t - (n - 6755399441055744.0);
+    double y = 4.44553827187081e-10;
+    y = fma(y, f, 7.054911620801121e-09);
+    y = fma(y, f, 1.0178086009239696e-07);
+    y = fma(y, f, 1.3215486790144305e-06);
+    y = fma(y, f, 1.5252733804059838e-05);
+    y = fma(y, f, 0.00015403530393381606);
+    y = fma(y, f, 0.0013333558146428441);
+    y = fma(y, f, 0.009618129107628477);
+    y = fma(y, f, 0.055504108664821576);
+    y = fma(y, f, 0.2402265069591007);
+    y = fma(y, f, 0.6931471805599453);
+    y = fma(y, f, 1.0);
+    // 2^(44 + n) by the exponent; then the nearest whole number by 2^52.
+    y = __hiloint2double(__double2hiint(y) + ((__double2loint(n) + 44) << 20), __double2loint(y));
+    return (uint64_t)__double_as_longlong(y + 4503599627370496.0) & 0xfffffffffffffull;
+  }
 };
 
 // The sum of s over the threads before this one, and over all of them in `all`.
@@ -135,6 +179,7 @@ __device__ __forceinline__ uint64_t scan_block(uint64_t s, uint64_t* warps, uint
 }
 
 // Sorts n (a power of two) pairs by their first, largest first.
+template <bool WITH>
 __device__ __forceinline__ void sort_block(uint64_t* by, uint64_t* with, int n) {
   for (int size = 2; size <= n; size <<= 1)
     for (int step = size / 2; step >= 1; step >>= 1) {
@@ -145,9 +190,11 @@ __device__ __forceinline__ void sort_block(uint64_t* by, uint64_t* with, int n) 
         if ((p < q) == ((lo & size) == 0)) {
           by[lo] = q;
           by[hi] = p;
-          const uint64_t w = with[lo];
-          with[lo] = with[hi];
-          with[hi] = w;
+          if constexpr (WITH) {
+            const uint64_t w = with[lo];
+            with[lo] = with[hi];
+            with[hi] = w;
+          }
         }
       }
     }
@@ -187,20 +234,18 @@ __device__ uint32_t border_of(cg::cluster_group& cluster, Shared& sh, const Row<
   uint32_t prefix = 0;
   above = 0;
   for (int shift = 24; shift >= 0; shift -= 8) {
-    sh.hist[tid] = 0;
+    for (int i = 0; i < 3; i++) sh.part[i][tid] = 0;
     __syncthreads();
     for (int at = tid; at < r.n; at += kThreads) {
       const uint32_t key = r.key(at);
-      if (key != 0 && (shift == 24 || key >> (shift + 8) == prefix))
-        if (const uint64_t part = f(key); part != 0)
-          atomicAdd(reinterpret_cast<unsigned long long*>(&sh.hist[key >> shift & 255]), (unsigned long long)part);
+      if (key != 0 && (shift == 24 || key >> (shift + 8) == prefix)) add_to_bin(sh, key >> shift & 255, f(key));
     }
-    cluster.sync();
+    sync_all(cluster);
     // Thread t has bin 255 - t: the sums before it are those above it.
     const int bin = 255 - tid;
     uint64_t own = 0;
 #pragma unroll
-    for (int b = 0; b < kMaxBlocks; b++) own += b < blocks ? cluster.map_shared_rank(&sh, b)->hist[bin] : 0;
+    for (int b = 0; b < kMaxBlocks; b++) own += b < blocks ? bin_sum(*cluster.map_shared_rank(&sh, b), bin) : 0;
     if (less != 0 && (shift == 24 || at_key >> (shift + 8) == prefix) && (int)(at_key >> shift & 255) == bin) own -= less;
     uint64_t all;
     const uint64_t before = above + scan_block(own, sh.scan, all);
@@ -208,39 +253,128 @@ __device__ uint32_t border_of(cg::cluster_group& cluster, Shared& sh, const Row<
       sh.border_bin = bin;
       sh.border_above = before;
     }
-    cluster.sync();  // and the block's own barrier
+    sync_all(cluster);  // and the block's own barrier
     prefix = prefix << 8 | (uint32_t)sh.border_bin;
     above = sh.border_above;
   }
   return prefix;
 }
 
+// Finds the token where the random number falls among the kept ones: `kept` of
+// (key, place), asked of a thread's contiguous tokens in order. before: the mass
+// before this block's, own: its own (both by whole blocks).
+template <typename T, typename F>
+__device__ void look_in_block(Shared& sh, const SampleArgs& a, int64_t row, const Row<T>& r, uint64_t before, uint64_t mass,
+                              uint64_t target, int count, F&& kept) {
+  const int each = (r.n + kThreads - 1) / kThreads, begin = min(r.n, (int)threadIdx.x * each), end = min(r.n, begin + each);
+  uint64_t own = 0, all;
+  for (int at = begin; at < end; at++) {
+    const uint32_t key = r.key(at);
+    if (kept(key, at)) own += r.weight(key);
+  }
+  before += scan_block(own, sh.scan, all);
+  if (!(before <= target && target < before + own)) return;
+  for (int at = begin; at < end; at++) {
+    const uint32_t key = r.key(at);
+    if (!kept(key, at)) continue;
+    const uint64_t w = r.weight(key);
+    before += w;
+    if (before > target) {
+      answer(a, row, r.first + at, log_share(w, mass), count);
+      return;
+    }
+  }
+}
+
+// The token among those whose keys are above `border`, the first `ties` of those
+// at it, less what min_p leaves out. Returns after the answer is written.
+template <typename T>
+__device__ void choose_by_border(cg::cluster_group& cluster, Shared& sh, const SampleArgs& a, int64_t row, const Row<T>& r,
+                                 uint32_t border, uint64_t ties, float min_p, float u) {
+  const int tid = threadIdx.x, rank = (int)cluster.block_rank();
+  // Threads have contiguous tokens, blocks and threads in index order.
+  const int each = (r.n + kThreads - 1) / kThreads, begin = min(r.n, tid * each), end = min(r.n, begin + each);
+  uint64_t all;
+  int last = INT32_MAX;  // the place of this thread's last tie that is in
+  if (ties != ~0ull) {
+    uint64_t own = 0;
+    for (int at = begin; at < end; at++) own += r.key(at) == border;
+    uint64_t before = scan_block(own, sh.scan, all), of_blocks;
+    if (tid == 0) sh.ties = (int)all;
+    sync_all(cluster);
+    over_blocks(cluster, sh, [](const Shared& o) { return o.ties; }, rank, of_blocks);
+    before += of_blocks;
+    if (before >= ties) {
+      last = -1;
+    } else if (before + own > ties) {
+      for (int at = begin; at < end; at++)
+        if (r.key(at) == border && before++ < ties) last = at;
+    }
+  }
+  auto kept = [&](uint32_t key, int at) {
+    return key != 0 && (key > border || (key == border && at <= last)) &&
+           (key == r.top || !(min_p > 0.0f) || r.share(key) >= (double)min_p);
+  };
+  uint64_t own = 0, count = 0;
+  for (int at = begin; at < end; at++) {
+    const uint32_t key = r.key(at);
+    if (!kept(key, at)) continue;
+    own += r.weight(key);
+    count++;
+  }
+  uint64_t counts;
+  scan_block(count, sh.scan, counts);
+  uint64_t before = scan_block(own, sh.scan, all);
+  if (tid == 0) {
+    sh.mass = all;
+    sh.count = (int)counts;
+  }
+  sync_all(cluster);
+  uint64_t of_blocks;
+  const uint64_t mass = over_blocks(cluster, sh, [](const Shared& o) { return o.mass; }, rank, of_blocks);
+  counts = over_blocks(cluster, sh, [](const Shared& o) { return o.count; });
+  sync_all(cluster);  // the others have read this block's
+  before += of_blocks;
+  const uint64_t target = target_of(u, mass);
+  if (!(before <= target && target < before + own)) return;
+  for (int at = begin; at < end; at++) {
+    const uint32_t key = r.key(at);
+    if (!kept(key, at)) continue;
+    const uint64_t w = r.weight(key);
+    before += w;
+    if (before > target) {
+      answer(a, row, r.first + at, log_share(w, mass), (int)counts);
+      return;
+    }
+  }
+}
+
 // Any rules, over the whole row. Returns after the answer is written.
 template <typename T>
 __device__ void choose_over_row(cg::cluster_group& cluster, Shared& sh, const SampleArgs& a, int64_t row, const Row<T>& r,
                                 int top_k, float top_p, float min_p, float u) {
-  const int tid = threadIdx.x, rank = (int)cluster.block_rank();
-  uint32_t border = 1;       // tokens below it are out,
-  uint64_t ties = ~0ull;     // of those at it the first so many are in
-  auto one = [](uint32_t) -> uint64_t { return 1; };
+  const int tid = threadIdx.x;
+  uint32_t border = 1;    // tokens below it are out,
+  uint64_t ties = ~0ull;  // of those at it the first so many are in
   // The sum of f over the cluster's tokens.
   auto sum_of = [&](auto&& f) {
     uint64_t own = 0, all;
     for (int at = tid; at < r.n; at += kThreads) own += f(r.key(at));
     scan_block(own, sh.scan, all);
     if (tid == 0) sh.mass = all;
-    cluster.sync();
+    sync_all(cluster);
     all = over_blocks(cluster, sh, [](const Shared& o) { return o.mass; });
-    cluster.sync();
+    sync_all(cluster);
     return all;
   };
   if (top_k > 0 && sum_of([](uint32_t key) -> uint64_t { return key != 0; }) > (uint64_t)top_k) {
     uint64_t above;
-    border = border_of(cluster, sh, r, (uint64_t)top_k, above, one, 0, 0);
+    border = border_of(cluster, sh, r, (uint64_t)top_k, above, [](uint32_t) -> uint64_t { return 1; }, 0, 0);
     ties = (uint64_t)top_k - above;
   }
   if (top_p < 1.0f) {
-    const uint64_t each = r.weight(border == 1 ? 0 : border), tied = border == 1 ? 0 : sum_of([&](uint32_t key) -> uint64_t { return key == border; });
+    const uint64_t each = border == 1 ? 0 : r.weight(border);
+    const uint64_t tied = border == 1 ? 0 : sum_of([&](uint32_t key) -> uint64_t { return key == border; });
     const uint64_t less = tied > ties ? (tied - ties) * each : 0;
     auto weight = [&](uint32_t key) { return key >= border ? r.weight(key) : 0; };
     const uint64_t total = sum_of(weight) - less, want = wanted_of(top_p, total);
@@ -250,55 +384,158 @@ __device__ void choose_over_row(cg::cluster_group& cluster, Shared& sh, const Sa
     if (at > border || need < ties) ties = need;
     border = at;
   }
-  // Threads have contiguous tokens from here on, blocks and threads in index order.
-  const int each = (r.n + kThreads - 1) / kThreads, begin = min(r.n, tid * each), end = min(r.n, begin + each);
-  uint64_t tie0 = 0;  // ties before this thread's
-  if (ties != ~0ull) {
-    uint64_t own = 0, all;
-    for (int at = begin; at < end; at++) own += r.key(at) == border;
-    tie0 = scan_block(own, sh.scan, all);
-    if (tid == 0) sh.ties = (int)all;
-    cluster.sync();
-    over_blocks(cluster, sh, [](const Shared& o) { return o.ties; }, rank, all);
-    tie0 += all;
-  }
-  // Calls f(at, weight) for this thread's kept tokens.
-  auto each_kept = [&](auto&& f) {
-    uint64_t tie = tie0;
-    for (int at = begin; at < end; at++) {
-      const uint32_t key = r.key(at);
-      if (key == 0 || key < border || (key == border && tie++ >= ties)) continue;
-      const double share = r.share(key);
-      if (key != r.top && min_p > 0.0f && share < (double)min_p) continue;
-      if (f(at, (uint64_t)__double2ull_rn(share * kOne))) break;
-    }
+  choose_by_border(cluster, sh, a, row, r, border, ties, min_p, u);
+}
+
+// top_p alone.
+template <typename T>
+__device__ void choose_by_share(cg::cluster_group& cluster, Shared& sh, const SampleArgs& a, int64_t row,
+                                const Row<T>& r, float top_p, float u) {
+  const int tid = threadIdx.x, blocks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+  constexpr int kOwn = kSteps / kThreads;  // bins of a thread
+  const float per = (float)r.per;
+  auto bin_of = [&](uint32_t key) {
+    return key == r.top ? 0 : (int)fminf((r.largest - value_of(key)) * per * kPerOctave, (float)(kSteps - 1));
   };
-  uint64_t own = 0, kept = 0, mass, count;
-  each_kept([&](int, uint64_t w) {
-    own += w;
-    kept++;
-    return false;
-  });
-  uint64_t before = scan_block(own, sh.scan, mass);
-  scan_block(kept, sh.scan, count);
+#pragma unroll
+  for (int i = 0; i < 3 * kOwn; i++) sh.part[i / kOwn][tid * kOwn + i % kOwn] = 0;
   if (tid == 0) {
-    sh.mass = mass;
-    sh.count = (int)count;
+    sh.most = 0;
+    sh.least = ~0u;
   }
-  cluster.sync();
-  uint64_t blocks_before;
-  mass = over_blocks(cluster, sh, [](const Shared& o) { return o.mass; }, rank, blocks_before);
-  before += blocks_before;
-  count = over_blocks(cluster, sh, [](const Shared& o) { return o.count; });
-  cluster.sync();  // the others have read this block's
+  __syncthreads();
+  uint64_t rest = 0, all;  // of the last bin, where most tokens may be
+  for (int at = tid; at < r.n; at += kThreads) {
+    const uint32_t key = r.key(at);
+    const uint64_t w = r.weight(key);
+    if (w == 0) continue;
+    if (const int bin = bin_of(key); bin < kSteps - 1) add_to_bin(sh, bin, w);
+    else rest += w;
+  }
+  scan_block(rest, sh.scan, all);
+  if (tid == 0) sh.rest = all;
+  sync_all(cluster);
+  uint64_t bins[kOwn] = {}, own = 0, total;
+#pragma unroll
+  for (int i = 0; i < kOwn; i++) {
+#pragma unroll
+    for (int b = 0; b < kMaxBlocks; b++) bins[i] += b < blocks ? bin_sum(*cluster.map_shared_rank(&sh, b), tid * kOwn + i) : 0;
+    own += bins[i];
+  }
+  rest = over_blocks(cluster, sh, [](const Shared& o) { return o.rest; });
+  if (tid == kThreads - 1) {
+    bins[kOwn - 1] += rest;
+    own += rest;
+  }
+  uint64_t run = scan_block(own, sh.scan, total);
+  const uint64_t want = wanted_of(top_p, total);
+#pragma unroll
+  for (int i = 0; i < kOwn; i++) {
+    if (run < want && run + bins[i] >= want) {
+      sh.border_bin = tid * kOwn + i;
+      sh.border_above = run;
+    }
+    run += bins[i];
+  }
+  __syncthreads();
+  const int border_bin = sh.border_bin;
+  const uint64_t above = sh.border_above;
+  // The border bin's tokens in a list, those above it counted.
+  uint64_t count = 0, counts, kept_above = 0;
+  uint32_t most = 0, least = ~0u;
+  for (int at = tid; at < r.n; at += kThreads) {
+    const uint32_t key = r.key(at);
+    if (key == 0) continue;
+    const int bin = bin_of(key);
+    count += bin < border_bin;
+    if (bin != border_bin) continue;
+    most = max(most, key);
+    least = min(least, key);
+    const int place = atomicAdd(&sh.listed, 1);
+    if (place < kListed) sh.list_at[place] = (uint16_t)at;
+  }
+  most = __reduce_max_sync(0xffffffffu, most);
+  least = __reduce_min_sync(0xffffffffu, least);
+  if (tid % 32 == 0) {
+    atomicMax(&sh.most, most);
+    atomicMin(&sh.least, least);
+  }
+#pragma unroll
+  for (int i = 0; i < kOwn; i++)
+    if (tid * kOwn + i < border_bin) kept_above += bin_sum(sh, tid * kOwn + i);
+  scan_block(count, sh.scan, counts);
+  scan_block(kept_above, sh.scan, kept_above);
+  const int listed = min(sh.listed, kListed);
+  for (int i = tid; i < listed; i += kThreads) sh.list_key[i] = r.key(sh.list_at[i]);
+  sync_all(cluster);
+  uint64_t before_block;
+  const int in_bin = (int)over_blocks(cluster, sh, [](const Shared& o) { return o.listed; }, rank, before_block);
+  if (over_blocks(cluster, sh, [](const Shared& o) { return o.listed > kListed; }) != 0 || in_bin > kSteps) {
+    uint64_t unused;
+    const uint64_t same_top = over_blocks(cluster, sh, [](const Shared& o) { return o.listed > 0 && o.most != o.least; });
+    // Keys that differ between blocks: the sums of the listed blocks' keys tell.
+    const uint64_t some = over_blocks(cluster, sh, [](const Shared& o) { return o.listed > 0; });
+    const uint64_t keys = over_blocks(cluster, sh, [](const Shared& o) { return o.listed > 0 ? (uint64_t)o.most : 0; }, rank, unused);
+    const uint32_t key = (uint32_t)(keys / some);
+    const uint64_t others = over_blocks(cluster, sh, [&](const Shared& o) { return o.listed > 0 && o.most != key; });
+    sync_all(cluster);  // the lists have been read
+    if (same_top == 0 && others == 0) {  // ties of one key
+      const uint64_t w = r.weight(key);
+      choose_by_border(cluster, sh, a, row, r, key, (want - above + w - 1) / w, 0.0f, u);
+    } else {
+      choose_over_row(cluster, sh, a, row, r, 0, top_p, 0.0f, u);
+    }
+    return;
+  }
+  uint64_t* by = cluster.map_shared_rank(&sh, 0)->sorted;  // over what has been read; the row is still needed
+  const int n2 = power_of_two(in_bin);
+  for (int i = tid; i < listed; i += kThreads)
+    by[before_block + i] = (uint64_t)sh.list_key[i] << 32 | (uint32_t)~(r.first + (int)sh.list_at[i]);
+  if (rank == 0)
+    for (int i = in_bin + tid; i < n2; i += kThreads) by[i] = 0;
+  sync_all(cluster);
+  if (rank == 0) {
+    sort_block<false>(sh.sorted, nullptr, n2);
+    const int each = (n2 + kThreads - 1) / kThreads, begin = min(n2, tid * each), end = min(n2, begin + each);
+    auto weight_at = [&](int i) { return r.weight((uint32_t)(sh.sorted[i] >> 32)); };
+    uint64_t sum = 0;
+    for (int i = begin; i < end; i++) sum += weight_at(i);
+    uint64_t upto = above + scan_block(sum, sh.scan, all);
+    if (upto < want && upto + sum >= want)
+      for (int i = begin; i < end; i++) {
+        upto += weight_at(i);
+        if (upto >= want) {
+          sh.border = sh.sorted[i];
+          break;
+        }
+      }
+  }
+  sync_all(cluster);
+  const uint64_t border = cluster.map_shared_rank(&sh, 0)->border;
+  auto composite = [&](uint32_t key, int at) { return (uint64_t)key << 32 | (uint32_t)~(r.first + at); };
+  uint64_t band = 0, band_count = 0;
+  for (int i = tid; i < listed; i += kThreads)
+    if (composite(sh.list_key[i], sh.list_at[i]) >= border) {
+      band += r.weight(sh.list_key[i]);
+      band_count++;
+    }
+  scan_block(band, sh.scan, all);
+  kept_above += all;
+  scan_block(band_count, sh.scan, all);
+  counts += all;
+  if (tid == 0) {
+    sh.mass = kept_above;
+    sh.count = (int)counts;
+  }
+  sync_all(cluster);
+  uint64_t before;
+  const uint64_t mass = over_blocks(cluster, sh, [](const Shared& o) { return o.mass; }, rank, before);
+  counts = over_blocks(cluster, sh, [](const Shared& o) { return o.count; });
+  sync_all(cluster);  // the others have read this block's
   const uint64_t target = target_of(u, mass);
-  if (before <= target && target < before + own)
-    each_kept([&](int at, uint64_t w) {
-      before += w;
-      if (before <= target) return false;
-      answer(a, row, r.first + at, log_share(w, mass), (int)count);
-      return true;
-    });
+  if (before <= target && target < before + kept_above)
+    look_in_block(sh, a, row, r, before, mass, target, (int)counts,
+                  [&](uint32_t key, int at) { return composite(key, at) >= border; });
 }
 
 template <typename T>
@@ -323,7 +560,6 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const __grid_consta
   if (tid == 0) {
     sh.top = 0;
     sh.listed = 0;
-    sh.head = sh.tail = 0;
     sh.first = INT32_MAX;
   }
   sh.near[tid] = 0;
@@ -358,7 +594,7 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const __grid_consta
   __syncthreads();
   const uint32_t warp_top = __reduce_max_sync(0xffffffffu, key_of(own));
   if (lane == 0) atomicMax(&sh.top, warp_top);
-  cluster.sync();
+  sync_all(cluster);
   uint32_t top = lane < blocks ? cluster.map_shared_rank(&sh, lane)->top : 0;
   r.top = top = __reduce_max_sync(0xffffffffu, top);
   r.largest = value_of(top);
@@ -373,6 +609,7 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const __grid_consta
   const float u = how.uniform[row];
   const bool p = top_p < 1.0f, m = min_p > 0.0f;
   r.inv = 1.0 / (double)temperature;
+  r.per = r.inv * 1.4426950408889634;
 
   if (top == 0 || !(temperature > 0.0f) || min_p > 1.0f) {  // no token, or the first one alone
     if (top != 0) {
@@ -382,18 +619,25 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const __grid_consta
       least = __reduce_min_sync(0xffffffffu, least);
       if (lane == 0 && least != INT32_MAX) atomicMin(&first->first, least);
     }
-    cluster.sync();
+    sync_all(cluster);
     if (rank == 0 && tid == 0) {
       if (top == 0) answer(a, row, -1, -INFINITY, 0);
       else answer(a, row, sh.first, 0.0f, 1);
     }
     return;
   }
-  const float per = (float)(1.4426950408889634 * r.inv);  // weights' log2 of a logit
-  if ((top_k == 0 && !p && !m) || top_k > kMostK || isinf(r.largest)) {
+  if (top_k > kMostK || isinf(r.largest) || (top_k == 0 && p && m)) {
     choose_over_row(cluster, sh, a, row, r, top_k, top_p, min_p, u);
     return;
   }
+  if (top_k == 0 && !m) {
+    if (p)
+      choose_by_share(cluster, sh, a, row, r, top_p, u);
+    else
+      choose_by_border(cluster, sh, a, row, r, 1, ~0ull, 0.0f, u);
+    return;
+  }
+  const float per = (float)r.per;
 
   // ---- how far below the largest a token may be and matter
   float far = NAN;  // in logits; NaN: any distance, an infinite one too
@@ -404,7 +648,7 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const __grid_consta
       const int bin = (int)(__float_as_uint(r.largest - own) >> 20) - kBase;
       atomicAdd(&sh.near[min(max(bin, 0), kBins - 1)], 1u);
     }
-    cluster.sync();
+    sync_all(cluster);
     uint32_t bin_own = 0;
 #pragma unroll
     for (int b = 0; b < kMaxBlocks; b++) bin_own += b < blocks ? cluster.map_shared_rank(&sh, b)->near[tid] : 0;
@@ -416,7 +660,6 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const __grid_consta
     __syncthreads();
     if (sh.border_bin < kBins - 1) far = __uint_as_float((uint32_t)(sh.border_bin + kBase + 1) << 20);
   }
-  auto log2_weight = [&](float z) { return (z - r.largest) * per; };
   // Calls f(place, logit) for this thread's tokens.
   auto each_token = [&](auto&& f) {
     for (int v = tid; v < r.n / V; v += kThreads) {
@@ -431,67 +674,22 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const __grid_consta
   // min_p's cut may not touch what top_p sums. The margin is what f32 may be off by.
   float low = -INFINITY;  // log2 of a weight
   if (m && !p) low = log2f(min_p) * 1.00001f - 0.001f;
-  const bool sums = p && top_k == 0;  // the rest of the row counts in top_p's sum
-  if (sums) {
-    // Weights in steps of 2^-16 by their log2, the small ones in the last bin.
-    each_token([&](int, float z) {
-      const float l = log2_weight(z);
-      const uint32_t w = __float2uint_rn(exp2f(l + 16.0f));
-      if (w != 0) atomicAdd(&sh.near[(int)min(-l, (float)(kLevels - 1))], w);
-    });
-    cluster.sync();
-    // A lane has a bin: enough are those that hold the share and a little more.
-    float bin_own = 0.0f;
-#pragma unroll
-    for (int b = 0; b < kMaxBlocks; b++)
-      if (b < blocks && lane < kLevels) bin_own += (float)cluster.map_shared_rank(&sh, b)->near[lane];
-    float upto = bin_own;
-#pragma unroll
-    for (int off = 1; off < 32; off <<= 1) {
-      const float y = __shfl_up_sync(0xffffffffu, upto, off);
-      if (lane >= off) upto += y;
-    }
-    const float whole = __shfl_sync(0xffffffffu, upto, 31);
-    const unsigned enough = __ballot_sync(0xffffffffu, upto >= (top_p + 0.002f) * whole);
-    low = -(float)min(enough != 0 ? __ffs(enough) : kLevels, kLevels - 1);
-  }
-  uint64_t head = 0, tail = 0;
   each_token([&](int place, float z) {
-    const float l = log2_weight(z);
-    if (!(r.largest - z >= far) && !(l < low)) {
+    if (!(r.largest - z >= far) && !((z - r.largest) * per < low)) {
       const int at = atomicAdd(&sh.listed, 1);
       if (at < kListed) sh.list_at[at] = (uint16_t)place;
-    } else if (sums) {
-      tail += l < kExact ? __float2uint_rn(exp2f(l + 44.0f)) : r.weight(key_of(z));
     }
   });
   __syncthreads();
   const int listed = min(sh.listed, kListed);
-  for (int i = tid; i < listed; i += kThreads) {
-    const uint32_t key = r.key(sh.list_at[i]);
-    const uint64_t w = r.weight(key);
-    sh.list_key[i] = key;
-    sh.list_weight[i] = w;
-    head += w;
-  }
-  if (sums) {
-    uint64_t all;
-    scan_block(head, sh.scan, all);
-    if (tid == 0) sh.head = all;
-    scan_block(tail, sh.scan, all);
-    if (tid == 0) sh.tail = all;
-  }
-  cluster.sync();
+  for (int i = tid; i < listed; i += kThreads) sh.list_key[i] = r.key(sh.list_at[i]);
+  sync_all(cluster);
   // ---- whether the lists hold what matters
   uint64_t before_block;
   const int total = (int)over_blocks(cluster, sh, [](const Shared& o) { return o.listed; }, rank, before_block);
   const bool over = over_blocks(cluster, sh, [](const Shared& o) { return o.listed > kListed; }) != 0;
-  if (sums) {
-    head = over_blocks(cluster, sh, [](const Shared& o) { return o.head; });
-    tail = over_blocks(cluster, sh, [](const Shared& o) { return o.tail; });
-  }
-  if (over || total > kSorted || (sums && head < wanted_of(top_p, head + tail))) {
-    cluster.sync();  // the lists have been read
+  if (over || total > kSorted) {
+    sync_all(cluster);  // the lists have been read
     choose_over_row(cluster, sh, a, row, r, top_k, top_p, min_p, u);
     return;
   }
@@ -501,15 +699,15 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const __grid_consta
   const int n2 = power_of_two(total);
   for (int i = tid; i < listed; i += kThreads) {
     by[before_block + i] = (uint64_t)sh.list_key[i] << 32 | (uint32_t)~(r.first + (int)sh.list_at[i]);
-    with[before_block + i] = sh.list_weight[i];
+    with[before_block + i] = r.weight(sh.list_key[i]);
   }
   if (rank == 0)
     for (int i = total + tid; i < n2; i += kThreads) by[i] = with[i] = 0;
-  cluster.sync();
+  sync_all(cluster);
   if (rank != 0) return;
   by = reinterpret_cast<uint64_t*>(smem);
   with = by + kSorted;
-  sort_block(by, with, n2);
+  sort_block<true>(by, with, n2);
   int kept = top_k > 0 ? min(top_k, total) : total;
   // Threads have contiguous places; `upto` is what lies before a thread's.
   const int each = (n2 + kThreads - 1) / kThreads, begin = min(n2, tid * each), end = min(n2, begin + each);
@@ -517,7 +715,7 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const __grid_consta
     uint64_t sum = 0, all;
     for (int i = begin; i < end; i++)
       if (i < kept) sum += with[i];
-    const uint64_t upto = scan_block(sum, sh.scan, all), want = wanted_of(top_p, all + tail);
+    const uint64_t upto = scan_block(sum, sh.scan, all), want = wanted_of(top_p, all);
     if (tid == 0) sh.count = kept;
     __syncthreads();
     if (upto < want && upto + sum >= want) {
@@ -550,7 +748,7 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const __grid_consta
     by[i] = i < kept ? by[i] & 0xffffffffu : 0;  // the complement of the token
     with[i] = i < kept ? with[i] : 0;
   }
-  sort_block(by, with, k2);
+  sort_block<true>(by, with, k2);
   const int per_thread = (k2 + kThreads - 1) / kThreads, from = min(k2, tid * per_thread), to = min(k2, from + per_thread);
   uint64_t sum = 0, mass;
   for (int i = from; i < to; i++) sum += with[i];

@@ -243,3 +243,17 @@ def test_shares(cuda_lib):
     for v in range(6):
         assert abs(tokens.count(v) - 4096 * w[v] / w.sum()) <= 1
     assert tokens == sorted(tokens) and kept == [4] * 4096
+
+
+@pytest.mark.parametrize("kind,vocab", [("f32", 4097), ("f16", 50257), ("bf16", 4100), ("f32", 151937)])
+def test_cuts_of_many_tokens_repeat(cuda_lib, kind, vocab):
+    """top_k over what the lists hold, with top_p's border on top: rows whose last tokens are few lanes' alone, the same
+    every time."""
+    n = 8
+    x = logits_of(kind, n, vocab, 7)
+    for k in (800, 1600, 3000):
+        for p in (0.5, 0.99):
+            rules = {"u": [0.3] * n, "top_k": [k] * n, "top_p": [p] * n}
+            first = check(cuda_lib, x, rules)
+            for _ in range(4):
+                assert run(cuda_lib, x, rules) == first
