@@ -130,29 +130,54 @@ struct Row {
     return exp(((double)value_of(key) - (double)largest) * inv);
   }
   // The same in steps of 2^-44, from the power series of 2^f about 0: |f| <= 1/2
-  // leaves (ln2 / 2)^12 / 12! = 2^-47 of it out. Half of exp's time, which it is
-  // all of (17 f64 operations a token).
+  // leaves (ln2 / 2)^12 / 12! = 2^-47 of it out. A few keys side by side: a chain
+  // of f64 operations is long (one at a time 151936 tokens take twice as long).
+  template <int N>
+  __device__ __forceinline__ void weights(const uint32_t (&key)[N], uint64_t (&w)[N]) const {
+    constexpr double kSeries[12] = {1.0, 0.6931471805599453, 0.2402265069591007, 0.055504108664821576, 0.009618129107628477, 0.0013333558146428441, 0.00015403530393381606, 1.5252733804059838e-05, 1.3215486790144305e-06, 1.0178086009239696e-07, 7.054911620801121e-09, 4.44553827187081e-10};
+    constexpr double kWhole = 6755399441055744.0;  // 1.5 2^52: the whole part of a sum lands in the low bits
+    double t[N], n[N], f[N], y[N];
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      t[i] = ((double)value_of(key[i]) - (double)largest) * per;  // log2
+      n[i] = t[i] + kWhole;
+      f[i] = t[i] - (n[i] - kWhole);
+      y[i] = kSeries[11];
+    }
+#pragma unroll
+    for (int k = 10; k >= 0; k--)
+#pragma unroll
+      for (int i = 0; i < N; i++) y[i] = fma(y[i], f[i], kSeries[k]);
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      // 2^(44 + n) by the exponent; then the nearest whole number by 2^52.
+      const int up = __double2loint(n[i]) + 44;
+      y[i] = __hiloint2double(__double2hiint(y[i]) + up * (1 << 20), __double2loint(y[i]));
+      w[i] = (uint64_t)__double_as_longlong(y[i] + 4503599627370496.0) & 0xfffffffffffffull;
+      if (!(t[i] > -46.0) || key[i] == 0) w[i] = 0;
+      if (key[i] == top) w[i] = (uint64_t)1 << 44;
+    }
+  }
   __device__ __forceinline__ uint64_t weight(uint32_t key) const {
-    if (key == top) return (uint64_t)1 << 44;
-    const double t = ((double)value_of(key) - (double)largest) * per;  // log2
-    if (!(t > -46.0) || key == 0) return 0;
-    const double n = t + 6755399441055744.0;  // 1.5 2^52: the whole part lands in the low bits
-    const double f = t - (n - 6755399441055744.0);
-    double y = 4.44553827187081e-10;
-    y = fma(y, f, 7.054911620801121e-09);
-    y = fma(y, f, 1.0178086009239696e-07);
-    y = fma(y, f, 1.3215486790144305e-06);
-    y = fma(y, f, 1.5252733804059838e-05);
-    y = fma(y, f, 0.00015403530393381606);
-    y = fma(y, f, 0.0013333558146428441);
-    y = fma(y, f, 0.009618129107628477);
-    y = fma(y, f, 0.055504108664821576);
-    y = fma(y, f, 0.2402265069591007);
-    y = fma(y, f, 0.6931471805599453);
-    y = fma(y, f, 1.0);
-    // 2^(44 + n) by the exponent; then the nearest whole number by 2^52.
-    y = __hiloint2double(__double2hiint(y) + ((__double2loint(n) + 44) << 20), __double2loint(y));
-    return (uint64_t)__double_as_longlong(y + 4503599627370496.0) & 0xfffffffffffffull;
+    const uint32_t keys[1] = {key};
+    uint64_t w[1];
+    weights(keys, w);
+    return w[0];
+  }
+  // Calls f(place, key, weight) for places at0, at0 + step, .. below end, in order.
+  template <typename F>
+  __device__ __forceinline__ void each_weight(int at0, int end, int step, F&& f) const {
+    constexpr int N = 4;
+    for (int at = at0; at < end; at += N * step) {
+      uint32_t k[N];
+      uint64_t w[N];
+#pragma unroll
+      for (int i = 0; i < N; i++) k[i] = at + i * step < end ? key(at + i * step) : 0;
+      weights(k, w);
+#pragma unroll
+      for (int i = 0; i < N; i++)
+        if (k[i] != 0) f(at + i * step, k[i], w[i]);
+    }
   }
 };
 
@@ -223,6 +248,57 @@ __device__ __forceinline__ float log_share(uint64_t weight, uint64_t mass) {
   return weight == mass ? 0.0f : (float)log((double)weight / (double)mass);
 }
 
+// Of the histograms that the cluster's blocks have in the first `bins` of theirs
+// (a power of two; `more` at the last bin besides), the bin in which the sum over
+// the bins before and with it, and `base`, comes to want(whole sum); above: the sum
+// before it. Every block sums a part of the bins over the blocks.
+template <typename F>
+__device__ int border_bin(cg::cluster_group& cluster, Shared& sh, int bins, uint64_t base, uint64_t more, int less_at,
+                          uint64_t less, F&& want_of, uint64_t& want, uint64_t& above) {
+  const int tid = threadIdx.x, lane = tid % 32, blocks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+  const int share = bins / blocks, per = max(1, share / kThreads), first = rank * share + tid * per;
+  uint64_t own[kSteps / kThreads], sum = 0, all;
+#pragma unroll
+  for (int i = 0; i < kSteps / kThreads; i++) {
+    own[i] = 0;
+    if (i >= per || tid * per + i >= share) continue;
+    const int bin = first + i;
+#pragma unroll
+    for (int b = 0; b < kMaxBlocks; b++) own[i] += b < blocks ? bin_sum(*cluster.map_shared_rank(&sh, b), bin) : 0;
+    own[i] += bin == bins - 1 ? more : 0;
+    own[i] -= bin == less_at ? less : 0;
+    sum += own[i];
+  }
+  uint64_t run = scan_block(sum, sh.scan, all);
+  if (tid == 0) sh.mass = all;
+  sync_all(cluster);
+  const uint64_t part = lane < blocks ? cluster.map_shared_rank(&sh, lane)->mass : 0;
+  uint64_t upto = part;
+#pragma unroll
+  for (int off = 1; off < kMaxBlocks; off <<= 1) {
+    const uint64_t y = __shfl_up_sync(0xffffffffu, upto, off);
+    if (lane >= off) upto += y;
+  }
+  want = want_of(__shfl_sync(0xffffffffu, upto, kMaxBlocks - 1));
+  const uint64_t before = base + upto - part;
+  const int owner = __ffs(__ballot_sync(0xffffffffu, lane < blocks && before < want && before + part >= want)) - 1;
+  run += __shfl_sync(0xffffffffu, before, rank);
+  if (owner == rank) {
+#pragma unroll
+    for (int i = 0; i < kSteps / kThreads; i++) {
+      if (run < want && run + own[i] >= want) {
+        sh.border_bin = first + i;
+        sh.border_above = run;
+      }
+      run += own[i];
+    }
+  }
+  sync_all(cluster);
+  const Shared* other = cluster.map_shared_rank(&sh, max(owner, 0));
+  above = other->border_above;
+  return other->border_bin;
+}
+
 // The largest key from which on f (counts or weights) sum to at least `want`
 // over the row, eight bits at a time, and the sum of the keys above it. `f`
 // gives a key's part of the sum; `less` of the sum is left out at key `at_key`.
@@ -230,32 +306,23 @@ __device__ __forceinline__ float log_share(uint64_t weight, uint64_t mass) {
 template <typename T, typename F>
 __device__ uint32_t border_of(cg::cluster_group& cluster, Shared& sh, const Row<T>& r, uint64_t want, uint64_t& above, F&& f,
                               uint32_t at_key, uint64_t less) {
-  const int tid = threadIdx.x, blocks = (int)cluster.num_blocks();
+  const int tid = threadIdx.x;
   uint32_t prefix = 0;
   above = 0;
   for (int shift = 24; shift >= 0; shift -= 8) {
+    auto inside = [&](uint32_t key) { return shift == 24 || key >> 8 >> shift == prefix; };
     for (int i = 0; i < 3; i++) sh.part[i][tid] = 0;
     __syncthreads();
     for (int at = tid; at < r.n; at += kThreads) {
       const uint32_t key = r.key(at);
-      if (key != 0 && (shift == 24 || key >> (shift + 8) == prefix)) add_to_bin(sh, key >> shift & 255, f(key));
+      if (key != 0 && inside(key)) add_to_bin(sh, 255 - (key >> shift & 255), f(key));  // large keys first
     }
     sync_all(cluster);
-    // Thread t has bin 255 - t: the sums before it are those above it.
-    const int bin = 255 - tid;
-    uint64_t own = 0;
-#pragma unroll
-    for (int b = 0; b < kMaxBlocks; b++) own += b < blocks ? bin_sum(*cluster.map_shared_rank(&sh, b), bin) : 0;
-    if (less != 0 && (shift == 24 || at_key >> (shift + 8) == prefix) && (int)(at_key >> shift & 255) == bin) own -= less;
-    uint64_t all;
-    const uint64_t before = above + scan_block(own, sh.scan, all);
-    if (before < want && before + own >= want) {
-      sh.border_bin = bin;
-      sh.border_above = before;
-    }
-    sync_all(cluster);  // and the block's own barrier
-    prefix = prefix << 8 | (uint32_t)sh.border_bin;
-    above = sh.border_above;
+    const int less_at = less != 0 && inside(at_key) ? 255 - (int)(at_key >> shift & 255) : -1;
+    uint64_t same;
+    const int bin = border_bin(cluster, sh, kBins, above, 0, less_at, less, [&](uint64_t) { return want; }, same, above);
+    prefix = prefix << 8 | (uint32_t)(255 - bin);
+    sync_all(cluster);  // the border has been read
   }
   return prefix;
 }
@@ -268,10 +335,7 @@ __device__ void look_in_block(Shared& sh, const SampleArgs& a, int64_t row, cons
                               uint64_t target, int count, F&& kept) {
   const int each = (r.n + kThreads - 1) / kThreads, begin = min(r.n, (int)threadIdx.x * each), end = min(r.n, begin + each);
   uint64_t own = 0, all;
-  for (int at = begin; at < end; at++) {
-    const uint32_t key = r.key(at);
-    if (kept(key, at)) own += r.weight(key);
-  }
+  r.each_weight(begin, end, 1, [&](int at, uint32_t key, uint64_t w) { own += kept(key, at) ? w : 0; });
   before += scan_block(own, sh.scan, all);
   if (!(before <= target && target < before + own)) return;
   for (int at = begin; at < end; at++) {
@@ -316,12 +380,11 @@ __device__ void choose_by_border(cg::cluster_group& cluster, Shared& sh, const S
            (key == r.top || !(min_p > 0.0f) || r.share(key) >= (double)min_p);
   };
   uint64_t own = 0, count = 0;
-  for (int at = begin; at < end; at++) {
-    const uint32_t key = r.key(at);
-    if (!kept(key, at)) continue;
-    own += r.weight(key);
-    count++;
-  }
+  r.each_weight(begin, end, 1, [&](int at, uint32_t key, uint64_t w) {
+    const bool in = kept(key, at);
+    own += in ? w : 0;
+    count += in;
+  });
   uint64_t counts;
   scan_block(count, sh.scan, counts);
   uint64_t before = scan_block(own, sh.scan, all);
@@ -391,7 +454,7 @@ __device__ void choose_over_row(cg::cluster_group& cluster, Shared& sh, const Sa
 template <typename T>
 __device__ void choose_by_share(cg::cluster_group& cluster, Shared& sh, const SampleArgs& a, int64_t row,
                                 const Row<T>& r, float top_p, float u) {
-  const int tid = threadIdx.x, blocks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+  const int tid = threadIdx.x, rank = (int)cluster.block_rank();
   constexpr int kOwn = kSteps / kThreads;  // bins of a thread
   const float per = (float)r.per;
   auto bin_of = [&](uint32_t key) {
@@ -405,41 +468,17 @@ __device__ void choose_by_share(cg::cluster_group& cluster, Shared& sh, const Sa
   }
   __syncthreads();
   uint64_t rest = 0, all;  // of the last bin, where most tokens may be
-  for (int at = tid; at < r.n; at += kThreads) {
-    const uint32_t key = r.key(at);
-    const uint64_t w = r.weight(key);
-    if (w == 0) continue;
-    if (const int bin = bin_of(key); bin < kSteps - 1) add_to_bin(sh, bin, w);
+  r.each_weight(tid, r.n, kThreads, [&](int, uint32_t key, uint64_t w) {
+    const int bin = bin_of(key);
+    if (bin < kSteps - 1) add_to_bin(sh, bin, w);
     else rest += w;
-  }
+  });
   scan_block(rest, sh.scan, all);
   if (tid == 0) sh.rest = all;
   sync_all(cluster);
-  uint64_t bins[kOwn] = {}, own = 0, total;
-#pragma unroll
-  for (int i = 0; i < kOwn; i++) {
-#pragma unroll
-    for (int b = 0; b < kMaxBlocks; b++) bins[i] += b < blocks ? bin_sum(*cluster.map_shared_rank(&sh, b), tid * kOwn + i) : 0;
-    own += bins[i];
-  }
   rest = over_blocks(cluster, sh, [](const Shared& o) { return o.rest; });
-  if (tid == kThreads - 1) {
-    bins[kOwn - 1] += rest;
-    own += rest;
-  }
-  uint64_t run = scan_block(own, sh.scan, total);
-  const uint64_t want = wanted_of(top_p, total);
-#pragma unroll
-  for (int i = 0; i < kOwn; i++) {
-    if (run < want && run + bins[i] >= want) {
-      sh.border_bin = tid * kOwn + i;
-      sh.border_above = run;
-    }
-    run += bins[i];
-  }
-  __syncthreads();
-  const int border_bin = sh.border_bin;
-  const uint64_t above = sh.border_above;
+  uint64_t want, above;
+  const int border_at = border_bin(cluster, sh, kSteps, 0, rest, -1, 0, [&](uint64_t sum) { return wanted_of(top_p, sum); }, want, above);
   // The border bin's tokens in a list, those above it counted.
   uint64_t count = 0, counts, kept_above = 0;
   uint32_t most = 0, least = ~0u;
@@ -447,8 +486,8 @@ __device__ void choose_by_share(cg::cluster_group& cluster, Shared& sh, const Sa
     const uint32_t key = r.key(at);
     if (key == 0) continue;
     const int bin = bin_of(key);
-    count += bin < border_bin;
-    if (bin != border_bin) continue;
+    count += bin < border_at;
+    if (bin != border_at) continue;
     most = max(most, key);
     least = min(least, key);
     const int place = atomicAdd(&sh.listed, 1);
@@ -462,7 +501,7 @@ __device__ void choose_by_share(cg::cluster_group& cluster, Shared& sh, const Sa
   }
 #pragma unroll
   for (int i = 0; i < kOwn; i++)
-    if (tid * kOwn + i < border_bin) kept_above += bin_sum(sh, tid * kOwn + i);
+    if (tid * kOwn + i < border_at) kept_above += bin_sum(sh, tid * kOwn + i);
   scan_block(count, sh.scan, counts);
   scan_block(kept_above, sh.scan, kept_above);
   const int listed = min(sh.listed, kListed);
