@@ -79,7 +79,8 @@ struct Shared {
   uint64_t mass, border, rest;
   uint32_t top, most, least;
   int listed, ties, count, first;
-  int border_bin;  // of this block alone
+  int border_bin, look_begin, look_end, look_last;
+  uint64_t look_before;
   uint64_t border_above;
 };
 
@@ -119,7 +120,8 @@ struct Row {
   const T* x;     // this block's part of the row
   int n, first;   // its elements (some before the row's begin or past its end hold -inf), the token of the first
   float largest;
-  double inv, per;  // 1 / temperature; of a logit, in log2 of a weight
+  double inv, per256;       // 1 / temperature; of a logit, in 256ths of an octave of weights
+  const double* powers;     // 2^(i / 256)
   uint32_t top;
 
   __device__ __forceinline__ uint32_t key(int at) const { return key_of(to_f32<T>(x[at])); }
@@ -129,32 +131,35 @@ struct Row {
     if (key == 0 || isinf(largest)) return 0.0;
     return exp(((double)value_of(key) - (double)largest) * inv);
   }
-  // The same in steps of 2^-44, from the power series of 2^f about 0: |f| <= 1/2
-  // leaves (ln2 / 2)^12 / 12! = 2^-47 of it out. A few keys side by side: a chain
-  // of f64 operations is long (one at a time 151936 tokens take twice as long).
+  // The same in steps of 2^-44: 2^t with t in 256ths, the whole ones' part from
+  // `powers`, and the power series of 2^(r / 256) about 0 for the rest: |r| <= 1/2
+  // leaves (ln2 / 512)^5 / 5! = 2^-54 of it out. A few keys side by side: a chain
+  // of f64 operations is long, and their number is what a row without cuts costs
+  // (11 a token; a series for all of 2^f took 17, and 256 rows 163 us for 121).
   template <int N>
   __device__ __forceinline__ void weights(const uint32_t (&key)[N], uint64_t (&w)[N]) const {
-    constexpr double kSeries[12] = {1.0, 0.6931471805599453, 0.2402265069591007, 0.055504108664821576, 0.009618129107628477, 0.0013333558146428441, 0.00015403530393381606, 1.5252733804059838e-05, 1.3215486790144305e-06, 1.0178086009239696e-07, 7.054911620801121e-09, 4.44553827187081e-10};
+    constexpr double kSeries[5] = {1.0, 0.0027076061740622863, 3.665565596910106e-06, 3.308302680541371e-09, 2.239395190875157e-12};
     constexpr double kWhole = 6755399441055744.0;  // 1.5 2^52: the whole part of a sum lands in the low bits
-    double t[N], n[N], f[N], y[N];
+    double t[N], n[N], r[N], y[N];
 #pragma unroll
     for (int i = 0; i < N; i++) {
-      t[i] = ((double)value_of(key[i]) - (double)largest) * per;  // log2
+      t[i] = ((double)value_of(key[i]) - (double)largest) * per256;
       n[i] = t[i] + kWhole;
-      f[i] = t[i] - (n[i] - kWhole);
-      y[i] = kSeries[11];
+      r[i] = t[i] - (n[i] - kWhole);
+      y[i] = kSeries[4];
     }
 #pragma unroll
-    for (int k = 10; k >= 0; k--)
+    for (int k = 3; k >= 0; k--)
 #pragma unroll
-      for (int i = 0; i < N; i++) y[i] = fma(y[i], f[i], kSeries[k]);
+      for (int i = 0; i < N; i++) y[i] = fma(y[i], r[i], kSeries[k]);
 #pragma unroll
     for (int i = 0; i < N; i++) {
-      // 2^(44 + n) by the exponent; then the nearest whole number by 2^52.
-      const int up = __double2loint(n[i]) + 44;
-      y[i] = __hiloint2double(__double2hiint(y[i]) + up * (1 << 20), __double2loint(y[i]));
+      // 2^(44 + n / 256) by the exponent; then the nearest whole number by 2^52.
+      const int whole = __double2loint(n[i]);
+      y[i] *= powers[whole & 255];
+      y[i] = __hiloint2double(__double2hiint(y[i]) + ((whole >> 8) + 44) * (1 << 20), __double2loint(y[i]));
       w[i] = (uint64_t)__double_as_longlong(y[i] + 4503599627370496.0) & 0xfffffffffffffull;
-      if (!(t[i] > -46.0) || key[i] == 0) w[i] = 0;
+      if (!(t[i] > -46.0 * 256) || key[i] == 0) w[i] = 0;
       if (key[i] == top) w[i] = (uint64_t)1 << 44;
     }
   }
@@ -263,8 +268,15 @@ __device__ int border_bin(cg::cluster_group& cluster, Shared& sh, int bins, uint
     own[i] = 0;
     if (i >= per || tid * per + i >= share) continue;
     const int bin = first + i;
+    // All blocks' at once: loads behind conditions would wait for one another.
+    uint32_t parts[kMaxBlocks][3];
 #pragma unroll
-    for (int b = 0; b < kMaxBlocks; b++) own[i] += b < blocks ? bin_sum(*cluster.map_shared_rank(&sh, b), bin) : 0;
+    for (int b = 0; b < kMaxBlocks; b++)
+#pragma unroll
+      for (int j = 0; j < 3; j++) parts[b][j] = cluster.map_shared_rank(&sh, min(b, blocks - 1))->part[j][bin];
+#pragma unroll
+    for (int b = 0; b < kMaxBlocks; b++)
+      if (b < blocks) own[i] += parts[b][0] + ((uint64_t)parts[b][1] << 15) + ((uint64_t)parts[b][2] << 30);
     own[i] += bin == bins - 1 ? more : 0;
     own[i] -= bin == less_at ? less : 0;
     sum += own[i];
@@ -327,26 +339,41 @@ __device__ uint32_t border_of(cg::cluster_group& cluster, Shared& sh, const Row<
   return prefix;
 }
 
-// Finds the token where the random number falls among the kept ones: `kept` of
-// (key, place), asked of a thread's contiguous tokens in order. before: the mass
-// before this block's, own: its own (both by whole blocks).
+// Finds the token where the random number falls: among this thread's contiguous
+// ones for one thread of the cluster's, which its block's first warp then looks at
+// together, with that thread's `last`. before: the kept mass before a thread's,
+// own: its own.
 template <typename T, typename F>
-__device__ void look_in_block(Shared& sh, const SampleArgs& a, int64_t row, const Row<T>& r, uint64_t before, uint64_t mass,
-                              uint64_t target, int count, F&& kept) {
-  const int each = (r.n + kThreads - 1) / kThreads, begin = min(r.n, (int)threadIdx.x * each), end = min(r.n, begin + each);
-  uint64_t own = 0, all;
-  r.each_weight(begin, end, 1, [&](int at, uint32_t key, uint64_t w) { own += kept(key, at) ? w : 0; });
-  before += scan_block(own, sh.scan, all);
-  if (!(before <= target && target < before + own)) return;
-  for (int at = begin; at < end; at++) {
-    const uint32_t key = r.key(at);
-    if (!kept(key, at)) continue;
-    const uint64_t w = r.weight(key);
-    before += w;
-    if (before > target) {
-      answer(a, row, r.first + at, log_share(w, mass), count);
+__device__ void look_among(Shared& sh, const SampleArgs& a, int64_t row, const Row<T>& r, uint64_t before, uint64_t own,
+                           int begin, int end, int last, uint64_t mass, uint64_t target, int count, F&& kept) {
+  const bool mine = before <= target && target < before + own;
+  if (mine) {
+    sh.look_begin = begin;
+    sh.look_end = end;
+    sh.look_last = last;
+    sh.look_before = before;
+  }
+  if (__syncthreads_or(mine) == 0 || threadIdx.x >= 32) return;
+  const int lane = threadIdx.x;
+  before = sh.look_before;
+  end = sh.look_end;
+  last = sh.look_last;
+  for (int at0 = sh.look_begin; at0 < end; at0 += 32) {
+    const int at = at0 + lane;
+    const uint32_t key = at < end ? r.key(at) : 0;
+    const uint64_t w = key != 0 && kept(key, at, last) ? r.weight(key) : 0;
+    uint64_t upto = w;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const uint64_t y = __shfl_up_sync(0xffffffffu, upto, off);
+      if (lane >= off) upto += y;
+    }
+    const unsigned past = __ballot_sync(0xffffffffu, before + upto > target);
+    if (past != 0) {
+      if (lane == __ffs(past) - 1) answer(a, row, r.first + at, log_share(w, mass), count);
       return;
     }
+    before += __shfl_sync(0xffffffffu, upto, 31);
   }
 }
 
@@ -375,13 +402,13 @@ __device__ void choose_by_border(cg::cluster_group& cluster, Shared& sh, const S
         if (r.key(at) == border && before++ < ties) last = at;
     }
   }
-  auto kept = [&](uint32_t key, int at) {
+  auto kept = [&](uint32_t key, int at, int last) {
     return key != 0 && (key > border || (key == border && at <= last)) &&
            (key == r.top || !(min_p > 0.0f) || r.share(key) >= (double)min_p);
   };
   uint64_t own = 0, count = 0;
   r.each_weight(begin, end, 1, [&](int at, uint32_t key, uint64_t w) {
-    const bool in = kept(key, at);
+    const bool in = kept(key, at, last);
     own += in ? w : 0;
     count += in;
   });
@@ -398,18 +425,7 @@ __device__ void choose_by_border(cg::cluster_group& cluster, Shared& sh, const S
   counts = over_blocks(cluster, sh, [](const Shared& o) { return o.count; });
   sync_all(cluster);  // the others have read this block's
   before += of_blocks;
-  const uint64_t target = target_of(u, mass);
-  if (!(before <= target && target < before + own)) return;
-  for (int at = begin; at < end; at++) {
-    const uint32_t key = r.key(at);
-    if (!kept(key, at)) continue;
-    const uint64_t w = r.weight(key);
-    before += w;
-    if (before > target) {
-      answer(a, row, r.first + at, log_share(w, mass), (int)counts);
-      return;
-    }
-  }
+  look_among(sh, a, row, r, before, own, begin, end, last, mass, target_of(u, mass), (int)counts, kept);
 }
 
 // Any rules, over the whole row. Returns after the answer is written.
@@ -456,7 +472,7 @@ __device__ void choose_by_share(cg::cluster_group& cluster, Shared& sh, const Sa
                                 const Row<T>& r, float top_p, float u) {
   const int tid = threadIdx.x, rank = (int)cluster.block_rank();
   constexpr int kOwn = kSteps / kThreads;  // bins of a thread
-  const float per = (float)r.per;
+  const float per = (float)(r.per256 / 256);
   auto bin_of = [&](uint32_t key) {
     return key == r.top ? 0 : (int)fminf((r.largest - value_of(key)) * per * kPerOctave, (float)(kSteps - 1));
   };
@@ -572,9 +588,13 @@ __device__ void choose_by_share(cg::cluster_group& cluster, Shared& sh, const Sa
   counts = over_blocks(cluster, sh, [](const Shared& o) { return o.count; });
   sync_all(cluster);  // the others have read this block's
   const uint64_t target = target_of(u, mass);
-  if (before <= target && target < before + kept_above)
-    look_in_block(sh, a, row, r, before, mass, target, (int)counts,
-                  [&](uint32_t key, int at) { return composite(key, at) >= border; });
+  if (!(before <= target && target < before + kept_above)) return;  // the whole block
+  auto kept = [&](uint32_t key, int at, int) { return composite(key, at) >= border; };
+  const int each = (r.n + kThreads - 1) / kThreads, begin = min(r.n, tid * each), end = min(r.n, begin + each);
+  uint64_t own = 0;
+  r.each_weight(begin, end, 1, [&](int at, uint32_t key, uint64_t w) { own += kept(key, at, 0) ? w : 0; });
+  before += scan_block(own, sh.scan, all);
+  look_among(sh, a, row, r, before, own, begin, end, 0, mass, target, (int)counts, kept);
 }
 
 template <typename T>
@@ -584,6 +604,7 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const __grid_consta
   constexpr int V = 16 / sizeof(T);
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ Shared sh;
+  __shared__ double powers[256];
   cg::cluster_group cluster = cg::this_cluster();
   const int tid = threadIdx.x, lane = tid % 32, blocks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int64_t row = blockIdx.x / (unsigned)blocks;
@@ -602,6 +623,7 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const __grid_consta
     sh.first = INT32_MAX;
   }
   sh.near[tid] = 0;
+  powers[tid] = exp2((double)tid / 256);
   float own = -INFINITY;  // this thread's largest
   constexpr int kAtOnce = 10;
   for (int v0 = tid; v0 < r.n / V; v0 += kThreads * kAtOnce) {
@@ -648,7 +670,8 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const __grid_consta
   const float u = how.uniform[row];
   const bool p = top_p < 1.0f, m = min_p > 0.0f;
   r.inv = 1.0 / (double)temperature;
-  r.per = r.inv * 1.4426950408889634;
+  r.per256 = r.inv * (1.4426950408889634 * 256);
+  r.powers = powers;
 
   if (top == 0 || !(temperature > 0.0f) || min_p > 1.0f) {  // no token, or the first one alone
     if (top != 0) {
@@ -676,7 +699,7 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const __grid_consta
       choose_by_border(cluster, sh, a, row, r, 1, ~0ull, 0.0f, u);
     return;
   }
-  const float per = (float)r.per;
+  const float per = (float)(r.per256 / 256);
 
   // ---- how far below the largest a token may be and matter
   float far = NAN;  // in logits; NaN: any distance, an infinite one too
@@ -688,9 +711,11 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const __grid_consta
       atomicAdd(&sh.near[min(max(bin, 0), kBins - 1)], 1u);
     }
     sync_all(cluster);
-    uint32_t bin_own = 0;
+    uint32_t bin_own = 0, of_block[kMaxBlocks];
 #pragma unroll
-    for (int b = 0; b < kMaxBlocks; b++) bin_own += b < blocks ? cluster.map_shared_rank(&sh, b)->near[tid] : 0;
+    for (int b = 0; b < kMaxBlocks; b++) of_block[b] = cluster.map_shared_rank(&sh, min(b, blocks - 1))->near[tid];
+#pragma unroll
+    for (int b = 0; b < kMaxBlocks; b++) bin_own += b < blocks ? of_block[b] : 0;
     uint64_t all;
     const uint64_t before = scan_block(bin_own, sh.scan, all);
     if (tid == 0) sh.border_bin = kBins - 1;
