@@ -615,7 +615,7 @@ int64_t dn_residual_norm(int64_t type, const void* y, int64_t y_stride, const fl
 
 /* How a batch's tokens are chosen; each array [n] or NULL. */
 typedef struct dn_sampling {
-  const float* temperature; /* NULL: 1; a row whose temperature is not > 0 takes its largest logit */
+  const float* temperature; /* NULL: 1; over 1e30: 1e30; a row whose temperature is not > 0 takes its largest logit */
   const int32_t* top_k;     /* at most so many tokens; NULL, or not > 0: any number */
   const float* top_p;       /* the likeliest with this share of what top_k leaves; NULL, or not < 1: all */
   const float* min_p;       /* at least this share of the likeliest token's probability; NULL: 0 */
