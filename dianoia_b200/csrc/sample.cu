@@ -17,13 +17,13 @@
 //    histogram of their distance from the largest one: at least k tokens are as
 //    near as the k-th of these;
 //  - min_p: the weight says it.
-// Their weights and keys go to the first block's shared memory, which sorts them
-// and decides alone while the others leave. top_p alone may keep any number of
+// Their weights and keys go to the first block's shared memory, which cuts them by
+// histograms of their keys' bytes and decides alone while the others leave. top_p alone may keep any number of
 // tokens: f32 sums by octaves of the weights tell where its border is to an octave
 // or two, whose weights go into a histogram (shared memory adds fewer than two
 // lanes a clock: all weights in one took 15 of 38 us), and the border bin's tokens
-// are the ones that are sorted; without a rule but the temperature there is nothing
-// to sort. Then the place that the random number falls to is looked for by sums of
+// are the ones that the first block cuts; without a rule but the temperature there is
+// nothing to cut. Then the place that the random number falls to is looked for by sums of
 // blocks, warps, segments. Where more tokens matter than the lists hold (thousands
 // of top_k, many ties) the border is found eight bits of the key at a time over all
 // of the row.
@@ -40,12 +40,13 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr int kMaxBlocks = 16;  // of a cluster
-constexpr int kSorted = 2048;   // tokens that the first block sorts
+constexpr int kGathered = 2048;  // tokens that the first block gathers
 constexpr int kMostK = 1536;    // top_k up to which the histogram is asked
 constexpr int kBins = 256;
 constexpr int kNears = 512;     // bins of distances: 32 to an octave, from 2^-8 to 2^8 of a logit
-constexpr int kOctaves = 16;    // of weights, that top_p's border is looked for in
-constexpr int kNear = 512;      // tokens of its border bin that are sorted
+constexpr int kDepths = 16;        // steps of weights that top_p's border is looked for in,
+constexpr float kDepth = 1.5f;     // so many octaves each
+constexpr int kNear = 512;         // tokens of its border bin that the first block gathers
 
 // The cluster's barrier counts whole warps: lanes that leave a loop a turn late
 // would be counted as there, their additions still to come (seen as sums that
@@ -71,7 +72,7 @@ __device__ __forceinline__ float value_of(uint32_t key) {
 template <bool WHOLE>
 struct Form {
   static constexpr int kThreads = WHOLE ? 1024 : 256, kWarps = kThreads / 32;
-  static constexpr int kListed = WHOLE ? kSorted : 512;  // tokens that a block lists
+  static constexpr int kListed = WHOLE ? kGathered : 512;  // tokens that a block lists
   static constexpr int kTops = WHOLE ? 4 : 1;            // largest logits that a thread has
 };
 
@@ -80,17 +81,15 @@ template <bool WHOLE>
 struct Shared {
   static constexpr int kWarps = Form<WHOLE>::kWarps, kListed = Form<WHOLE>::kListed;
   // A histogram's sums in three parts of 15 bits, which shared memory adds by
-  // itself (64-bit additions are loops there); the share's border tokens over it.
-  union {
-    uint32_t part[3][kBins];
-    uint64_t sorted[kNear];
-  };
+  // itself (64-bit additions are loops there).
+  uint32_t part[3][kBins];
+  uint64_t gathered[kNear];
   uint32_t near[kNears];
   uint32_t list_key[kListed];
   typename std::conditional<WHOLE, uint32_t, uint16_t>::type list_at[kListed];
   uint64_t scan[kWarps];  // of this block alone, as the next two
   uint64_t mass, border, above, rest;
-  float octave[kOctaves + 1];
+  float octave[kDepths + 1];
   uint32_t top, most, least;
   int listed, ties, count, first;
   int border_bin, place;
@@ -262,30 +261,74 @@ __device__ __forceinline__ uint64_t scan_block(uint64_t s, Shared<W>& sh, uint64
   return before + up - s;
 }
 
-// Sorts n (a power of two) pairs by their first, largest first.
-template <int kThreads, bool WITH>
-__device__ __forceinline__ void sort_block(uint64_t* by, uint64_t* with, int n) {
-  for (int size = 2; size <= n; size <<= 1)
-    for (int step = size / 2; step >= 1; step >>= 1) {
-      __syncthreads();
-      for (int i = threadIdx.x; i < n / 2; i += kThreads) {
-        const int lo = (i & -step) * 2 | (i & (step - 1)), hi = lo + step;
-        const uint64_t p = by[lo], q = by[hi];
-        if ((p < q) == ((lo & size) == 0)) {
-          by[lo] = q;
-          by[hi] = p;
-          if constexpr (WITH) {
-            const uint64_t w = with[lo];
-            with[lo] = with[hi];
-            with[hi] = w;
-          }
-        }
-      }
+// The largest of n keys of shift + 8 bits from which on the parts sum to at least
+// `want`, a byte at a time, and the sum above it; within a block.
+template <bool W, typename K, typename F>
+__device__ uint32_t list_border(Shared<W>& sh, int n, int shift, uint64_t want, uint64_t& above, K&& key_at, F&& part_at) {
+  constexpr int kThreads = Form<W>::kThreads;
+  const int tid = threadIdx.x;
+  uint32_t prefix = 0;
+  above = 0;
+  for (; shift >= 0; shift -= 8) {
+    for (int i = tid; i < 3 * kBins; i += kThreads) sh.part[i / kBins][i % kBins] = 0;
+    __syncthreads();
+    for (int i = tid; i < n; i += kThreads) {
+      const uint32_t key = key_at(i);
+      if (key >> 8 >> shift == prefix) add_to_bin(sh, 255 - (key >> shift & 255), part_at(i));
     }
-  __syncthreads();
+    __syncthreads();
+    const uint64_t own = tid < kBins ? bin_sum(sh, tid) : 0;
+    uint64_t all;
+    const uint64_t before = above + scan_block(own, sh, all);
+    if (before < want && before + own >= want) {
+      sh.border_bin = tid;
+      sh.border_above = before;
+    }
+    __syncthreads();
+    prefix = prefix << 8 | (uint32_t)(255 - sh.border_bin);
+    above = sh.border_above;
+  }
+  return prefix;
 }
 
-__device__ __forceinline__ int power_of_two(int n) { return n <= 2 ? 2 : 1 << (32 - __clz(n - 1)); }
+struct Gathered {
+  uint64_t weight;
+  uint32_t key, token;
+};
+
+// A border among listed tokens: larger keys are in, and those at `key` up to `token`.
+struct Border {
+  uint32_t key, token;
+  __device__ __forceinline__ bool in(uint32_t k, uint32_t t) const { return k > key || (k == key && t <= token); }
+};
+
+constexpr uint32_t kLastToken = 0xffffff;  // three bytes of token; kLastToken - token orders them down
+
+// Where the first tokens of n, by key and token, come to `want` by part_of(i)
+// (0 for what is out, else the same for equal keys).
+template <bool W, typename K, typename I, typename F>
+__device__ Border cut_list(Shared<W>& sh, int n, uint64_t want, K&& key_at, I&& token_at, F&& part_at) {
+  const int tid = threadIdx.x;
+  uint64_t above, unused, own = 0, tied, each = 0;
+  Border b{0, ~0u};
+  b.key = list_border(sh, n, 24, want, above, key_at, part_at);
+  for (int i = tid; i < n; i += Form<W>::kThreads)
+    if (key_at(i) == b.key && part_at(i) != 0) {
+      own++;
+      each = part_at(i);
+    }
+  scan_block(own, sh, tied);
+  if (own != 0) sh.border_above = each;  // all the same
+  __syncthreads();
+  each = sh.border_above;
+  __syncthreads();
+  const uint64_t need = (want - above + each - 1) / each;
+  if (need < tied)
+    b.token = kLastToken - list_border(
+                               sh, n, 16, need, unused, [&](int i) { return kLastToken - token_at(i); },
+                               [&](int i) -> uint64_t { return key_at(i) == b.key && part_at(i) != 0; });
+  return b;
+}
 
 // What top_p asks of a sum, and the place that a random number has in one.
 __device__ __forceinline__ uint64_t wanted_of(float top_p, uint64_t total) {
@@ -558,22 +601,22 @@ __device__ void choose_by_share(cg::cluster_group& cluster, Shared<W>& sh, const
   auto depth_of = [&](float z) { return z == r.largest ? 0.0f : (r.largest - z) * per; };
   // ---- the sums to each octave, and of all
   {
-    float sum[kOctaves] = {}, whole = 0.0f;
+    float sum[kDepths] = {}, whole = 0.0f;
     r.each_logit(tid, r.n, kThreads, [&](int, float z) {
       const float d = z > -INFINITY ? depth_of(z) : INFINITY, w = power2(-d);
       whole += w;
 #pragma unroll
-      for (int i = 0; i < kOctaves; i++) sum[i] += d <= (float)(i + 1) ? w : 0.0f;
+      for (int i = 0; i < kDepths; i++) sum[i] += d <= kDepth * (float)(i + 1) ? w : 0.0f;
     });
     float mine = 0.0f;
 #pragma unroll
-    for (int i = 0; i <= kOctaves; i++) {
-      float x = i < kOctaves ? sum[i < kOctaves ? i : 0] : whole;
+    for (int i = 0; i <= kDepths; i++) {
+      float x = i < kDepths ? sum[i < kDepths ? i : 0] : whole;
 #pragma unroll
       for (int off = 16; off >= 1; off >>= 1) x += __shfl_xor_sync(0xffffffffu, x, off);
       if (lane == i) mine = x;
     }
-    constexpr int kRow = kOctaves + 1;
+    constexpr int kRow = kDepths + 1;
     static_assert(kWarps * kRow <= 3 * kBins, "the histogram's place holds the warps' sums");
     float* warps = reinterpret_cast<float*>(sh.part);
     if (lane < kRow) warps[tid / 32 * kRow + lane] = mine;
@@ -592,14 +635,14 @@ __device__ void choose_by_share(cg::cluster_group& cluster, Shared<W>& sh, const
   sync_all(cluster);
   float upto = 0.0f, of_block[kMaxBlocks];
 #pragma unroll
-  for (int b = 0; b < kMaxBlocks; b++) of_block[b] = cluster.map_shared_rank(&sh, min(b, blocks - 1))->octave[min(lane, kOctaves)];
+  for (int b = 0; b < kMaxBlocks; b++) of_block[b] = cluster.map_shared_rank(&sh, min(b, blocks - 1))->octave[min(lane, kDepths)];
 #pragma unroll
   for (int b = 0; b < kMaxBlocks; b++) upto += b < blocks ? of_block[b] : 0.0f;
-  const float whole = __shfl_sync(0xffffffffu, upto, kOctaves);
+  const float whole = __shfl_sync(0xffffffffu, upto, kDepths);
   // The border lies from depth `near` to `far`, whatever f32 sums may be off by.
-  const unsigned enough = __ballot_sync(0xffffffffu, lane < kOctaves && upto >= (top_p + 0.001f) * whole);
-  const unsigned short_of = __ballot_sync(0xffffffffu, lane < kOctaves && upto <= (top_p - 0.001f) * whole);
-  const float near = (float)__popc(short_of), far = enough != 0 ? (float)__ffs(enough) : 3.0f * kOctaves;
+  const unsigned enough = __ballot_sync(0xffffffffu, lane < kDepths && upto >= (top_p + 0.001f) * whole);
+  const unsigned short_of = __ballot_sync(0xffffffffu, lane < kDepths && upto <= (top_p - 0.001f) * whole);
+  const float near = kDepth * (float)__popc(short_of), far = enough != 0 ? kDepth * (float)__ffs(enough) : 46.0f;
   const float per_bin = (float)kBins / (far - near);
   // -1 above all bins, kBins below.
   auto bin_of = [&](float z) {
@@ -673,36 +716,23 @@ __device__ void choose_by_share(cg::cluster_group& cluster, Shared<W>& sh, const
     }
     return;
   }
-  uint64_t* by = cluster.map_shared_rank(&sh, 0)->sorted;  // over what has been read; the row is still needed
-  const int n2 = power_of_two(in_bin);
+  uint64_t* to = cluster.map_shared_rank(&sh, 0)->gathered;
   for (int i = tid; i < listed; i += kThreads)
-    by[before_block + i] = (uint64_t)sh.list_key[i] << 32 | (uint32_t)~(r.first + (int)sh.list_at[i]);
-  if (rank == 0)
-    for (int i = in_bin + tid; i < n2; i += kThreads) by[i] = 0;
+    to[before_block + i] = (uint64_t)sh.list_key[i] << 32 | (uint32_t)(r.first + (int)sh.list_at[i]);
   sync_all(cluster);
   if (rank == 0) {
-    sort_block<kThreads, false>(sh.sorted, nullptr, n2);
-    const int each = (n2 + kThreads - 1) / kThreads, begin = min(n2, tid * each), end = min(n2, begin + each);
-    auto weight_at = [&](int i) { return r.weight(value_of((uint32_t)(sh.sorted[i] >> 32))); };
-    uint64_t sum = 0;
-    for (int i = begin; i < end; i++)
-      if (i < in_bin) sum += weight_at(i);
-    uint64_t upto = above + scan_block(sum, sh, all);
-    if (upto < want && upto + sum >= want)
-      for (int i = begin; i < min(end, in_bin); i++) {
-        upto += weight_at(i);
-        if (upto >= want) {
-          sh.border = sh.sorted[i];
-          break;
-        }
-      }
+    auto key_at = [&](int i) { return (uint32_t)(sh.gathered[i] >> 32); };
+    const Border b = cut_list(
+        sh, in_bin, want - above, key_at, [&](int i) { return (uint32_t)sh.gathered[i]; },
+        [&](int i) { return r.weight(value_of(key_at(i))); });
+    if (tid == 0) sh.border = (uint64_t)b.key << 32 | b.token;
   }
   sync_all(cluster);
-  const uint64_t border = cluster.map_shared_rank(&sh, 0)->border;
-  auto composite = [&](uint32_t key, int at) { return (uint64_t)key << 32 | (uint32_t)~(r.first + at); };
+  const uint64_t packed = cluster.map_shared_rank(&sh, 0)->border;
+  const Border border{(uint32_t)(packed >> 32), (uint32_t)packed};
   uint64_t band = 0, band_count = 0;
   for (int i = tid; i < listed; i += kThreads)
-    if (composite(sh.list_key[i], sh.list_at[i]) >= border) {
+    if (border.in(sh.list_key[i], (uint32_t)(r.first + (int)sh.list_at[i]))) {
       band += r.weight(value_of(sh.list_key[i]));
       band_count++;
     }
@@ -721,7 +751,7 @@ __device__ void choose_by_share(cg::cluster_group& cluster, Shared<W>& sh, const
   sync_all(cluster);  // the others have read this block's
   const uint64_t target = target_of(u, mass);
   if (!(before <= target && target < before + kept_above)) return;  // the whole block
-  auto kept = [&](float z, int token) { return composite(key_of(z), token - r.first) >= border; };
+  auto kept = [&](float z, int token) { return border.in(key_of(z), (uint32_t)token); };
   const Segments<W, T> segments(r);
   const uint64_t mine =
       segments.template sums<true>(r, [&](int at, float z, uint64_t w) { return kept(z, r.first + at) ? w : 0; });
@@ -898,80 +928,55 @@ __global__ void __launch_bounds__(Form<W>::kThreads, W ? 1 : 4) sample_kernel(co
   uint64_t before_block;
   const int total = (int)over_blocks(cluster, sh, [](const auto& o) { return o.listed; }, rank, before_block);
   const bool over = over_blocks(cluster, sh, [](const auto& o) { return o.listed > kListed; }) != 0;
-  if (over || total > kSorted) {
+  if (over || total > kGathered) {
     sync_all(cluster);  // the lists have been read
     choose_over_row(cluster, sh, a, row, r, top_k, top_p, min_p, u);
     return;
   }
-  // ---- the first block sorts and decides, over its part of the row
-  uint64_t* by = reinterpret_cast<uint64_t*>(cluster.map_shared_rank(smem, 0));
-  uint64_t* with = by + kSorted;
-  const int n2 = power_of_two(total);
-  for (int i = tid; i < listed; i += kThreads) {
-    by[before_block + i] = (uint64_t)sh.list_key[i] << 32 | (uint32_t)~(r.first + (int)sh.list_at[i]);
-    with[before_block + i] = r.weight(value_of(sh.list_key[i]));
-  }
-  if (rank == 0)
-    for (int i = total + tid; i < n2; i += kThreads) by[i] = with[i] = 0;
+  // ---- the first block cuts and decides, over its part of the row
+  Gathered* list = reinterpret_cast<Gathered*>(cluster.map_shared_rank(smem, 0));
+  for (int i = tid; i < listed; i += kThreads)
+    list[before_block + i] = Gathered{r.weight(value_of(sh.list_key[i])), sh.list_key[i], (uint32_t)(r.first + (int)sh.list_at[i])};
   sync_all(cluster);
   if (rank != 0) return;
-  by = reinterpret_cast<uint64_t*>(smem);
-  with = by + kSorted;
-  sort_block<kThreads, true>(by, with, n2);
-  int kept = top_k > 0 ? min(top_k, total) : total;
-  // Threads have contiguous places; `upto` is what lies before a thread's.
-  const int each = (n2 + kThreads - 1) / kThreads, begin = min(n2, tid * each), end = min(n2, begin + each);
+  list = reinterpret_cast<Gathered*>(smem);
+  auto key_at = [&](int i) { return list[i].key; };
+  auto token_at = [&](int i) { return list[i].token; };
+  Border border{0, ~0u};
+  if (top_k > 0 && total > top_k) border = cut_list(sh, total, top_k, key_at, token_at, [](int) -> uint64_t { return 1; });
+  auto part_at = [&](int i) { return border.in(list[i].key, list[i].token) ? list[i].weight : 0; };
+  auto sum_kept = [&](uint64_t& count) {
+    uint64_t sum = 0, some = 0;
+    for (int i = tid; i < total; i += kThreads) {
+      const uint64_t w = part_at(i);
+      sum += w;
+      some += border.in(list[i].key, list[i].token);
+    }
+    scan_block(some, sh, count);
+    scan_block(sum, sh, sum);
+    return sum;
+  };
+  uint64_t kept, mass = sum_kept(kept);
   if (p) {
-    uint64_t sum = 0, all;
-    for (int i = begin; i < end; i++)
-      if (i < kept) sum += with[i];
-    const uint64_t upto = scan_block(sum, sh, all), want = wanted_of(top_p, all);
-    if (tid == 0) sh.count = kept;
+    Border by_share = cut_list(sh, total, wanted_of(top_p, mass), key_at, token_at, part_at);
+    if (by_share.key == border.key) by_share.token = min(by_share.token, border.token);  // top_k's cut among equals stays
+    border = by_share;
+    mass = sum_kept(kept);
+  }
+  if (m) {  // these are the last ones, but for the largest
     __syncthreads();
-    if (upto < want && upto + sum >= want) {
-      uint64_t run = upto;
-      for (int i = begin; i < end && i < kept; i++) {
-        run += with[i];
-        if (run >= want) {
-          sh.count = i + 1;
-          break;
-        }
-      }
-    }
+    for (int i = tid; i < total; i += kThreads)
+      if (const uint32_t key = list[i].key; key != top && !(r.share(value_of(key)) >= (double)min_p)) list[i].key = 0;
+    if (border.key == 0) border.key = 1;
     __syncthreads();
-    kept = sh.count;
+    mass = sum_kept(kept);
   }
-  if (m) {
-    int in = 0;
-    for (int i = begin; i < end && i < kept; i++) {
-      const uint32_t key = (uint32_t)(by[i] >> 32);
-      in += key == top || r.share(value_of(key)) >= (double)min_p;
-    }
-    uint64_t all;
-    scan_block((uint64_t)in, sh, all);
-    kept = (int)all;
-  }
-  // The kept ones in index order.
-  const int k2 = power_of_two(kept);
-  __syncthreads();
-  for (int i = tid; i < k2; i += kThreads) {
-    by[i] = i < kept ? by[i] & 0xffffffffu : 0;  // the complement of the token
-    with[i] = i < kept ? with[i] : 0;
-  }
-  sort_block<kThreads, true>(by, with, k2);
-  const int per_thread = (k2 + kThreads - 1) / kThreads, from = min(k2, tid * per_thread), to = min(k2, from + per_thread);
-  uint64_t sum = 0, mass;
-  for (int i = from; i < to; i++) sum += with[i];
-  uint64_t run = scan_block(sum, sh, mass);
-  const uint64_t target = target_of(u, mass);
-  if (run <= target && target < run + sum)
-    for (int i = from; i < to; i++) {
-      run += with[i];
-      if (run > target) {
-        answer(a, row, (int)~(uint32_t)by[i], log_share(with[i], mass), kept);
-        break;
-      }
-    }
+  uint64_t unused;
+  const uint32_t token = kLastToken - list_border(
+                                          sh, total, 16, target_of(u, mass) + 1, unused,
+                                          [&](int i) { return kLastToken - list[i].token; }, part_at);
+  for (int i = tid; i < total; i += kThreads)
+    if (list[i].token == token) answer(a, row, (int)token, log_share(list[i].weight, mass), (int)kept);
 }
 
 // From so many rows on a row is one block's: 49 rows are more than the 32 or so
@@ -1000,17 +1005,17 @@ template <typename T>
 cudaError_t launch_type(const SampleArgs& a, cudaStream_t stream, bool pdl) {
   constexpr int V = 16 / sizeof(T);
   if (a.n >= kMany) {
-    if (cudaError_t e = allow_smem<sample_kernel<T, true>>(kSorted * 16); e != cudaSuccess) return e;
-    return launch_form<T, true>(a, 1, 0, kSorted * 16, stream, pdl);
+    if (cudaError_t e = allow_smem<sample_kernel<T, true>>(kGathered * 16); e != cudaSuccess) return e;
+    return launch_form<T, true>(a, 1, 0, kGathered * 16, stream, pdl);
   }
   // The fewest blocks whose part of a row is 40 KB at most, so that four of them share an SM.
   const int64_t vecs = (a.vocab + 2 * V - 2) / V;
   int blocks = 1;
   while (blocks < kMaxBlocks && (vecs + blocks - 1) / blocks * 16 > 40960) blocks *= 2;
   const int64_t block_vecs = (vecs + blocks - 1) / blocks < 1 ? 1 : (vecs + blocks - 1) / blocks;
-  const int bytes = block_vecs * 16 > kSorted * 16 ? (int)block_vecs * 16 : kSorted * 16;
+  const int bytes = block_vecs * 16 > kGathered * 16 ? (int)block_vecs * 16 : kGathered * 16;
   constexpr int most = (int)(kMaxSampleVocab / kMaxBlocks + V) * (int)sizeof(T);
-  if (cudaError_t e = allow_smem<sample_kernel<T, false>>(most > kSorted * 16 ? most : kSorted * 16); e != cudaSuccess)
+  if (cudaError_t e = allow_smem<sample_kernel<T, false>>(most > kGathered * 16 ? most : kGathered * 16); e != cudaSuccess)
     return e;
   if (blocks > 8)
     if (cudaError_t e = cudaFuncSetAttribute(sample_kernel<T, false>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);

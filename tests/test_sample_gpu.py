@@ -257,3 +257,54 @@ def test_cuts_of_many_tokens_repeat(cuda_lib, kind, vocab):
             first = check(cuda_lib, x, rules)
             for _ in range(4):
                 assert run(cuda_lib, x, rules) == first
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("which", ["", "k", "p", "m", "kp", "tkpm", "pm"])
+@pytest.mark.parametrize("vocab,offset,pad", [(1, 0, 0), (70, 1, 0), (4097, 0, 1), (30011, 3, 2)])
+def test_many_rows(cuda_lib, kind, which, vocab, offset, pad):
+    """Rows enough for a block each, those on both sides of that number alike."""
+    n = 60
+    x = logits_of(kind, n, vocab, vocab, offset=offset, pad=pad)
+    rules = rules_of(n, which, vocab, vocab)
+    whole = check(cuda_lib, x, rules)
+    few = run(cuda_lib, x[:40], {k: v[:40] for k, v in rules.items()})
+    assert [o[:40] for o in whole] == list(few)
+
+
+@pytest.mark.parametrize("n", [5, 55])
+def test_ties_at_every_cut(cuda_lib, n):
+    """Equal logits at top_k's border and at top_p's, in the lists and over the row, the two at the same logit."""
+    g = torch.Generator(device="cuda").manual_seed(n)
+    rng = random.Random(n)
+    for vocab, levels in ((300, 5), (20000, 40), (20000, 4000)):
+        x = torch.randint(0, levels, (n, vocab), generator=g, device="cuda").float().mul_(8.0 / levels)
+        for k in (3, 17, 100, 900, 2500):
+            rules = {"u": [0.001 + 0.998 * rng.random() for _ in range(n)], "top_k": [min(k, vocab - 1)] * n,
+                     "top_p": [rng.choice([0.3111, 0.5123, 0.9017, 0.9917]) for _ in range(n)]}
+            check(cuda_lib, x, rules)
+            check(cuda_lib, x, {"u": rules["u"], "top_k": rules["top_k"]})
+        check(cuda_lib, x, {"u": rules["u"], "top_p": rules["top_p"]})
+
+
+@pytest.mark.parametrize("n", [3, 60])
+def test_masks_of_finite_numbers(cuda_lib, n):
+    """Masked logits of the type's lowest value, or of a large negative one, among which a cut may fall."""
+    for kind in TYPES:
+        for low in (-1e4, torch.finfo(TYPES[kind][0]).min):
+            x = logits_of(kind, n, 9001, 5)
+            few = torch.rand(x.shape, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda") < 0.002
+            x.copy_(torch.where(few, x, torch.full_like(x, low)))
+            for which in ("k", "p", "kp", "m", ""):
+                check(cuda_lib, x, rules_of(n, which, 3, 9001))
+
+
+@pytest.mark.parametrize("n", [4, 64])
+def test_logits_and_temperatures_of_every_size(cuda_lib, n):
+    """Spreads from a billionth to a billion, temperatures that make weights steep or level."""
+    for spread, offset in ((1e-9, 0.0), (1e-3, 5.0), (50.0, 0.0), (1e9, 0.0), (1e30, 0.0), (1.0, 1e6)):
+        x = logits_of("f32", n, 5003, 11, spread=spread) + offset
+        for t in (1e-3, 1.0, 1e4, 1e20):
+            for which in ("", "k", "p", "m", "kp"):
+                rules = {**rules_of(n, which, 13, 5003), "temperature": [t] * n}
+                check(cuda_lib, x, rules)
