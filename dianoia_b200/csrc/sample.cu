@@ -92,7 +92,7 @@ struct Shared {
   float octave[kDepths + 1];
   uint32_t top, most, least;
   int listed, ties, count, first;
-  int border_bin, place;
+  int border_bin, band_first, band_last, place;
   uint64_t border_above;
 };
 
@@ -529,8 +529,13 @@ __device__ void choose_by_border(cg::cluster_group& cluster, Shared<W>& sh, cons
     last = lane < (int)cluster.num_blocks() ? cluster.map_shared_rank(&sh, lane)->place : INT32_MAX;
     last = __reduce_min_sync(0xffffffffu, last);
   }
+  // Logits that min_p surely lets in, and that it surely does not; in f64 between.
+  const float cut = min_p > 0.0f ? (float)((double)r.largest + log((double)min_p) / r.inv) : -INFINITY;
+  const float in_from = min_p > 0.0f ? cut + fabsf(cut) * 1e-6f + fabsf(r.largest) * 1e-6f : -INFINITY;
+  const float out_to = min_p > 0.0f ? cut - fabsf(cut) * 1e-6f - fabsf(r.largest) * 1e-6f : -INFINITY;
   auto kept = [&](float z, int token) {
-    return (z > border || (z == border && token <= last)) && (!(min_p > 0.0f) || z == r.largest || r.share(z) >= (double)min_p);
+    return (z > border || (z == border && token <= last)) &&
+           (z >= in_from || z == r.largest || (z >= out_to && r.share(z) >= (double)min_p));
   };
   uint64_t counts, count = 0;
   const uint64_t mine = segments.template sums<true>(r, [&](int at, float z, uint64_t w) {
@@ -643,77 +648,97 @@ __device__ void choose_by_share(cg::cluster_group& cluster, Shared<W>& sh, const
   const unsigned enough = __ballot_sync(0xffffffffu, lane < kDepths && upto >= (top_p + 0.001f) * whole);
   const unsigned short_of = __ballot_sync(0xffffffffu, lane < kDepths && upto <= (top_p - 0.001f) * whole);
   const float near = kDepth * (float)__popc(short_of), far = enough != 0 ? kDepth * (float)__ffs(enough) : 46.0f;
+  const float base_sum = short_of != 0 ? __shfl_sync(0xffffffffu, upto, __popc(short_of) - 1) : 0.0f;
   const float per_bin = (float)kBins / (far - near);
   // -1 above all bins, kBins below.
-  auto bin_of = [&](float z) {
-    const float d = depth_of(z);
+  auto bin_of = [&](float d) {
     return d <= near && near > 0.0f ? -1 : !(d <= far) ? kBins : min((int)((d - near) * per_bin), kBins - 1);
   };
-  for (int i = tid; i < 3 * kBins; i += kThreads) sh.part[i / kBins][i % kBins] = 0;
-  __syncthreads();
-  uint64_t above_bins = 0, rest = 0, all;
-  r.each_weight(tid, r.n, kThreads, [&](int, float z, uint64_t w) {
-    const int bin = bin_of(z);
-    above_bins += bin < 0 ? w : 0;
-    rest += bin == kBins ? w : 0;
-    if (bin >= 0 && bin < kBins) add_to_bin(sh, bin, w);
-  });
-  scan_block(rest, sh, all);
-  if (tid == 0) sh.rest = all;
-  scan_block(above_bins, sh, above_bins);
-  if (tid == 0) sh.above = above_bins;
-  sync_all(cluster);
-  rest = over_blocks(cluster, sh, [](const auto& o) { return o.rest; });
-  const uint64_t base = over_blocks(cluster, sh, [](const auto& o) { return o.above; });
-  uint64_t want, above;
-  const int border_at =
-      border_bin(cluster, sh, base, -1, 0, [&](uint64_t sum) { return wanted_of(top_p, base + sum + rest); }, want, above);
-  if (border_at < 0) {
-    choose_over_row(cluster, sh, a, row, r, 0, top_p, 0.0f, u);
-    return;
+  // ---- the bins of those depths, in steps of 2^-16 of the first one's weights
+  if (tid < kBins) sh.part[0][tid] = 0;
+  if (tid == 0) {
+    sh.band_first = 0;
+    sh.band_last = kBins - 1;
   }
-  // The border bin's tokens in a list, those above it counted.
-  uint64_t count = 0, counts, kept_above;
+  __syncthreads();
+  r.each_logit(tid, r.n, kThreads, [&](int, float z) {
+    const float d = depth_of(z);
+    const int bin = bin_of(d);
+    if (bin >= 0 && bin < kBins) atomicAdd(&sh.part[0][bin], __float2uint_rn(power2(near - d + 16.0f)));
+  });
+  sync_all(cluster);
+  uint64_t all;
+  {
+    uint32_t of_block[kMaxBlocks];
+    uint64_t own = 0;
+#pragma unroll
+    for (int b = 0; b < (W ? 1 : kMaxBlocks); b++) of_block[b] = cluster.map_shared_rank(&sh, min(b, blocks - 1))->part[0][tid % kBins];
+#pragma unroll
+    for (int b = 0; b < (W ? 1 : kMaxBlocks); b++) own += b < blocks && tid < kBins ? of_block[b] : 0;
+    const uint64_t before = scan_block(own, sh, all);
+    const float unit = power2(-16.0f - near), from = base_sum + (float)before * unit, to = base_sum + (float)(before + own) * unit;
+    const float less = (top_p - 2e-5f) * whole, more = (top_p + 2e-5f) * whole;
+    if (tid < kBins && from <= less && less < to) sh.band_first = tid;
+    if (tid < kBins && from < more && more <= to) sh.band_last = tid;
+  }
+  __syncthreads();
+  const int band_first = sh.band_first, band_last = sh.band_last;
+  // ---- all weights: those above the band by segments, the band's tokens in a list
+  uint64_t count = 0, counts, rest = 0;
   uint32_t most = 0, least = ~0u;
-  r.each_logit(tid, r.n, kThreads, [&](int at, float z) {
-    const int bin = bin_of(z);
-    count += bin < border_at;
-    if (bin != border_at) return;
+  const Segments<W, T> segments(r);
+  uint64_t mine = segments.template sums<true>(r, [&](int at, float z, uint64_t w) -> uint64_t {
+    const int bin = bin_of(depth_of(z));
+    if (bin < band_first) {
+      count++;
+      return w;
+    }
+    if (bin > band_last) {
+      rest += w;
+      return 0;
+    }
     const uint32_t key = key_of(z);
     most = max(most, key);
     least = min(least, key);
     const int place = atomicAdd(&sh.listed, 1);
     if (place < kListed) sh.list_at[place] = at;
+    return 0;
   });
   most = __reduce_max_sync(0xffffffffu, most);
   least = __reduce_min_sync(0xffffffffu, least);
-  if (tid % 32 == 0) {
+  if (lane == 0) {
     atomicMax(&sh.most, most);
     atomicMin(&sh.least, least);
   }
+  uint64_t above;
   scan_block(count, sh, counts);
-  scan_block(tid < border_at ? bin_sum(sh, tid) : 0, sh, kept_above);
-  kept_above += above_bins;
+  scan_block(mine, sh, above);
+  scan_block(rest, sh, rest);
+  if (tid == 0) {
+    sh.above = above;
+    sh.rest = rest;
+  }
   const int listed = min(sh.listed, kListed);
   for (int i = tid; i < listed; i += kThreads) sh.list_key[i] = r.key(sh.list_at[i]);
   sync_all(cluster);
   uint64_t before_block;
-  const int in_bin = (int)over_blocks(cluster, sh, [](const auto& o) { return o.listed; }, rank, before_block);
-  if (over_blocks(cluster, sh, [](const auto& o) { return o.listed > kListed; }) != 0 || in_bin > kNear) {
+  const int in_band = (int)over_blocks(cluster, sh, [](const auto& o) { return o.listed; }, rank, before_block);
+  const uint64_t base = over_blocks(cluster, sh, [](const auto& o) { return o.above; });
+  rest = over_blocks(cluster, sh, [](const auto& o) { return o.rest; });
+  if (over_blocks(cluster, sh, [](const auto& o) { return o.listed > kListed; }) != 0 || in_band > kNear) {
     uint64_t unused;
-    const uint64_t same_top = over_blocks(cluster, sh, [](const auto& o) { return o.listed > 0 && o.most != o.least; });
-    // Keys that differ between blocks: the sums of the listed blocks' keys tell.
+    const uint64_t several = over_blocks(cluster, sh, [](const auto& o) { return o.listed > 0 && o.most != o.least; });
+    // Keys that differ between blocks: their mean is not all of theirs.
     const uint64_t some = over_blocks(cluster, sh, [](const auto& o) { return o.listed > 0; });
     const uint64_t keys = over_blocks(cluster, sh, [](const auto& o) { return o.listed > 0 ? (uint64_t)o.most : 0; }, rank, unused);
     const uint32_t key = (uint32_t)(keys / some);
     const uint64_t others = over_blocks(cluster, sh, [&](const auto& o) { return o.listed > 0 && o.most != key; });
     sync_all(cluster);  // the lists have been read
-    if (same_top == 0 && others == 0) {  // ties of one key
-      const uint64_t w = r.weight(value_of(key));
-      choose_by_border(cluster, sh, a, row, r, value_of(key), (want - above + w - 1) / w, 0.0f, u);
-    } else {
+    const uint64_t w = r.weight(value_of(key)), want = wanted_of(top_p, base + in_band * w + rest);
+    if (several == 0 && others == 0 && base < want && want <= base + in_band * w)  // ties of one key
+      choose_by_border(cluster, sh, a, row, r, value_of(key), (want - base + w - 1) / w, 0.0f, u);
+    else
       choose_over_row(cluster, sh, a, row, r, 0, top_p, 0.0f, u);
-    }
     return;
   }
   uint64_t* to = cluster.map_shared_rank(&sh, 0)->gathered;
@@ -722,41 +747,46 @@ __device__ void choose_by_share(cg::cluster_group& cluster, Shared<W>& sh, const
   sync_all(cluster);
   if (rank == 0) {
     auto key_at = [&](int i) { return (uint32_t)(sh.gathered[i] >> 32); };
-    const Border b = cut_list(
-        sh, in_bin, want - above, key_at, [&](int i) { return (uint32_t)sh.gathered[i]; },
-        [&](int i) { return r.weight(value_of(key_at(i))); });
+    auto weight_at = [&](int i) { return r.weight(value_of(key_at(i))); };
+    uint64_t band = 0;
+    for (int i = tid; i < in_band; i += kThreads) band += weight_at(i);
+    scan_block(band, sh, band);
+    const uint64_t want = wanted_of(top_p, base + band + rest);
+    Border b{0, 0};  // not in the band after all
+    if (base < want && want <= base + band)
+      b = cut_list(sh, in_band, want - base, key_at, [&](int i) { return (uint32_t)sh.gathered[i]; }, weight_at);
     if (tid == 0) sh.border = (uint64_t)b.key << 32 | b.token;
   }
   sync_all(cluster);
   const uint64_t packed = cluster.map_shared_rank(&sh, 0)->border;
   const Border border{(uint32_t)(packed >> 32), (uint32_t)packed};
-  uint64_t band = 0, band_count = 0;
-  for (int i = tid; i < listed; i += kThreads)
-    if (border.in(sh.list_key[i], (uint32_t)(r.first + (int)sh.list_at[i]))) {
-      band += r.weight(value_of(sh.list_key[i]));
-      band_count++;
-    }
-  scan_block(band, sh, all);
-  kept_above += all;
+  if (border.key == 0) {
+    choose_over_row(cluster, sh, a, row, r, 0, top_p, 0.0f, u);
+    return;
+  }
+  // The band's kept tokens count in their segments.
+  uint64_t band_count = 0;
+  for (int i = tid; i < listed; i += kThreads) {
+    const bool in = border.in(sh.list_key[i], (uint32_t)(r.first + (int)sh.list_at[i]));
+    sh.gathered[i] = in ? r.weight(value_of(sh.list_key[i])) : 0;
+    band_count += in;
+  }
   scan_block(band_count, sh, all);
   counts += all;
+  const int begin = segments.base + lane * segments.size, end = min(segments.last, begin + segments.size);
+  for (int i = 0; i < listed; i++)
+    if (const int at = (int)sh.list_at[i]; at >= begin && at < end) mine += sh.gathered[i];
+  uint64_t before = scan_block(mine, sh, all), of_blocks;
   if (tid == 0) {
-    sh.mass = kept_above;
+    sh.mass = all;
     sh.count = (int)counts;
   }
   sync_all(cluster);
-  uint64_t before;
-  const uint64_t mass = over_blocks(cluster, sh, [](const auto& o) { return o.mass; }, rank, before);
+  const uint64_t mass = over_blocks(cluster, sh, [](const auto& o) { return o.mass; }, rank, of_blocks);
   counts = over_blocks(cluster, sh, [](const auto& o) { return o.count; });
   sync_all(cluster);  // the others have read this block's
-  const uint64_t target = target_of(u, mass);
-  if (!(before <= target && target < before + kept_above)) return;  // the whole block
-  auto kept = [&](float z, int token) { return border.in(key_of(z), (uint32_t)token); };
-  const Segments<W, T> segments(r);
-  const uint64_t mine =
-      segments.template sums<true>(r, [&](int at, float z, uint64_t w) { return kept(z, r.first + at) ? w : 0; });
-  before += scan_block(mine, sh, all);
-  find_token(sh, a, row, r, segments, before, mine, mass, u, (int)counts, kept);
+  find_token(sh, a, row, r, segments, before + of_blocks, mine, mass, u, (int)counts,
+             [&](float z, int token) { return border.in(key_of(z), (uint32_t)token); });
 }
 
 template <typename T, bool W>

@@ -48,13 +48,17 @@ def run(L, logits, rules, flags=0):
     return tokens.tolist(), logprobs.tolist(), kept.tolist()
 
 
-def check(L, logits, rules):
-    got = run(L, logits, rules)
+def check(L, logits, rules, some=False):
+    """Every row's choice is determined, or, with `some`, is looked at where it is, in half of the rows at least."""
+    got, unclear = run(L, logits, rules), 0
     x = logits.double().cpu().numpy()
     n, vocab = x.shape
     for r in range(n):
         one = {k: (np.float32(v[r]) if k != "top_k" else v[r]) for k, v in rules.items()}
         token, logprob, kept, margin = ref.choose(x[r], **one)
+        if some and not margin > 1:
+            unclear += 1
+            continue
         assert margin > 1, "a border next to a place that decides: another seed"
         assert (got[0][r], got[2][r]) == (token, kept), (r, one)
         # The share's rounding to f32 after steps of 2^-45 of each weight: relative to the token's own weight.
@@ -62,6 +66,7 @@ def check(L, logits, rules):
             assert got[1][r] == logprob
         else:
             assert abs(got[1][r] - logprob) <= 2.0 ** -24 * abs(logprob) + 2.0 ** -45 * vocab / math.exp(max(logprob, -20)) + 1e-12
+    assert 2 * unclear <= n
     return got
 
 
@@ -307,4 +312,4 @@ def test_logits_and_temperatures_of_every_size(cuda_lib, n):
         for t in (1e-3, 1.0, 1e4, 1e20):
             for which in ("", "k", "p", "m", "kp"):
                 rules = {**rules_of(n, which, 13, 5003), "temperature": [t] * n}
-                check(cuda_lib, x, rules)
+                check(cuda_lib, x, rules, some=True)  # where all weights are equal, borders lie on round numbers
