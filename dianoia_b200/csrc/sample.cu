@@ -46,7 +46,6 @@ constexpr int kBins = 256;
 constexpr int kNears = 512;     // bins of distances: 32 to an octave, from 2^-8 to 2^8 of a logit
 constexpr int kDepths = 16;        // steps of weights that top_p's border is looked for in,
 constexpr float kDepth = 1.5f;     // so many octaves each
-constexpr int kNear = 512;         // tokens of its border bin that the first block gathers
 
 // The cluster's barrier counts whole warps: lanes that leave a loop a turn late
 // would be counted as there, their additions still to come (seen as sums that
@@ -74,6 +73,7 @@ struct Form {
   static constexpr int kThreads = WHOLE ? 1024 : 256, kWarps = kThreads / 32;
   static constexpr int kListed = WHOLE ? kGathered : 512;  // tokens that a block lists
   static constexpr int kTops = WHOLE ? 4 : 1;            // largest logits that a thread has
+  static constexpr int kNear = WHOLE ? 2048 : 1024;      // tokens of top_p's border that the first block gathers
 };
 
 // What the blocks of a cluster read of one another.
@@ -83,7 +83,7 @@ struct Shared {
   // A histogram's sums in three parts of 15 bits, which shared memory adds by
   // itself (64-bit additions are loops there).
   uint32_t part[3][kBins];
-  uint64_t gathered[kNear];
+  uint64_t gathered[Form<WHOLE>::kNear];
   uint32_t near[kNears];
   uint32_t list_key[kListed];
   typename std::conditional<WHOLE, uint32_t, uint16_t>::type list_at[kListed];
@@ -725,7 +725,7 @@ __device__ void choose_by_share(cg::cluster_group& cluster, Shared<W>& sh, const
   const int in_band = (int)over_blocks(cluster, sh, [](const auto& o) { return o.listed; }, rank, before_block);
   const uint64_t base = over_blocks(cluster, sh, [](const auto& o) { return o.above; });
   rest = over_blocks(cluster, sh, [](const auto& o) { return o.rest; });
-  if (over_blocks(cluster, sh, [](const auto& o) { return o.listed > kListed; }) != 0 || in_band > kNear) {
+  if (over_blocks(cluster, sh, [](const auto& o) { return o.listed > kListed; }) != 0 || in_band > Form<W>::kNear) {
     uint64_t unused;
     const uint64_t several = over_blocks(cluster, sh, [](const auto& o) { return o.listed > 0 && o.most != o.least; });
     // Keys that differ between blocks: their mean is not all of theirs.
@@ -766,7 +766,7 @@ __device__ void choose_by_share(cg::cluster_group& cluster, Shared<W>& sh, const
   }
   // The band's kept tokens count in their segments.
   uint64_t band_count = 0;
-  for (int i = tid; i < listed; i += kThreads) {
+  for (int i = tid; i < listed; i += kThreads) {  // no more than were gathered
     const bool in = border.in(sh.list_key[i], (uint32_t)(r.first + (int)sh.list_at[i]));
     sh.gathered[i] = in ? r.weight(value_of(sh.list_key[i])) : 0;
     band_count += in;
