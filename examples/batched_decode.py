@@ -12,9 +12,19 @@ cache names; then each step, for all requests together and in each layer:
 
 and at its end the lm_head and the rules on its logits (penalties for what a
 request has said so far, a bias, a mask) with dn_logits_apply, before the
-greedy choice. Needs a B200 and torch:
+greedy choice. With `--cache q8` the keys and values are kept in 8 bits, half the
+room of bf16, and a block's output is added to the residual stream in the pass
+that norms it for the next block:
+
+    cache append, head norms, RoPE    dn_paged_q8_append
+    attention, per request            dn_paged_q8_attention
+    residual add, next RMSNorm        dn_residual_norm
+
+With `--temperature` above 0 the tokens are drawn (dn_sample, with `--top-k`,
+`--top-p` and `--min-p`) in place of the greedy choice. Needs a B200 and torch:
 
     python examples/batched_decode.py --requests 32 --prefix 1024 --steps 16
+    python examples/batched_decode.py --cache q8 --temperature 0.7 --top-p 0.9
 """
 from __future__ import annotations
 
@@ -63,6 +73,13 @@ def stream():
     return torch.cuda.current_stream().cuda_stream
 
 
+def add_norm(x, y, w, h):
+    """x + y into x, and the norm of that into h."""
+    _lib.check(_lib.lib().dn_residual_norm(_lib.DN_F32, y.data_ptr(), y.shape[1], None, None, 0, 1.0, _lib.DN_F32, x.data_ptr(),
+                                           x.shape[1], x.data_ptr(), x.shape[1], w.data_ptr(), EPS, h.data_ptr(), h.shape[1],
+                                           None, 0, x.shape[0], x.shape[1], 0, stream()))
+
+
 def norm(x, w):
     out = torch.empty_like(x)
     _lib.check(_lib.lib().dn_rms_norm(x.data_ptr(), w.data_ptr(), out.data_ptr(), None, 0, x.shape[0], x.shape[1], EPS, 0, 0,
@@ -71,7 +88,7 @@ def norm(x, w):
 
 
 class Layer:
-    def __init__(self, pages, table, gen):
+    def __init__(self, pages, table, gen, cache):
         weight = lambda n: 1 + 0.1 * torch.randn(n, device="cuda", generator=gen)
         self.qkv = Linear((HEADS + 2 * KV_HEADS) * HEAD_DIM, HIDDEN, gen)
         self.o = Linear(HIDDEN, HEADS * HEAD_DIM, gen)
@@ -79,6 +96,13 @@ class Layer:
         self.down = Linear(HIDDEN, INTER, gen)
         self.norm1, self.norm2, self.q_norm, self.k_norm = weight(HIDDEN), weight(HIDDEN), weight(HEAD_DIM), weight(HEAD_DIM)
         shape = (pages, KV_HEADS, PAGE, HEAD_DIM)
+        if cache == "q8":
+            self.keys, self.values = (torch.zeros(shape, dtype=torch.int8, device="cuda") for _ in range(2))
+            self.key_scales, self.value_scales = (torch.zeros(shape[:3], device="cuda") for _ in range(2))
+            self.cache = _lib.PagedQ8Cache(self.keys.data_ptr(), self.values.data_ptr(), self.key_scales.data_ptr(),
+                                           self.value_scales.data_ptr(), table.data_ptr(), pages, PAGE, KV_HEADS, HEAD_DIM,
+                                           table.shape[0], table.shape[1], KV_HEADS * PAGE * HEAD_DIM, KV_HEADS * PAGE)
+            return
         self.keys, self.values = (torch.zeros(shape, dtype=torch.bfloat16, device="cuda") for _ in range(2))
         self.cache = _lib.PagedCache(self.keys.data_ptr(), self.values.data_ptr(), table.data_ptr(), _lib.DN_BF16, pages, PAGE,
                                      KV_HEADS, HEAD_DIM, table.shape[0], table.shape[1], KV_HEADS * PAGE * HEAD_DIM)
@@ -87,8 +111,9 @@ class Layer:
 class Model:
     """`requests` sequences; row `requests` of the page table is the prompt's own."""
 
-    def __init__(self, layers, vocab, requests, prefix, room, seed=0):
+    def __init__(self, layers, vocab, requests, prefix, room, seed=0, cache="bf16"):
         gen = torch.Generator(device="cuda").manual_seed(seed)
+        self.kind = cache
         self.requests, self.prefix, self.vocab = requests, prefix, vocab
         shared, each = -(-prefix // PAGE), -(-room // PAGE) + 1
         self.width = shared + each
@@ -108,7 +133,7 @@ class Model:
             -torch.arange(HEAD_DIM // 2, device="cuda") * 2 / HEAD_DIM)
         self.rope = torch.cat([angle.cos(), angle.sin()], 1).float().contiguous()
         self.embed = torch.randn((vocab, HIDDEN), device="cuda", generator=gen)
-        self.layers = [Layer(at, self.table, gen) for _ in range(layers)]
+        self.layers = [Layer(at, self.table, gen, cache) for _ in range(layers)]
         self.final, self.head = 1 + 0.1 * torch.randn(HIDDEN, device="cuda", generator=gen), Linear(vocab, HIDDEN, gen)
 
     def forward(self, tokens, seq, pos, starts, lengths, prefix):
@@ -137,18 +162,50 @@ class Model:
             x = x + layer.down(g)
         return x
 
+    def forward_q8(self, tokens, seq, pos, starts, lengths):
+        """forward() over an 8-bit cache; gives the hidden states behind the final norm."""
+        L, n = _lib.lib(), tokens.numel()
+        x = self.embed[tokens.long()]
+        q = torch.empty((n, HEADS * HEAD_DIM), dtype=torch.bfloat16, device="cuda")
+        out = torch.empty_like(q)
+        need = L.dn_paged_q8_attention_workspace(self.layers[0].cache, HEADS, n, self.max_length)
+        work = torch.empty(need, dtype=torch.uint8, device="cuda")
+        h = norm(x, self.layers[0].norm1)
+        for layer, after in zip(self.layers, [layer.norm1 for layer in self.layers[1:]] + [self.final]):
+            qkv = layer.qkv(h)
+            k = qkv.data_ptr() + HEADS * HEAD_DIM * 4
+            row = qkv.shape[1]
+            _lib.check(L.dn_paged_q8_append(layer.cache, _lib.DN_F32, qkv.data_ptr(), row, k, row, k + KV_HEADS * HEAD_DIM * 4,
+                                            row, seq.data_ptr(), pos.data_ptr(), self.rope.data_ptr(), self.rope.shape[0],
+                                            HEAD_DIM, layer.q_norm.data_ptr(), layer.k_norm.data_ptr(), EPS, _lib.DN_BF16,
+                                            q.data_ptr(), q.shape[1], HEADS, n, 0, stream()))
+            _lib.check(L.dn_paged_q8_attention(layer.cache, _lib.DN_BF16, q.data_ptr(), q.shape[1], starts.data_ptr(),
+                                               lengths.data_ptr(), self.max_length, HEAD_DIM ** -0.5, 0, out.data_ptr(),
+                                               out.shape[1], HEADS, n, work.data_ptr(), need, 0, stream()))
+            add_norm(x, layer.o(out.float()), layer.norm2, h)
+            g, u = layer.gate(h), layer.up(h)
+            _lib.check(L.dn_swiglu(g.data_ptr(), u.data_ptr(), None, g.numel(), 0, stream()))
+            add_norm(x, layer.down(g), after, h)
+        return h
+
+    def states(self, tokens, seq, pos, starts, lengths, prefix):
+        """Hidden states behind the final norm."""
+        if self.kind == "q8":
+            return self.forward_q8(tokens, seq, pos, starts, lengths)
+        return norm(self.forward(tokens, seq, pos, starts, lengths, prefix), self.final)
+
     def prompt(self, tokens):
         """Runs the shared prompt once, as the table's last sequence."""
         n, r = tokens.numel(), self.requests
-        self.forward(tokens, ints([r] * n), torch.arange(n, dtype=torch.int32, device="cuda"), ints([0] * (r + 1) + [n]),
+        self.states(tokens, ints([r] * n), torch.arange(n, dtype=torch.int32, device="cuda"), ints([0] * (r + 1) + [n]),
                      ints([0] * r + [n]), 0)
 
     def step(self, tokens, done):
         """Logits of one token for each request, `done` tokens of its own behind it."""
         r = self.requests
         seq, pos = torch.arange(r, dtype=torch.int32, device="cuda"), ints([self.prefix + done] * r)
-        x = self.forward(tokens, seq, pos, ints(list(range(r + 1)) + [r]), ints([self.prefix + done + 1] * r + [0]), self.prefix)
-        return self.head(norm(x, self.final))
+        return self.head(self.states(tokens, seq, pos, ints(list(range(r + 1)) + [r]),
+                                     ints([self.prefix + done + 1] * r + [0]), self.prefix))
 
 
 def rules_of(history, vocab, banned):
@@ -170,8 +227,32 @@ def rules_of(history, vocab, banned):
     return rules, keep
 
 
-def decode(model, prompt, first, steps, banned=(1, 2, 3), forced=None):
-    """Greedy tokens [steps][requests] and each step's ruled logits; with `forced`, those tokens are fed instead."""
+class Chooser:
+    """Draws the tokens of `requests` rows of logits by the same rules; a request's random numbers are its own."""
+
+    def __init__(self, requests, temperature, top_k=0, top_p=1.0, min_p=0.0, seed=0):
+        full = lambda v, t: torch.full((requests,), v, dtype=t, device="cuda")
+        self.rules = [full(temperature, torch.float32), full(top_k, torch.int32), full(top_p, torch.float32),
+                      full(min_p, torch.float32)]
+        self.gens = [torch.Generator(device="cuda").manual_seed(seed + r) for r in range(requests)]
+        self.uniform, self.used = None, 0
+
+    def __call__(self, logits):
+        n, vocab = logits.shape
+        if self.uniform is None or self.used == len(self.uniform):  # the next 64 steps' numbers
+            self.uniform = torch.stack([torch.rand(64, device="cuda", generator=g) for g in self.gens], 1).contiguous()
+            self.used = 0
+        uniform = self.uniform[self.used]
+        self.used += 1
+        how = _lib.Sampling(*(t.data_ptr() for t in self.rules + [uniform]))
+        tokens = torch.empty(n, dtype=torch.int32, device="cuda")
+        _lib.check(_lib.lib().dn_sample(_lib.DN_F32, logits.data_ptr(), vocab, n, vocab, how, tokens.data_ptr(), None, None, 0,
+                                        stream()))
+        return tokens
+
+
+def decode(model, prompt, first, steps, banned=(1, 2, 3), forced=None, choose=lambda logits: logits.argmax(-1)):
+    """Chosen tokens (by default greedily) [steps][requests] and each step's ruled logits; with `forced`, those are fed instead."""
     model.prompt(prompt)
     tokens, history, said, seen = first, [[t] for t in first.tolist()], [], []
     for i in range(steps):
@@ -180,7 +261,7 @@ def decode(model, prompt, first, steps, banned=(1, 2, 3), forced=None):
         _lib.check(_lib.lib().dn_logits_apply(_lib.DN_F32, logits.data_ptr(), model.vocab, logits.data_ptr(), model.vocab,
                                               model.requests, model.vocab, rules, 0, stream()))
         seen.append(logits)
-        tokens = (logits.argmax(-1) if forced is None else forced[i]).int()
+        tokens = (choose(logits) if forced is None else forced[i]).int()
         said.append(tokens)
         for h, t in zip(history, tokens.tolist()):
             h.append(t)
@@ -194,15 +275,23 @@ def main():
     ap.add_argument("--steps", type=int, default=16)
     ap.add_argument("--layers", type=int, default=4)
     ap.add_argument("--vocab", type=int, default=151936)
+    ap.add_argument("--cache", choices=("bf16", "q8"), default="bf16")
+    ap.add_argument("--temperature", type=float, default=0.0)
+    ap.add_argument("--top-k", type=int, default=0)
+    ap.add_argument("--top-p", type=float, default=1.0)
+    ap.add_argument("--min-p", type=float, default=0.0)
     a = ap.parse_args()
-    model = Model(a.layers, a.vocab, a.requests, a.prefix, a.steps + 1)
+    model = Model(a.layers, a.vocab, a.requests, a.prefix, a.steps + 1, cache=a.cache)
+    how = {}
+    if a.temperature > 0:
+        how["choose"] = Chooser(a.requests, a.temperature, a.top_k, a.top_p, a.min_p)
     gen = torch.Generator(device="cuda").manual_seed(1)
     prompt = torch.randint(0, a.vocab, (a.prefix,), device="cuda", generator=gen, dtype=torch.int32)
     first = torch.randint(0, a.vocab, (a.requests,), device="cuda", generator=gen, dtype=torch.int32)
-    decode(model, prompt, first, 2)
+    decode(model, prompt, first, 2, **how)
     begin, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
     begin.record()
-    said, _ = decode(model, prompt, first, a.steps)
+    said, _ = decode(model, prompt, first, a.steps, **how)
     end.record()
     torch.cuda.synchronize()
     ms = begin.elapsed_time(end)
