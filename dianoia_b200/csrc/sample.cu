@@ -27,6 +27,9 @@
 // blocks, warps, segments. Where more tokens matter than the lists hold (thousands
 // of top_k, many ties) the border is found eight bits of the key at a time over all
 // of the row.
+#include <algorithm>
+#include <cfloat>
+
 #include <cooperative_groups.h>
 
 #include "dn_common.cuh"
@@ -44,8 +47,9 @@ constexpr int kGathered = 2048;  // tokens that the first block gathers
 constexpr int kMostK = 1536;    // top_k up to which the histogram is asked
 constexpr int kBins = 256;
 constexpr int kNears = 512;     // bins of distances: 32 to an octave, from 2^-8 to 2^8 of a logit
-constexpr int kDepths = 16;        // steps of weights that top_p's border is looked for in,
-constexpr float kDepth = 1.5f;     // so many octaves each
+constexpr int kDepths = 16;       // steps of weights that top_p's border is looked for in,
+constexpr float kDepth = 1.5f;    // so many octaves each,
+constexpr float kDeepest = 31.0f;  // and the last of them that any weight is in: 2^-46 of the largest
 
 // The cluster's barrier counts whole warps: lanes that leave a loop a turn late
 // would be counted as there, their additions still to come (seen as sums that
@@ -424,13 +428,15 @@ __device__ uint32_t border_of(cg::cluster_group& cluster, Shared<W>& sh, const R
 template <bool W, typename T>
 struct Segments {
   static constexpr int kChunk = 128;
-  int size, base, last;  // tokens of a segment; the warp's run
+  int run, size, base, last;  // tokens of a warp, of a segment; this warp's run
   __device__ __forceinline__ explicit Segments(const Row<T>& r) {
-    const int run = ((r.n + Form<W>::kWarps - 1) / Form<W>::kWarps + kChunk - 1) / kChunk * kChunk;
+    run = ((r.n + Form<W>::kWarps - 1) / Form<W>::kWarps + kChunk - 1) / kChunk * kChunk;
     size = (run + 32 * kChunk - 1) / (32 * kChunk) * kChunk;
     base = (int)threadIdx.x / 32 * run;
     last = min(r.n, base + run);
   }
+  // The thread that has the segment of a place.
+  __device__ __forceinline__ int lane_of(int at) const { return at / run * 32 + at % run / size; }
   // f(place, logit, weight) gives a token's part of the sum; a lane gets the sum
   // over its segment.
   template <bool WEIGHTS, typename F>
@@ -598,21 +604,38 @@ __device__ void choose_over_row(cg::cluster_group& cluster, Shared<W>& sh, const
 // top_p alone.
 template <bool W, typename T>
 __device__ void choose_by_share(cg::cluster_group& cluster, Shared<W>& sh, const SampleArgs& a, int64_t row, const Row<T>& r,
-                                float top_p, float u) {
+                                float top_p, float u, uint8_t* smem) {
   constexpr int kThreads = Form<W>::kThreads, kWarps = Form<W>::kWarps, kListed = Form<W>::kListed;
   const int tid = threadIdx.x, lane = tid % 32, blocks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const float per = (float)(r.per256 / 256);
-  // How far a token lies below the largest, in octaves of weights.
-  auto depth_of = [&](float z) { return z == r.largest ? 0.0f : (r.largest - z) * per; };
-  // ---- the sums to each octave, and of all
+  // How far a token lies below the largest, in steps of kDepth octaves of weights.
+  const float per_step = per / kDepth;
+  auto depth_of = [&](float z) { return z == r.largest ? 0.0f : z > -INFINITY ? (r.largest - z) * per_step : INFINITY; };
+  // ---- the sums to each step, and of all
   {
     float sum[kDepths] = {}, whole = 0.0f;
-    r.each_logit(tid, r.n, kThreads, [&](int, float z) {
-      const float d = z > -INFINITY ? depth_of(z) : INFINITY, w = power2(-d);
-      whole += w;
+    if constexpr (W) {
+      // A column of shared memory to a thread, with its sums of each step: 17 us of
+      // 152 thousand tokens where 16 comparisons a token took 53.
+      float* column = reinterpret_cast<float*>(smem) + tid;
 #pragma unroll
-      for (int i = 0; i < kDepths; i++) sum[i] += d <= kDepth * (float)(i + 1) ? w : 0.0f;
-    });
+      for (int i = 0; i < kDepths; i++) column[i * kThreads] = 0.0f;
+      r.each_logit(tid, r.n, kThreads, [&](int, float z) {
+        const float d = depth_of(z), w = power2(-kDepth * d);
+        whole += w;
+        if (d < (float)kDepths) column[(int)d * kThreads] += w;
+      });
+#pragma unroll
+      for (int i = 0; i < kDepths; i++) sum[i] = column[i * kThreads] + (i > 0 ? sum[i > 0 ? i - 1 : 0] : 0.0f);
+    } else {
+      r.each_logit(tid, r.n, kThreads, [&](int, float z) {
+        const float d = depth_of(z), w = power2(-kDepth * d);
+        whole += w;
+#pragma unroll
+        for (int i = 0; i < kDepths; i++)
+          if (d < (float)(i + 1)) sum[i] += w;
+      });
+    }
     float mine = 0.0f;
 #pragma unroll
     for (int i = 0; i <= kDepths; i++) {
@@ -644,17 +667,13 @@ __device__ void choose_by_share(cg::cluster_group& cluster, Shared<W>& sh, const
 #pragma unroll
   for (int b = 0; b < kMaxBlocks; b++) upto += b < blocks ? of_block[b] : 0.0f;
   const float whole = __shfl_sync(0xffffffffu, upto, kDepths);
-  // The border lies from depth `near` to `far`, whatever f32 sums may be off by.
+  // The border lies from step `near` to `far`, whatever f32 sums may be off by.
   const unsigned enough = __ballot_sync(0xffffffffu, lane < kDepths && upto >= (top_p + 0.001f) * whole);
   const unsigned short_of = __ballot_sync(0xffffffffu, lane < kDepths && upto <= (top_p - 0.001f) * whole);
-  const float near = kDepth * (float)__popc(short_of), far = enough != 0 ? kDepth * (float)__ffs(enough) : 46.0f;
+  const float near = (float)__popc(short_of), far = enough != 0 ? (float)__ffs(enough) : kDeepest;
   const float base_sum = short_of != 0 ? __shfl_sync(0xffffffffu, upto, __popc(short_of) - 1) : 0.0f;
   const float per_bin = (float)kBins / (far - near);
-  // -1 above all bins, kBins below.
-  auto bin_of = [&](float d) {
-    return d <= near && near > 0.0f ? -1 : !(d <= far) ? kBins : min((int)((d - near) * per_bin), kBins - 1);
-  };
-  // ---- the bins of those depths, in steps of 2^-16 of the first one's weights
+  // ---- the bins of those steps, in units of 2^-16 of the first one's weights
   if (tid < kBins) sh.part[0][tid] = 0;
   if (tid == 0) {
     sh.band_first = 0;
@@ -663,8 +682,8 @@ __device__ void choose_by_share(cg::cluster_group& cluster, Shared<W>& sh, const
   __syncthreads();
   r.each_logit(tid, r.n, kThreads, [&](int, float z) {
     const float d = depth_of(z);
-    const int bin = bin_of(d);
-    if (bin >= 0 && bin < kBins) atomicAdd(&sh.part[0][bin], __float2uint_rn(power2(near - d + 16.0f)));
+    if (d >= near && d < far)
+      atomicAdd(&sh.part[0][min((int)((d - near) * per_bin), kBins - 1)], __float2uint_rn(power2(kDepth * (near - d) + 16.0f)));
   });
   sync_all(cluster);
   uint64_t all;
@@ -676,24 +695,29 @@ __device__ void choose_by_share(cg::cluster_group& cluster, Shared<W>& sh, const
 #pragma unroll
     for (int b = 0; b < (W ? 1 : kMaxBlocks); b++) own += b < blocks && tid < kBins ? of_block[b] : 0;
     const uint64_t before = scan_block(own, sh, all);
-    const float unit = power2(-16.0f - near), from = base_sum + (float)before * unit, to = base_sum + (float)(before + own) * unit;
+    const float unit = power2(-16.0f - kDepth * near), from = base_sum + (float)before * unit, to = base_sum + (float)(before + own) * unit;
     const float less = (top_p - 2e-5f) * whole, more = (top_p + 2e-5f) * whole;
     if (tid < kBins && from <= less && less < to) sh.band_first = tid;
     if (tid < kBins && from < more && more <= to) sh.band_last = tid;
   }
   __syncthreads();
-  const int band_first = sh.band_first, band_last = sh.band_last;
+  // The band in logits, a little wider than what f32 rounds its ends by; what it
+  // holds is checked below.
+  const float high_step = near + (float)sh.band_first / per_bin, low_step = near + (float)(sh.band_last + 1) / per_bin;
+  auto at_step = [&](float step) { return r.largest - step / per_step; };
+  const float wider = (fabsf(r.largest) + low_step / per_step) * 1e-6f;
+  const float high = high_step > 0.0f ? at_step(high_step) + wider : INFINITY;
+  const float low = low_step < kDeepest ? at_step(low_step) - wider : -FLT_MAX;
   // ---- all weights: those above the band by segments, the band's tokens in a list
   uint64_t count = 0, counts, rest = 0;
   uint32_t most = 0, least = ~0u;
   const Segments<W, T> segments(r);
   uint64_t mine = segments.template sums<true>(r, [&](int at, float z, uint64_t w) -> uint64_t {
-    const int bin = bin_of(depth_of(z));
-    if (bin < band_first) {
+    if (z > high) {
       count++;
       return w;
     }
-    if (bin > band_last) {
+    if (!(z >= low)) {
       rest += w;
       return 0;
     }
@@ -764,18 +788,21 @@ __device__ void choose_by_share(cg::cluster_group& cluster, Shared<W>& sh, const
     choose_over_row(cluster, sh, a, row, r, 0, top_p, 0.0f, u);
     return;
   }
-  // The band's kept tokens count in their segments.
+  // The band's kept tokens count in their segments. (A lane that looked through the
+  // list for its own took a third of the time.)
+  static_assert(Form<W>::kNear >= kThreads, "the gathered ones' place holds a sum for each segment");
+  sh.gathered[tid] = 0;
+  __syncthreads();
   uint64_t band_count = 0;
   for (int i = tid; i < listed; i += kThreads) {  // no more than were gathered
-    const bool in = border.in(sh.list_key[i], (uint32_t)(r.first + (int)sh.list_at[i]));
-    sh.gathered[i] = in ? r.weight(value_of(sh.list_key[i])) : 0;
-    band_count += in;
+    const int at = (int)sh.list_at[i];
+    if (!border.in(sh.list_key[i], (uint32_t)(r.first + at))) continue;
+    atomicAdd(reinterpret_cast<unsigned long long*>(&sh.gathered[segments.lane_of(at)]), r.weight(value_of(sh.list_key[i])));
+    band_count++;
   }
   scan_block(band_count, sh, all);
   counts += all;
-  const int begin = segments.base + lane * segments.size, end = min(segments.last, begin + segments.size);
-  for (int i = 0; i < listed; i++)
-    if (const int at = (int)sh.list_at[i]; at >= begin && at < end) mine += sh.gathered[i];
+  mine += sh.gathered[tid];
   uint64_t before = scan_block(mine, sh, all), of_blocks;
   if (tid == 0) {
     sh.mass = all;
@@ -898,7 +925,7 @@ __global__ void __launch_bounds__(Form<W>::kThreads, W ? 1 : 4) sample_kernel(co
   }
   if (top_k == 0 && !m) {
     if (p)
-      choose_by_share(cluster, sh, a, row, r, top_p, u);
+      choose_by_share(cluster, sh, a, row, r, top_p, u, smem);
     else
       choose_by_border(cluster, sh, a, row, r, -INFINITY, ~0ull, 0.0f, u);
     return;
@@ -1035,8 +1062,10 @@ template <typename T>
 cudaError_t launch_type(const SampleArgs& a, cudaStream_t stream, bool pdl) {
   constexpr int V = 16 / sizeof(T);
   if (a.n >= kMany) {
-    if (cudaError_t e = allow_smem<sample_kernel<T, true>>(kGathered * 16); e != cudaSuccess) return e;
-    return launch_form<T, true>(a, 1, 0, kGathered * 16, stream, pdl);
+    // The gathered tokens, or the columns of top_p's steps.
+    constexpr int bytes = std::max(kGathered * 16, kDepths * Form<true>::kThreads * (int)sizeof(float));
+    if (cudaError_t e = allow_smem<sample_kernel<T, true>>(bytes); e != cudaSuccess) return e;
+    return launch_form<T, true>(a, 1, 0, bytes, stream, pdl);
   }
   // The fewest blocks whose part of a row is 40 KB at most, so that four of them share an SM.
   const int64_t vecs = (a.vocab + 2 * V - 2) / V;
