@@ -18,15 +18,24 @@
 //    near as the k-th of these;
 //  - min_p: the weight says it.
 // Their weights and keys go to the first block's shared memory, which cuts them by
-// histograms of their keys' bytes and decides alone while the others leave. top_p alone may keep any number of
-// tokens: f32 sums by octaves of the weights tell where its border is to an octave
-// or two, whose weights go into a histogram (shared memory adds fewer than two
-// lanes a clock: all weights in one took 15 of 38 us), and the border bin's tokens
-// are the ones that the first block cuts; without a rule but the temperature there is
-// nothing to cut. Then the place that the random number falls to is looked for by sums of
-// blocks, warps, segments. Where more tokens matter than the lists hold (thousands
-// of top_k, many ties) the border is found eight bits of the key at a time over all
-// of the row.
+// histograms of their keys' bytes and decides alone while the others leave. top_p
+// alone may keep any number of tokens: f32 sums by steps of 1.5 octaves of the
+// weights tell where its border is to a step or two, whose weights go into a
+// histogram (shared memory adds fewer than two lanes a clock: all weights in one
+// took 15 of 38 us), and the border bin's tokens are the ones that the first block
+// cuts; without a rule but the temperature there is nothing to cut. Then the place
+// that the random number falls to is looked for by sums of blocks, warps, segments.
+// Where more tokens matter than the lists hold (thousands of top_k, many ties) the
+// border is found eight bits of the key at a time over all of the row.
+//
+// Measured at 151936 f32 logits, one row / 256 rows, us: the largest alone 5 / 51,
+// no rules 13 / 116, min_p 11 / 73 to 94, top_k 17 / 88, top_k with top_p 21 / 102,
+// top_p alone 33 / 230; reading 256 rows takes 24. A row without rules is bound by
+// its f64 weights (30 of 54 us on an SM: about 11 operations at 64 a clock and the
+// conversions), top_p by four passes: 8 the maximum, 17 the steps, 20 the bins, 43
+// the weights with the band. 256 rows are 1.7 to an SM, so the last ones run on 108
+// of 148 SMs; two blocks of 512 threads to an SM instead, all rows at once, were
+// slower (top_k 111, top_p 362: 156 MB do not stay in L2).
 #include <algorithm>
 #include <cfloat>
 
@@ -201,31 +210,49 @@ struct Row {
     weights(one, w);
     return w[0];
   }
-  // Calls f(place, logit) for places at0, at0 + step, .. below end, in order; past
-  // the end, too, with -inf.
-  template <typename F>
-  __device__ __forceinline__ void each_logit(int at0, int end, int step, F&& f) const {
-    constexpr int N = 4;
-    for (int at = at0; at < end; at += N * step) {
-      float z[N];
+  // Elements of the 16 bytes that begin at place `at`, of this part's alone; -inf
+  // for the others. Where the caller has the row, places begin `shift` before it
+  // at a 16-byte boundary.
+  static constexpr int V = 16 / sizeof(T);
+  __device__ __forceinline__ uint4 vector(int at, int end) const {
+    if (at >= 0 && at + V <= end) return *reinterpret_cast<const uint4*>(x + at);
+    T e[V];
 #pragma unroll
-      for (int i = 0; i < N; i++) z[i] = at + i * step < end ? logit(at + i * step) : -INFINITY;
-#pragma unroll
-      for (int i = 0; i < N; i++) f(at + i * step, z[i]);
-    }
+    for (int j = 0; j < V; j++) e[j] = at + j >= 0 && at + j < end ? x[at + j] : from_f32<T>(-INFINITY);
+    uint4 raw;
+    memcpy(&raw, e, 16);
+    return raw;
   }
-  // The same with the weights.
-  template <typename F>
-  __device__ __forceinline__ void each_weight(int at0, int end, int step, F&& f) const {
-    constexpr int N = 4;
-    for (int at = at0; at < end; at += N * step) {
-      float z[N];
-      uint64_t w[N];
+  __device__ __forceinline__ int shift() const { return (int)(((uintptr_t)x & 15) / sizeof(T)); }
+  // Calls f(place, logit) for all of this part's tokens; for places outside, too, with -inf.
+  template <bool W, typename F>
+  __device__ __forceinline__ void each_logit(F&& f) const {
+    constexpr int kThreads = Form<W>::kThreads;
+    if constexpr (W) {
+      // From L2: 48 bytes a thread on the way, as single elements 16.
+      constexpr int N = 3;
+      const int step = kThreads * V;
+      for (int at = (int)threadIdx.x * V - shift(); at < n; at += N * step) {
+        uint4 raw[N];
 #pragma unroll
-      for (int i = 0; i < N; i++) z[i] = at + i * step < end ? logit(at + i * step) : -INFINITY;
-      weights(z, w);
+        for (int i = 0; i < N; i++) raw[i] = vector(at + i * step, n);
 #pragma unroll
-      for (int i = 0; i < N; i++) f(at + i * step, z[i], w[i]);
+        for (int i = 0; i < N; i++) {
+          T e[V];
+          memcpy(e, &raw[i], 16);
+#pragma unroll
+          for (int j = 0; j < V; j++) f(at + i * step + j, to_f32<T>(e[j]));
+        }
+      }
+    } else {
+      constexpr int N = 4;
+      for (int at = threadIdx.x; at < n; at += N * kThreads) {
+        float z[N];
+#pragma unroll
+        for (int i = 0; i < N; i++) z[i] = at + i * kThreads < n ? logit(at + i * kThreads) : -INFINITY;
+#pragma unroll
+        for (int i = 0; i < N; i++) f(at + i * kThreads, z[i]);
+      }
     }
   }
 };
@@ -620,7 +647,7 @@ __device__ void choose_by_share(cg::cluster_group& cluster, Shared<W>& sh, const
       float* column = reinterpret_cast<float*>(smem) + tid;
 #pragma unroll
       for (int i = 0; i < kDepths; i++) column[i * kThreads] = 0.0f;
-      r.each_logit(tid, r.n, kThreads, [&](int, float z) {
+      r.template each_logit<W>([&](int, float z) {
         const float d = depth_of(z), w = power2(-kDepth * d);
         whole += w;
         if (d < (float)kDepths) column[(int)d * kThreads] += w;
@@ -628,7 +655,7 @@ __device__ void choose_by_share(cg::cluster_group& cluster, Shared<W>& sh, const
 #pragma unroll
       for (int i = 0; i < kDepths; i++) sum[i] = column[i * kThreads] + (i > 0 ? sum[i > 0 ? i - 1 : 0] : 0.0f);
     } else {
-      r.each_logit(tid, r.n, kThreads, [&](int, float z) {
+      r.template each_logit<W>([&](int, float z) {
         const float d = depth_of(z), w = power2(-kDepth * d);
         whole += w;
 #pragma unroll
@@ -680,7 +707,7 @@ __device__ void choose_by_share(cg::cluster_group& cluster, Shared<W>& sh, const
     sh.band_last = kBins - 1;
   }
   __syncthreads();
-  r.each_logit(tid, r.n, kThreads, [&](int, float z) {
+  r.template each_logit<W>([&](int, float z) {
     const float d = depth_of(z);
     if (d >= near && d < far)
       atomicAdd(&sh.part[0][min((int)((d - near) * per_bin), kBins - 1)], __float2uint_rn(power2(kDepth * (near - d) + 16.0f)));
@@ -907,8 +934,9 @@ __global__ void __launch_bounds__(Form<W>::kThreads, W ? 1 : 4) sample_kernel(co
   if (top == 0 || !(temperature > 0.0f) || min_p > 1.0f) {  // no token, or the first one alone
     if (top != 0) {
       int least = INT32_MAX;
-      for (int at = tid; at < r.n; at += kThreads)
-        if (r.key(at) == top) least = min(least, r.first + at);
+      r.template each_logit<W>([&](int at, float z) {
+        if (z == r.largest) least = min(least, r.first + at);
+      });
       least = __reduce_min_sync(0xffffffffu, least);
       if (lane == 0 && least != INT32_MAX) atomicMin(&first->first, least);
     }
@@ -971,7 +999,7 @@ __global__ void __launch_bounds__(Form<W>::kThreads, W ? 1 : 4) sample_kernel(co
   // min_p's cut may not touch what top_p sums. The margin is what f32 may be off by.
   float low = -INFINITY;  // log2 of a weight
   if (m && !p) low = log2f(min_p) * 1.00001f - 0.001f;
-  r.each_logit(tid, r.n, kThreads, [&](int place, float z) {
+  r.template each_logit<W>([&](int place, float z) {
     if (z > -INFINITY && !(r.largest - z >= far) && !((z - r.largest) * per < low)) {
       const int at = atomicAdd(&sh.listed, 1);
       if (at < kListed) sh.list_at[at] = place;
