@@ -576,15 +576,22 @@ int64_t dn_paged_q8_read(const dn_paged_q8_cache* cache, int64_t type, const int
  * positions, window, outputs and the rows that see nothing as for
  * dn_paged_attention, every position read through its sequence's table row
  * (there is no shared prefix; sequences may name the same pages). q and out
- * are elements of `type`. It is made for decode steps, one to a few tokens a
- * sequence: a sequence's keys are split over the GPU by length and joined, and
- * read once for up to 32 rows (tokens times heads of a kv head; fewer for
- * heads over 128). Any number of tokens is computed right. Scores, softmax and
- * sums are in f32; the int8 values enter the tensor cores as they are, the
- * queries and each weight (probability times its value's scale) as bf16 parts
- * of 8 bits each: one and two of them (bf16), two (f16) or three (f32).
- * max_length and
- * `workspace` as for dn_paged_attention. */
+ * are elements of `type`; out may be q (the same address and stride). It is
+ * made for decode steps, one to a few tokens a sequence: a sequence's keys are
+ * read once for the rows (its tokens times the heads of a kv head) of a tile of
+ * 8, 16 or 32 (32 for bf16 and heads up to 128 only), tiled by the average
+ * number of tokens a sequence. Any number of tokens is computed right. Scores,
+ * softmax and sums are in f32; the int8 values enter the tensor cores as they
+ * are, the queries and each weight (probability times its value's scale) as
+ * bf16 parts of 8 bits each: one and two of them (bf16), two (f16) or three
+ * (f32). The batch's work is divided over the GPU on the device, by the lengths
+ * it finds there; max_length (the longest that the batch may have, a hint: any
+ * lengths are computed right) says whether long sequences are split at all,
+ * which batches of up to 256 positions are not, and with it what workspace the
+ * parts need. `workspace` (16-byte aligned, at least
+ * dn_paged_q8_attention_workspace bytes, from the same cache, heads, n and
+ * max_length) is undefined before and after, and calls that overlap in time
+ * need one each. */
 int64_t dn_paged_q8_attention_workspace(const dn_paged_q8_cache* cache, int64_t heads, int64_t n,
                                         int64_t max_length);
 int64_t dn_paged_q8_attention(const dn_paged_q8_cache* cache, int64_t type, const void* q, int64_t q_stride,
