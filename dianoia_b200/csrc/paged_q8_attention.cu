@@ -34,9 +34,8 @@
 // Measured, device time and share of a copy's 6.5 TB/s: 64 sequences of up to 16384
 // positions, 32 heads on 8 of 128, bf16: 204 us, 83 %; f16 215 us; f32 at half the
 // sequences 124 us, 68 %; 64 heads on 4 (16 rows a tile) 163 us, 52 %. One sequence
-// of 131072, 28 heads on 4: 39 us, 54 % (filling the rings and the join are a
-// quarter of it). Prompts run too, though this is made for decode steps: 2048 bf16
-// tokens of 16 heads on 8 in 250 us.
+// of 131072, 28 heads on 4: 39 us, 54 %, of which the join 5. Prompts run too, though
+// this is made for decode steps: 2048 bf16 tokens of 16 heads on 8 in 250 us.
 #include "dn_common.cuh"
 #include "dn_launch.h"
 #include "elem.cuh"
