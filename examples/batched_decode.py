@@ -199,6 +199,15 @@ class Model:
         n, r = tokens.numel(), self.requests
         self.states(tokens, ints([r] * n), torch.arange(n, dtype=torch.int32, device="cuda"), ints([0] * (r + 1) + [n]),
                      ints([0] * r + [n]), 0)
+        whole = n // PAGE
+        if self.kind != "q8" or n % PAGE == 0:
+            return
+        # The 8-bit attention reads every position through a request's own table: the
+        # prompt's last page, which the requests write on, becomes a copy for each.
+        own = self.table[:r, whole].long()
+        for layer in self.layers:
+            for pool in (layer.keys, layer.values, layer.key_scales, layer.value_scales):
+                pool[own] = pool[int(self.table[r, whole])].clone()
 
     def step(self, tokens, done):
         """Logits of one token for each request, `done` tokens of its own behind it."""

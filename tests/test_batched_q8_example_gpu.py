@@ -72,12 +72,18 @@ def test_cache_holds_the_prompt(cuda_lib):
     for model in models:
         model.prompt(prompt)
     wide, narrow = (model.layers[0] for model in models)
-    seq, pos = ex.ints([1] * prefix), torch.arange(prefix, dtype=torch.int32, device="cuda")
+    seq, first, pos = ex.ints([1] * prefix), ex.ints([0] * prefix), torch.arange(prefix, dtype=torch.int32, device="cuda")
     row = ex.KV_HEADS * ex.HEAD_DIM
     k, v = (torch.empty((prefix, row), device="cuda") for _ in range(2))
     assert cuda_lib.dn_paged_q8_read(narrow.cache, 0, seq.data_ptr(), pos.data_ptr(), k.data_ptr(), row, v.data_ptr(), row,
                                      prefix, 0, ex.stream()) == 0
     torch.cuda.synchronize()
+    # A request finds the same rows through its own table.
+    mine = [torch.empty_like(k) for _ in range(2)]
+    assert cuda_lib.dn_paged_q8_read(narrow.cache, 0, first.data_ptr(), pos.data_ptr(), mine[0].data_ptr(), row,
+                                     mine[1].data_ptr(), row, prefix, 0, ex.stream()) == 0
+    torch.cuda.synchronize()
+    assert torch.equal(mine[0], k) and torch.equal(mine[1], v)
     pages = models[0].table[1].long()[:-(-prefix // ex.PAGE)]
     for got, pool in ((k, wide.keys), (v, wide.values)):
         got = got.view(prefix, ex.KV_HEADS, ex.HEAD_DIM)
