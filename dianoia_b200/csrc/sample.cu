@@ -30,10 +30,10 @@
 //
 // Measured at 151936 f32 logits, one row / 256 rows, us: the largest alone 5 / 51,
 // no rules 13 / 116, min_p 11 / 73 to 94, top_k 17 / 88, top_k with top_p 21 / 102,
-// top_p alone 33 / 230; reading 256 rows takes 24. A row without rules is bound by
+// top_p alone 33 / 227; reading 256 rows takes 24. A row without rules is bound by
 // its f64 weights (30 of 54 us on an SM: about 11 operations at 64 a clock and the
-// conversions), top_p by four passes: 8 the maximum, 17 the steps, 20 the bins, 43
-// the weights with the band. 256 rows are 1.7 to an SM, so the last ones run on 108
+// conversions), top_p by four passes and the cuts, of 114 us with a row on every SM: 8
+// the maximum, 20 the steps, 16 to 25 the bins, 42 the weights with the band, 7 the cuts. 256 rows are 1.7 to an SM, so the last ones run on 108
 // of 148 SMs; two blocks of 512 threads to an SM instead, all rows at once, were
 // slower (top_k 111, top_p 362: 156 MB do not stay in L2).
 #include <algorithm>
@@ -147,6 +147,10 @@ __device__ __forceinline__ float power2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+
+// The whole part of 0 <= x < 2^23: by an addition, which four times as many lanes
+// do as a conversion.
+__device__ __forceinline__ int whole_part(float x) { return __float_as_int(__fadd_rd(x, 8388608.0f)) & 0x7fffff; }
 
 template <typename T>
 struct Row {
@@ -642,7 +646,7 @@ __device__ void choose_by_share(cg::cluster_group& cluster, Shared<W>& sh, const
   {
     float sum[kDepths] = {}, whole = 0.0f;
     if constexpr (W) {
-      // A column of shared memory to a thread, with its sums of each step: 17 us of
+      // A column of shared memory to a thread, with its sums of each step: 20 us of
       // 152 thousand tokens where 16 comparisons a token took 53.
       float* column = reinterpret_cast<float*>(smem) + tid;
 #pragma unroll
@@ -650,7 +654,7 @@ __device__ void choose_by_share(cg::cluster_group& cluster, Shared<W>& sh, const
       r.template each_logit<W>([&](int, float z) {
         const float d = depth_of(z), w = power2(-kDepth * d);
         whole += w;
-        if (d < (float)kDepths) column[(int)d * kThreads] += w;
+        if (d < (float)kDepths) column[whole_part(d) * kThreads] += w;
       });
 #pragma unroll
       for (int i = 0; i < kDepths; i++) sum[i] = column[i * kThreads] + (i > 0 ? sum[i > 0 ? i - 1 : 0] : 0.0f);
@@ -710,7 +714,7 @@ __device__ void choose_by_share(cg::cluster_group& cluster, Shared<W>& sh, const
   r.template each_logit<W>([&](int, float z) {
     const float d = depth_of(z);
     if (d >= near && d < far)
-      atomicAdd(&sh.part[0][min((int)((d - near) * per_bin), kBins - 1)], __float2uint_rn(power2(kDepth * (near - d) + 16.0f)));
+      atomicAdd(&sh.part[0][min(whole_part((d - near) * per_bin), kBins - 1)], __float2uint_rn(power2(kDepth * (near - d) + 16.0f)));
   });
   sync_all(cluster);
   uint64_t all;
