@@ -32,10 +32,11 @@
 // no rules 13 / 116, min_p 11 / 73 to 94, top_k 17 / 88, top_k with top_p 21 / 102,
 // top_p alone 33 / 227; reading 256 rows takes 24. A row without rules is bound by
 // its f64 weights (30 of 54 us on an SM: about 11 operations at 64 a clock and the
-// conversions), top_p by four passes and the cuts, of 114 us with a row on every SM: 8
-// the maximum, 20 the steps, 16 to 25 the bins, 42 the weights with the band, 7 the cuts. 256 rows are 1.7 to an SM, so the last ones run on 108
-// of 148 SMs; two blocks of 512 threads to an SM instead, all rows at once, were
-// slower (top_k 111, top_p 362: 156 MB do not stay in L2).
+// conversions), top_p by four passes and the cuts, of 114 us with a row on every
+// SM: 8 the maximum, 20 the steps, 16 to 25 the bins, 42 the weights with the band, 7
+// the cuts. 256 rows are 1.7 to an SM, so the last ones run on 108 of 148 SMs; two
+// blocks of 512 threads to an SM instead, all rows at once, were slower (top_k 111,
+// top_p 362: 156 MB do not stay in L2).
 #include <algorithm>
 #include <cfloat>
 
