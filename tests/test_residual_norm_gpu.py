@@ -126,6 +126,15 @@ def test_qa_blocks(cuda_lib, kind, cols, pad):
     assert torch.equal(c.qa[:, :blocks], got)
 
 
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("cols", [2056, 2080, 3000, 4064, 4088, 4104, 4128, 8160, 8200, 16384, 16416])
+def test_runs_that_do_not_fill_the_threads(cuda_lib, kind, cols):
+    """Rows in runs of 8 values on either side of each number of runs a thread, with QA blocks where a row is whole blocks."""
+    if cols % 32 == 0:
+        test_qa_blocks(cuda_lib, kind, cols, 0)
+    Case(kind, "f32", 300, cols, gate="one", seed=cols).check(cuda_lib)
+
+
 def test_values_of_every_size(cuda_lib):
     c = Case("f32", "f32", 4, 256)
     c.y[0], c.y[1] = 0, c.y[1] * 1e15
